@@ -267,6 +267,73 @@ int nd_op_silu(const float* x, long long n, float* out, void* stream);
  * scale). An id outside [0, vocab) gives a row of zeros. */
 int nd_op_gather(const nd_model* m, const int* ids, int T, float* out, void* stream);
 
+/* ---- Serving from one pool of pages: a 4-bit cache shared by sequences of
+ * different lengths, attention over it, page bookkeeping, draft checking.
+ * No counterpart in the reference, whose cache is one session's int8 ring.
+ * Device pointers of GPU `device`, whichever device is current; queued on
+ * `stream` (of that device; NULL = its legacy default stream) and not waited
+ * for; 0 on success, -1 with nd_last_error() and nothing queued. No call
+ * allocates or keeps anything, so all may be captured into a graph; a
+ * workspace `ws` is the caller's, holds nothing between calls, and must not
+ * be used by two calls that overlap on the GPU. Lengths, tables and ids are
+ * read on the device and may change between replays; whatever they hold, no
+ * kernel reads or writes outside the buffers named here. */
+
+/* Types of rows and logits. */
+enum { ND_F32 = 0, ND_F16 = 1, ND_BF16 = 2 };
+
+/* A 4-bit cache and the rows of one call. pool: num_pages pages,
+ * page_stride bytes apart (a multiple of 16; the pointer 16-byte aligned),
+ * each [heads][page / 16] tiles of 16 * (dk / 2 + dv / 2 + 8) bytes: key codes
+ * [16][dk / 2], value codes [16][dv / 2] (two a byte, lower dimension in the
+ * low nibble), f16 (scale, minimum) of the 16 keys, of the 16 values; a value
+ * is minimum + scale * code. page is a multiple of 16; (dk, dv) is (48, 64),
+ * (64, 64) or (128, 128); at most 2^20 sequences. table[seqs][max_pages] (rows table_stride apart)
+ * names each sequence's pages in order; positions past its columns, or on a
+ * page id outside [0, num_pages), do not exist. lens[seqs]: positions each
+ * sequence holds, this call's rows included. The call's `rows` rows belong to
+ * the sequences in order, start[s] .. start[s + 1] - 1 to sequence s
+ * (start[seqs + 1], ascending; NULL: rows / seqs each): row i of the n of
+ * sequence s is position lens[s] - n + i. Rows behind start[seqs] are left
+ * alone. */
+typedef struct nd_kv4 {
+    int device;
+    void* pool;
+    long long page_stride;
+    int num_pages, page, heads, dk, dv;
+    const int* table;
+    int table_stride, max_pages, seqs;
+    const int* lens;
+    const int* start;
+    int rows;
+} nd_kv4;
+
+/* Quantize rows k[rows][heads][dk], v[rows][heads][dv] of `type` (element
+ * strides k_row, k_head, ..; the last dimension contiguous) into their
+ * places. Per row and head, in f32: scale = f16(min((max - min) / 15, 65504)),
+ * minimum = f16(min, clamped to +-65504), code = rint((x - minimum) / scale)
+ * in [0, 15], 0 where scale is 0. A row of values holding a NaN or an infinity
+ * is stored as NaN. Rows whose position does not exist are dropped. */
+int nd_op_kv4_append(const nd_kv4* kv, int type, const void* k, long long k_row, long long k_head, const void* v,
+                     long long v_row, long long v_head, void* stream);
+
+/* The cache's values at the rows' positions, rounded once to `type`; zeros
+ * where a position does not exist. */
+int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long long k_head, void* v, long long v_row,
+                   long long v_head, void* stream);
+
+/* Attention of the rows q[rows][q_heads][dk] over the cache (which holds the
+ * rows' own keys already): out[rows][q_heads][dv] of the same `type`. Query
+ * head g reads kv head g / (q_heads / heads), q_heads / heads <= 64. A row at
+ * position p sees the positions j <= p that exist, with window > 0 only those
+ * with j > p - window or j < sink. out = softmax(scale q.k) v; zeros for a row
+ * that sees nothing. out must not overlap q. ws: nd_op_kv4_attend_ws(kv,
+ * q_heads) bytes, 16-byte aligned. */
+unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads);
+int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row, long long q_head, int q_heads, float scale,
+                     int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
+                     void* stream);
+
 /* The last failure on this thread (empty if none). */
 const char* nd_last_error(void);
 

@@ -1,0 +1,227 @@
+// Rows into and out of the paged 4-bit cache (nd_op_kv4_append,
+// nd_op_kv4_read). A row of values x (one position, one kv head, its key or
+// its value) is kept as codes c in 0 .. 15 with an f16 scale s and minimum m,
+// x ~ m + s c; every step is an IEEE f32 operation rounded once, so codes do
+// not depend on how the work is split.
+
+#include <cfloat>
+#include <stdexcept>
+#include <string>
+
+#include "kernels.h"
+#include "kv4.cuh"
+#include "kv4_host.h"
+
+namespace nd {
+
+// A warp takes one row of the call: its 2 * heads vectors, L lanes each with
+// eight values a lane (so a lane forms one 32-bit word of codes), 32 / L
+// vectors at a time. HBM bound: each value is read once by 16-byte loads and
+// the codes leave as runs of dk / 2 bytes; the search for the row's sequence
+// costs two or three dependent loads of a warp, not log2(seqs).
+template <int DK, int DV>
+struct RowSplit {
+    static constexpr int L = DK > 64 || DV > 64 ? 16 : 8;
+    static constexpr int PER = 32 / L;
+};
+
+constexpr int ROW_WARPS = 8;
+
+template <int DK, int DV, typename T>
+__global__ void __launch_bounds__(32 * ROW_WARPS) kv4_append_kernel(Kv4Args a, const T* __restrict__ k, long long k_row, long long k_head,
+                                                                    const T* __restrict__ v, long long v_row, long long v_head, bool vec) {
+    constexpr int TB = kv4_tile_bytes(DK, DV), L = RowSplit<DK, DV>::L, PER = RowSplit<DK, DV>::PER;
+    const int lane = threadIdx.x & 31, r = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    if (r >= a.rows) return;
+    int s, first, n;
+    if (!kv4_find_row(a, r, lane, &s, &first, &n)) return;
+    const long long pos = (long long)__ldg(a.lens + s) - n + (r - first);
+    uint8_t* tile0 = kv4_tile_of(a, s, pos, TB);
+    if (!tile0) return;
+    const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
+    for (int j = blockIdx.y * PER + lane / L; j - lane / L < 2 * a.heads; j += gridDim.y * PER) {
+        const bool val = j >= a.heads;
+        const int h = val ? j - a.heads : j, D = val ? DV : DK;
+        const bool on = j < 2 * a.heads && d0 < D;
+        float x[8];
+        float lo = FLT_MAX, hi = -FLT_MAX;
+        bool bad = false;
+        if (on) {
+            load8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                bad |= !(fabsf(x[i]) <= FLT_MAX);
+                lo = fminf(lo, x[i]);
+                hi = fmaxf(hi, x[i]);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < L; o *= 2) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+        }
+        if (!on) continue;
+        __half sh = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), 65504.0f));
+        __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
+        const float sf = __half2float(sh), mf = __half2float(mh);
+        uint32_t w = 0;
+        if (bad) {
+            sh = mh = __ushort_as_half(0x7fff);
+        } else if (sf > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), sf)), 0.f), 15.f);
+                w |= (uint32_t)(int)c << (4 * i);
+            }
+        }
+        uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
+        *(uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub) = w;
+        if (sub == 0) *(__half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot) = __halves2half2(sh, mh);
+    }
+}
+
+template <int DK, int DV, typename T>
+__global__ void __launch_bounds__(32 * ROW_WARPS) kv4_read_kernel(Kv4Args a, T* __restrict__ k, long long k_row, long long k_head,
+                                                                  T* __restrict__ v, long long v_row, long long v_head, bool vec) {
+    constexpr int TB = kv4_tile_bytes(DK, DV), L = RowSplit<DK, DV>::L, PER = RowSplit<DK, DV>::PER;
+    const int lane = threadIdx.x & 31, r = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    if (r >= a.rows) return;
+    int s, first, n;
+    if (!kv4_find_row(a, r, lane, &s, &first, &n)) return;
+    const long long pos = (long long)__ldg(a.lens + s) - n + (r - first);
+    const uint8_t* tile0 = kv4_tile_of(a, s, pos, TB);
+    const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
+    for (int j = blockIdx.y * PER + lane / L; j < 2 * a.heads; j += gridDim.y * PER) {
+        const bool val = j >= a.heads;
+        const int h = val ? j - a.heads : j, D = val ? DV : DK;
+        if (d0 >= D) continue;
+        float x[8];
+        if (tile0) {
+            const uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
+            const uint32_t w = *(const uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub);
+            const float2 sm = __half22float2(*(const __half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot));
+            // the product of an f16 and a code is exact: one rounding
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __fmaf_rn(sm.x, (float)((w >> (4 * i)) & 15), sm.y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 0.f;
+        }
+        store8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x);
+    }
+}
+
+Kv4Args kv4_args(const nd_kv4* kv, const char* what) {
+    auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
+    if (!kv) fail("null cache");
+    if (!kv->pool || !kv->table || !kv->lens) fail("null pointer");
+    if (kv->num_pages < 1 || kv->heads < 1 || kv->max_pages < 1 || kv->seqs < 1 || kv->rows < 0) fail("sizes must be positive");
+    if (kv->heads > 65535 || kv->seqs > (1 << 20)) fail("at most 65535 heads and 2^20 sequences");
+    if (kv->page < 16 || kv->page % 16) fail("page must be a multiple of 16 positions");
+    if (!((kv->dk == 48 && kv->dv == 64) || (kv->dk == 64 && kv->dv == 64) || (kv->dk == 128 && kv->dv == 128)))
+        fail("(dk, dv) must be (48, 64), (64, 64) or (128, 128)");
+    if (kv->table_stride < kv->max_pages) fail("table rows overlap");
+    if ((uintptr_t)kv->pool % 16 || kv->page_stride % 16) fail("the pool and its page stride must be 16-byte aligned");
+    const long long bytes = (long long)kv->heads * (kv->page / 16) * kv4_tile_bytes(kv->dk, kv->dv);
+    if (kv->page_stride < bytes) fail("pages overlap");
+    if ((long long)kv->max_pages * kv->page > 0x7fffffffLL) fail("more than 2^31 - 1 positions a sequence");
+    if (!kv->start && kv->rows % kv->seqs) fail("without start, rows must be a multiple of the sequences");
+    return Kv4Args{(uint8_t*)kv->pool, kv->page_stride, kv->table,   kv->table_stride, kv->max_pages, kv->num_pages,
+                   kv->page / 16,      kv->heads,       kv->seqs,    kv->rows,         kv->lens,      kv->start};
+}
+
+bool kv4_vec(int type, const void* p, long long row, long long head) {
+    const int e = type == ND_F32 ? 4 : 2;
+    return (uintptr_t)p % 16 == 0 && row * e % 16 == 0 && head * e % 16 == 0;
+}
+
+void kv4_check_rows(const char* what, int type, const void* p, long long row, long long head) {
+    auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
+    if (type != ND_F32 && type != ND_F16 && type != ND_BF16) fail("unknown type");
+    if (!p) fail("null pointer");
+    if ((uintptr_t)p % (type == ND_F32 ? 4 : 2)) fail("rows must be aligned to their type");
+    if (row < 0 || head < 0) fail("negative strides");
+}
+
+// Rows that are written may not share memory.
+static void check_distinct(const char* what, long long row, long long head, int rows, int heads, int d) {
+    const bool row_major = head >= d && (rows <= 1 || row >= (long long)(heads - 1) * head + d);
+    const bool head_major = row >= d && (heads <= 1 || head >= (long long)(rows - 1) * row + d);
+    const bool one = heads == 1 && (rows <= 1 || row >= d);
+    if (!row_major && !head_major && !one) throw std::runtime_error(std::string(what) + ": output rows overlap");
+}
+
+void kv4_check_out(const char* what, int type, const void* p, long long row, long long head, int rows, int heads, int d) {
+    kv4_check_rows(what, type, p, row, head);
+    check_distinct(what, row, head, rows, heads, d);
+}
+
+// Calls f with the cache's head dimensions and the rows' type as templates.
+template <typename F>
+static void dispatch(int dk, int type, F&& f) {
+    auto typed = [&](auto dkc, auto dvc) {
+        if (type == ND_F32) f(dkc, dvc, (float*)nullptr);
+        else if (type == ND_F16) f(dkc, dvc, (__half*)nullptr);
+        else f(dkc, dvc, (__nv_bfloat16*)nullptr);
+    };
+    if (dk == 48) typed(std::integral_constant<int, 48>(), std::integral_constant<int, 64>());
+    else if (dk == 64) typed(std::integral_constant<int, 64>(), std::integral_constant<int, 64>());
+    else typed(std::integral_constant<int, 128>(), std::integral_constant<int, 128>());
+}
+
+// Rows go eight to a CTA; with few rows the vectors of a row are spread over
+// grid.y so that a handful of rows of many heads still fills the GPU.
+static dim3 row_grid(const Kv4Args& a, int per) {
+    const int x = (a.rows + ROW_WARPS - 1) / ROW_WARPS, steps = (2 * a.heads + per - 1) / per;
+    const int want = (4 * device_sm_count() + x - 1) / x;
+    return dim3(x, std::min(std::min(steps, std::max(want, 1)), 65535));
+}
+
+}  // namespace nd
+
+using namespace nd;
+
+extern "C" {
+
+int nd_op_kv4_append(const nd_kv4* kv, int type, const void* k, long long k_row, long long k_head, const void* v,
+                     long long v_row, long long v_head, void* stream) {
+    return op_call([&] {
+        const char* what = "nd_op_kv4_append";
+        const Kv4Args a = kv4_args(kv, what);
+        if (a.rows == 0) return;
+        kv4_check_rows(what, type, k, k_row, k_head);
+        kv4_check_rows(what, type, v, v_row, v_head);
+        const bool vec = kv4_vec(type, k, k_row, k_head) && kv4_vec(type, v, v_row, v_head);
+        OnDevice on(kv->device, what);
+        dispatch(kv->dk, type, [&](auto dk, auto dv, auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
+            kv4_append_kernel<DK, DV, T><<<row_grid(a, RowSplit<DK, DV>::PER), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(
+                a, (const T*)k, k_row, k_head, (const T*)v, v_row, v_head, vec);
+        });
+        op_launched(what);
+    });
+}
+
+int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long long k_head, void* v, long long v_row,
+                   long long v_head, void* stream) {
+    return op_call([&] {
+        const char* what = "nd_op_kv4_read";
+        const Kv4Args a = kv4_args(kv, what);
+        if (a.rows == 0) return;
+        kv4_check_out(what, type, k, k_row, k_head, a.rows, a.heads, kv->dk);
+        kv4_check_out(what, type, v, v_row, v_head, a.rows, a.heads, kv->dv);
+        const bool vec = kv4_vec(type, k, k_row, k_head) && kv4_vec(type, v, v_row, v_head);
+        OnDevice on(kv->device, what);
+        dispatch(kv->dk, type, [&](auto dk, auto dv, auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
+            kv4_read_kernel<DK, DV, T><<<row_grid(a, RowSplit<DK, DV>::PER), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(
+                a, (T*)k, k_row, k_head, (T*)v, v_row, v_head, vec);
+        });
+        op_launched(what);
+    });
+}
+
+}  // extern "C"

@@ -72,6 +72,9 @@ def lib():
             "needle_reset": (None, []),
             "needle_last_error": (C.c_char_p, []),
         }
+        from ._abi import SIGNATURES
+
+        sig.update(SIGNATURES)
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
             fn.restype = res
@@ -467,3 +470,18 @@ def op_gather(model, ids, out=None):
     if lib().nd_op_gather(model._h, _p(ids), T, _p(out), _stream_of(ids)) != 0:
         raise _err()
     return out
+
+
+# ----------------------------------------- serving from one pool of pages
+
+# These live in serving.py, which needs torch; the rest of the package does not.
+_SERVING = ("KV4Pool", "op_kv4_append", "op_kv4_read", "op_kv4_attend")
+
+
+def __getattr__(name):
+    if name in _SERVING:
+        from . import serving
+
+        globals().update({n: getattr(serving, n) for n in _SERVING})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
