@@ -15,9 +15,20 @@
 // bits make 16 c * 2^-24, whose 16 is taken out of the matching query value
 // beforehand (q is scaled per row by a power of two so that its f16 keeps it)
 // or out of the accumulator row afterwards. 2^24 is put back in f32.
-// f32 queries are split into two f16 terms (22 bits); weights p sv into two
-// terms for f32 and f16 rows. For bf16 rows one f16 term: its 2^-12 is far
-// below the output's own 2^-9.
+// Weights p sv are split into two f16 terms (22 bits) for f32 and f16 rows;
+// bf16 rows take one: its 2^-12 is far below the output's own 2^-9.
+//
+// f32 rows. The tensor cores truncate their sums near the 24th bit, and codes
+// counted from the minimum add up to much more than the result, so what is
+// enough for 16-bit outputs loses f32's last bits twice over. For f32:
+// - q is split in fixed point: q = q1 + q2 with 11 bits each below the row's
+//   largest value (2^-24 of it is left). A k-sum of codes times either term,
+//   started at -8 sum(q_i) so that codes count from the middle, stays below
+//   2^24 units: it is exact, whatever the order.
+// - value codes are made the f16 e - 8 (one more instruction a pair), each
+//   tile's sum starts at zero and is added to the accumulator rounded.
+// Measured: 5e-7 of the result against 64 bits where the plain way had 4e-5
+// (keys and values with outlying channels).
 //
 // A warp keeps the softmax's running reference M per query row (a power-of-
 // two argument: scores carry log2 e) and rescales only when a new exponent
@@ -129,6 +140,20 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return *(const uint32_t*)&h;
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t x) { return __half22float2(*(const __half2*)&x); }
+// Codes (in the low four bits of each half; in the next four) to f16 c - 8:
+// 1024 + c and 1024 + 16 c are the f16 with those bits under 1024's exponent.
+__device__ __forceinline__ uint32_t code_mid(uint32_t x) {
+    x |= 0x64006400u;
+    uint32_t y;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0xe408e408u));  // -1032
+    return y;
+}
+__device__ __forceinline__ uint32_t code16_mid(uint32_t x) {
+    x |= 0x64006400u;
+    uint32_t y;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
+    return y;
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
@@ -151,6 +176,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
     kv4_attend_kernel(AttendArgs a, const T* __restrict__ q, T* __restrict__ out) {
     using Sh = AttendShape<DK, DV, NT, T>;
     constexpr int TB = Sh::TB, QS = Sh::QS, WS = Sh::WS, KS = Sh::KSTEPS, MT = DV / 16, VW = DV / 64;
+    constexpr bool MID = std::is_same<T, float>::value;  // codes count from 8
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long sums[32 * ATT_WARPS + 1];
     __shared__ long long warp_sums[ATT_WARPS];
@@ -258,7 +284,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         // the query block: lane (g, c) holds of query row 8 t + g the
         // dimensions whose codes it will hold of every key
         uint32_t qreg[Sh::Q_SMEM ? 1 : NT * Sh::QREGS];
-        float f0[NT][2], f1[NT][2];
+        float f0[NT][2], f1[NT][2], mid[QS == 2 ? NT : 1][2][2];
         int seen_hi[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -299,14 +325,20 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             float fac0 = a.scale_log2e * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * 16777216.f;
             float fac1 = a.scale_log2e * sum;
             if (bad) fac0 = fac1 = __uint_as_float(0x7fc00000u);
+            float q1 = 0.f, q2 = 0.f;  // sums of the fixed-point terms: exact
             auto put = [&](int k, int half, float x0, float x1) {  // operand `half` of k-step k
-                const uint32_t hi = pack_half2(x0, x1);
-                const int at = (t * KS + k) * 2 * QS + half * QS;
-                uint32_t lo = 0;
+                const float mul = half ? 0.0625f : 1.f;  // the second operand's codes come 16-fold
+                uint32_t hi, lo = 0;
                 if (QS == 2) {
-                    const float2 r = unpack_half2(hi);
-                    lo = pack_half2(x0 - r.x, x1 - r.y);
+                    // multiples of 16 up to 2^15, then of 2^-8 up to 8
+                    const float a0 = __fmul_rn(rintf(x0 * 0.0625f), 16.f), a1 = __fmul_rn(rintf(x1 * 0.0625f), 16.f);
+                    const float b0 = __fmul_rn(rintf((x0 - a0) * 256.f), 0.00390625f), b1 = __fmul_rn(rintf((x1 - a1) * 256.f), 0.00390625f);
+                    q1 += a0 + a1, q2 += b0 + b1;
+                    hi = pack_half2(a0 * mul, a1 * mul), lo = pack_half2(b0 * mul, b1 * mul);
+                } else {
+                    hi = pack_half2(x0 * mul, x1 * mul);
                 }
+                const int at = (t * KS + k) * 2 * QS + half * QS;
                 if constexpr (Sh::Q_SMEM) {
                     qsm[at * 32] = hi;
                     if (QS == 2) qsm[(at + 1) * 32] = lo;
@@ -321,13 +353,19 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             for (int w = 0; w < DK / 32; w++) {
                 const float* y = v + 8 * w;
                 put(2 * w, 0, y[0], y[4]);
-                put(2 * w, 1, y[1] * 0.0625f, y[5] * 0.0625f);
+                put(2 * w, 1, y[1], y[5]);
                 put(2 * w + 1, 0, y[2], y[6]);
-                put(2 * w + 1, 1, y[3] * 0.0625f, y[7] * 0.0625f);
+                put(2 * w + 1, 1, y[3], y[7]);
             }
             if constexpr (DK == 48) {
                 put(2, 0, v[8], v[10]);
-                put(2, 1, v[9] * 0.0625f, v[11] * 0.0625f);
+                put(2, 1, v[9], v[11]);
+            }
+            if (QS == 2) {
+                q1 += __shfl_xor_sync(0xffffffffu, q1, 1);
+                q2 += __shfl_xor_sync(0xffffffffu, q2, 1);
+                q1 += __shfl_xor_sync(0xffffffffu, q1, 2);
+                q2 += __shfl_xor_sync(0xffffffffu, q2, 2);
             }
             const int hi = on ? (int)min(max(rows.pos0 + x / a.group, -1LL), 0x7fffffffLL) : -1;
 #pragma unroll
@@ -335,6 +373,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
                 f0[t][j] = __shfl_sync(0xffffffffu, fac0, 4 * (2 * c + j));
                 f1[t][j] = __shfl_sync(0xffffffffu, fac1, 4 * (2 * c + j));
                 seen_hi[t][j] = __shfl_sync(0xffffffffu, hi, 4 * (2 * c + j));
+                if (QS == 2) {  // -8 of the codes' unit, 2^-24
+                    mid[t][j][0] = __shfl_sync(0xffffffffu, q1, 4 * (2 * c + j)) * -4.76837158203125e-7f;
+                    mid[t][j][1] = __shfl_sync(0xffffffffu, q2, 4 * (2 * c + j)) * -4.76837158203125e-7f;
+                }
             }
         }
         // tiles wholly inside every row's span need no masks
@@ -362,9 +404,14 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             const int k0 = tl.at(off + i) * KV4_TILE;
 
             // scores: keys g and g + 8 against query rows 2 c, 2 c + 1
-            float sc[NT][4];
+            float sc[NT][4], sc2[QS == 2 ? NT : 1][4];
 #pragma unroll
-            for (int t = 0; t < NT; t++) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    sc[t][j] = QS == 2 ? mid[QS == 2 ? t : 0][j & 1][0] : 0.f;
+                    if (QS == 2) sc2[QS == 2 ? t : 0][j] = mid[QS == 2 ? t : 0][j & 1][1];
+                }
             auto qop = [&](int t, int k, int half, int term) -> uint32_t {
                 const int at = (t * KS + k) * 2 * QS + half * QS + term;
                 if constexpr (Sh::Q_SMEM) return qsm[at * 32];
@@ -372,9 +419,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             };
             auto step = [&](int k, uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int term = 0; term < QS; term++) mma16816(sc[t], x0, y0, x1, y1, qop(t, k, 0, term), qop(t, k, 1, term));
+                for (int t = 0; t < NT; t++) {
+                    mma16816(sc[t], x0, y0, x1, y1, qop(t, k, 0, 0), qop(t, k, 1, 0));
+                    if (QS == 2) mma16816(sc2[QS == 2 ? t : 0], x0, y0, x1, y1, qop(t, k, 0, QS - 1), qop(t, k, 1, QS - 1));
+                }
             };
             const uint8_t *ka = tile + g * (DK / 2), *kb = tile + (g + 8) * (DK / 2);
             uint32_t wa[DK / 32], wb[DK / 32];
@@ -402,8 +450,12 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
                 step(2, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
             }
             const uint8_t* par = tile + 8 * (DK + DV);
-            const float2 kpa = unpack_half2(*(const uint32_t*)(par + 4 * g)), kpb = unpack_half2(*(const uint32_t*)(par + 4 * (g + 8)));
-            const float2 vpa = unpack_half2(*(const uint32_t*)(par + 64 + 4 * g)), vpb = unpack_half2(*(const uint32_t*)(par + 64 + 4 * (g + 8)));
+            float2 kpa = unpack_half2(*(const uint32_t*)(par + 4 * g)), kpb = unpack_half2(*(const uint32_t*)(par + 4 * (g + 8)));
+            float2 vpa = unpack_half2(*(const uint32_t*)(par + 64 + 4 * g)), vpb = unpack_half2(*(const uint32_t*)(par + 64 + 4 * (g + 8)));
+            if (QS == 2) {  // the middle of the codes instead of the minimum
+                kpa.y = __fmaf_rn(8.f, kpa.x, kpa.y), kpb.y = __fmaf_rn(8.f, kpb.x, kpb.y);
+                vpa.y = __fmaf_rn(8.f, vpa.x, vpa.y), vpb.y = __fmaf_rn(8.f, vpb.x, vpb.y);
+            }
             const float la = lg2(fmaxf(vpa.x, 5.9604645e-8f)), lb = lg2(fmaxf(vpb.x, 5.9604645e-8f));
             const bool whole = page_ok && k0 + 15 <= p_first && (a.window <= 0 || k0 > p_last - a.window || k0 + 15 < a.sink);
             uint32_t vis = 0xffffffffu;
@@ -412,6 +464,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             for (int t = 0; t < NT; t++) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
+                    if (QS == 2) sc[t][j] += sc2[QS == 2 ? t : 0][j], sc[t][2 + j] += sc2[QS == 2 ? t : 0][2 + j];
                     sc[t][j] = __fmaf_rn(kpa.x, sc[t][j] * f0[t][j], kpa.y * f1[t][j]);
                     sc[t][2 + j] = __fmaf_rn(kpb.x, sc[t][2 + j] * f0[t][j], kpb.y * f1[t][j]);
                 }
@@ -490,13 +543,12 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
                     const uint32_t sel = quarter < 2 ? 0x5410 : 0x7632;
                     const uint32_t x = __byte_perm(vw[0][w], vw[1][w], sel) >> (quarter & 1 ? 8 : 0);
                     const uint32_t y = __byte_perm(vw[2][w], vw[3][w], sel) >> (quarter & 1 ? 8 : 0);
-                    const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                    uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                    if (MID) a0 = code_mid(a0), a1 = code16_mid(a1), a2 = code_mid(a2), a3 = code16_mid(a3);
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
                         float* d = acc[t][4 * w + quarter];
-                        if constexpr (std::is_same<T, float>::value) {
-                            // the tensor cores truncate what they add to a sum:
-                            // a tile's own sum starts at zero and is added rounded
+                        if constexpr (MID) {
                             float z[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                             for (int term = 0; term < WS; term++) mma16816(z, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
@@ -531,8 +583,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
                     float v[8];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        v[2 * k] = __fmaf_rn(acc[t][4 * w + k][j], 16777216.f, mn[t][j]) * norm;
-                        v[2 * k + 1] = __fmaf_rn(acc[t][4 * w + k][2 + j], 1048576.f, mn[t][j]) * norm;
+                        v[2 * k] = __fmaf_rn(acc[t][4 * w + k][j], MID ? 1.f : 16777216.f, mn[t][j]) * norm;
+                        v[2 * k + 1] = __fmaf_rn(acc[t][4 * w + k][2 + j], MID ? 1.f : 1048576.f, mn[t][j]) * norm;
                     }
                     const int d0 = 8 * (VW * g + w);
                     if (starts && ends) {
