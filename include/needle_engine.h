@@ -281,6 +281,9 @@ int nd_op_gather(const nd_model* m, const int* ids, int T, float* out, void* str
 
 /* Types of rows and logits. */
 enum { ND_F32 = 0, ND_F16 = 1, ND_BF16 = 2 };
+/* In `flags`: output rows behind the last sequence are set to zero instead
+ * of left as they were. */
+enum { ND_ZERO_REST = 2 };
 
 /* A 4-bit cache and the rows of one call. pool: num_pages pages,
  * page_stride bytes apart (a multiple of 16; the pointer 16-byte aligned),
@@ -320,19 +323,20 @@ int nd_op_kv4_append(const nd_kv4* kv, int type, const void* k, long long k_row,
 /* The cache's values at the rows' positions, rounded once to `type`; zeros
  * where a position does not exist. */
 int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long long k_head, void* v, long long v_row,
-                   long long v_head, void* stream);
+                   long long v_head, int flags, void* stream);
 
 /* Attention of the rows q[rows][q_heads][dk] over the cache (which holds the
  * rows' own keys already): out[rows][q_heads][dv] of the same `type`. Query
  * head g reads kv head g / (q_heads / heads), q_heads / heads <= 64. A row at
  * position p sees the positions j <= p that exist, with window > 0 only those
  * with j > p - window or j < sink. out = softmax(scale q.k) v; zeros for a row
- * that sees nothing. out must not overlap q. ws: nd_op_kv4_attend_ws(kv,
- * q_heads) bytes, 16-byte aligned. */
-unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads);
+ * that sees nothing. out must not overlap q. ws:
+ * nd_op_kv4_attend_ws(the same arguments) bytes, 16-byte aligned; NULL where
+ * that is 0. */
+unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads, int window, int sink);
 int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row, long long q_head, int q_heads, float scale,
                      int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
-                     void* stream);
+                     int flags, void* stream);
 
 /* The last failure on this thread (empty if none). */
 const char* nd_last_error(void);

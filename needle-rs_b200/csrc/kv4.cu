@@ -83,14 +83,19 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_append_kernel(Kv4Args a, c
 
 template <int DK, int DV, typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_read_kernel(Kv4Args a, T* __restrict__ k, long long k_row, long long k_head,
-                                                                  T* __restrict__ v, long long v_row, long long v_head, bool vec) {
+                                                                  T* __restrict__ v, long long v_row, long long v_head, bool vec, bool zero_rest) {
     constexpr int TB = kv4_tile_bytes(DK, DV), L = RowSplit<DK, DV>::L, PER = RowSplit<DK, DV>::PER;
     const int lane = threadIdx.x & 31, r = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     if (r >= a.rows) return;
     int s, first, n;
-    if (!kv4_find_row(a, r, lane, &s, &first, &n)) return;
-    const long long pos = (long long)__ldg(a.lens + s) - n + (r - first);
-    const uint8_t* tile0 = kv4_tile_of(a, s, pos, TB);
+    long long pos = 0;
+    const uint8_t* tile0 = nullptr;
+    if (kv4_find_row(a, r, lane, &s, &first, &n)) {
+        pos = (long long)__ldg(a.lens + s) - n + (r - first);
+        tile0 = kv4_tile_of(a, s, pos, TB);
+    } else if (!zero_rest) {
+        return;
+    }
     const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
     for (int j = blockIdx.y * PER + lane / L; j < 2 * a.heads; j += gridDim.y * PER) {
         const bool val = j >= a.heads;
@@ -205,10 +210,11 @@ int nd_op_kv4_append(const nd_kv4* kv, int type, const void* k, long long k_row,
 }
 
 int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long long k_head, void* v, long long v_row,
-                   long long v_head, void* stream) {
+                   long long v_head, int flags, void* stream) {
     return op_call([&] {
         const char* what = "nd_op_kv4_read";
         const Kv4Args a = kv4_args(kv, what);
+        if (flags & ~ND_ZERO_REST) throw std::runtime_error("nd_op_kv4_read: unknown flags");
         if (a.rows == 0) return;
         kv4_check_out(what, type, k, k_row, k_head, a.rows, a.heads, kv->dk);
         kv4_check_out(what, type, v, v_row, v_head, a.rows, a.heads, kv->dv);
@@ -218,7 +224,7 @@ int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long lo
             using T = std::remove_pointer_t<decltype(t)>;
             constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
             kv4_read_kernel<DK, DV, T><<<row_grid(a, RowSplit<DK, DV>::PER), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(
-                a, (T*)k, k_row, k_head, (T*)v, v_row, v_head, vec);
+                a, (T*)k, k_row, k_head, (T*)v, v_row, v_head, vec, flags & ND_ZERO_REST);
         });
         op_launched(what);
     });

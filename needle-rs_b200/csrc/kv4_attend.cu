@@ -52,43 +52,57 @@
 namespace nd {
 
 constexpr int ATT_WARPS = 4, ATT_STAGES = 4;
-constexpr int ATT_MIN_SHARE = 4;  // tiles: a shorter run costs more to join than it takes
+// Tiles: a shorter run of a cut unit costs more to join than it takes.
+constexpr int ATT_MIN_SHARE = 4;
+// A call whose units all have at most this many tiles deals whole units out
+// to the warps and needs no second kernel.
+constexpr int ATT_WHOLE_TILES = 16;
+
+// n / d for 0 <= n < 2^31 by a multiplication.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv(uint32_t x = 1) : d(x), mul(0), shift(0) {
+        while ((1ull << shift) < d) shift++;
+        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
 
 struct AttendArgs {
     Kv4Args kv;
     long long q_row, q_head, o_row, o_head;
-    int group;  // query heads a kv head
+    FastDiv group;       // query heads a kv head
+    FastDiv page_tiles;
     int window, sink;
     float scale_log2e;
-    int q_vec, o_vec;
-    float* parts;   // [warps][2][8 NT * (DV + 2)]
-    int4* joins;    // [warps]: (sequence, kv head, query block, further warps) of the cut unit that starts there, w < 0: none
+    bool q_vec, o_vec, whole, zero_rest;
+    float* parts;   // [runners][2][8 NT * (DV + 2)]; a runner is a warp, for NT = 1 a CTA
+    int4* joins;    // [runners]: (sequence, kv head, query block, further runners) of the cut unit that starts there, w < 0: none
 };
 
 // The key tiles a block of query rows reads: those of the first `sink`
-// positions, then lo .. hi of the window.
+// positions, then lo .. of the window.
 struct Tiles {
     int sink, lo, n;  // n >= 1, so that a block that sees nothing is still written
     __device__ __forceinline__ int at(int i) const { return i < sink ? i : lo + (i - sink); }
 };
 
 __device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, long long first, long long last) {
-    const long long cap = (long long)a.kv.max_pages * a.kv.page_tiles * KV4_TILE;
-    const long long hi = min(last, cap - 1);
-    long long lo = a.window > 0 ? max(first - a.window + 1, 0LL) : 0LL;
+    const int cap = a.kv.max_pages * a.kv.page_tiles * KV4_TILE;  // positions of the table: below 2^31
+    const int end = last < 0 ? 0 : (int)min(last, (long long)cap - 1) / KV4_TILE + 1;
     Tiles t;
-    t.lo = (int)(min(lo, cap) / KV4_TILE);
-    const int end = hi < 0 ? 0 : (int)(hi / KV4_TILE) + 1;
-    int sink = 0;
-    if (a.window > 0 && a.sink > 0) sink = min((int)((min((long long)a.sink, cap) + KV4_TILE - 1) / KV4_TILE), min(t.lo, end));
-    t.sink = sink;
-    t.n = max(1, sink + max(0, end - t.lo));
+    t.lo = t.sink = 0;
+    if (a.window > 0) {
+        t.lo = (int)(min(max(first - a.window + 1, 0LL), (long long)cap)) / KV4_TILE;
+        if (a.sink > 0) t.sink = min((min(a.sink, cap) - 1) / KV4_TILE + 1, min(t.lo, end));
+    }
+    t.n = max(1, t.sink + max(0, end - t.lo));
     return t;
 }
 
 struct SeqRows {
-    int first, n;        // rows of the call
-    long long pos0;      // position of the first
+    int first, n;    // rows of the call
+    long long pos0;  // position of the first
 };
 
 __device__ __forceinline__ SeqRows seq_rows(const AttendArgs& a, int s) {
@@ -103,13 +117,16 @@ __device__ __forceinline__ SeqRows seq_rows(const AttendArgs& a, int s) {
 // head x % group of token x / group. Block b holds 8 NT of them.
 template <int NT>
 __device__ __forceinline__ Tiles block_tiles(const AttendArgs& a, const SeqRows& r, int b) {
-    const int x0 = b * 8 * NT, x1 = min(x0 + 8 * NT, r.n * a.group) - 1;
-    return tiles_of(a, r.pos0 + x0 / a.group, r.pos0 + x1 / a.group);
+    const int x0 = b * 8 * NT, x1 = min(x0 + 8 * NT, r.n * (int)a.group.d) - 1;
+    return tiles_of(a, r.pos0 + a.group(x0), r.pos0 + a.group(x1));
 }
 
+// What a sequence and kv head adds to the list of work: its tiles, or its
+// units where they are dealt out whole.
 template <int NT>
-__device__ __forceinline__ long long seq_tiles(const AttendArgs& a, const SeqRows& r) {
-    const int blocks = (r.n * a.group + 8 * NT - 1) / (8 * NT);
+__device__ __forceinline__ long long seq_work(const AttendArgs& a, const SeqRows& r) {
+    const int blocks = (r.n * (int)a.group.d + 8 * NT - 1) / (8 * NT);
+    if (a.whole) return blocks;
     long long t = 0;
     for (int b = 0; b < blocks; b++) t += block_tiles<NT>(a, r, b).n;
     return t;
@@ -158,36 +175,123 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
+// Two f32 operations in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(f32x2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Below every score that is not -infinity: the softmax's reference before the
+// first key is seen.
+constexpr float ATT_LOW = -3.0e38f;
+
 template <int DK, int DV, int NT, typename T>
 struct AttendShape {
     static constexpr int TB = kv4_tile_bytes(DK, DV);
-    static constexpr int QS = std::is_same<T, float>::value ? 2 : 1;           // f16 terms of a query value
+    static constexpr bool F32 = std::is_same<T, float>::value;
+    static constexpr int QS = F32 ? 2 : 1;                                     // f16 terms of a query value
     static constexpr int WS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // f16 terms of a weight
     static constexpr int KSTEPS = DK / 16;
-    static constexpr int QREGS = KSTEPS * 2 * QS;                 // a query block's operands, per 8 rows
-    static constexpr bool Q_SMEM = NT * QREGS > 32;               // else they stay in registers
-    static constexpr int SMEM = ATT_WARPS * (ATT_STAGES * TB + (Q_SMEM ? NT * QREGS * 128 : 0));
+    static constexpr int QOPS = NT * KSTEPS * QS;  // a query block's operands: pairs of registers
+    static constexpr bool Q_SMEM = QOPS > 16;      // else they stay in registers
+    // For one block of eight rows the warps of a CTA join their parts in
+    // shared memory first: decoding cuts few units into many parts.
+    static constexpr bool MERGE = NT == 1;
+    static constexpr int PART = 8 * NT * (DV + 2);  // floats
+    static constexpr int RING = ATT_STAGES * TB > 4 * PART || !MERGE ? ATT_STAGES * TB : 4 * PART;
+    static constexpr int WARP_SMEM = RING + (MERGE ? 4 * PART : 0) + (Q_SMEM ? QOPS * 256 : 0);
+    static constexpr int SMEM = ATT_WARPS * WARP_SMEM;
     static constexpr int CTAS = NT == 1 ? 4 : NT == 2 ? 3 : 2;
-    static constexpr int PART = 8 * NT * (DV + 2);                // floats
+};
+
+// acc (8 VW g + .. as the main loop holds it), M, l of a part of 8 rows.
+template <int DV>
+struct PartRegs {
+    float v[2][DV / 8], M[2], l[2];  // rows 2 c, 2 c + 1; dimensions (DV / 8) g ..
+    __device__ __forceinline__ void load(const float* p, int g, int c) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int y = 2 * c + j;
+#pragma unroll
+            for (int k = 0; k < DV / 32; k++) *(float4*)&v[j][4 * k] = *(const float4*)(p + y * DV + (DV / 8) * g + 4 * k);
+            M[j] = p[8 * DV + y];
+            l[j] = p[8 * (DV + 1) + y];
+        }
+    }
+    __device__ __forceinline__ void add(const PartRegs& o) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const float m = fmaxf(M[j], o.M[j]);
+            const float r = ex2(M[j] - m), s = ex2(o.M[j] - m);
+            M[j] = m;
+            l[j] = __fmaf_rn(l[j], r, o.l[j] * s);
+#pragma unroll
+            for (int k = 0; k < DV / 8; k++) v[j][k] = __fmaf_rn(v[j][k], r, o.v[j][k] * s);
+        }
+    }
+};
+
+// rows y (of a block) from x0 on of one sequence and kv head
+template <typename T>
+struct OutRows {
+    T* out;
+    const AttendArgs& a;
+    int first, h, nrows;
+    __device__ __forceinline__ T* at(int x) const {
+        const int tok = a.group(x);
+        return out + (long long)(first + tok) * a.o_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.o_head;
+    }
 };
 
 template <int DK, int DV, int NT, typename T>
 __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CTAS)
     kv4_attend_kernel(AttendArgs a, const T* __restrict__ q, T* __restrict__ out) {
     using Sh = AttendShape<DK, DV, NT, T>;
-    constexpr int TB = Sh::TB, QS = Sh::QS, WS = Sh::WS, KS = Sh::KSTEPS, MT = DV / 16, VW = DV / 64;
-    constexpr bool MID = std::is_same<T, float>::value;  // codes count from 8
+    constexpr int TB = Sh::TB, QS = Sh::QS, WS = Sh::WS, KS = Sh::KSTEPS, MT = DV / 16, VW = DV / 64, PART = Sh::PART;
+    constexpr bool F32 = Sh::F32, MERGE = Sh::MERGE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long sums[32 * ATT_WARPS + 1];
     __shared__ long long warp_sums[ATT_WARPS];
+    __shared__ int4 cut_start[ATT_WARPS];   // the cut unit that starts in a warp's run: (sequence, kv head, block, 1), w = 0: none
+    __shared__ int cut_rest[ATT_WARPS];     // the run begins inside a unit: 1, and ends it too: 2
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int H = a.kv.heads, S = a.kv.seqs;
+    const int warps = gridDim.x * ATT_WARPS, wid = blockIdx.x * ATT_WARPS + warp;
+
+    if (a.zero_rest && a.kv.start)
+        for (int r = kv4_first_row(a.kv, S) + wid; r < a.kv.rows; r += warps)
+            for (int hq = 0; hq < H * (int)a.group.d; hq++)
+                for (int d = lane; d < DV; d += 32) out[r * a.o_row + hq * a.o_head + d] = (T)0.f;
 
     // the list's length, and its prefix at every chunk of `per` sequences
     const int per = (S + 32 * ATT_WARPS - 1) / (32 * ATT_WARPS);
     {
         long long mine = 0;
-        for (int s = tid * per; s < min((tid + 1) * per, S); s++) mine += seq_tiles<NT>(a, seq_rows(a, s)) * H;
+#pragma unroll 4
+        for (int s = tid * per; s < min((tid + 1) * per, S); s++) mine += seq_work<NT>(a, seq_rows(a, s)) * H;
         long long incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -195,6 +299,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             if (lane >= o) incl += up;
         }
         if (lane == 31) warp_sums[warp] = incl;
+        if (lane == 0) cut_start[warp] = make_int4(0, 0, 0, 0), cut_rest[warp] = 0;
         __syncthreads();
         for (int w = 0; w < warp; w++) incl += warp_sums[w];
         sums[tid + 1] = incl;
@@ -202,449 +307,556 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         __syncthreads();
     }
     const long long total = sums[32 * ATT_WARPS];
-    const int warps = gridDim.x * ATT_WARPS, wid = blockIdx.x * ATT_WARPS + warp;
-    const long long share = max((total + warps - 1) / warps, (long long)ATT_MIN_SHARE);
+    const long long share = max((total + warps - 1) / warps, (long long)(a.whole ? 1 : ATT_MIN_SHARE));
     const long long begin = min(wid * share, total), end = min(begin + share, total);
-    if (lane == 0) a.joins[wid] = make_int4(0, 0, 0, -1);
-    if (begin >= end) return;
+    if (!MERGE && !a.whole && lane == 0) a.joins[wid] = make_int4(0, 0, 0, -1);
 
-    // the unit at `begin`
-    int s;
-    {
-        int lo = 0, hi = 32 * ATT_WARPS;  // sums[lo] <= begin < sums[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (sums[mid] <= begin) lo = mid;
-            else hi = mid;
+    uint8_t* mine = smem + warp * Sh::WARP_SMEM;
+    float* first_part = (float*)(mine + Sh::RING);  // MERGE: a part of a unit that an earlier run begins
+    float* last_part = (float*)mine;                // MERGE: of a unit that a later run ends, over the ring
+
+    if (begin < end) {
+        // the unit at `begin`
+        int s;
+        {
+            int lo = 0, hi = 32 * ATT_WARPS;  // sums[lo] <= begin < sums[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (sums[mid] <= begin) lo = mid;
+                else hi = mid;
+            }
+            s = lo;
         }
-        s = lo * per;
-        hi = lo;
-    }
-    long long rem = begin - sums[s / per];
-    SeqRows rows = seq_rows(a, s);
-    long long per_head = seq_tiles<NT>(a, rows);
-    while (rem >= per_head * H) {
-        rem -= per_head * H;
-        rows = seq_rows(a, ++s);
-        per_head = seq_tiles<NT>(a, rows);
-    }
-    int h = (int)(rem / per_head), b = 0;
-    rem -= h * per_head;
-    Tiles tl = block_tiles<NT>(a, rows, 0);
-    while (rem >= tl.n) {
-        rem -= tl.n;
-        tl = block_tiles<NT>(a, rows, ++b);
-    }
-    int off = (int)rem;
-
-    uint8_t* ring = smem + warp * ATT_STAGES * TB;
-    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-    uint32_t* qsm = (uint32_t*)(smem + ATT_WARPS * ATT_STAGES * TB) + warp * (NT * Sh::QREGS * 32) + lane;
-    const size_t head_stride = (size_t)a.kv.page_tiles * TB;
-
-    long long cur = begin;
-    while (true) {
-        const int m = (int)min((long long)(tl.n - off), end - cur);
-        const int nrows = rows.n * a.group;
-
-        // page ids of the next tiles, 32 at a time, one batch ahead
-        const int32_t* trow = a.kv.table + (size_t)s * a.kv.table_stride;
-        const int i_end = off + m;
-        auto fetch_page = [&](int i) {
-            const int t = i < i_end ? tl.at(i) / a.kv.page_tiles : 0;
-            return i < i_end && t < a.kv.max_pages ? __ldg(trow + t) : -1;
-        };
-        int ids = fetch_page(off + lane), ids_next = fetch_page(off + 32 + lane);
-        uint32_t okbits = 0;  // by stage: the tile's page exists
-        int issued = 0;
-        auto issue = [&]() {
-            if (issued < m) {
-                const int i = off + issued, page = __shfl_sync(0xffffffffu, ids, issued & 31);
-                const bool ok = page >= 0 && page < a.kv.num_pages;
-                const int st = issued % ATT_STAGES;
-                okbits = (okbits & ~(1u << st)) | ((uint32_t)ok << st);
-                if (ok) {
-                    const uint8_t* src = a.kv.pool + (size_t)page * a.kv.page_stride + h * head_stride + (size_t)(tl.at(i) % a.kv.page_tiles) * TB;
-#pragma unroll
-                    for (int j = 0; j < (TB / 16 + 31) / 32; j++)
-                        if (j * 32 + lane < TB / 16) copy16(ring_s + st * TB + (j * 32 + lane) * 16, src + (j * 32 + lane) * 16);
-                }
-                issued++;
-                if ((issued & 31) == 0) {
-                    ids = ids_next;
-                    ids_next = fetch_page(off + issued + 32 + lane);
-                }
-            }
-            asm volatile("cp.async.commit_group;\n" ::: "memory");
-        };
-        __syncwarp();  // the ring's last tile has been read by every lane
-#pragma unroll
-        for (int i = 0; i < ATT_STAGES - 1; i++) issue();
-
-        // the query block: lane (g, c) holds of query row 8 t + g the
-        // dimensions whose codes it will hold of every key
-        uint32_t qreg[Sh::Q_SMEM ? 1 : NT * Sh::QREGS];
-        float f0[NT][2], f1[NT][2], mid[QS == 2 ? NT : 1][2][2];
-        int seen_hi[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int x = b * 8 * NT + 8 * t + g;
-            const bool on = x < nrows;
-            float v[DK / 4];
-#pragma unroll
-            for (int i = 0; i < DK / 4; i++) v[i] = 0.f;
-            if (on) {
-                const T* p = q + (rows.first + x / a.group) * a.q_row + (h * a.group + x % a.group) * a.q_head;
-                if constexpr (DK == 48) {
-                    load8(p + 8 * c, a.q_vec, v);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[8 + i] = (float)p[32 + 4 * c + i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < DK / 32; i++) load8(p + (DK / 4) * c + 8 * i, a.q_vec, v + 8 * i);
-                }
-            }
-            float top = 0.f, sum = 0.f;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < DK / 4; i++) {
-                top = fmaxf(top, fabsf(v[i]));
-                bad |= !(fabsf(v[i]) <= FLT_MAX);
-                sum += v[i];
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
-            bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2) != 0;
-            // 2^e <= top < 2^(e+1) goes to 2^14: f16's largest values
-            int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-            e = min(max(e, -100), 127);
-            const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-            float fac0 = a.scale_log2e * __uint_as_float((uint32_t)(e - 14 + 127) << 23) * 16777216.f;
-            float fac1 = a.scale_log2e * sum;
-            if (bad) fac0 = fac1 = __uint_as_float(0x7fc00000u);
-            float q1 = 0.f, q2 = 0.f;  // sums of the fixed-point terms: exact
-            auto put = [&](int k, int half, float x0, float x1) {  // operand `half` of k-step k
-                const float mul = half ? 0.0625f : 1.f;  // the second operand's codes come 16-fold
-                uint32_t hi, lo = 0;
-                if (QS == 2) {
-                    // multiples of 16 up to 2^15, then of 2^-8 up to 8
-                    const float a0 = __fmul_rn(rintf(x0 * 0.0625f), 16.f), a1 = __fmul_rn(rintf(x1 * 0.0625f), 16.f);
-                    const float b0 = __fmul_rn(rintf((x0 - a0) * 256.f), 0.00390625f), b1 = __fmul_rn(rintf((x1 - a1) * 256.f), 0.00390625f);
-                    q1 += a0 + a1, q2 += b0 + b1;
-                    hi = pack_half2(a0 * mul, a1 * mul), lo = pack_half2(b0 * mul, b1 * mul);
-                } else {
-                    hi = pack_half2(x0 * mul, x1 * mul);
-                }
-                const int at = (t * KS + k) * 2 * QS + half * QS;
-                if constexpr (Sh::Q_SMEM) {
-                    qsm[at * 32] = hi;
-                    if (QS == 2) qsm[(at + 1) * 32] = lo;
-                } else {
-                    qreg[at] = hi;
-                    if (QS == 2) qreg[at + QS - 1] = lo;
-                }
-            };
-#pragma unroll
-            for (int i = 0; i < DK / 4; i++) v[i] = bad ? 0.f : v[i] * up;
-#pragma unroll
-            for (int w = 0; w < DK / 32; w++) {
-                const float* y = v + 8 * w;
-                put(2 * w, 0, y[0], y[4]);
-                put(2 * w, 1, y[1], y[5]);
-                put(2 * w + 1, 0, y[2], y[6]);
-                put(2 * w + 1, 1, y[3], y[7]);
-            }
-            if constexpr (DK == 48) {
-                put(2, 0, v[8], v[10]);
-                put(2, 1, v[9], v[11]);
-            }
-            if (QS == 2) {
-                q1 += __shfl_xor_sync(0xffffffffu, q1, 1);
-                q2 += __shfl_xor_sync(0xffffffffu, q2, 1);
-                q1 += __shfl_xor_sync(0xffffffffu, q1, 2);
-                q2 += __shfl_xor_sync(0xffffffffu, q2, 2);
-            }
-            const int hi = on ? (int)min(max(rows.pos0 + x / a.group, -1LL), 0x7fffffffLL) : -1;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                f0[t][j] = __shfl_sync(0xffffffffu, fac0, 4 * (2 * c + j));
-                f1[t][j] = __shfl_sync(0xffffffffu, fac1, 4 * (2 * c + j));
-                seen_hi[t][j] = __shfl_sync(0xffffffffu, hi, 4 * (2 * c + j));
-                if (QS == 2) {  // -8 of the codes' unit, 2^-24
-                    mid[t][j][0] = __shfl_sync(0xffffffffu, q1, 4 * (2 * c + j)) * -4.76837158203125e-7f;
-                    mid[t][j][1] = __shfl_sync(0xffffffffu, q2, 4 * (2 * c + j)) * -4.76837158203125e-7f;
-                }
-            }
+        long long rem = begin - sums[s];
+        s *= per;
+        SeqRows rows = seq_rows(a, s);
+        long long per_head = seq_work<NT>(a, rows);
+        while (rem >= per_head * H) {
+            rem -= per_head * H;
+            rows = seq_rows(a, ++s);
+            per_head = seq_work<NT>(a, rows);
         }
-        // tiles wholly inside every row's span need no masks
-        const int x_last = min((b + 1) * 8 * NT, nrows) - 1;
-        const long long p_first = rows.pos0 + (b * 8 * NT) / a.group, p_last = rows.pos0 + x_last / a.group;
-
-        float acc[NT][MT][4], M[NT][2], l[NT][2], mn[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-#pragma unroll
-            for (int i = 0; i < MT; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[t][i][j] = 0.f;
-#pragma unroll
-            for (int j = 0; j < 2; j++) M[t][j] = -INFINITY, l[t][j] = mn[t][j] = 0.f;
+        int h = (int)(rem / per_head), b = 0;
+        rem -= h * per_head;
+        if (a.whole) b = (int)rem, rem = 0;
+        Tiles tl = block_tiles<NT>(a, rows, b);
+        while (rem >= tl.n) {
+            rem -= tl.n;
+            tl = block_tiles<NT>(a, rows, ++b);
         }
+        int off = (int)rem;
 
-        for (int i = 0; i < m; i++) {
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(ATT_STAGES - 2) : "memory");
-            __syncwarp();
-            const int st = i % ATT_STAGES;
-            const bool page_ok = (okbits >> st) & 1;
-            issue();  // into the stage read in the last round
-            const uint8_t* tile = ring + st * TB;
-            const int k0 = tl.at(off + i) * KV4_TILE;
+        const uint8_t* ring = mine;
+        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+        uint2* qsm = (uint2*)(mine + Sh::RING + (MERGE ? 4 * PART : 0)) + lane;
+        const size_t head_stride = (size_t)a.kv.page_tiles * TB;
 
-            // scores: keys g and g + 8 against query rows 2 c, 2 c + 1
-            float sc[NT][4], sc2[QS == 2 ? NT : 1][4];
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    sc[t][j] = QS == 2 ? mid[QS == 2 ? t : 0][j & 1][0] : 0.f;
-                    if (QS == 2) sc2[QS == 2 ? t : 0][j] = mid[QS == 2 ? t : 0][j & 1][1];
-                }
-            auto qop = [&](int t, int k, int half, int term) -> uint32_t {
-                const int at = (t * KS + k) * 2 * QS + half * QS + term;
-                if constexpr (Sh::Q_SMEM) return qsm[at * 32];
-                else return qreg[at];
+        long long cur = begin;
+        while (true) {
+            const int m = a.whole ? tl.n : (int)min((long long)(tl.n - off), end - cur);
+            const int nrows = rows.n * (int)a.group.d;
+
+            // addresses of the next tiles, 32 at a time, one batch ahead; 0: no such page
+            const int32_t* trow = a.kv.table + (size_t)s * a.kv.table_stride;
+            const uint8_t* head = a.kv.pool + h * head_stride + lane * 16;
+            auto fetch = [&](int i) -> unsigned long long {
+                if (i >= off + m) return 0;
+                const int t = tl.at(i), p = a.page_tiles(t);
+                const int page = p < a.kv.max_pages ? __ldg(trow + p) : -1;
+                if (page < 0 || page >= a.kv.num_pages) return 0;
+                return (unsigned long long)(head - lane * 16 + (size_t)page * a.kv.page_stride + (size_t)(t - p * a.kv.page_tiles) * TB);
             };
-            auto step = [&](int k, uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
+            unsigned long long src = fetch(off + lane), src_next = fetch(off + 32 + lane);
+            uint32_t ok_hist = 0;  // bit k: the tile issued k issues ago has a page
+            int issued = 0;
+            uint32_t put_at = 0;
+            auto issue = [&]() {
+                ok_hist <<= 1;
+                if (issued < m) {
+                    const unsigned long long from = __shfl_sync(0xffffffffu, src, issued & 31);
+                    if (from) {
+                        ok_hist |= 1;
+                        const uint8_t* p = (const uint8_t*)from + lane * 16;
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    mma16816(sc[t], x0, y0, x1, y1, qop(t, k, 0, 0), qop(t, k, 1, 0));
-                    if (QS == 2) mma16816(sc2[QS == 2 ? t : 0], x0, y0, x1, y1, qop(t, k, 0, QS - 1), qop(t, k, 1, QS - 1));
+                        for (int j = 0; j < TB / 512; j++) copy16(ring_s + put_at + j * 512, p + j * 512);
+                        if (TB % 512 && lane * 16 < TB % 512) copy16(ring_s + put_at + TB / 512 * 512, p + TB / 512 * 512);
+                    }
+                    put_at = put_at == (ATT_STAGES - 1) * TB ? 0 : put_at + TB;
+                    issued++;
+                    if ((issued & 31) == 0) {
+                        src = src_next;
+                        src_next = fetch(off + issued + 32 + lane);
+                    }
                 }
+                asm volatile("cp.async.commit_group;\n" ::: "memory");
             };
-            const uint8_t *ka = tile + g * (DK / 2), *kb = tile + (g + 8) * (DK / 2);
-            uint32_t wa[DK / 32], wb[DK / 32];
-            if constexpr (DK == 128) {
-                const uint4 x = *(const uint4*)(ka + 16 * c), y = *(const uint4*)(kb + 16 * c);
-                wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
-                wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
-            } else if constexpr (DK == 64) {
-                const uint2 x = *(const uint2*)(ka + 8 * c), y = *(const uint2*)(kb + 8 * c);
-                wa[0] = x.x, wa[1] = x.y;
-                wb[0] = y.x, wb[1] = y.y;
-            } else {
-                wa[0] = *(const uint32_t*)(ka + 4 * c);
-                wb[0] = *(const uint32_t*)(kb + 4 * c);
-            }
+            __syncwarp();  // the ring's last tile has been read by every lane
+#pragma unroll 1
+            for (int i = 0; i < ATT_STAGES - 1; i++) issue();
+
+            // the query block: lane (g, c) holds of query row 8 t + g the
+            // dimensions whose codes it will hold of every key
+            uint2 qreg[Sh::Q_SMEM ? 1 : Sh::QOPS];
+            f32x2 f0[NT], f1[NT], mid[F32 ? NT : 1][2];
+            int seen_hi[NT][2];
 #pragma unroll
-            for (int w = 0; w < DK / 32; w++) {
-                step(2 * w, wa[w] & 0x000f000fu, wa[w] & 0x00f000f0u, wb[w] & 0x000f000fu, wb[w] & 0x00f000f0u);
-                const uint32_t xa = wa[w] >> 8, xb = wb[w] >> 8;
-                step(2 * w + 1, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
+            for (int t = 0; t < NT; t++) {
+                const int x = b * 8 * NT + 8 * t + g;
+                const bool on = x < nrows;
+                float v[DK / 4];
+#pragma unroll
+                for (int i = 0; i < DK / 4; i++) v[i] = 0.f;
+                const int tok = a.group(x);
+                if (on) {
+                    const T* p = q + (long long)(rows.first + tok) * a.q_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.q_head;
+                    if constexpr (DK == 48) {
+                        load8(p + 8 * c, a.q_vec, v);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[8 + i] = (float)p[32 + 4 * c + i];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < DK / 32; i++) load8(p + (DK / 4) * c + 8 * i, a.q_vec, v + 8 * i);
+                    }
+                }
+                float top = 0.f, sum = 0.f;
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < DK / 4; i++) {
+                    top = fmaxf(top, fabsf(v[i]));
+                    bad |= !(fabsf(v[i]) <= FLT_MAX);
+                    sum += v[i];
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
+                bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2) != 0;
+                // 2^e <= top < 2^(e+1) goes to 2^14: f16's largest values
+                const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+                const float up = bad ? 0.f : __uint_as_float((uint32_t)(14 - min(e, 127) + 127) << 23);
+                float fac0 = a.scale_log2e * __uint_as_float((uint32_t)(min(e, 127) - 14 + 127) << 23) * 16777216.f;
+                float fac1 = a.scale_log2e * sum;
+                if (bad) fac0 = fac1 = __uint_as_float(0x7fc00000u);
+                float q1 = 0.f, q2 = 0.f;  // sums of the fixed-point terms: exact
+                auto terms = [&](float x0, float x1, float mul, uint32_t& hi, uint32_t& lo) {
+                    if (F32) {
+                        // multiples of 16 up to 2^15, then of 2^-8 up to 8
+                        const float a0 = rintf(x0 * 0.0625f) * 16.f, a1 = rintf(x1 * 0.0625f) * 16.f;
+                        const float b0 = rintf((x0 - a0) * 256.f) * 0.00390625f, b1 = rintf((x1 - a1) * 256.f) * 0.00390625f;
+                        q1 += a0 + a1, q2 += b0 + b1;
+                        hi = pack_half2(a0 * mul, a1 * mul), lo = pack_half2(b0 * mul, b1 * mul);
+                    } else {
+                        hi = pack_half2(x0 * mul, x1 * mul);
+                    }
+                };
+                // operands of k-step k: codes (x0, x1) as they are, (y0, y1) 16-fold
+                auto put = [&](int k, float x0, float x1, float y0, float y1) {
+                    uint2 hi, lo;
+                    terms(x0, x1, 1.f, hi.x, lo.x);
+                    terms(y0, y1, 0.0625f, hi.y, lo.y);
+                    const int at = (t * KS + k) * QS;
+                    if constexpr (Sh::Q_SMEM) {
+                        qsm[at * 32] = hi;
+                        if (F32) qsm[(at + 1) * 32] = lo;
+                    } else {
+                        qreg[at] = hi;
+                        if (F32) qreg[at + QS - 1] = lo;
+                    }
+                };
+#pragma unroll
+                for (int i = 0; i < DK / 4; i++) v[i] = bad ? 0.f : v[i] * up;
+#pragma unroll
+                for (int w = 0; w < DK / 32; w++) {
+                    const float* y = v + 8 * w;
+                    put(2 * w, y[0], y[4], y[1], y[5]);
+                    put(2 * w + 1, y[2], y[6], y[3], y[7]);
+                }
+                if constexpr (DK == 48) put(2, v[8], v[10], v[9], v[11]);
+                const int hi = on ? (int)min(max(rows.pos0 + tok, -1LL), 0x7fffffffLL) : -1;
+                auto cols = [&](float x) { return pair(__shfl_sync(0xffffffffu, x, 8 * c), __shfl_sync(0xffffffffu, x, 8 * c + 4)); };
+                f0[t] = cols(fac0);
+                f1[t] = cols(fac1);
+                seen_hi[t][0] = __shfl_sync(0xffffffffu, hi, 8 * c);
+                seen_hi[t][1] = __shfl_sync(0xffffffffu, hi, 8 * c + 4);
+                if (F32) {  // -8 of the codes' unit, 2^-24
+                    q1 += __shfl_xor_sync(0xffffffffu, q1, 1);
+                    q2 += __shfl_xor_sync(0xffffffffu, q2, 1);
+                    q1 += __shfl_xor_sync(0xffffffffu, q1, 2);
+                    q2 += __shfl_xor_sync(0xffffffffu, q2, 2);
+                    mid[F32 ? t : 0][0] = cols(q1 * -4.76837158203125e-7f);
+                    mid[F32 ? t : 0][1] = cols(q2 * -4.76837158203125e-7f);
+                }
             }
-            if constexpr (DK == 48) {  // dimensions 32 .. 47: four codes a lane
-                const uint32_t ha = *(const uint16_t*)(ka + 16 + 2 * c), hb = *(const uint16_t*)(kb + 16 + 2 * c);
-                const uint32_t xa = __byte_perm(ha, 0, 0x4140), xb = __byte_perm(hb, 0, 0x4140);
-                step(2, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
-            }
-            const uint8_t* par = tile + 8 * (DK + DV);
-            float2 kpa = unpack_half2(*(const uint32_t*)(par + 4 * g)), kpb = unpack_half2(*(const uint32_t*)(par + 4 * (g + 8)));
-            float2 vpa = unpack_half2(*(const uint32_t*)(par + 64 + 4 * g)), vpb = unpack_half2(*(const uint32_t*)(par + 64 + 4 * (g + 8)));
-            if (QS == 2) {  // the middle of the codes instead of the minimum
-                kpa.y = __fmaf_rn(8.f, kpa.x, kpa.y), kpb.y = __fmaf_rn(8.f, kpb.x, kpb.y);
-                vpa.y = __fmaf_rn(8.f, vpa.x, vpa.y), vpb.y = __fmaf_rn(8.f, vpb.x, vpb.y);
-            }
-            const float la = lg2(fmaxf(vpa.x, 5.9604645e-8f)), lb = lg2(fmaxf(vpb.x, 5.9604645e-8f));
-            const bool whole = page_ok && k0 + 15 <= p_first && (a.window <= 0 || k0 > p_last - a.window || k0 + 15 < a.sink);
-            uint32_t vis = 0xffffffffu;
-            bool raise = false;
+            // tiles wholly inside every row's span need no masks
+            const int x_last = min((b + 1) * 8 * NT, nrows) - 1;
+            const long long p_first = rows.pos0 + a.group(b * 8 * NT), p_last = rows.pos0 + a.group(x_last);
+            const int all_hi = (int)min(max(p_first, -1LL), 0x7fffffffLL) - 15;              // whole: k0 <= all_hi and
+            const int all_lo = a.window > 0 ? (int)min(max(p_last - a.window, -1LL), 0x7fffffffLL) : -1;  // k0 > all_lo or k0 + 15 < sink
+
+            float acc[NT][MT][4];
+            f32x2 nM[NT], l[NT], mn[NT];  // -M, sum p, sum p mv for columns 2 c, 2 c + 1 (the sums over this lane's keys)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if (QS == 2) sc[t][j] += sc2[QS == 2 ? t : 0][j], sc[t][2 + j] += sc2[QS == 2 ? t : 0][2 + j];
-                    sc[t][j] = __fmaf_rn(kpa.x, sc[t][j] * f0[t][j], kpa.y * f1[t][j]);
-                    sc[t][2 + j] = __fmaf_rn(kpb.x, sc[t][2 + j] * f0[t][j], kpb.y * f1[t][j]);
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[t][i][j] = 0.f;
+                nM[t] = pair(-ATT_LOW, -ATT_LOW);
+                l[t] = mn[t] = 0;
+            }
+
+            int k0 = tl.at(off) * KV4_TILE;
+            uint32_t get_at = 0;
+#pragma unroll 1
+            for (int i = 0; i < m; i++) {
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(ATT_STAGES - 2) : "memory");
+                __syncwarp();
+                const bool page_ok = (ok_hist >> (ATT_STAGES - 2)) & 1;
+                issue();  // into the stage read in the last round
+                const uint8_t* tile = ring + get_at;
+                get_at = get_at == (ATT_STAGES - 1) * TB ? 0 : get_at + TB;
+
+                // scores: keys g and g + 8 against query rows 2 c, 2 c + 1
+                float sc[NT][4], sc2[F32 ? NT : 1][4];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if (F32) {
+                        const float2 x = unpair(mid[F32 ? t : 0][0]), y = unpair(mid[F32 ? t : 0][1]);
+                        sc[t][0] = sc[t][2] = x.x, sc[t][1] = sc[t][3] = x.y;
+                        sc2[F32 ? t : 0][0] = sc2[F32 ? t : 0][2] = y.x, sc2[F32 ? t : 0][1] = sc2[F32 ? t : 0][3] = y.y;
+                    } else {
+                        sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+                    }
+                }
+                auto qop = [&](int t, int k, int term) -> uint2 {
+                    const int at = (t * KS + k) * QS + term;
+                    if constexpr (Sh::Q_SMEM) return qsm[at * 32];
+                    else return qreg[at];
+                };
+                auto step = [&](int k, uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const uint2 o = qop(t, k, 0);
+                        mma16816(sc[t], x0, y0, x1, y1, o.x, o.y);
+                        if (F32) {
+                            const uint2 o2 = qop(t, k, QS - 1);
+                            mma16816(sc2[F32 ? t : 0], x0, y0, x1, y1, o2.x, o2.y);
+                        }
+                    }
+                };
+                const uint8_t *ka = tile + g * (DK / 2), *kb = tile + (g + 8) * (DK / 2);
+                uint32_t wa[DK / 32], wb[DK / 32];
+                if constexpr (DK == 128) {
+                    const uint4 x = *(const uint4*)(ka + 16 * c), y = *(const uint4*)(kb + 16 * c);
+                    wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
+                    wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
+                } else if constexpr (DK == 64) {
+                    const uint2 x = *(const uint2*)(ka + 8 * c), y = *(const uint2*)(kb + 8 * c);
+                    wa[0] = x.x, wa[1] = x.y;
+                    wb[0] = y.x, wb[1] = y.y;
+                } else {
+                    wa[0] = *(const uint32_t*)(ka + 4 * c);
+                    wb[0] = *(const uint32_t*)(kb + 4 * c);
+                }
+                const uint8_t* par = tile + 8 * (DK + DV) + 4 * g;
+                float2 kpa = unpack_half2(*(const uint32_t*)par), kpb = unpack_half2(*(const uint32_t*)(par + 32));
+                float2 vpa = unpack_half2(*(const uint32_t*)(par + 64)), vpb = unpack_half2(*(const uint32_t*)(par + 96));
+#pragma unroll
+                for (int w = 0; w < DK / 32; w++) {
+                    step(2 * w, wa[w] & 0x000f000fu, wa[w] & 0x00f000f0u, wb[w] & 0x000f000fu, wb[w] & 0x00f000f0u);
+                    const uint32_t xa = wa[w] >> 8, xb = wb[w] >> 8;
+                    step(2 * w + 1, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
+                }
+                if constexpr (DK == 48) {  // dimensions 32 .. 47: four codes a lane
+                    const uint32_t ha = *(const uint16_t*)(ka + 16 + 2 * c), hb = *(const uint16_t*)(kb + 16 + 2 * c);
+                    const uint32_t xa = __byte_perm(ha, 0, 0x4140), xb = __byte_perm(hb, 0, 0x4140);
+                    step(2, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
+                }
+                if (F32) {  // the middle of the codes instead of the minimum
+                    kpa.y = __fmaf_rn(8.f, kpa.x, kpa.y), kpb.y = __fmaf_rn(8.f, kpb.x, kpb.y);
+                    vpa.y = __fmaf_rn(8.f, vpa.x, vpa.y), vpb.y = __fmaf_rn(8.f, vpb.x, vpb.y);
+                }
+                // a score may pass M by this much before M is raised
+                const float ta = 4.f - lg2(fmaxf(vpa.x, 5.9604645e-8f)), tb = 4.f - lg2(fmaxf(vpb.x, 5.9604645e-8f));
+                const bool whole = page_ok && k0 <= all_hi && (k0 > all_lo || k0 + 15 < a.sink);
+                const f32x2 ksa = pair(kpa.x, kpa.x), ksb = pair(kpb.x, kpb.x), kma = pair(kpa.y, kpa.y), kmb = pair(kpb.y, kpb.y);
+                f32x2 sa[NT], sb[NT];  // keys g, g + 8
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    sa[t] = pair(sc[t][0], sc[t][1]), sb[t] = pair(sc[t][2], sc[t][3]);
+                    if (F32) {
+                        sa[t] = add2(sa[t], pair(sc2[F32 ? t : 0][0], sc2[F32 ? t : 0][1]));
+                        sb[t] = add2(sb[t], pair(sc2[F32 ? t : 0][2], sc2[F32 ? t : 0][3]));
+                    }
+                    sa[t] = fma2(mul2(sa[t], f0[t]), ksa, mul2(f1[t], kma));
+                    sb[t] = fma2(mul2(sb[t], f0[t]), ksb, mul2(f1[t], kmb));
                 }
                 if (!whole) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int key = k0 + g + (j >= 2 ? 8 : 0), hi = seen_hi[t][j & 1];
-                        const bool ok = page_ok && key <= hi && (a.window <= 0 || key > hi - a.window || key < a.sink);
-                        if (!ok) vis &= ~(1u << (4 * t + j));
+                    for (int t = 0; t < NT; t++) {
+                        auto mask = [&](f32x2 x, int key) {
+                            float2 f = unpair(x);
+                            const bool in = page_ok, sunk = key < a.sink;
+                            if (!(in && key <= seen_hi[t][0] && (a.window <= 0 || sunk || key > seen_hi[t][0] - a.window))) f.x = -INFINITY;
+                            if (!(in && key <= seen_hi[t][1] && (a.window <= 0 || sunk || key > seen_hi[t][1] - a.window))) f.y = -INFINITY;
+                            return pair(f.x, f.y);
+                        };
+                        sa[t] = mask(sa[t], k0 + g);
+                        sb[t] = mask(sb[t], k0 + g + 8);
                     }
                 }
+                bool raise = false;
+                float2 xa[NT], xb[NT];  // exponents
 #pragma unroll
-                for (int j = 0; j < 4; j++) raise |= ((vis >> (4 * t + j)) & 1) && sc[t][j] + (j >= 2 ? lb : la) > M[t][j & 1] + 4.f;
-            }
-            if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        float mx = M[t][j];
-                        if ((vis >> (4 * t + j)) & 1) mx = fmaxf(mx, sc[t][j] + la);
-                        if ((vis >> (4 * t + 2 + j)) & 1) mx = fmaxf(mx, sc[t][2 + j] + lb);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float r = mx == -INFINITY ? 1.f : ex2(M[t][j] - mx);
-                        M[t][j] = mx;
-                        l[t][j] *= r;
-                        mn[t][j] *= r;
-#pragma unroll
-                        for (int k = 0; k < MT; k++) acc[t][k][j] *= r, acc[t][k][2 + j] *= r;
-                    }
-            }
-            // weights, and their operands: rows of the transpose are query rows
-            uint32_t wop[NT][2][WS];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                float w[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const bool ok = (vis >> (4 * t + j)) & 1;
-                    const float p = ok ? ex2(sc[t][j] - M[t][j & 1]) : 0.f;
-                    const float2 vp = j >= 2 ? vpb : vpa;
-                    w[j] = ok ? p * vp.x : 0.f;
-                    l[t][j & 1] += p;
-                    mn[t][j & 1] = __fmaf_rn(p, ok ? vp.y : 0.f, mn[t][j & 1]);
+                for (int t = 0; t < NT; t++) {
+                    xa[t] = unpair(add2(sa[t], nM[t])), xb[t] = unpair(add2(sb[t], nM[t]));
+                    raise |= xa[t].x > ta || xa[t].y > ta || xb[t].x > tb || xb[t].y > tb;
                 }
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const uint32_t hi = pack_half2(w[2 * half], w[2 * half + 1]);
-                    wop[t][half][0] = transpose8(hi);
-                    if (WS == 2) {
-                        const float2 r = unpack_half2(hi);
-                        wop[t][half][WS - 1] = transpose8(pack_half2(w[2 * half] - r.x, w[2 * half + 1] - r.y));
-                    }
-                }
-            }
-            // values: lane (g, c) holds dimensions 8 (VW g + w) .. + 7 of keys 2c, 2c+1, 2c+8, 2c+9
-            const uint8_t* vt = tile + 8 * DK + g * 4 * VW;
-            uint32_t vw[4][VW];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint8_t* p = vt + (2 * c + (j & 1) + (j >= 2 ? 8 : 0)) * (DV / 2);
-                if constexpr (VW == 2) {
-                    const uint2 x = *(const uint2*)p;
-                    vw[j][0] = x.x, vw[j][1] = x.y;
-                } else {
-                    vw[j][0] = *(const uint32_t*)p;
-                }
-            }
-#pragma unroll
-            for (int w = 0; w < VW; w++)
-#pragma unroll
-                for (int quarter = 0; quarter < 4; quarter++) {
-                    // dimensions 2 quarter (row g), 2 quarter + 1 (row g + 8)
-                    const uint32_t sel = quarter < 2 ? 0x5410 : 0x7632;
-                    const uint32_t x = __byte_perm(vw[0][w], vw[1][w], sel) >> (quarter & 1 ? 8 : 0);
-                    const uint32_t y = __byte_perm(vw[2][w], vw[3][w], sel) >> (quarter & 1 ? 8 : 0);
-                    uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
-                    if (MID) a0 = code_mid(a0), a1 = code16_mid(a1), a2 = code_mid(a2), a3 = code16_mid(a3);
+                if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        float* d = acc[t][4 * w + quarter];
-                        if constexpr (MID) {
-                            float z[4] = {0.f, 0.f, 0.f, 0.f};
+                        const float2 fa = unpair(sa[t]), fb = unpair(sb[t]), old = unpair(nM[t]);
+                        float m0 = fmaxf(-old.x, fmaxf(fa.x + (4.f - ta), fb.x + (4.f - tb)));
+                        float m1 = fmaxf(-old.y, fmaxf(fa.y + (4.f - ta), fb.y + (4.f - tb)));
 #pragma unroll
-                            for (int term = 0; term < WS; term++) mma16816(z, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
+                        for (int o = 4; o < 32; o *= 2) {
+                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                        }
+                        const float r0 = ex2(-old.x - m0), r1 = ex2(-old.y - m1);
+                        const f32x2 r = pair(r0, r1);
+                        nM[t] = pair(-m0, -m1);
+                        l[t] = mul2(l[t], r);
+                        mn[t] = mul2(mn[t], r);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) d[j] += z[j];
-                        } else {
+                        for (int k = 0; k < MT; k++) acc[t][k][0] *= r0, acc[t][k][1] *= r1, acc[t][k][2] *= r0, acc[t][k][3] *= r1;
+                        xa[t] = unpair(add2(sa[t], nM[t])), xb[t] = unpair(add2(sb[t], nM[t]));
+                    }
+                }
+                // weights, and their operands: rows of the transpose are query rows
+                uint32_t wop[NT][2][WS];
+                const f32x2 vsa = pair(vpa.x, vpa.x), vsb = pair(vpb.x, vpb.x), vma = pair(vpa.y, vpa.y), vmb = pair(vpb.y, vpb.y);
 #pragma unroll
-                            for (int term = 0; term < WS; term++) mma16816(d, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
+                for (int t = 0; t < NT; t++) {
+                    const float2 ea = make_float2(ex2(xa[t].x), ex2(xa[t].y)), eb = make_float2(ex2(xb[t].x), ex2(xb[t].y));
+                    const f32x2 pa = pair(ea.x, ea.y), pb = pair(eb.x, eb.y);
+                    l[t] = add2(l[t], add2(pa, pb));
+                    float2 wa2, wb2;
+                    if (whole) {
+                        mn[t] = fma2(pa, vma, fma2(pb, vmb, mn[t]));
+                        wa2 = unpair(mul2(pa, vsa)), wb2 = unpair(mul2(pb, vsb));
+                    } else {  // a masked place may hold NaN or infinity
+                        float2 y = unpair(mn[t]);
+                        y.x = __fmaf_rn(ea.x, ea.x == 0.f ? 0.f : vpa.y, __fmaf_rn(eb.x, eb.x == 0.f ? 0.f : vpb.y, y.x));
+                        y.y = __fmaf_rn(ea.y, ea.y == 0.f ? 0.f : vpa.y, __fmaf_rn(eb.y, eb.y == 0.f ? 0.f : vpb.y, y.y));
+                        mn[t] = pair(y.x, y.y);
+                        wa2 = make_float2(ea.x == 0.f ? 0.f : ea.x * vpa.x, ea.y == 0.f ? 0.f : ea.y * vpa.x);
+                        wb2 = make_float2(eb.x == 0.f ? 0.f : eb.x * vpb.x, eb.y == 0.f ? 0.f : eb.y * vpb.x);
+                    }
+                    const uint32_t ha = pack_half2(wa2.x, wa2.y), hb = pack_half2(wb2.x, wb2.y);
+                    wop[t][0][0] = transpose8(ha), wop[t][1][0] = transpose8(hb);
+                    if (WS == 2) {
+                        const float2 ra = unpack_half2(ha), rb = unpack_half2(hb);
+                        wop[t][0][WS - 1] = transpose8(pack_half2(wa2.x - ra.x, wa2.y - ra.y));
+                        wop[t][1][WS - 1] = transpose8(pack_half2(wb2.x - rb.x, wb2.y - rb.y));
+                    }
+                }
+                // values: lane (g, c) holds dimensions 8 (VW g + w) .. + 7 of keys 2c, 2c+1, 2c+8, 2c+9
+                const uint8_t* vt = tile + 8 * DK + g * 4 * VW + c * DV;
+                uint32_t vw[4][VW];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint8_t* p = vt + ((j & 1) + (j >= 2 ? 8 : 0)) * (DV / 2);
+                    if constexpr (VW == 2) {
+                        const uint2 x = *(const uint2*)p;
+                        vw[j][0] = x.x, vw[j][1] = x.y;
+                    } else {
+                        vw[j][0] = *(const uint32_t*)p;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < VW; w++)
+#pragma unroll
+                    for (int quarter = 0; quarter < 4; quarter++) {
+                        // dimensions 2 quarter (row g), 2 quarter + 1 (row g + 8)
+                        const uint32_t sel = quarter < 2 ? 0x5410 : 0x7632;
+                        const uint32_t x = __byte_perm(vw[0][w], vw[1][w], sel) >> (quarter & 1 ? 8 : 0);
+                        const uint32_t y = __byte_perm(vw[2][w], vw[3][w], sel) >> (quarter & 1 ? 8 : 0);
+                        uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                        if (F32) a0 = code_mid(a0), a1 = code16_mid(a1), a2 = code_mid(a2), a3 = code16_mid(a3);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            float* d = acc[t][4 * w + quarter];
+                            if constexpr (F32) {
+                                float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int term = 0; term < WS; term++) mma16816(z, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
+#pragma unroll
+                                for (int j = 0; j < 4; j++) d[j] += z[j];
+                            } else {
+#pragma unroll
+                                for (int term = 0; term < WS; term++) mma16816(d, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
+                            }
                         }
                     }
-                }
-        }
-        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                k0 = off + i + 1 == tl.sink ? tl.lo * KV4_TILE : k0 + KV4_TILE;
+            }
+            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            __syncwarp();
 
-        // this run's part of the unit: sums over the keys' lanes, 2^24 back
-        const bool starts = off == 0, ends = off + m == tl.n;
-        float* part = a.parts + ((size_t)wid * 2 + (starts ? 1 : 0)) * Sh::PART;
+            // this run's part of the unit: sums over the keys' lanes, 2^24 back
+            const bool starts = off == 0, ends = off + m == tl.n, done = starts && ends;
+            float* part = MERGE ? (starts ? last_part : first_part) : a.parts + ((size_t)wid * 2 + (starts ? 1 : 0)) * PART;
+            const OutRows<T> to{out, a, rows.first, h, nrows};
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int t = 0; t < NT; t++) {
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) {
-                    l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], o);
-                    mn[t][j] += __shfl_xor_sync(0xffffffffu, mn[t][j], o);
+                    l[t] = add2(l[t], __shfl_xor_sync(0xffffffffu, l[t], o));
+                    mn[t] = add2(mn[t], __shfl_xor_sync(0xffffffffu, mn[t], o));
                 }
-                const int y = 8 * t + 2 * c + j, x = b * 8 * NT + y;  // query row in the block, in the sequence
-                const float norm = starts && ends ? (l[t][j] == 0.f ? 0.f : 1.f / l[t][j]) : 1.f;
-                T* o = out + (rows.first + x / a.group) * a.o_row + (h * a.group + x % a.group) * a.o_head;
+                const float2 l2 = unpair(l[t]), mn2 = unpair(mn[t]), M2 = unpair(nM[t]);
 #pragma unroll
-                for (int w = 0; w < VW; w++) {
-                    float v[8];
+                for (int j = 0; j < 2; j++) {
+                    const float lj = j ? l2.y : l2.x, mj = j ? mn2.y : mn2.x;
+                    const int y = 8 * t + 2 * c + j, x = b * 8 * NT + y;  // query row in the block, in the sequence
+                    const float norm = done ? (lj == 0.f ? 0.f : 1.f / lj) : 1.f;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        v[2 * k] = __fmaf_rn(acc[t][4 * w + k][j], MID ? 1.f : 16777216.f, mn[t][j]) * norm;
-                        v[2 * k + 1] = __fmaf_rn(acc[t][4 * w + k][2 + j], MID ? 1.f : 1048576.f, mn[t][j]) * norm;
+                    for (int w = 0; w < VW; w++) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            v[2 * k] = __fmaf_rn(acc[t][4 * w + k][j], F32 ? 1.f : 16777216.f, mj) * norm;
+                            v[2 * k + 1] = __fmaf_rn(acc[t][4 * w + k][2 + j], F32 ? 1.f : 1048576.f, mj) * norm;
+                        }
+                        const int d0 = 8 * (VW * g + w);
+                        if (!done) store8(part + y * DV + d0, true, v);
+                        else if (x < nrows) store8(to.at(x) + d0, a.o_vec, v);
                     }
-                    const int d0 = 8 * (VW * g + w);
-                    if (starts && ends) {
-                        if (x < nrows) store8(o + d0, a.o_vec, v);
-                    } else {
-                        store8(part + y * DV + d0, true, v);
+                    if (!done && g == 0) {
+                        part[8 * NT * DV + y] = j ? -M2.y : -M2.x;
+                        part[8 * NT * (DV + 1) + y] = lj;
                     }
-                }
-                if (!(starts && ends) && g == 0) {
-                    part[8 * NT * DV + y] = M[t][j];
-                    part[8 * NT * (DV + 1) + y] = l[t][j];
                 }
             }
-        if (starts && !ends && lane == 0) {
-            const int further = (int)((cur + tl.n - 1) / share - wid);
-            a.joins[wid] = make_int4(s, h, b, further);
-        }
+            if (!done && lane == 0) {
+                if (MERGE) {
+                    if (starts) cut_start[warp] = make_int4(s, h, b, 1);
+                    else cut_rest[warp] = ends ? 2 : 1;
+                }
+                if (starts) {
+                    const long long last = (cur + tl.n - 1) / share;  // the warp that ends the unit
+                    const int runner = MERGE ? blockIdx.x : wid, further = (int)((MERGE ? last / ATT_WARPS : last) - runner);
+                    if (!MERGE) a.joins[wid] = make_int4(s, h, b, further);
+                    else cut_start[warp].w = 1 + further;
+                }
+            }
 
-        // the next unit
-        cur += m;
-        if (cur >= end) break;
-        off = 0;
-        if (++b * 8 * NT >= nrows) {
-            b = 0;
-            if (++h == H) {
-                h = 0;
-                do rows = seq_rows(a, ++s);
-                while (rows.n == 0);
+            // the next unit
+            cur += a.whole ? 1 : m;
+            if (cur >= end) break;
+            off = 0;
+            if (++b * 8 * NT >= nrows) {
+                b = 0;
+                if (++h == H) {
+                    h = 0;
+                    do rows = seq_rows(a, ++s);
+                    while (rows.n == 0);
+                }
             }
+            tl = block_tiles<NT>(a, rows, b);
         }
-        tl = block_tiles<NT>(a, rows, b);
+    }
+
+    if constexpr (MERGE) {
+        if (a.whole) return;
+        __syncthreads();
+        // A unit's parts in this CTA, from the warp where it starts (or warp
+        // 0, if an earlier CTA has its start) to the one that ends it.
+        auto slot = [&](int w, bool start) { return (const float*)(smem + w * Sh::WARP_SMEM + (start ? 0 : Sh::RING)); };
+        auto chain = [&](bool start) {
+            PartRegs<DV> sum, more;
+            sum.load(slot(warp, start), g, c);
+            bool ended = !start && cut_rest[warp] == 2;
+            for (int w = warp + 1; w < ATT_WARPS && !ended && cut_rest[w]; w++) {
+                more.load(slot(w, false), g, c);
+                sum.add(more);
+                ended = cut_rest[w] == 2;
+            }
+            if (start && ended) {
+                const int4 u = cut_start[warp];
+                const SeqRows rows = seq_rows(a, u.x);
+                const OutRows<T> to{out, a, rows.first, u.y, rows.n * (int)a.group.d};
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int x = u.z * 8 + 2 * c + j;
+                    const float norm = sum.l[j] == 0.f ? 0.f : 1.f / sum.l[j];
+#pragma unroll
+                    for (int k = 0; k < DV / 8; k++) sum.v[j][k] *= norm;
+                    if (x < to.nrows)
+#pragma unroll
+                        for (int k = 0; k < DV / 64; k++) store8(to.at(x) + (DV / 8) * g + 8 * k, a.o_vec, sum.v[j] + 8 * k);
+                }
+                return false;
+            }
+            float* part = a.parts + ((size_t)blockIdx.x * 2 + (start ? 1 : 0)) * PART;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int y = 2 * c + j;
+#pragma unroll
+                for (int k = 0; k < DV / 64; k++) store8(part + y * DV + (DV / 8) * g + 8 * k, true, sum.v[j] + 8 * k);
+                if (g == 0) part[8 * DV + y] = sum.M[j], part[8 * (DV + 1) + y] = sum.l[j];
+            }
+            return true;
+        };
+        if (warp == 0 && cut_rest[0]) chain(false);
+        if (cut_start[warp].w && chain(true) && lane == 0) {
+            const int4 u = cut_start[warp];
+            a.joins[blockIdx.x] = make_int4(u.x, u.y, u.z, u.w - 1);
+        }
+        // a CTA whose last cut unit ends here, or that has none, joins nothing
+        if (tid == 0) {
+            bool open = false;
+            for (int w = 0; w < ATT_WARPS; w++) {
+                if (open && cut_rest[w] != 1) open = false;
+                if (cut_start[w].w) open = true;
+            }
+            if (!open) a.joins[blockIdx.x] = make_int4(0, 0, 0, -1);
+        }
     }
 }
 
-// out = sum_w 2^(M_w - M) acc_w / sum_w 2^(M_w - M) l_w over the warps w that
-// share a unit, in their order. A CTA per warp of the first kernel; those
-// where no cut unit starts return at once.
+// out = sum_w 2^(M_w - M) acc_w / sum_w 2^(M_w - M) l_w over the runners w
+// that share a unit, in their order. A CTA per runner of the first kernel;
+// those where no cut unit starts return at once.
 template <int DV, int NT, typename T>
-__global__ void __launch_bounds__(128) kv4_join_kernel(AttendArgs a, T* __restrict__ out) {
-    constexpr int PART = 8 * NT * (DV + 2), ROWS = 128 / DV;
+__global__ void __launch_bounds__(512) kv4_join_kernel(AttendArgs a, T* __restrict__ out) {
+    constexpr int PART = 8 * NT * (DV + 2), ROWS = 512 / DV;
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int4 job = a.joins[blockIdx.x];
     if (job.w < 0) return;
     const SeqRows rows = seq_rows(a, job.x);
-    const int y = blockIdx.y * ROWS + threadIdx.x / DV, d = threadIdx.x % DV, x = job.z * 8 * NT + y;
-    if (x >= rows.n * a.group) return;
-    auto part = [&](int i) { return a.parts + ((size_t)(blockIdx.x + i) * 2 + (i == 0)) * PART; };
-    float M = -INFINITY;
-    for (int i = 0; i <= job.w; i++) M = fmaxf(M, __ldg(part(i) + 8 * NT * DV + y));
-    float l = 0.f, v = 0.f;
-    for (int i = 0; i <= job.w; i++) {
-        const float* p = part(i);
-        const float m = __ldg(p + 8 * NT * DV + y);
-        const float li = __ldg(p + 8 * NT * (DV + 1) + y);
-        const float r = m == M ? 1.f : ex2(m - M);
-        l = __fmaf_rn(li, r, l);
-        v = __fmaf_rn(__ldg(p + y * DV + d), r, v);
+    const OutRows<T> to{out, a, rows.first, job.y, rows.n * (int)a.group.d};
+    const float* part = a.parts + (size_t)blockIdx.x * 2 * PART;
+    const int d = threadIdx.x % DV;
+    for (int y = threadIdx.x / DV; y < 8 * NT; y += ROWS) {
+        const int x = job.z * 8 * NT + y;
+        if (x >= to.nrows) return;
+        // the starting runner's second slot, then the first slot of each further one
+        float M = part[PART + 8 * NT * DV + y];
+#pragma unroll 8
+        for (int i = 1; i <= job.w; i++) M = fmaxf(M, part[(size_t)i * 2 * PART + 8 * NT * DV + y]);
+        float l = 0.f, v = 0.f;
+#pragma unroll 8
+        for (int i = 0; i <= job.w; i++) {
+            const float* p = part + (i ? (size_t)i * 2 * PART : PART);
+            const float r = ex2(p[8 * NT * DV + y] - M);
+            l = __fmaf_rn(p[8 * NT * (DV + 1) + y], r, l);
+            v = __fmaf_rn(p[y * DV + d], r, v);
+        }
+        to.at(x)[d] = (T)(l == 0.f ? 0.f : v / l);
     }
-    v = l == 0.f ? 0.f : v / l;
-    T* o = out + (rows.first + x / a.group) * a.o_row + (job.y * a.group + x % a.group) * a.o_head;
-    o[d] = (T)v;
 }
 
 // Query rows a block: the fewest blocks of 8, 16 or 32 rows that hold what a
@@ -654,40 +866,81 @@ static int query_tiles(const nd_kv4* kv, int group) {
     return mean <= 8 ? 1 : mean <= 16 ? 2 : 4;
 }
 
-static int attend_ctas(int nt) { return device_sm_count() * (nt == 1 ? 4 : nt == 2 ? 3 : 2); }
+struct AttendPlan {
+    int nt, ctas;
+    bool whole;
+    size_t ws;
+};
 
-static size_t attend_ws_bytes(int nt, int dv, int ctas) {
-    const size_t warps = (size_t)ctas * ATT_WARPS;
-    return warps * (sizeof(int4) + 2 * sizeof(float) * 8 * nt * (dv + 2));
+// Grid and workspace from what the host knows: the sizes, not the lengths.
+static AttendPlan attend_plan(const nd_kv4* kv, int group, int window, int sink) {
+    AttendPlan p;
+    p.nt = query_tiles(kv, group);
+    // tiles a unit can have: the table's, or those of the window (of 8 nt rows' tokens) and the sinks
+    const long long table = (long long)kv->max_pages * (kv->page / KV4_TILE);
+    long long tiles = table;
+    if (window > 0) tiles = std::min(table, ((long long)window + 8 * p.nt + 2 * KV4_TILE) / KV4_TILE + (sink + KV4_TILE - 1LL) / KV4_TILE);
+    p.whole = tiles <= ATT_WHOLE_TILES;
+    const long long units = kv->heads * ((long long)kv->rows * group / (8 * p.nt) + std::min(kv->seqs, kv->rows));
+    const long long runs = p.whole ? units : (units * tiles + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
+    const int full = device_sm_count() * (p.nt == 1 ? 4 : p.nt == 2 ? 3 : 2);
+    p.ctas = (int)std::max(1LL, std::min<long long>(full, (runs + ATT_WARPS - 1) / ATT_WARPS));
+    const size_t runners = (size_t)p.ctas * (p.nt == 1 ? 1 : ATT_WARPS);
+    p.ws = p.whole ? 0 : runners * (sizeof(int4) + 2 * sizeof(float) * 8 * p.nt * (kv->dv + 2));
+    return p;
 }
 
 template <int DK, int DV, int NT, typename T>
-static void attend_launch(const AttendArgs& a0, const void* q, void* out, void* ws, int ctas, cudaStream_t st) {
+static void attend_launch(const AttendArgs& a0, const AttendPlan& plan, const void* q, void* out, void* ws, cudaStream_t st) {
     using Sh = AttendShape<DK, DV, NT, T>;
     AttendArgs a = a0;
+    const int runners = plan.ctas * (Sh::MERGE ? 1 : ATT_WARPS);
     a.joins = (int4*)ws;
-    a.parts = (float*)((char*)ws + (size_t)ctas * ATT_WARPS * sizeof(int4));
+    a.parts = (float*)((char*)ws + (size_t)runners * sizeof(int4));
     auto kernel = kv4_attend_kernel<DK, DV, NT, T>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM);
-    if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
-    kernel<<<ctas, 32 * ATT_WARPS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
+    auto check = [](cudaError_t e) {
+        if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
+    };
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    kernel<<<plan.ctas, 32 * ATT_WARPS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
-    kv4_join_kernel<DV, NT, T><<<dim3(ctas * ATT_WARPS, 8 * NT * DV / 128), 128, 0, st>>>(a, (T*)out);
-    op_launched("nd_op_kv4_attend");
+    if (plan.whole) return;
+    // launched early where the stream allows it; it waits for the first kernel's results
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(runners);
+    cfg.blockDim = dim3(512);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = st ? 1 : 0;
+    check(cudaLaunchKernelEx(&cfg, kv4_join_kernel<DV, NT, T>, (AttendArgs)a, (T*)out));
+    add_launches(1);
 }
 
 template <int DK, int DV, typename T>
-static void attend_nt(int nt, const AttendArgs& a, const void* q, void* out, void* ws, int ctas, cudaStream_t st) {
-    if (nt == 1) attend_launch<DK, DV, 1, T>(a, q, out, ws, ctas, st);
-    else if (nt == 2) attend_launch<DK, DV, 2, T>(a, q, out, ws, ctas, st);
-    else attend_launch<DK, DV, 4, T>(a, q, out, ws, ctas, st);
+static void attend_nt(const AttendArgs& a, const AttendPlan& p, const void* q, void* out, void* ws, cudaStream_t st) {
+    if (p.nt == 1) attend_launch<DK, DV, 1, T>(a, p, q, out, ws, st);
+    else if (p.nt == 2) attend_launch<DK, DV, 2, T>(a, p, q, out, ws, st);
+    else attend_launch<DK, DV, 4, T>(a, p, q, out, ws, st);
 }
 
 template <int DK, int DV>
-static void attend_type(int type, int nt, const AttendArgs& a, const void* q, void* out, void* ws, int ctas, cudaStream_t st) {
-    if (type == ND_F32) attend_nt<DK, DV, float>(nt, a, q, out, ws, ctas, st);
-    else if (type == ND_F16) attend_nt<DK, DV, __half>(nt, a, q, out, ws, ctas, st);
-    else attend_nt<DK, DV, __nv_bfloat16>(nt, a, q, out, ws, ctas, st);
+static void attend_type(int type, const AttendArgs& a, const AttendPlan& p, const void* q, void* out, void* ws, cudaStream_t st) {
+    if (type == ND_F32) attend_nt<DK, DV, float>(a, p, q, out, ws, st);
+    else if (type == ND_F16) attend_nt<DK, DV, __half>(a, p, q, out, ws, st);
+    else attend_nt<DK, DV, __nv_bfloat16>(a, p, q, out, ws, st);
+}
+
+static int attend_group(const nd_kv4* kv, int q_heads, int window, int sink, const char* what) {
+    auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
+    if (q_heads < 1 || q_heads % kv->heads) fail("q_heads must be a multiple of heads");
+    const int group = q_heads / kv->heads;
+    if (group > 64) fail("more than 64 query heads a kv head");
+    if ((long long)kv->rows * group > 0x7fffffffLL / 2) fail("too many rows");
+    if (window < 0 || sink < 0) fail("window and sink must not be negative");
+    return group;
 }
 
 }  // namespace nd
@@ -696,47 +949,47 @@ using namespace nd;
 
 extern "C" {
 
-unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads) {
+unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads, int window, int sink) {
     unsigned long long bytes = 0;
     op_call([&] {
-        kv4_args(kv, "nd_op_kv4_attend_ws");
-        if (q_heads < 1 || q_heads % kv->heads) throw std::runtime_error("nd_op_kv4_attend_ws: q_heads must be a multiple of heads");
-        OnDevice on(kv->device, "nd_op_kv4_attend_ws");
-        const int nt = query_tiles(kv, q_heads / kv->heads);
-        bytes = attend_ws_bytes(nt, kv->dv, attend_ctas(nt));
+        const char* what = "nd_op_kv4_attend_ws";
+        kv4_args(kv, what);
+        const int group = attend_group(kv, q_heads, window, sink, what);
+        OnDevice on(kv->device, what);
+        bytes = attend_plan(kv, group, window, sink).ws;
     });
     return bytes;
 }
 
 int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row, long long q_head, int q_heads, float scale,
                      int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
-                     void* stream) {
+                     int flags, void* stream) {
     return op_call([&] {
         const char* what = "nd_op_kv4_attend";
         auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
         AttendArgs a{};
         a.kv = kv4_args(kv, what);
-        if (a.kv.rows == 0) return;
-        if (q_heads < 1 || q_heads % a.kv.heads) fail("q_heads must be a multiple of heads");
-        a.group = q_heads / a.kv.heads;
-        if (a.group > 64) fail("more than 64 query heads a kv head");
-        if ((long long)a.kv.rows * a.group > 0x7fffffffLL / 2) fail("too many rows");
-        if (window < 0 || sink < 0) fail("window and sink must not be negative");
+        const int group = attend_group(kv, q_heads, window, sink, what);
         if (!(fabsf(scale) <= FLT_MAX)) fail("scale must be finite");
+        if (flags & ~ND_ZERO_REST) fail("unknown flags");
+        if (a.kv.rows == 0) return;
         kv4_check_rows(what, type, q, q_row, q_head);
         kv4_check_out(what, type, out, o_row, o_head, a.kv.rows, q_heads, kv->dv);
-        if (!ws || (uintptr_t)ws % 16) fail("the workspace must be 16-byte aligned");
+        if ((uintptr_t)ws % 16) fail("the workspace must be 16-byte aligned");
+        a.group = FastDiv(group), a.page_tiles = FastDiv(a.kv.page_tiles);
         a.q_row = q_row, a.q_head = q_head, a.o_row = o_row, a.o_head = o_head;
         a.window = window, a.sink = sink;
         a.scale_log2e = (float)((double)scale * 1.4426950408889634);
         a.q_vec = kv4_vec(type, q, q_row, q_head), a.o_vec = kv4_vec(type, out, o_row, o_head);
+        a.zero_rest = flags & ND_ZERO_REST;
         OnDevice on(kv->device, what);
-        const int nt = query_tiles(kv, a.group), ctas = attend_ctas(nt);
-        if (ws_bytes < attend_ws_bytes(nt, kv->dv, ctas)) fail("the workspace is too small");
+        const AttendPlan plan = attend_plan(kv, group, window, sink);
+        a.whole = plan.whole;
+        if (plan.ws && (!ws || ws_bytes < plan.ws)) fail("the workspace is too small");
         cudaStream_t st = (cudaStream_t)stream;
-        if (kv->dk == 48) attend_type<48, 64>(type, nt, a, q, out, ws, ctas, st);
-        else if (kv->dk == 64) attend_type<64, 64>(type, nt, a, q, out, ws, ctas, st);
-        else attend_type<128, 128>(type, nt, a, q, out, ws, ctas, st);
+        if (kv->dk == 48) attend_type<48, 64>(type, a, plan, q, out, ws, st);
+        else if (kv->dk == 64) attend_type<64, 64>(type, a, plan, q, out, ws, st);
+        else attend_type<128, 128>(type, a, plan, q, out, ws, st);
     });
 }
 

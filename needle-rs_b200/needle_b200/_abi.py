@@ -11,12 +11,12 @@ class KV4(C.Structure):
 
 
 SIGNATURES = {
-    "nd_op_kv4_append": (C.c_int, [C.POINTER(KV4), C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p,
+    "nd_op_kv4_append": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p,
                                    C.c_longlong, C.c_longlong, C.c_void_p]),
-    "nd_op_kv4_read": (C.c_int, [C.POINTER(KV4), C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p,
-                                 C.c_longlong, C.c_longlong, C.c_void_p]),
-    "nd_op_kv4_attend_ws": (C.c_ulonglong, [C.POINTER(KV4), C.c_int]),
-    "nd_op_kv4_attend": (C.c_int, [C.POINTER(KV4), C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_int, C.c_float,
+    "nd_op_kv4_read": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p,
+                                 C.c_longlong, C.c_longlong, C.c_int, C.c_void_p]),
+    "nd_op_kv4_attend_ws": (C.c_ulonglong, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "nd_op_kv4_attend": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_int, C.c_float,
                                    C.c_int, C.c_int, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p, C.c_ulonglong,
-                                   C.c_void_p]),
+                                   C.c_int, C.c_void_p]),
 }

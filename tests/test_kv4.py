@@ -412,7 +412,7 @@ def test_entry_points_refuse_without_a_gpu():
 
     def attend(row=576, heads=12, type=0, window=0, ws=4096, nbytes=0, q=4096, o_row=768, **bad):
         a = KV4(**{**good, **bad})
-        return lib.nd_op_kv4_attend(C.byref(a), type, q, row, 48, heads, 0.1, window, 0, 4096, o_row, 64, ws, nbytes, None)
+        return lib.nd_op_kv4_attend(C.byref(a), type, q, row, 48, heads, 0.1, window, 0, 4096, o_row, 64, ws, nbytes, 0, None)
 
     for bad, message in ((dict(page=20), b"multiple of 16"), (dict(dk=50), b"(dk, dv)"), (dict(pool=4100), b"aligned"),
                          (dict(page_stride=1024), b"overlap"), (dict(table_stride=1), b"overlap"), (dict(seqs=0), b"positive"),
@@ -424,7 +424,7 @@ def test_entry_points_refuse_without_a_gpu():
         assert attend(heads=heads, **bad) == -1, bad
         assert message in lib.nd_last_error(), (bad, lib.nd_last_error())
     assert attend(heads=13) == -1 and b"multiple of heads" in lib.nd_last_error()
-    assert lib.nd_op_kv4_attend(None, 0, 4096, 576, 48, 12, 0.1, 0, 0, 4096, 768, 64, 4096, 0, None) == -1
+    assert lib.nd_op_kv4_attend(None, 0, 4096, 576, 48, 12, 0.1, 0, 0, 4096, 768, 64, 4096, 0, 0, None) == -1
     a = KV4(**good)
     assert lib.nd_op_kv4_append(C.byref(a), 0, None, 96, 48, 4096, 128, 64, None) == -1 and b"null" in lib.nd_last_error()
-    assert lib.nd_op_kv4_read(C.byref(a), 0, 4096, 96, 0, 4096, 128, 64, None) == -1 and b"overlap" in lib.nd_last_error()
+    assert lib.nd_op_kv4_read(C.byref(a), 0, 4096, 96, 0, 4096, 128, 64, 0, None) == -1 and b"overlap" in lib.nd_last_error()
