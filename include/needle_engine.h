@@ -338,6 +338,71 @@ int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row,
                      int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
                      int flags, void* stream);
 
+/* A pool as bytes: page p of layer l lies at pool + p * page_stride + l *
+ * layer_stride, page_bytes long (all multiples of 16; pool 16-byte aligned;
+ * pages do not overlap; at most 2^28). A nd_kv4 pool is one layer of it. */
+typedef struct nd_pages {
+    int device;
+    void* pool;
+    long long page_stride, layer_stride, page_bytes;
+    int num_pages, layers;
+} nd_pages;
+
+/* From a table of old sequences to one of new ones: forking, truncating,
+ * growing and freeing in one call. New sequence d (of n) keeps the first
+ * keep[d] positions of old sequence src[d] (none where src[d] is not in
+ * [0, seqs)) and gets room for need[d]; both are cut to the row's cols * page
+ * positions, need to keep at least. Whole kept pages are shared. A kept page
+ * that is partly filled and will be written (need > keep) is copied, in
+ * every layer, unless d alone refers to it, or all that refer to it will
+ * write on it and d is the first of them. Pages that no new sequence refers
+ * to and whose pinned[] byte (num_pages, may be NULL) is 0 are free; fresh
+ * pages are the free ones in ascending order, given to the new sequences in
+ * order, each first its copy, then its columns. Pinned pages are never
+ * written: they count as referred to by one more that does not write.
+ * table_out[n][cols] (not the old table): -1 where there is no page, where a
+ * kept entry was outside [0, num_pages), and where free pages ran out.
+ * refs[num_pages]: references from table_out. info[4]: pages referred to or
+ * pinned, fresh pages given, copies made, fresh pages wanted but not had.
+ * The call reads the old table only, and overwrites free pages alone, so it
+ * may be repeated. ws: nd_op_pages_fork_ws bytes, 16-byte aligned. */
+unsigned long long nd_op_pages_fork_ws(int num_pages, int n);
+int nd_op_pages_fork(const nd_pages* pool, const int* table, int table_stride, int seqs, int cols, int page, const int* src,
+                     const int* keep, const int* need, int n, const unsigned char* pinned, int* table_out, int* refs, int* info,
+                     void* ws, unsigned long long ws_bytes, void* stream);
+
+/* Live pages (in the table, or pinned) to the front: with n of them, those
+ * at ids >= n that are not pinned move, in ascending order, to the ids < n
+ * that are not live. table_out[seqs][cols] (not the old table): the new
+ * ids, -1 for entries outside [0, num_pages). map[num_pages]: each live
+ * page's new id, -1 for the others. info[2]: n, pages moved. Moved pages'
+ * old places keep their bytes. ws as above. */
+unsigned long long nd_op_pages_compact_ws(int num_pages);
+int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride, int seqs, int cols, const unsigned char* pinned,
+                        int* table_out, int* map, int* info, void* ws, unsigned long long ws_bytes, void* stream);
+
+/* Check drafted tokens against the target and draw the next one, for each
+ * of seqs sequences. logits (of `type`; element strides l_seq, l_row): row i
+ * of T + 1 is the target's for the place of draft[s][i], row counts[s] for
+ * the token after the last one. counts[seqs] (NULL: T each; cut to [0, T])
+ * says how many of draft[seqs][T] there are; T <= 64. p_i = softmax(logits_i /
+ * temperature[s]), or one at the first largest logit where the temperature
+ * is not above 0. q[seqs][T][V] f32 (strides q_seq, q_row; NULL: the draft
+ * was certain of its tokens): the draft's probabilities. u[seqs][T + 1] in
+ * [0, 1). Draft i is accepted, while all before it are, if u[i] q_i(draft_i)
+ * < p_i(draft_i). The next token is drawn from max(p_i - q_i, 0) (p_i if that
+ * is all zero) at the first i refused, from p after the last: the first j
+ * whose running sum over 0 .. j exceeds u[T] times the whole. accepted[seqs];
+ * tokens[seqs][T + 1]: the accepted drafts, the drawn token, then -1;
+ * probs[seqs][T + 1]: p of each of them, then 0. A row that holds a NaN, a
+ * +infinity at a temperature above 0, or nothing above -infinity accepts
+ * nothing and draws -1 with probability 0; so does a residual that holds a
+ * NaN. A drafted id outside [0, V) is refused. Sums and comparisons that
+ * decide are exact to f64 rounding. */
+int nd_op_verify(int device, int type, const void* logits, long long l_seq, long long l_row, const int* draft,
+                 const int* counts, const float* u, const float* temperature, const float* q, long long q_seq,
+                 long long q_row, int seqs, int T, int V, int* tokens, int* accepted, float* probs, void* stream);
+
 /* The last failure on this thread (empty if none). */
 const char* nd_last_error(void);
 

@@ -475,7 +475,7 @@ def op_gather(model, ids, out=None):
 # ----------------------------------------- serving from one pool of pages
 
 # These live in serving.py, which needs torch; the rest of the package does not.
-_SERVING = ("KV4Pool", "op_kv4_append", "op_kv4_read", "op_kv4_attend")
+_SERVING = ("KV4Pool", "op_kv4_append", "op_kv4_read", "op_kv4_attend", "op_pages_fork", "op_pages_compact", "op_verify")
 
 
 def __getattr__(name):

@@ -1,6 +1,7 @@
 """Serving from one pool of pages (include/needle_engine.h, "Serving from one
 pool of pages"): a 4-bit key/value cache that sequences of different lengths
-share, and attention over it.
+share, attention over it, forking and compacting of pages, and the check of
+drafted tokens.
 
 Tensors are CUDA tensors of one device; work is queued on that device's
 current torch stream. Tables, lengths and offsets are int32 and read on the
@@ -15,6 +16,7 @@ import torch
 
 from . import _err, lib
 from ._abi import KV4 as _KV4
+from ._abi import PAGES as _PAGES
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TILE = 16  # positions a tile
@@ -66,12 +68,8 @@ class KV4Pool:
     def _args(self, table, lens, start, rows):
         """The C view of a call; its tensors must outlive the call."""
         dev = self.device
-        if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev:
-            raise ValueError(f"table must be an int32 tensor [seqs, pages] on {dev}")
-        (s, p), (stride, inner) = table.shape, table.stride()
-        if not s or not p or (inner != 1 and p > 1):
-            raise ValueError("table must have sequences and columns, each row contiguous")
-        return C.byref(_KV4(*self._fixed, table.data_ptr(), stride if s > 1 else p, p, s, _int32(lens, s, dev, "lens"),
+        s, p, stride = _table(table, dev)
+        return C.byref(_KV4(*self._fixed, table.data_ptr(), stride, p, s, _int32(lens, s, dev, "lens"),
                             None if start is None else _int32(start, s + 1, dev, "start"), rows))
 
     def _rows(self, x, heads, d, name):
@@ -139,3 +137,115 @@ def op_kv4_attend(kv, q, table, lens, start=None, scale=None, window=0, sink=0, 
                           ws.data_ptr() if n else None, n, _ZERO_REST if new else 0, _stream(kv.device)) != 0:
         raise _err()
     return out
+
+
+def _pages(pool, axis):
+    """The C view of a pool whose pages lie along `axis` (0: [pages, ..], 1:
+    [layers, pages, ..])."""
+    if not pool.is_cuda or axis not in (0, 1) or pool.dim() <= axis or not pool.numel():
+        raise ValueError("pool must be a CUDA tensor [pages, ..], or [layers, pages, ..] with axis=1")
+    n, layers = pool.shape[axis], pool.shape[0] if axis else 1
+    size = pool.element_size()
+    nbytes = pool.numel() // (n * layers) * size
+    if not pool[0 if axis == 0 else (0, 0)].is_contiguous():
+        raise ValueError("a page must be contiguous")
+    return C.byref(_PAGES(pool.device.index, pool.data_ptr(), pool.stride(axis) * size if n > 1 else nbytes,
+                          pool.stride(0) * size if axis and layers > 1 else 0, nbytes, n, layers)), n
+
+
+def _table(table, device):
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.device != device:
+        raise ValueError(f"table must be an int32 tensor [seqs, pages] on {device}")
+    (s, p), (stride, inner) = table.shape, table.stride()
+    if not s or not p or (inner != 1 and p > 1):
+        raise ValueError("table must have sequences and columns, each row contiguous")
+    return s, p, stride if s > 1 else p
+
+
+def _pinned(pinned, n, device):
+    if pinned is None:
+        return None
+    if (pinned.dtype not in (torch.uint8, torch.bool) or pinned.device != device or pinned.shape != (n,)
+            or not pinned.is_contiguous()):
+        raise ValueError(f"pinned must be a contiguous uint8 or bool tensor [{n}] on {device}")
+    return pinned.data_ptr()
+
+
+def op_pages_fork(pool, table, src, keep, need, page, pinned=None, axis=0):
+    """A new set of sequences from the old ones' pages (nd_op_pages_fork):
+    sequence d keeps ``keep[d]`` positions of old sequence ``src[d]`` (-1: of
+    none) and gets pages for ``need[d]``, ``page`` positions a page. Whole
+    pages are shared, a partly filled one that will be written is copied in
+    ``pool`` (any type; [pages, ..], or [layers, pages, ..] with axis=1), pages
+    nothing refers to are free. Returns (table [n, columns], refs [pages],
+    info [4]: pages in use, given, copied, wanted but not had)."""
+    dev = pool.device
+    pv, n_pages = _pages(pool, axis)
+    s, p, stride = _table(table, dev)
+    n = src.shape[0] if src.dim() else 0
+    if not n:
+        raise ValueError("src must name at least one sequence")
+    out = torch.empty((n, p), dtype=torch.int32, device=dev)
+    refs = torch.empty(n_pages, dtype=torch.int32, device=dev)
+    info = torch.empty(4, dtype=torch.int32, device=dev)
+    L = lib()
+    size = L.nd_op_pages_fork_ws(n_pages, n)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    if L.nd_op_pages_fork(pv, table.data_ptr(), stride, s, p, page, _int32(src, n, dev, "src"), _int32(keep, n, dev, "keep"),
+                          _int32(need, n, dev, "need"), n, _pinned(pinned, n_pages, dev), out.data_ptr(), refs.data_ptr(),
+                          info.data_ptr(), ws.data_ptr(), size, _stream(dev)) != 0:
+        raise _err()
+    return out, refs, info
+
+
+def op_pages_compact(pool, table, pinned=None, axis=0):
+    """Live pages to the front of the pool (nd_op_pages_compact). Returns
+    (table, map [pages]: each live page's new id or -1, info [2]: live pages,
+    pages moved)."""
+    dev = pool.device
+    pv, n_pages = _pages(pool, axis)
+    s, p, stride = _table(table, dev)
+    out = torch.empty((s, p), dtype=torch.int32, device=dev)
+    to = torch.empty(n_pages, dtype=torch.int32, device=dev)
+    info = torch.empty(2, dtype=torch.int32, device=dev)
+    L = lib()
+    size = L.nd_op_pages_compact_ws(n_pages)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    if L.nd_op_pages_compact(pv, table.data_ptr(), stride, s, p, _pinned(pinned, n_pages, dev), out.data_ptr(), to.data_ptr(),
+                             info.data_ptr(), ws.data_ptr(), size, _stream(dev)) != 0:
+        raise _err()
+    return out, to, info
+
+
+def op_verify(logits, draft, u, temperature, q=None, counts=None):
+    """Check drafted tokens and draw the next (nd_op_verify): logits
+    [seqs, T + 1, V] float32, float16 or bfloat16, draft [seqs, T] int32,
+    u [seqs, T + 1] float32 in [0, 1), temperature [seqs] float32 (not above
+    0: greedy), q [seqs, T, V] float32 the draft's probabilities (None: it was
+    certain), counts [seqs] int32 how many drafts there are (None: T). Returns
+    (tokens [seqs, T + 1]: accepted drafts, the drawn token, then -1;
+    accepted [seqs]; probs [seqs, T + 1])."""
+    dev = logits.device
+    if logits.dtype not in _TYPES or logits.dim() != 3 or not logits.is_cuda or logits.stride(2) != 1 or not logits.numel():
+        raise ValueError("logits must be a float32, float16 or bfloat16 CUDA tensor [seqs, T + 1, V], rows contiguous")
+    s, t1, v = logits.shape
+    t = t1 - 1
+    if draft.dtype is not torch.int32 or draft.shape != (s, t) or draft.device != dev or not draft.is_contiguous():
+        raise ValueError(f"draft must be a contiguous int32 tensor [{s}, {t}] on {dev}")
+    if u.dtype is not torch.float32 or u.shape != (s, t1) or u.device != dev or not u.is_contiguous():
+        raise ValueError(f"u must be a contiguous float32 tensor [{s}, {t1}] on {dev}")
+    if temperature.dtype is not torch.float32 or temperature.shape != (s,) or temperature.device != dev or not temperature.is_contiguous():
+        raise ValueError(f"temperature must be a contiguous float32 tensor [{s}] on {dev}")
+    if q is not None and (q.dtype is not torch.float32 or q.shape != (s, t, v) or q.device != dev
+                          or (t and q.stride(2) != 1 and v > 1)):
+        raise ValueError(f"q must be a float32 tensor [{s}, {t}, {v}] on {dev}, rows contiguous")
+    c = None if counts is None else _int32(counts, s, dev, "counts")
+    tokens = torch.empty((s, t1), dtype=torch.int32, device=dev)
+    accepted = torch.empty(s, dtype=torch.int32, device=dev)
+    probs = torch.empty((s, t1), dtype=torch.float32, device=dev)
+    qa = (None, 0, 0) if q is None or not t else (q.data_ptr(), q.stride(0), q.stride(1))
+    if lib().nd_op_verify(dev.index, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
+                          draft.data_ptr(), c, u.data_ptr(), temperature.data_ptr(), *qa, s, t, v, tokens.data_ptr(),
+                          accepted.data_ptr(), probs.data_ptr(), _stream(dev)) != 0:
+        raise _err()
+    return tokens, accepted, probs
