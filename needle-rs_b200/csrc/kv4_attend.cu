@@ -51,7 +51,10 @@
 
 namespace nd {
 
-constexpr int ATT_WARPS = 4, ATT_STAGES = 4;
+constexpr int ATT_WARPS = 4;
+constexpr int ATT_KT(int nt) { return nt == 4 ? 1 : 2; }
+constexpr int ATT_STAGES(int nt) { return nt == 4 ? 4 : 3; }
+constexpr int ATT_CTAS(int nt, int dv) { return nt == 4 ? 2 : nt == 2 || dv == 128 ? 3 : 4; }  // an SM
 // Tiles: a shorter run of a cut unit costs more to join than it takes.
 constexpr int ATT_MIN_SHARE = 4;
 // A call whose units all have at most this many tiles deals whole units out
@@ -75,10 +78,32 @@ struct AttendArgs {
     FastDiv page_tiles;
     int window, sink;
     float scale_log2e;
-    bool q_vec, o_vec, whole, zero_rest;
+    bool q_vec, o_vec, zero_rest;
     float* parts;   // [runners][2][8 NT * (DV + 2)]; a runner is a warp, for NT = 1 a CTA
     int4* joins;    // [runners]: (sequence, kv head, query block, further runners) of the cut unit that starts there, w < 0: none
 };
+
+// Whole units are numbered without sums: sequence s has the places
+// from s + start[s] * group / (8 NT) on, one more than its whole blocks of
+// rows at least, of which it leaves at most one empty.
+template <int NT>
+__device__ __forceinline__ int first_place(const AttendArgs& a, int s) {
+    return s + (int)((long long)kv4_first_row(a.kv, s) * a.group.d / (8 * NT));
+}
+
+// The sequence of place u, by the whole warp 32 at a time.
+template <int NT>
+__device__ __forceinline__ int seq_of_place(const AttendArgs& a, int u, int lane) {
+    int lo = 0, size = a.kv.seqs;  // sequences that may begin at or before u
+    while (size > 0) {
+        const int step = (size + 31) / 32, at = lane * step + step - 1;
+        const bool before = at < size && first_place<NT>(a, lo + at) <= u;
+        const int c = __popc(__ballot_sync(0xffffffffu, before));
+        lo += c * step;
+        size = min(step - 1, size - c * step);
+    }
+    return lo - 1;
+}
 
 // The key tiles a block of query rows reads: those of the first `sink`
 // positions, then lo .. of the window.
@@ -121,12 +146,10 @@ __device__ __forceinline__ Tiles block_tiles(const AttendArgs& a, const SeqRows&
     return tiles_of(a, r.pos0 + a.group(x0), r.pos0 + a.group(x1));
 }
 
-// What a sequence and kv head adds to the list of work: its tiles, or its
-// units where they are dealt out whole.
+// What a sequence and kv head adds to the list of work: its tiles.
 template <int NT>
 __device__ __forceinline__ long long seq_work(const AttendArgs& a, const SeqRows& r) {
     const int blocks = (r.n * (int)a.group.d + 8 * NT - 1) / (8 * NT);
-    if (a.whole) return blocks;
     long long t = 0;
     for (int b = 0; b < blocks; b++) t += block_tiles<NT>(a, r, b).n;
     return t;
@@ -171,8 +194,8 @@ __device__ __forceinline__ uint32_t code16_mid(uint32_t x) {
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
     return y;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {  // 16 of them, or none and zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // Two f32 operations in one instruction.
@@ -216,14 +239,19 @@ struct AttendShape {
     static constexpr int KSTEPS = DK / 16;
     static constexpr int QOPS = NT * KSTEPS * QS;  // a query block's operands: pairs of registers
     static constexpr bool Q_SMEM = QOPS > 16;      // else they stay in registers
+    // Tiles a round of the main loop, and rounds in flight: two tiles give a
+    // warp two independent chains of products, and share a round's overhead.
+    static constexpr int KT = ATT_KT(NT), STAGES = ATT_STAGES(NT);
     // For one block of eight rows the warps of a CTA join their parts in
     // shared memory first: decoding cuts few units into many parts.
     static constexpr bool MERGE = NT == 1;
     static constexpr int PART = 8 * NT * (DV + 2);  // floats
-    static constexpr int RING = ATT_STAGES * TB > 4 * PART || !MERGE ? ATT_STAGES * TB : 4 * PART;
-    static constexpr int WARP_SMEM = RING + (MERGE ? 4 * PART : 0) + (Q_SMEM ? QOPS * 256 : 0);
-    static constexpr int SMEM = ATT_WARPS * WARP_SMEM;
-    static constexpr int CTAS = NT == 1 ? 4 : NT == 2 ? 3 : 2;
+    static constexpr int SLOTS = STAGES * KT * TB;
+    static constexpr int RING = SLOTS > 4 * PART || !MERGE ? SLOTS : 4 * PART;
+    static constexpr int QBYTES = Q_SMEM ? QOPS * 256 : 0;
+    static constexpr int WARP_SMEM = RING + QBYTES + (MERGE ? 4 * PART : 0);
+    static constexpr int SMEM = ATT_WARPS * WARP_SMEM, WHOLE_SMEM = ATT_WARPS * (RING + QBYTES);
+    static constexpr int CTAS = ATT_CTAS(NT, DV);
 };
 
 // acc (8 VW g + .. as the main loop holds it), M, l of a part of 8 rows.
@@ -265,12 +293,484 @@ struct OutRows {
     }
 };
 
+// A warp's part of a unit: tiles off .. off + m - 1 of query block b of
+// sequence s and kv head h. With `part` NULL they are all it has and the
+// result goes to its place; else the sums go to `part`, unnormalised.
+template <int DK, int DV, int NT, typename T>
+__device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __restrict__ q, T* __restrict__ out, int s, int h, int b,
+                                            const SeqRows& rows, const Tiles& tl, int off, int m, uint8_t* ring, uint2* qsm0,
+                                            float* part) {
+    using Sh = AttendShape<DK, DV, NT, T>;
+    constexpr int TB = Sh::TB, QS = Sh::QS, WS = Sh::WS, KS = Sh::KSTEPS, MT = DV / 16, VW = DV / 64, KT = Sh::KT, STAGES = Sh::STAGES;
+    constexpr bool F32 = Sh::F32;
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int nrows = rows.n * (int)a.group.d;
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+    uint2* qsm = qsm0 + lane;
+
+    // addresses of the next tiles, 32 at a time, one batch ahead; 0: no such page
+    const int32_t* trow = a.kv.table + (size_t)s * a.kv.table_stride;
+    const uint8_t* head = a.kv.pool + (size_t)h * a.kv.page_tiles * TB;
+    auto fetch = [&](int i) -> unsigned long long {
+        if (i >= off + m) return 0;
+        const int t = tl.at(i), p = a.page_tiles(t);
+        const int page = p < a.kv.max_pages ? __ldg(trow + p) : -1;
+        if (page < 0 || page >= a.kv.num_pages) return 0;
+        return (unsigned long long)(head + (size_t)page * a.kv.page_stride + (size_t)(t - p * a.kv.page_tiles) * TB);
+    };
+    unsigned long long src = fetch(off + lane), src_next = fetch(off + 32 + lane);
+    uint32_t have = 0;  // bit k: the tile issued k issues ago exists (others are zeros in the ring)
+    int issued = 0;
+    uint32_t put_at = 0;
+    auto issue = [&]() {
+#pragma unroll
+        for (int u = 0; u < KT; u++) {
+            const unsigned long long from = __shfl_sync(0xffffffffu, src, (issued + u) & 31);
+            const uint32_t bytes = from ? 16 : 0;
+            have = have << 1 | (from != 0);
+            const uint8_t* p = (from ? (const uint8_t*)from : a.kv.pool) + lane * 16;
+            const uint32_t d = ring_s + put_at + u * TB;
+#pragma unroll
+            for (int j = 0; j < TB / 512; j++) copy16(d + j * 512, p + j * 512, bytes);
+            if (TB % 512 && lane * 16 < TB % 512) copy16(d + TB / 512 * 512, p + TB / 512 * 512, bytes);
+        }
+        put_at = put_at == (STAGES - 1) * KT * TB ? 0 : put_at + KT * TB;
+        issued += KT;
+        if (__builtin_expect((issued & 31) == 0, 0)) {
+            src = src_next;
+            src_next = fetch(off + issued + 32 + lane);
+        }
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+    };
+    __syncwarp();  // the ring's last tile has been read by every lane
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; i++) issue();
+
+    // the query block: lane (g, c) holds of query row 8 t + g the
+    // dimensions whose codes it will hold of every key
+    uint2 qreg[Sh::Q_SMEM ? 1 : Sh::QOPS];
+    f32x2 f0[NT], f1[NT], mid[F32 ? NT : 1][2];
+    int seen_hi[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int x = b * 8 * NT + 8 * t + g;
+        const bool on = x < nrows;
+        float v[DK / 4];
+#pragma unroll
+        for (int i = 0; i < DK / 4; i++) v[i] = 0.f;
+        const int tok = a.group(x);
+        if (on) {
+            const T* p = q + (long long)(rows.first + tok) * a.q_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.q_head;
+            if constexpr (DK == 48) {
+                load8(p + 8 * c, a.q_vec, v);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[8 + i] = (float)p[32 + 4 * c + i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < DK / 32; i++) load8(p + (DK / 4) * c + 8 * i, a.q_vec, v + 8 * i);
+            }
+        }
+        float top = 0.f, sum = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < DK / 4; i++) {
+            top = fmaxf(top, fabsf(v[i]));
+            bad |= !(fabsf(v[i]) <= FLT_MAX);
+            sum += v[i];
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
+        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2) != 0;
+        // 2^e <= top < 2^(e+1) goes to 2^14: f16's largest values
+        const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+        const float up = bad ? 0.f : __uint_as_float((uint32_t)(14 - min(e, 127) + 127) << 23);
+        float fac0 = a.scale_log2e * __uint_as_float((uint32_t)(min(e, 127) - 14 + 127) << 23) * 16777216.f;
+        float fac1 = a.scale_log2e * sum;
+        if (bad) fac0 = fac1 = __uint_as_float(0x7fc00000u);
+        float q1 = 0.f, q2 = 0.f;  // sums of the fixed-point terms: exact
+        auto terms = [&](float x0, float x1, float mul, uint32_t& hi, uint32_t& lo) {
+            if (F32) {
+                // multiples of 16 up to 2^15, then of 2^-8 up to 8
+                const float a0 = rintf(x0 * 0.0625f) * 16.f, a1 = rintf(x1 * 0.0625f) * 16.f;
+                const float b0 = rintf((x0 - a0) * 256.f) * 0.00390625f, b1 = rintf((x1 - a1) * 256.f) * 0.00390625f;
+                q1 += a0 + a1, q2 += b0 + b1;
+                hi = pack_half2(a0 * mul, a1 * mul), lo = pack_half2(b0 * mul, b1 * mul);
+            } else {
+                hi = pack_half2(x0 * mul, x1 * mul);
+            }
+        };
+        // operands of k-step k: codes (x0, x1) as they are, (y0, y1) 16-fold
+        auto put = [&](int k, float x0, float x1, float y0, float y1) {
+            uint2 hi, lo;
+            terms(x0, x1, 1.f, hi.x, lo.x);
+            terms(y0, y1, 0.0625f, hi.y, lo.y);
+            const int at = (t * KS + k) * QS;
+            if constexpr (Sh::Q_SMEM) {
+                qsm[at * 32] = hi;
+                if (F32) qsm[(at + 1) * 32] = lo;
+            } else {
+                qreg[at] = hi;
+                if (F32) qreg[at + QS - 1] = lo;
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < DK / 4; i++) v[i] = bad ? 0.f : v[i] * up;
+#pragma unroll
+        for (int w = 0; w < DK / 32; w++) {
+            const float* y = v + 8 * w;
+            put(2 * w, y[0], y[4], y[1], y[5]);
+            put(2 * w + 1, y[2], y[6], y[3], y[7]);
+        }
+        if constexpr (DK == 48) put(2, v[8], v[10], v[9], v[11]);
+        const int hi = on ? (int)min(max(rows.pos0 + tok, -1LL), 0x7fffffffLL) : -1;
+        auto cols = [&](float x) { return pair(__shfl_sync(0xffffffffu, x, 8 * c), __shfl_sync(0xffffffffu, x, 8 * c + 4)); };
+        f0[t] = cols(fac0);
+        f1[t] = cols(fac1);
+        seen_hi[t][0] = __shfl_sync(0xffffffffu, hi, 8 * c);
+        seen_hi[t][1] = __shfl_sync(0xffffffffu, hi, 8 * c + 4);
+        if (F32) {  // -8 of the codes' unit, 2^-24
+            q1 += __shfl_xor_sync(0xffffffffu, q1, 1);
+            q2 += __shfl_xor_sync(0xffffffffu, q2, 1);
+            q1 += __shfl_xor_sync(0xffffffffu, q1, 2);
+            q2 += __shfl_xor_sync(0xffffffffu, q2, 2);
+            mid[F32 ? t : 0][0] = cols(q1 * -4.76837158203125e-7f);
+            mid[F32 ? t : 0][1] = cols(q2 * -4.76837158203125e-7f);
+        }
+    }
+    // tiles wholly inside every row's span need no masks
+    const int x_last = min((b + 1) * 8 * NT, nrows) - 1;
+    const long long p_first = rows.pos0 + a.group(b * 8 * NT), p_last = rows.pos0 + a.group(x_last);
+    const int all_hi = (int)min(max(p_first, -1LL), 0x7fffffffLL) - 15;              // whole: k0 <= all_hi and
+    const int all_lo = a.window > 0 ? (int)min(max(p_last - a.window, -1LL), 0x7fffffffLL) : -1;  // k0 > all_lo or k0 + 15 < sink
+
+    float acc[NT][MT][4];
+    f32x2 nM[NT], l[NT], mn[NT];  // -M, sum p, sum p mv for columns 2 c, 2 c + 1 (the sums over this lane's keys)
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[t][i][j] = 0.f;
+        nM[t] = pair(-ATT_LOW, -ATT_LOW);
+        l[t] = mn[t] = 0;
+    }
+
+    int key0 = tl.at(off) * KV4_TILE;
+    uint32_t get_at = 0;
+#pragma unroll 1
+    for (int i = 0; i < m; i += KT) {
+        asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();
+        const uint32_t here = have >> ((STAGES - 2) * KT);  // bit KT - 1 - u: tile u of this round
+        issue();  // into the slots read in the last round
+        const uint8_t* round = ring + get_at;
+        get_at = get_at == (STAGES - 1) * KT * TB ? 0 : get_at + KT * TB;
+        int k0[KT];
+#pragma unroll
+        for (int u = 0; u < KT; u++) {
+            k0[u] = key0;
+            key0 = off + i + u + 1 == tl.sink ? tl.lo * KV4_TILE : key0 + KV4_TILE;
+        }
+        bool whole = true;
+#pragma unroll
+        for (int u = 0; u < KT; u++) whole &= k0[u] <= all_hi && (k0[u] > all_lo || k0[u] + 15 < a.sink);
+        whole &= (here & ((1u << KT) - 1)) == (1u << KT) - 1;
+
+        // scores: keys g and g + 8 against query rows 2 c, 2 c + 1
+        float sc[KT][NT][4], sc2[F32 ? KT : 1][F32 ? NT : 1][4];
+#pragma unroll
+        for (int u = 0; u < KT; u++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                if (F32) {
+                    const float2 x = unpair(mid[F32 ? t : 0][0]), y = unpair(mid[F32 ? t : 0][1]);
+                    sc[u][t][0] = sc[u][t][2] = x.x, sc[u][t][1] = sc[u][t][3] = x.y;
+                    float* z = sc2[F32 ? u : 0][F32 ? t : 0];
+                    z[0] = z[2] = y.x, z[1] = z[3] = y.y;
+                } else {
+                    sc[u][t][0] = sc[u][t][1] = sc[u][t][2] = sc[u][t][3] = 0.f;
+                }
+            }
+        auto qop = [&](int t, int k, int term) -> uint2 {
+            const int at = (t * KS + k) * QS + term;
+            if constexpr (Sh::Q_SMEM) return qsm[at * 32];
+            else return qreg[at];
+        };
+        uint32_t wa[KT][DK / 32], wb[KT][DK / 32];
+        float2 kpa[KT], kpb[KT], vpa[KT], vpb[KT];
+#pragma unroll
+        for (int u = 0; u < KT; u++) {
+            const uint8_t *ka = round + u * TB + g * (DK / 2), *kb = ka + 4 * DK;
+            if constexpr (DK == 128) {
+                const uint4 x = *(const uint4*)(ka + 16 * c), y = *(const uint4*)(kb + 16 * c);
+                wa[u][0] = x.x, wa[u][1] = x.y, wa[u][2] = x.z, wa[u][3] = x.w;
+                wb[u][0] = y.x, wb[u][1] = y.y, wb[u][2] = y.z, wb[u][3] = y.w;
+            } else if constexpr (DK == 64) {
+                const uint2 x = *(const uint2*)(ka + 8 * c), y = *(const uint2*)(kb + 8 * c);
+                wa[u][0] = x.x, wa[u][1] = x.y;
+                wb[u][0] = y.x, wb[u][1] = y.y;
+            } else {
+                wa[u][0] = *(const uint32_t*)(ka + 4 * c);
+                wb[u][0] = *(const uint32_t*)(kb + 4 * c);
+            }
+            const uint8_t* par = round + u * TB + 8 * (DK + DV) + 4 * g;
+            kpa[u] = unpack_half2(*(const uint32_t*)par), kpb[u] = unpack_half2(*(const uint32_t*)(par + 32));
+            vpa[u] = unpack_half2(*(const uint32_t*)(par + 64)), vpb[u] = unpack_half2(*(const uint32_t*)(par + 96));
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            uint32_t x0[KT], x1[KT], y0[KT], y1[KT];
+#pragma unroll
+            for (int u = 0; u < KT; u++) {
+                uint32_t xa, xb;
+                if (DK == 48 && k == 2) {  // dimensions 32 .. 47: four codes a lane
+                    const uint8_t* p = round + u * TB + g * (DK / 2) + 16 + 2 * c;
+                    xa = __byte_perm(*(const uint16_t*)p, 0, 0x4140), xb = __byte_perm(*(const uint16_t*)(p + 4 * DK), 0, 0x4140);
+                } else {
+                    xa = wa[u][k / 2 < DK / 32 ? k / 2 : 0], xb = wb[u][k / 2 < DK / 32 ? k / 2 : 0];
+                    if (k & 1) xa >>= 8, xb >>= 8;
+                }
+                x0[u] = xa & 0x000f000fu, x1[u] = xa & 0x00f000f0u, y0[u] = xb & 0x000f000fu, y1[u] = xb & 0x00f000f0u;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const uint2 o = qop(t, k, 0);
+#pragma unroll
+                for (int u = 0; u < KT; u++) mma16816(sc[u][t], x0[u], y0[u], x1[u], y1[u], o.x, o.y);
+                if (F32) {
+                    const uint2 o2 = qop(t, k, QS - 1);
+#pragma unroll
+                    for (int u = 0; u < KT; u++) mma16816(sc2[F32 ? u : 0][F32 ? t : 0], x0[u], y0[u], x1[u], y1[u], o2.x, o2.y);
+                }
+            }
+        }
+        f32x2 sa[KT][NT], sb[KT][NT];  // keys g, g + 8
+        float ta[KT], tb[KT];          // a score may pass M by this much before M is raised
+#pragma unroll
+        for (int u = 0; u < KT; u++) {
+            if (F32) {  // the middle of the codes instead of the minimum
+                kpa[u].y = __fmaf_rn(8.f, kpa[u].x, kpa[u].y), kpb[u].y = __fmaf_rn(8.f, kpb[u].x, kpb[u].y);
+                vpa[u].y = __fmaf_rn(8.f, vpa[u].x, vpa[u].y), vpb[u].y = __fmaf_rn(8.f, vpb[u].x, vpb[u].y);
+            }
+            ta[u] = 4.f - lg2(fmaxf(vpa[u].x, 5.9604645e-8f)), tb[u] = 4.f - lg2(fmaxf(vpb[u].x, 5.9604645e-8f));
+            const f32x2 ksa = pair(kpa[u].x, kpa[u].x), ksb = pair(kpb[u].x, kpb[u].x);
+            const f32x2 kma = pair(kpa[u].y, kpa[u].y), kmb = pair(kpb[u].y, kpb[u].y);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                f32x2 da = pair(sc[u][t][0], sc[u][t][1]), db = pair(sc[u][t][2], sc[u][t][3]);
+                if (F32) {
+                    const float* z = sc2[F32 ? u : 0][F32 ? t : 0];
+                    da = add2(da, pair(z[0], z[1])), db = add2(db, pair(z[2], z[3]));
+                }
+                sa[u][t] = fma2(mul2(da, f0[t]), ksa, mul2(f1[t], kma));
+                sb[u][t] = fma2(mul2(db, f0[t]), ksb, mul2(f1[t], kmb));
+            }
+        }
+        if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+            for (int u = 0; u < KT; u++) {
+                const bool in = here >> (KT - 1 - u) & 1;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    auto mask = [&](f32x2 x, int key) {
+                        float2 f = unpair(x);
+                        const bool sunk = key < a.sink;
+                        if (!(in && key <= seen_hi[t][0] && (a.window <= 0 || sunk || key > seen_hi[t][0] - a.window))) f.x = -INFINITY;
+                        if (!(in && key <= seen_hi[t][1] && (a.window <= 0 || sunk || key > seen_hi[t][1] - a.window))) f.y = -INFINITY;
+                        return pair(f.x, f.y);
+                    };
+                    sa[u][t] = mask(sa[u][t], k0[u] + g);
+                    sb[u][t] = mask(sb[u][t], k0[u] + g + 8);
+                }
+            }
+        }
+        bool raise = false;
+        float2 xa[KT][NT], xb[KT][NT];  // exponents
+#pragma unroll
+        for (int u = 0; u < KT; u++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                xa[u][t] = unpair(add2(sa[u][t], nM[t])), xb[u][t] = unpair(add2(sb[u][t], nM[t]));
+                raise |= xa[u][t].x > ta[u] || xa[u][t].y > ta[u] || xb[u][t].x > tb[u] || xb[u][t].y > tb[u];
+            }
+        if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const float2 old = unpair(nM[t]);
+                float m0 = -old.x, m1 = -old.y;
+#pragma unroll
+                for (int u = 0; u < KT; u++) {
+                    const float2 fa = unpair(sa[u][t]), fb = unpair(sb[u][t]);
+                    m0 = fmaxf(m0, fmaxf(fa.x + (4.f - ta[u]), fb.x + (4.f - tb[u])));
+                    m1 = fmaxf(m1, fmaxf(fa.y + (4.f - ta[u]), fb.y + (4.f - tb[u])));
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) {
+                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+                }
+                const float r0 = ex2(-old.x - m0), r1 = ex2(-old.y - m1);
+                const f32x2 r = pair(r0, r1);
+                nM[t] = pair(-m0, -m1);
+                l[t] = mul2(l[t], r);
+                mn[t] = mul2(mn[t], r);
+#pragma unroll
+                for (int k = 0; k < MT; k++) acc[t][k][0] *= r0, acc[t][k][1] *= r1, acc[t][k][2] *= r0, acc[t][k][3] *= r1;
+#pragma unroll
+                for (int u = 0; u < KT; u++) xa[u][t] = unpair(add2(sa[u][t], nM[t])), xb[u][t] = unpair(add2(sb[u][t], nM[t]));
+            }
+        }
+        // weights, and their operands: rows of the transpose are query rows
+        uint32_t wop[KT][NT][2][WS];
+#pragma unroll
+        for (int u = 0; u < KT; u++) {
+            const f32x2 vsa = pair(vpa[u].x, vpa[u].x), vsb = pair(vpb[u].x, vpb[u].x), vma = pair(vpa[u].y, vpa[u].y), vmb = pair(vpb[u].y, vpb[u].y);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const f32x2 pa = pair(ex2(xa[u][t].x), ex2(xa[u][t].y)), pb = pair(ex2(xb[u][t].x), ex2(xb[u][t].y));
+                l[t] = add2(l[t], add2(pa, pb));
+                f32x2 wa2 = mul2(pa, vsa), wb2 = mul2(pb, vsb), ma = mul2(pa, vma), mb = mul2(pb, vmb);
+                if (__builtin_expect(!whole, 0)) {  // a masked place may hold NaN or infinity
+                    auto clean = [](f32x2 x, float2 e) {
+                        const float2 f = unpair(x);
+                        return pair(e.x == -INFINITY ? 0.f : f.x, e.y == -INFINITY ? 0.f : f.y);
+                    };
+                    wa2 = clean(wa2, xa[u][t]), wb2 = clean(wb2, xb[u][t]), ma = clean(ma, xa[u][t]), mb = clean(mb, xb[u][t]);
+                }
+                mn[t] = add2(mn[t], add2(ma, mb));
+                const float2 fa = unpair(wa2), fb = unpair(wb2);
+                const uint32_t ha = pack_half2(fa.x, fa.y), hb = pack_half2(fb.x, fb.y);
+                wop[u][t][0][0] = transpose8(ha), wop[u][t][1][0] = transpose8(hb);
+                if (WS == 2) {
+                    const float2 ra = unpack_half2(ha), rb = unpack_half2(hb);
+                    wop[u][t][0][WS - 1] = transpose8(pack_half2(fa.x - ra.x, fa.y - ra.y));
+                    wop[u][t][1][WS - 1] = transpose8(pack_half2(fb.x - rb.x, fb.y - rb.y));
+                }
+            }
+        }
+        // values: lane (g, c) holds dimensions 8 (VW g + w) .. + 7 of keys 2c, 2c+1, 2c+8, 2c+9
+        uint32_t vw[KT][4][VW];
+#pragma unroll
+        for (int u = 0; u < KT; u++) {
+            const uint8_t* vt = round + u * TB + 8 * DK + g * 4 * VW + c * DV;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint8_t* p = vt + ((j & 1) + (j >= 2 ? 8 : 0)) * (DV / 2);
+                if constexpr (VW == 2) {
+                    const uint2 x = *(const uint2*)p;
+                    vw[u][j][0] = x.x, vw[u][j][1] = x.y;
+                } else {
+                    vw[u][j][0] = *(const uint32_t*)p;
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; w++)
+#pragma unroll
+            for (int quarter = 0; quarter < 4; quarter++) {
+                // dimensions 2 quarter (row g), 2 quarter + 1 (row g + 8)
+                float z[F32 ? NT : 1][4];
+#pragma unroll
+                for (int u = 0; u < KT; u++) {
+                    const uint32_t sel = quarter < 2 ? 0x5410 : 0x7632;
+                    const uint32_t x = __byte_perm(vw[u][0][w], vw[u][1][w], sel) >> (quarter & 1 ? 8 : 0);
+                    const uint32_t y = __byte_perm(vw[u][2][w], vw[u][3][w], sel) >> (quarter & 1 ? 8 : 0);
+                    uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                    if (F32) a0 = code_mid(a0), a1 = code16_mid(a1), a2 = code_mid(a2), a3 = code16_mid(a3);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        float* d = F32 ? z[F32 ? t : 0] : acc[t][4 * w + quarter];
+                        if (F32 && u == 0) d[0] = d[1] = d[2] = d[3] = 0.f;
+#pragma unroll
+                        for (int term = 0; term < WS; term++) mma16816(d, a0, a1, a2, a3, wop[u][t][0][term], wop[u][t][1][term]);
+                    }
+                }
+                if (F32)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) acc[t][4 * w + quarter][j] += z[F32 ? t : 0][j];
+            }
+    }
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    __syncwarp();
+
+    // this run's part of the unit: sums over the keys' lanes, 2^24 back
+    const bool done = !part;
+    const OutRows<T> to{out, a, rows.first, h, nrows};
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) {
+            l[t] = add2(l[t], __shfl_xor_sync(0xffffffffu, l[t], o));
+            mn[t] = add2(mn[t], __shfl_xor_sync(0xffffffffu, mn[t], o));
+        }
+        const float2 l2 = unpair(l[t]), mn2 = unpair(mn[t]), M2 = unpair(nM[t]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const float lj = j ? l2.y : l2.x, mj = j ? mn2.y : mn2.x;
+            const int y = 8 * t + 2 * c + j, x = b * 8 * NT + y;  // query row in the block, in the sequence
+            const float norm = done ? (lj == 0.f ? 0.f : 1.f / lj) : 1.f;
+#pragma unroll
+            for (int w = 0; w < VW; w++) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v[2 * k] = __fmaf_rn(acc[t][4 * w + k][j], F32 ? 1.f : 16777216.f, mj) * norm;
+                    v[2 * k + 1] = __fmaf_rn(acc[t][4 * w + k][2 + j], F32 ? 1.f : 1048576.f, mj) * norm;
+                }
+                const int d0 = 8 * (VW * g + w);
+                if (!done) store8(part + y * DV + d0, true, v);
+                else if (x < nrows) store8(to.at(x) + d0, a.o_vec, v);
+            }
+            if (!done && g == 0) {
+                part[8 * NT * DV + y] = j ? -M2.y : -M2.x;
+                part[8 * NT * (DV + 1) + y] = lj;
+            }
+        }
+    }
+}
+
+// Output rows behind the last sequence, where the caller wants them zero.
+template <int DV, typename T>
+__device__ __forceinline__ void zero_rest(const AttendArgs& a, T* out, int wid, int warps, int lane) {
+    if (!a.zero_rest || !a.kv.start) return;
+    for (int r = kv4_first_row(a.kv, a.kv.seqs) + wid; r < a.kv.rows; r += warps)
+        for (int hq = 0; hq < a.kv.heads * (int)a.group.d; hq++)
+            for (int d = lane; d < DV; d += 32) out[r * a.o_row + hq * a.o_head + d] = (T)0.f;
+}
+
+// Short units, dealt out whole: unit by unit, no sums over the sequences, no joins.
+template <int DK, int DV, int NT, typename T>
+__global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CTAS)
+    kv4_attend_whole_kernel(AttendArgs a, const T* __restrict__ q, T* __restrict__ out) {
+    using Sh = AttendShape<DK, DV, NT, T>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warps = gridDim.x * ATT_WARPS, wid = blockIdx.x * ATT_WARPS + warp;
+    zero_rest<DV>(a, out, wid, warps, lane);
+    uint8_t* ring = smem + warp * (Sh::RING + Sh::QBYTES);
+    const long long units = ((long long)a.kv.seqs + (long long)a.kv.rows * a.group.d / (8 * NT)) * a.kv.heads;
+    for (long long x = wid; x < units; x += warps) {
+        const int u = (int)(x / a.kv.heads), h = (int)(x % a.kv.heads), s = seq_of_place<NT>(a, u, lane);
+        if (s < 0) continue;
+        const int b = u - first_place<NT>(a, s);
+        const SeqRows rows = seq_rows(a, s);
+        if (b * 8 * NT >= rows.n * (int)a.group.d) continue;
+        const Tiles tl = block_tiles<NT>(a, rows, b);
+        attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, 0, tl.n, ring, (uint2*)(ring + Sh::RING), nullptr);
+    }
+}
+
 template <int DK, int DV, int NT, typename T>
 __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CTAS)
     kv4_attend_kernel(AttendArgs a, const T* __restrict__ q, T* __restrict__ out) {
     using Sh = AttendShape<DK, DV, NT, T>;
-    constexpr int TB = Sh::TB, QS = Sh::QS, WS = Sh::WS, KS = Sh::KSTEPS, MT = DV / 16, VW = DV / 64, PART = Sh::PART;
-    constexpr bool F32 = Sh::F32, MERGE = Sh::MERGE;
+    constexpr int PART = Sh::PART;
+    constexpr bool MERGE = Sh::MERGE;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long sums[32 * ATT_WARPS + 1];
     __shared__ long long warp_sums[ATT_WARPS];
@@ -281,10 +781,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
     const int H = a.kv.heads, S = a.kv.seqs;
     const int warps = gridDim.x * ATT_WARPS, wid = blockIdx.x * ATT_WARPS + warp;
 
-    if (a.zero_rest && a.kv.start)
-        for (int r = kv4_first_row(a.kv, S) + wid; r < a.kv.rows; r += warps)
-            for (int hq = 0; hq < H * (int)a.group.d; hq++)
-                for (int d = lane; d < DV; d += 32) out[r * a.o_row + hq * a.o_head + d] = (T)0.f;
+    zero_rest<DV>(a, out, wid, warps, lane);
 
     // the list's length, and its prefix at every chunk of `per` sequences
     const int per = (S + 32 * ATT_WARPS - 1) / (32 * ATT_WARPS);
@@ -307,12 +804,12 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         __syncthreads();
     }
     const long long total = sums[32 * ATT_WARPS];
-    const long long share = max((total + warps - 1) / warps, (long long)(a.whole ? 1 : ATT_MIN_SHARE));
+    const long long share = max((total + warps - 1) / warps, (long long)ATT_MIN_SHARE);
     const long long begin = min(wid * share, total), end = min(begin + share, total);
-    if (!MERGE && !a.whole && lane == 0) a.joins[wid] = make_int4(0, 0, 0, -1);
+    if (!MERGE && lane == 0) a.joins[wid] = make_int4(0, 0, 0, -1);
 
     uint8_t* mine = smem + warp * Sh::WARP_SMEM;
-    float* first_part = (float*)(mine + Sh::RING);  // MERGE: a part of a unit that an earlier run begins
+    float* first_part = (float*)(mine + Sh::RING + Sh::QBYTES);  // MERGE: a part of a unit that an earlier run begins
     float* last_part = (float*)mine;                // MERGE: of a unit that a later run ends, over the ring
 
     if (begin < end) {
@@ -338,7 +835,6 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         }
         int h = (int)(rem / per_head), b = 0;
         rem -= h * per_head;
-        if (a.whole) b = (int)rem, rem = 0;
         Tiles tl = block_tiles<NT>(a, rows, b);
         while (rem >= tl.n) {
             rem -= tl.n;
@@ -346,400 +842,12 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         }
         int off = (int)rem;
 
-        const uint8_t* ring = mine;
-        const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
-        uint2* qsm = (uint2*)(mine + Sh::RING + (MERGE ? 4 * PART : 0)) + lane;
-        const size_t head_stride = (size_t)a.kv.page_tiles * TB;
-
         long long cur = begin;
         while (true) {
-            const int m = a.whole ? tl.n : (int)min((long long)(tl.n - off), end - cur);
-            const int nrows = rows.n * (int)a.group.d;
-
-            // addresses of the next tiles, 32 at a time, one batch ahead; 0: no such page
-            const int32_t* trow = a.kv.table + (size_t)s * a.kv.table_stride;
-            const uint8_t* head = a.kv.pool + h * head_stride + lane * 16;
-            auto fetch = [&](int i) -> unsigned long long {
-                if (i >= off + m) return 0;
-                const int t = tl.at(i), p = a.page_tiles(t);
-                const int page = p < a.kv.max_pages ? __ldg(trow + p) : -1;
-                if (page < 0 || page >= a.kv.num_pages) return 0;
-                return (unsigned long long)(head - lane * 16 + (size_t)page * a.kv.page_stride + (size_t)(t - p * a.kv.page_tiles) * TB);
-            };
-            unsigned long long src = fetch(off + lane), src_next = fetch(off + 32 + lane);
-            uint32_t ok_hist = 0;  // bit k: the tile issued k issues ago has a page
-            int issued = 0;
-            uint32_t put_at = 0;
-            auto issue = [&]() {
-                ok_hist <<= 1;
-                if (issued < m) {
-                    const unsigned long long from = __shfl_sync(0xffffffffu, src, issued & 31);
-                    if (from) {
-                        ok_hist |= 1;
-                        const uint8_t* p = (const uint8_t*)from + lane * 16;
-#pragma unroll
-                        for (int j = 0; j < TB / 512; j++) copy16(ring_s + put_at + j * 512, p + j * 512);
-                        if (TB % 512 && lane * 16 < TB % 512) copy16(ring_s + put_at + TB / 512 * 512, p + TB / 512 * 512);
-                    }
-                    put_at = put_at == (ATT_STAGES - 1) * TB ? 0 : put_at + TB;
-                    issued++;
-                    if ((issued & 31) == 0) {
-                        src = src_next;
-                        src_next = fetch(off + issued + 32 + lane);
-                    }
-                }
-                asm volatile("cp.async.commit_group;\n" ::: "memory");
-            };
-            __syncwarp();  // the ring's last tile has been read by every lane
-#pragma unroll 1
-            for (int i = 0; i < ATT_STAGES - 1; i++) issue();
-
-            // the query block: lane (g, c) holds of query row 8 t + g the
-            // dimensions whose codes it will hold of every key
-            uint2 qreg[Sh::Q_SMEM ? 1 : Sh::QOPS];
-            f32x2 f0[NT], f1[NT], mid[F32 ? NT : 1][2];
-            int seen_hi[NT][2];
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const int x = b * 8 * NT + 8 * t + g;
-                const bool on = x < nrows;
-                float v[DK / 4];
-#pragma unroll
-                for (int i = 0; i < DK / 4; i++) v[i] = 0.f;
-                const int tok = a.group(x);
-                if (on) {
-                    const T* p = q + (long long)(rows.first + tok) * a.q_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.q_head;
-                    if constexpr (DK == 48) {
-                        load8(p + 8 * c, a.q_vec, v);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) v[8 + i] = (float)p[32 + 4 * c + i];
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < DK / 32; i++) load8(p + (DK / 4) * c + 8 * i, a.q_vec, v + 8 * i);
-                    }
-                }
-                float top = 0.f, sum = 0.f;
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < DK / 4; i++) {
-                    top = fmaxf(top, fabsf(v[i]));
-                    bad |= !(fabsf(v[i]) <= FLT_MAX);
-                    sum += v[i];
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
-                bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 2) != 0;
-                // 2^e <= top < 2^(e+1) goes to 2^14: f16's largest values
-                const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);
-                const float up = bad ? 0.f : __uint_as_float((uint32_t)(14 - min(e, 127) + 127) << 23);
-                float fac0 = a.scale_log2e * __uint_as_float((uint32_t)(min(e, 127) - 14 + 127) << 23) * 16777216.f;
-                float fac1 = a.scale_log2e * sum;
-                if (bad) fac0 = fac1 = __uint_as_float(0x7fc00000u);
-                float q1 = 0.f, q2 = 0.f;  // sums of the fixed-point terms: exact
-                auto terms = [&](float x0, float x1, float mul, uint32_t& hi, uint32_t& lo) {
-                    if (F32) {
-                        // multiples of 16 up to 2^15, then of 2^-8 up to 8
-                        const float a0 = rintf(x0 * 0.0625f) * 16.f, a1 = rintf(x1 * 0.0625f) * 16.f;
-                        const float b0 = rintf((x0 - a0) * 256.f) * 0.00390625f, b1 = rintf((x1 - a1) * 256.f) * 0.00390625f;
-                        q1 += a0 + a1, q2 += b0 + b1;
-                        hi = pack_half2(a0 * mul, a1 * mul), lo = pack_half2(b0 * mul, b1 * mul);
-                    } else {
-                        hi = pack_half2(x0 * mul, x1 * mul);
-                    }
-                };
-                // operands of k-step k: codes (x0, x1) as they are, (y0, y1) 16-fold
-                auto put = [&](int k, float x0, float x1, float y0, float y1) {
-                    uint2 hi, lo;
-                    terms(x0, x1, 1.f, hi.x, lo.x);
-                    terms(y0, y1, 0.0625f, hi.y, lo.y);
-                    const int at = (t * KS + k) * QS;
-                    if constexpr (Sh::Q_SMEM) {
-                        qsm[at * 32] = hi;
-                        if (F32) qsm[(at + 1) * 32] = lo;
-                    } else {
-                        qreg[at] = hi;
-                        if (F32) qreg[at + QS - 1] = lo;
-                    }
-                };
-#pragma unroll
-                for (int i = 0; i < DK / 4; i++) v[i] = bad ? 0.f : v[i] * up;
-#pragma unroll
-                for (int w = 0; w < DK / 32; w++) {
-                    const float* y = v + 8 * w;
-                    put(2 * w, y[0], y[4], y[1], y[5]);
-                    put(2 * w + 1, y[2], y[6], y[3], y[7]);
-                }
-                if constexpr (DK == 48) put(2, v[8], v[10], v[9], v[11]);
-                const int hi = on ? (int)min(max(rows.pos0 + tok, -1LL), 0x7fffffffLL) : -1;
-                auto cols = [&](float x) { return pair(__shfl_sync(0xffffffffu, x, 8 * c), __shfl_sync(0xffffffffu, x, 8 * c + 4)); };
-                f0[t] = cols(fac0);
-                f1[t] = cols(fac1);
-                seen_hi[t][0] = __shfl_sync(0xffffffffu, hi, 8 * c);
-                seen_hi[t][1] = __shfl_sync(0xffffffffu, hi, 8 * c + 4);
-                if (F32) {  // -8 of the codes' unit, 2^-24
-                    q1 += __shfl_xor_sync(0xffffffffu, q1, 1);
-                    q2 += __shfl_xor_sync(0xffffffffu, q2, 1);
-                    q1 += __shfl_xor_sync(0xffffffffu, q1, 2);
-                    q2 += __shfl_xor_sync(0xffffffffu, q2, 2);
-                    mid[F32 ? t : 0][0] = cols(q1 * -4.76837158203125e-7f);
-                    mid[F32 ? t : 0][1] = cols(q2 * -4.76837158203125e-7f);
-                }
-            }
-            // tiles wholly inside every row's span need no masks
-            const int x_last = min((b + 1) * 8 * NT, nrows) - 1;
-            const long long p_first = rows.pos0 + a.group(b * 8 * NT), p_last = rows.pos0 + a.group(x_last);
-            const int all_hi = (int)min(max(p_first, -1LL), 0x7fffffffLL) - 15;              // whole: k0 <= all_hi and
-            const int all_lo = a.window > 0 ? (int)min(max(p_last - a.window, -1LL), 0x7fffffffLL) : -1;  // k0 > all_lo or k0 + 15 < sink
-
-            float acc[NT][MT][4];
-            f32x2 nM[NT], l[NT], mn[NT];  // -M, sum p, sum p mv for columns 2 c, 2 c + 1 (the sums over this lane's keys)
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[t][i][j] = 0.f;
-                nM[t] = pair(-ATT_LOW, -ATT_LOW);
-                l[t] = mn[t] = 0;
-            }
-
-            int k0 = tl.at(off) * KV4_TILE;
-            uint32_t get_at = 0;
-#pragma unroll 1
-            for (int i = 0; i < m; i++) {
-                asm volatile("cp.async.wait_group %0;\n" ::"n"(ATT_STAGES - 2) : "memory");
-                __syncwarp();
-                const bool page_ok = (ok_hist >> (ATT_STAGES - 2)) & 1;
-                issue();  // into the stage read in the last round
-                const uint8_t* tile = ring + get_at;
-                get_at = get_at == (ATT_STAGES - 1) * TB ? 0 : get_at + TB;
-
-                // scores: keys g and g + 8 against query rows 2 c, 2 c + 1
-                float sc[NT][4], sc2[F32 ? NT : 1][4];
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    if (F32) {
-                        const float2 x = unpair(mid[F32 ? t : 0][0]), y = unpair(mid[F32 ? t : 0][1]);
-                        sc[t][0] = sc[t][2] = x.x, sc[t][1] = sc[t][3] = x.y;
-                        sc2[F32 ? t : 0][0] = sc2[F32 ? t : 0][2] = y.x, sc2[F32 ? t : 0][1] = sc2[F32 ? t : 0][3] = y.y;
-                    } else {
-                        sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-                    }
-                }
-                auto qop = [&](int t, int k, int term) -> uint2 {
-                    const int at = (t * KS + k) * QS + term;
-                    if constexpr (Sh::Q_SMEM) return qsm[at * 32];
-                    else return qreg[at];
-                };
-                auto step = [&](int k, uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const uint2 o = qop(t, k, 0);
-                        mma16816(sc[t], x0, y0, x1, y1, o.x, o.y);
-                        if (F32) {
-                            const uint2 o2 = qop(t, k, QS - 1);
-                            mma16816(sc2[F32 ? t : 0], x0, y0, x1, y1, o2.x, o2.y);
-                        }
-                    }
-                };
-                const uint8_t *ka = tile + g * (DK / 2), *kb = tile + (g + 8) * (DK / 2);
-                uint32_t wa[DK / 32], wb[DK / 32];
-                if constexpr (DK == 128) {
-                    const uint4 x = *(const uint4*)(ka + 16 * c), y = *(const uint4*)(kb + 16 * c);
-                    wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
-                    wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
-                } else if constexpr (DK == 64) {
-                    const uint2 x = *(const uint2*)(ka + 8 * c), y = *(const uint2*)(kb + 8 * c);
-                    wa[0] = x.x, wa[1] = x.y;
-                    wb[0] = y.x, wb[1] = y.y;
-                } else {
-                    wa[0] = *(const uint32_t*)(ka + 4 * c);
-                    wb[0] = *(const uint32_t*)(kb + 4 * c);
-                }
-                const uint8_t* par = tile + 8 * (DK + DV) + 4 * g;
-                float2 kpa = unpack_half2(*(const uint32_t*)par), kpb = unpack_half2(*(const uint32_t*)(par + 32));
-                float2 vpa = unpack_half2(*(const uint32_t*)(par + 64)), vpb = unpack_half2(*(const uint32_t*)(par + 96));
-#pragma unroll
-                for (int w = 0; w < DK / 32; w++) {
-                    step(2 * w, wa[w] & 0x000f000fu, wa[w] & 0x00f000f0u, wb[w] & 0x000f000fu, wb[w] & 0x00f000f0u);
-                    const uint32_t xa = wa[w] >> 8, xb = wb[w] >> 8;
-                    step(2 * w + 1, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
-                }
-                if constexpr (DK == 48) {  // dimensions 32 .. 47: four codes a lane
-                    const uint32_t ha = *(const uint16_t*)(ka + 16 + 2 * c), hb = *(const uint16_t*)(kb + 16 + 2 * c);
-                    const uint32_t xa = __byte_perm(ha, 0, 0x4140), xb = __byte_perm(hb, 0, 0x4140);
-                    step(2, xa & 0x000f000fu, xa & 0x00f000f0u, xb & 0x000f000fu, xb & 0x00f000f0u);
-                }
-                if (F32) {  // the middle of the codes instead of the minimum
-                    kpa.y = __fmaf_rn(8.f, kpa.x, kpa.y), kpb.y = __fmaf_rn(8.f, kpb.x, kpb.y);
-                    vpa.y = __fmaf_rn(8.f, vpa.x, vpa.y), vpb.y = __fmaf_rn(8.f, vpb.x, vpb.y);
-                }
-                // a score may pass M by this much before M is raised
-                const float ta = 4.f - lg2(fmaxf(vpa.x, 5.9604645e-8f)), tb = 4.f - lg2(fmaxf(vpb.x, 5.9604645e-8f));
-                const bool whole = page_ok && k0 <= all_hi && (k0 > all_lo || k0 + 15 < a.sink);
-                const f32x2 ksa = pair(kpa.x, kpa.x), ksb = pair(kpb.x, kpb.x), kma = pair(kpa.y, kpa.y), kmb = pair(kpb.y, kpb.y);
-                f32x2 sa[NT], sb[NT];  // keys g, g + 8
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    sa[t] = pair(sc[t][0], sc[t][1]), sb[t] = pair(sc[t][2], sc[t][3]);
-                    if (F32) {
-                        sa[t] = add2(sa[t], pair(sc2[F32 ? t : 0][0], sc2[F32 ? t : 0][1]));
-                        sb[t] = add2(sb[t], pair(sc2[F32 ? t : 0][2], sc2[F32 ? t : 0][3]));
-                    }
-                    sa[t] = fma2(mul2(sa[t], f0[t]), ksa, mul2(f1[t], kma));
-                    sb[t] = fma2(mul2(sb[t], f0[t]), ksb, mul2(f1[t], kmb));
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        auto mask = [&](f32x2 x, int key) {
-                            float2 f = unpair(x);
-                            const bool in = page_ok, sunk = key < a.sink;
-                            if (!(in && key <= seen_hi[t][0] && (a.window <= 0 || sunk || key > seen_hi[t][0] - a.window))) f.x = -INFINITY;
-                            if (!(in && key <= seen_hi[t][1] && (a.window <= 0 || sunk || key > seen_hi[t][1] - a.window))) f.y = -INFINITY;
-                            return pair(f.x, f.y);
-                        };
-                        sa[t] = mask(sa[t], k0 + g);
-                        sb[t] = mask(sb[t], k0 + g + 8);
-                    }
-                }
-                bool raise = false;
-                float2 xa[NT], xb[NT];  // exponents
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    xa[t] = unpair(add2(sa[t], nM[t])), xb[t] = unpair(add2(sb[t], nM[t]));
-                    raise |= xa[t].x > ta || xa[t].y > ta || xb[t].x > tb || xb[t].y > tb;
-                }
-                if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        const float2 fa = unpair(sa[t]), fb = unpair(sb[t]), old = unpair(nM[t]);
-                        float m0 = fmaxf(-old.x, fmaxf(fa.x + (4.f - ta), fb.x + (4.f - tb)));
-                        float m1 = fmaxf(-old.y, fmaxf(fa.y + (4.f - ta), fb.y + (4.f - tb)));
-#pragma unroll
-                        for (int o = 4; o < 32; o *= 2) {
-                            m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                            m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-                        }
-                        const float r0 = ex2(-old.x - m0), r1 = ex2(-old.y - m1);
-                        const f32x2 r = pair(r0, r1);
-                        nM[t] = pair(-m0, -m1);
-                        l[t] = mul2(l[t], r);
-                        mn[t] = mul2(mn[t], r);
-#pragma unroll
-                        for (int k = 0; k < MT; k++) acc[t][k][0] *= r0, acc[t][k][1] *= r1, acc[t][k][2] *= r0, acc[t][k][3] *= r1;
-                        xa[t] = unpair(add2(sa[t], nM[t])), xb[t] = unpair(add2(sb[t], nM[t]));
-                    }
-                }
-                // weights, and their operands: rows of the transpose are query rows
-                uint32_t wop[NT][2][WS];
-                const f32x2 vsa = pair(vpa.x, vpa.x), vsb = pair(vpb.x, vpb.x), vma = pair(vpa.y, vpa.y), vmb = pair(vpb.y, vpb.y);
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const float2 ea = make_float2(ex2(xa[t].x), ex2(xa[t].y)), eb = make_float2(ex2(xb[t].x), ex2(xb[t].y));
-                    const f32x2 pa = pair(ea.x, ea.y), pb = pair(eb.x, eb.y);
-                    l[t] = add2(l[t], add2(pa, pb));
-                    float2 wa2, wb2;
-                    if (whole) {
-                        mn[t] = fma2(pa, vma, fma2(pb, vmb, mn[t]));
-                        wa2 = unpair(mul2(pa, vsa)), wb2 = unpair(mul2(pb, vsb));
-                    } else {  // a masked place may hold NaN or infinity
-                        float2 y = unpair(mn[t]);
-                        y.x = __fmaf_rn(ea.x, ea.x == 0.f ? 0.f : vpa.y, __fmaf_rn(eb.x, eb.x == 0.f ? 0.f : vpb.y, y.x));
-                        y.y = __fmaf_rn(ea.y, ea.y == 0.f ? 0.f : vpa.y, __fmaf_rn(eb.y, eb.y == 0.f ? 0.f : vpb.y, y.y));
-                        mn[t] = pair(y.x, y.y);
-                        wa2 = make_float2(ea.x == 0.f ? 0.f : ea.x * vpa.x, ea.y == 0.f ? 0.f : ea.y * vpa.x);
-                        wb2 = make_float2(eb.x == 0.f ? 0.f : eb.x * vpb.x, eb.y == 0.f ? 0.f : eb.y * vpb.x);
-                    }
-                    const uint32_t ha = pack_half2(wa2.x, wa2.y), hb = pack_half2(wb2.x, wb2.y);
-                    wop[t][0][0] = transpose8(ha), wop[t][1][0] = transpose8(hb);
-                    if (WS == 2) {
-                        const float2 ra = unpack_half2(ha), rb = unpack_half2(hb);
-                        wop[t][0][WS - 1] = transpose8(pack_half2(wa2.x - ra.x, wa2.y - ra.y));
-                        wop[t][1][WS - 1] = transpose8(pack_half2(wb2.x - rb.x, wb2.y - rb.y));
-                    }
-                }
-                // values: lane (g, c) holds dimensions 8 (VW g + w) .. + 7 of keys 2c, 2c+1, 2c+8, 2c+9
-                const uint8_t* vt = tile + 8 * DK + g * 4 * VW + c * DV;
-                uint32_t vw[4][VW];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint8_t* p = vt + ((j & 1) + (j >= 2 ? 8 : 0)) * (DV / 2);
-                    if constexpr (VW == 2) {
-                        const uint2 x = *(const uint2*)p;
-                        vw[j][0] = x.x, vw[j][1] = x.y;
-                    } else {
-                        vw[j][0] = *(const uint32_t*)p;
-                    }
-                }
-#pragma unroll
-                for (int w = 0; w < VW; w++)
-#pragma unroll
-                    for (int quarter = 0; quarter < 4; quarter++) {
-                        // dimensions 2 quarter (row g), 2 quarter + 1 (row g + 8)
-                        const uint32_t sel = quarter < 2 ? 0x5410 : 0x7632;
-                        const uint32_t x = __byte_perm(vw[0][w], vw[1][w], sel) >> (quarter & 1 ? 8 : 0);
-                        const uint32_t y = __byte_perm(vw[2][w], vw[3][w], sel) >> (quarter & 1 ? 8 : 0);
-                        uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
-                        if (F32) a0 = code_mid(a0), a1 = code16_mid(a1), a2 = code_mid(a2), a3 = code16_mid(a3);
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            float* d = acc[t][4 * w + quarter];
-                            if constexpr (F32) {
-                                float z[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                for (int term = 0; term < WS; term++) mma16816(z, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
-#pragma unroll
-                                for (int j = 0; j < 4; j++) d[j] += z[j];
-                            } else {
-#pragma unroll
-                                for (int term = 0; term < WS; term++) mma16816(d, a0, a1, a2, a3, wop[t][0][term], wop[t][1][term]);
-                            }
-                        }
-                    }
-                k0 = off + i + 1 == tl.sink ? tl.lo * KV4_TILE : k0 + KV4_TILE;
-            }
-            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-            __syncwarp();
-
-            // this run's part of the unit: sums over the keys' lanes, 2^24 back
+            const int m = (int)min((long long)(tl.n - off), end - cur);
             const bool starts = off == 0, ends = off + m == tl.n, done = starts && ends;
             float* part = MERGE ? (starts ? last_part : first_part) : a.parts + ((size_t)wid * 2 + (starts ? 1 : 0)) * PART;
-            const OutRows<T> to{out, a, rows.first, h, nrows};
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-#pragma unroll
-                for (int o = 4; o < 32; o *= 2) {
-                    l[t] = add2(l[t], __shfl_xor_sync(0xffffffffu, l[t], o));
-                    mn[t] = add2(mn[t], __shfl_xor_sync(0xffffffffu, mn[t], o));
-                }
-                const float2 l2 = unpair(l[t]), mn2 = unpair(mn[t]), M2 = unpair(nM[t]);
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float lj = j ? l2.y : l2.x, mj = j ? mn2.y : mn2.x;
-                    const int y = 8 * t + 2 * c + j, x = b * 8 * NT + y;  // query row in the block, in the sequence
-                    const float norm = done ? (lj == 0.f ? 0.f : 1.f / lj) : 1.f;
-#pragma unroll
-                    for (int w = 0; w < VW; w++) {
-                        float v[8];
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            v[2 * k] = __fmaf_rn(acc[t][4 * w + k][j], F32 ? 1.f : 16777216.f, mj) * norm;
-                            v[2 * k + 1] = __fmaf_rn(acc[t][4 * w + k][2 + j], F32 ? 1.f : 1048576.f, mj) * norm;
-                        }
-                        const int d0 = 8 * (VW * g + w);
-                        if (!done) store8(part + y * DV + d0, true, v);
-                        else if (x < nrows) store8(to.at(x) + d0, a.o_vec, v);
-                    }
-                    if (!done && g == 0) {
-                        part[8 * NT * DV + y] = j ? -M2.y : -M2.x;
-                        part[8 * NT * (DV + 1) + y] = lj;
-                    }
-                }
-            }
+            attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, off, m, mine, (uint2*)(mine + Sh::RING), done ? nullptr : part);
             if (!done && lane == 0) {
                 if (MERGE) {
                     if (starts) cut_start[warp] = make_int4(s, h, b, 1);
@@ -754,10 +862,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             }
 
             // the next unit
-            cur += a.whole ? 1 : m;
+            cur += m;
             if (cur >= end) break;
             off = 0;
-            if (++b * 8 * NT >= nrows) {
+            if (++b * 8 * NT >= rows.n * (int)a.group.d) {
                 b = 0;
                 if (++h == H) {
                     h = 0;
@@ -770,11 +878,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
     }
 
     if constexpr (MERGE) {
-        if (a.whole) return;
         __syncthreads();
         // A unit's parts in this CTA, from the warp where it starts (or warp
         // 0, if an earlier CTA has its start) to the one that ends it.
-        auto slot = [&](int w, bool start) { return (const float*)(smem + w * Sh::WARP_SMEM + (start ? 0 : Sh::RING)); };
+        auto slot = [&](int w, bool start) { return (const float*)(smem + w * Sh::WARP_SMEM + (start ? 0 : Sh::RING + Sh::QBYTES)); };
         auto chain = [&](bool start) {
             PartRegs<DV> sum, more;
             sum.load(slot(warp, start), g, c);
@@ -883,7 +990,7 @@ static AttendPlan attend_plan(const nd_kv4* kv, int group, int window, int sink)
     p.whole = tiles <= ATT_WHOLE_TILES;
     const long long units = kv->heads * ((long long)kv->rows * group / (8 * p.nt) + std::min(kv->seqs, kv->rows));
     const long long runs = p.whole ? units : (units * tiles + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
-    const int full = device_sm_count() * (p.nt == 1 ? 4 : p.nt == 2 ? 3 : 2);
+    const int full = device_sm_count() * ATT_CTAS(p.nt, kv->dv);
     p.ctas = (int)std::max(1LL, std::min<long long>(full, (runs + ATT_WARPS - 1) / ATT_WARPS));
     const size_t runners = (size_t)p.ctas * (p.nt == 1 ? 1 : ATT_WARPS);
     p.ws = p.whole ? 0 : runners * (sizeof(int4) + 2 * sizeof(float) * 8 * p.nt * (kv->dv + 2));
@@ -897,12 +1004,13 @@ static void attend_launch(const AttendArgs& a0, const AttendPlan& plan, const vo
     const int runners = plan.ctas * (Sh::MERGE ? 1 : ATT_WARPS);
     a.joins = (int4*)ws;
     a.parts = (float*)((char*)ws + (size_t)runners * sizeof(int4));
-    auto kernel = kv4_attend_kernel<DK, DV, NT, T>;
+    auto kernel = plan.whole ? kv4_attend_whole_kernel<DK, DV, NT, T> : kv4_attend_kernel<DK, DV, NT, T>;
+    const int smem = plan.whole ? Sh::WHOLE_SMEM : Sh::SMEM;
     auto check = [](cudaError_t e) {
         if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
     };
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
-    kernel<<<plan.ctas, 32 * ATT_WARPS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<plan.ctas, 32 * ATT_WARPS, smem, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
     if (plan.whole) return;
     // launched early where the stream allows it; it waits for the first kernel's results
@@ -984,7 +1092,6 @@ int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row,
         a.zero_rest = flags & ND_ZERO_REST;
         OnDevice on(kv->device, what);
         const AttendPlan plan = attend_plan(kv, group, window, sink);
-        a.whole = plan.whole;
         if (plan.ws && (!ws || ws_bytes < plan.ws)) fail("the workspace is too small");
         cudaStream_t st = (cudaStream_t)stream;
         if (kv->dk == 48) attend_type<48, 64>(type, a, plan, q, out, ws, st);

@@ -12,10 +12,16 @@
 // with the sum in f64. Only the one row a sequence draws from is summed in
 // f64 throughout.
 //
-// A cluster a sequence: its CTAs take the rows between them (one read of each
-// from HBM, which bounds the large calls), the verdicts meet in the first
-// CTA's shared memory, then all share the drawn row, in slices in order, so
-// that the prefix sums over slices, threads and values give the index.
+// Two kernels: one takes every row's statistics (one read of the logits, which
+// bounds the large calls: a CTA a row, or several where rows are few), the
+// second, a cluster of CTAs a sequence, decides and draws. There every warp
+// has a run of the drawn row: the runs' sums meet through the cluster's
+// shared memory, each CTA adds them up in order, and the warp whose run holds
+// the place walks it 32 values at a time.
+//
+// Measured (us, GPU alone; 256 sequences of up to 7 drafts, 16384 f32 logits,
+// 98 MB in all): one kernel with a CTA a row and f64 terms taken twice 236; as
+// it is now VERIFY_US.
 
 #include <cooperative_groups.h>
 
@@ -27,8 +33,21 @@ namespace nd {
 
 namespace cg = cooperative_groups;
 
-constexpr int VF_THREADS = 512, VF_MAX_DRAFT = 64;
+constexpr int VF_MAX_DRAFT = 64, VF_MAX_SEQS = 1 << 20;
+constexpr int VF_STATS = 256;        // threads of the first kernel
+constexpr int VF_CHUNK = 4096;       // logits a CTA of it takes at a time
+constexpr int VF_MAX_PARTS = 32;
+constexpr int VF_DRAW = 512, VF_WARPS = VF_DRAW / 32;
+constexpr int VF_CACHE = 512;        // f64 terms of its run that a warp keeps
 constexpr float LOG2E = 1.4426950408889634f;
+
+// Of a row, or a part of it: the largest logit, its first place (-1: a NaN is
+// there), and sum exp((l - top) / temperature).
+struct RowStats {
+    float top;
+    int at;
+    double sum;
+};
 
 struct VerifyArgs {
     long long l_seq, l_row, q_seq, q_row;
@@ -37,17 +56,11 @@ struct VerifyArgs {
     const float* u;         // [seqs][T + 1]
     const float* temp;      // [seqs]
     const float* q;         // or NULL
-    int seqs, T, V;
+    int seqs, T, V, parts;
     bool l_vec;
+    RowStats* stats;             // [seqs][T + 1][parts]
     int32_t *tokens, *accepted;  // [seqs][T + 1], [seqs]
     float* probs;                // [seqs][T + 1]
-};
-
-// A row's largest logit, its first place, and sum exp((l - top) / temperature).
-struct RowStats {
-    float top;
-    int at;       // -1: a NaN, or nothing above -infinity
-    double sum;
 };
 
 __device__ __forceinline__ float vf_ex2(float x) {
@@ -56,276 +69,349 @@ __device__ __forceinline__ float vf_ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ int drafts_of(const VerifyArgs& a, int s) { return a.counts ? min(max(__ldg(a.counts + s), 0), a.T) : a.T; }
+
+struct Temperature {
+    bool greedy;
+    double inv;
+    float scale2;  // of an exponent of two
+    __device__ explicit Temperature(float t) {
+        greedy = !(t > 0.f && LOG2E / t <= FLT_MAX);
+        inv = greedy ? 1.0 : 1.0 / (double)t;
+        scale2 = greedy ? LOG2E : LOG2E / t;
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, const T* __restrict__ logits) {
+    constexpr int PER = 16 / sizeof(T), LOADS = VF_CHUNK / VF_STATS / PER, N = LOADS * PER;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts, s = r / (a.T + 1), i = r % (a.T + 1), tid = threadIdx.x;
+    if (i > drafts_of(a, s)) return;
+    const float scale2 = Temperature(__ldg(a.temp + s)).scale2;
+    const T* row = logits + s * a.l_seq + i * a.l_row;
+    const int chunks = (a.V + VF_CHUNK - 1) / VF_CHUNK, per = (chunks + a.parts - 1) / a.parts;
+    const int lo = min(part * per, chunks), hi = min(lo + per, chunks);
+    float top = -INFINITY, sum = 0.f;
+    int at = a.V;
+    bool nan = false;
+    for (int ch = lo; ch < hi; ch++) {
+        float x[N];
+        const int base = ch * VF_CHUNK;
+        if (a.l_vec && base + VF_CHUNK <= a.V) {
+            uint4 raw[LOADS];
+#pragma unroll
+            for (int k = 0; k < LOADS; k++) raw[k] = __ldg((const uint4*)(row + base) + k * VF_STATS + tid);
+#pragma unroll
+            for (int k = 0; k < LOADS; k++) {
+                const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (sizeof(T) == 4) {
+                        x[4 * k + j] = __uint_as_float(w[j]);
+                    } else {
+                        const T* h = (const T*)&w[j];
+                        x[8 * k + 2 * j] = (float)h[0], x[8 * k + 2 * j + 1] = (float)h[1];
+                    }
+                }
+            }
+        } else {  // the same places one by one
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const int p = base + (j / PER * VF_STATS + tid) * PER + j % PER;
+                x[j] = p < a.V ? (float)row[p] : -INFINITY;
+            }
+        }
+        float m = top;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            nan |= x[j] != x[j];
+            if (x[j] > m) m = x[j], at = base + (j / PER * VF_STATS + tid) * PER + j % PER;
+        }
+        if (m == -INFINITY) continue;
+        if (m > top) sum *= vf_ex2((top - m) * scale2), top = m;  // top = -infinity: sum is 0
+#pragma unroll
+        for (int j = 0; j < N; j++) sum += vf_ex2((x[j] - top) * scale2);
+    }
+    // the block's largest, its first place, the sum against it
+    __shared__ float tops[VF_STATS / 32];
+    __shared__ int ats[VF_STATS / 32];
+    __shared__ double sums[VF_STATS / 32];
+    const int lane = tid & 31, warp = tid >> 5;
+    float m = top;
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, o);
+        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+        if (om > m || (om == m && oa < at)) m = om, at = oa;
+        nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
+    }
+    if (lane == 0) tops[warp] = m, ats[warp] = nan ? -1 : at;
+    __syncthreads();
+    m = tops[0], at = ats[0], nan = at < 0;
+#pragma unroll
+    for (int w = 1; w < VF_STATS / 32; w++) {
+        nan |= ats[w] < 0;
+        if (tops[w] > m || (tops[w] == m && ats[w] < at)) m = tops[w], at = ats[w];
+    }
+    double z = top == -INFINITY ? 0.0 : (double)sum * (double)vf_ex2((top - m) * scale2);
+#pragma unroll
+    for (int o = 16; o; o /= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if (lane == 0) sums[warp] = z;
+    __syncthreads();
+    if (tid == 0) {
+        z = 0.0;
+        for (int w = 0; w < VF_STATS / 32; w++) z += sums[w];
+        a.stats[blockIdx.x] = RowStats{m, nan ? -1 : at, z};
+    }
+}
+
 template <typename T>
 __device__ __forceinline__ double term(const T* row, int j, float top, double inv) {
     return exp(((double)(float)row[j] - (double)top) * inv);
 }
 
-__device__ __forceinline__ double block_sum(double x, double* red) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ double warp_sum(double x) {
 #pragma unroll
     for (int o = 16; o; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
-    __syncthreads();
-    if (lane == 0) red[warp] = x;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < VF_THREADS / 32; w++) s += red[w];
-    return s;
+    return x;
 }
 
-// One pass over a row by the CTA; every thread returns the result.
-template <typename T>
-__device__ RowStats row_stats(const T* row, int V, float scale2, bool vec, double* red, float* redf, int* redi) {
-    constexpr int PER = 16 / sizeof(T);
-    float top = -INFINITY, sum = 0.f;
-    int at = V;
-    bool nan = false;
-    auto take = [&](const float* x, int n, int j0) {
-        float m = top;
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (i < n) {
-                nan |= x[i] != x[i];
-                if (x[i] > m) m = x[i], at = j0 + i;
-            }
-        if (m > top) {
-            sum *= vf_ex2((top - m) * scale2);  // top = -infinity: sum is 0
-            top = m;
-        }
-        if (top == -INFINITY) return;
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (i < n) sum += vf_ex2((x[i] - top) * scale2);
-    };
-    if (vec) {
-        const int units = V / PER;
-        for (int k = threadIdx.x; k < units; k += VF_THREADS) {
-            float x[8];
-            if constexpr (sizeof(T) == 4) {
-                const float4 f = __ldg((const float4*)row + k);
-                x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-            } else {
-                load8(row + 8 * k, true, x);
-            }
-            take(x, PER, k * PER);
-        }
-        for (int j = units * PER + threadIdx.x; j < V; j += VF_THREADS) {
-            const float x[8] = {(float)row[j]};
-            take(x, 1, j);
-        }
-    } else {
-        for (int j = threadIdx.x; j < V; j += VF_THREADS) {
-            const float x[8] = {(float)row[j]};
-            take(x, 1, j);
-        }
-    }
-    // the block's largest, the first place that has it
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float m = top;
-    int place = at;
+// A row's statistics from its parts, in their order; at < 0 where it is no
+// distribution. For a whole warp.
+__device__ __forceinline__ RowStats join_stats(const RowStats* parts, int n, float scale2, int lane) {
+    RowStats r{-INFINITY, 0x7fffffff, 0.0};
+    if (lane < n) r = parts[lane];
+    float m = r.top;
+    int at = r.at;
+    bool nan = r.at < 0;
 #pragma unroll
     for (int o = 16; o; o /= 2) {
         const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        const int op = __shfl_xor_sync(0xffffffffu, place, o);
-        if (om > m || (om == m && op < place)) m = om, place = op;
+        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+        if (om > m || (om == m && oa < at)) m = om, at = oa;
         nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
     }
-    __syncthreads();
-    if (lane == 0) redf[warp] = m, redi[warp] = nan ? -1 : place;
-    __syncthreads();
-    m = redf[0], place = redi[0];
-    nan = place < 0;
-    for (int w = 1; w < VF_THREADS / 32; w++) {
-        nan |= redi[w] < 0;
-        if (redf[w] > m || (redf[w] == m && redi[w] < place)) m = redf[w], place = redi[w];
-    }
-    RowStats r;
-    r.top = m;
-    r.at = nan || m == -INFINITY ? -1 : place;
-    r.sum = block_sum(top == -INFINITY ? 0.0 : (double)sum * (double)vf_ex2((top - m) * scale2), red);
-    return r;
+    RowStats out{m, nan || m == -INFINITY ? -1 : at, 0.0};
+    out.sum = warp_sum(r.top == -INFINITY ? 0.0 : r.sum * (double)vf_ex2((r.top - m) * scale2));
+    return out;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(VF_THREADS) verify_kernel(VerifyArgs a, const T* __restrict__ logits) {
+__global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, const T* __restrict__ logits) {
     cg::cluster_group cluster = cg::this_cluster();
     const int C = cluster.num_blocks(), rank = cluster.block_rank(), s = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    __shared__ double red[VF_THREADS / 32];
-    __shared__ float redf[VF_THREADS / 32];
-    __shared__ int redi[VF_THREADS / 32];
-    // of the first CTA: each row's verdict and statistics, met through the cluster
-    __shared__ int ok[VF_MAX_DRAFT + 1];
-    __shared__ float tops[VF_MAX_DRAFT + 1], probs[VF_MAX_DRAFT + 1];
-    __shared__ int places[VF_MAX_DRAFT + 1];
-    __shared__ double part[2];      // this CTA's sum of exponentials, of the residual
-    __shared__ int found, last;     // the drawn place (of the first CTA); the last place that could be drawn
-    const int T_ = a.T, V = a.V, n = min(max(a.counts ? __ldg(a.counts + s) : T_, 0), T_);
-    const float temp = __ldg(a.temp + s);
-    const bool greedy = !(temp > 0.f && LOG2E / temp <= FLT_MAX);
-    const double inv = greedy ? 1.0 : 1.0 / (double)temp;
-    const float scale2 = greedy ? LOG2E : LOG2E / temp;
+    __shared__ RowStats rows[VF_MAX_DRAFT + 1];
+    __shared__ int verdict[VF_MAX_DRAFT + 1];  // 0 refused, 1 accepted, 2 too close to say
+    __shared__ double probs[VF_MAX_DRAFT + 1];
+    __shared__ double sums[2][VF_WARPS];  // by warp: of its run's terms, of its residuals
+    __shared__ double all[8 * VF_WARPS];  // those of every run
+    extern __shared__ double cache_all[];
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const int T_ = a.T, V = a.V, n = drafts_of(a, s);
+    const Temperature tp(__ldg(a.temp + s));
     const float* u = a.u + (size_t)s * (T_ + 1);
-    const T* rows = logits + s * a.l_seq;
-    if (tid == 0) found = V, last = -1;
-    int* ok0 = cluster.map_shared_rank(ok, 0);
-    float *tops0 = cluster.map_shared_rank(tops, 0), *probs0 = cluster.map_shared_rank(probs, 0);
-    int* places0 = cluster.map_shared_rank(places, 0);
-    cluster.sync();
+    const T* l0 = logits + s * a.l_seq;
 
-    for (int i = rank; i <= n; i += C) {
-        const T* row = rows + i * a.l_row;
-        const RowStats st = row_stats(row, V, scale2, a.l_vec, red, redf, redi);
-        bool take = false;
-        double p = 0.0;
-        if (i < n && st.at >= 0) {
-            const int x = __ldg(a.draft + (size_t)s * T_ + i);
-            if (x >= 0 && x < V) {
-                const double uq = (double)__ldg(u + i) * (a.q ? (double)__ldg(a.q + s * a.q_seq + i * a.q_row + x) : 1.0);
-                if (greedy) {
-                    p = x == st.at;
-                    take = uq < p;
-                } else {
-                    const double e = term(row, x, st.top, inv);
-                    double z = st.sum;
-                    if (fabs(uq * z - e) <= 1e-4 * (fabs(uq * z) + e)) {  // every thread sees the same values
-                        double mine = 0.0;
-                        for (int j = tid; j < V; j += VF_THREADS) mine += term(row, j, st.top, inv);
-                        z = block_sum(mine, red);
-                    }
-                    p = e / z;
-                    take = uq < p;
-                }
-            }
+    // p of a drafted token and its verdict, given the row's sum
+    auto judge = [&](int i, const RowStats& st, bool sure, double* p) -> int {
+        *p = 0.0;
+        const int x = __ldg(a.draft + (size_t)s * T_ + i);
+        if (st.at < 0 || x < 0 || x >= V) return 0;
+        const double uq = (double)__ldg(u + i) * (a.q ? (double)__ldg(a.q + s * a.q_seq + i * a.q_row + x) : 1.0);
+        if (tp.greedy) {
+            *p = x == st.at;
+            return uq < *p;
         }
-        if (tid == 0) ok0[i] = take, tops0[i] = st.top, places0[i] = st.at, probs0[i] = (float)p;
-        __syncthreads();
+        const double e = term(l0 + i * a.l_row, x, st.top, tp.inv);
+        *p = e / st.sum;
+        if (!sure && fabs(uq * st.sum - e) <= 1e-4 * (fabs(uq * st.sum) + e)) return 2;
+        return uq < *p;
+    };
+    for (int i = warp; i <= n; i += VF_WARPS) {
+        const RowStats st = join_stats(a.stats + ((size_t)s * (T_ + 1) + i) * a.parts, a.parts, tp.scale2, lane);
+        if (lane == 0) {
+            rows[i] = st;
+            if (i < n) verdict[i] = judge(i, st, false, &probs[i]);
+        }
     }
-    cluster.sync();
+    __syncthreads();
     int kept = 0;
-    while (kept < n && ok0[kept]) kept++;
-    const float top = tops0[kept];
-    const int place = places0[kept];
-
-    // the drawn row
-    int token = -1;
-    float prob = 0.f;
-    if (place >= 0 && greedy) {
-        // p is one at `place`; what q takes from it leaves it the only token
-        token = place;
-        prob = 1.f;
-    } else if (place >= 0) {
-        const T* row = rows + kept * a.l_row;
-        const float* q = kept < n && a.q ? a.q + s * a.q_seq + kept * a.q_row : nullptr;
-        const int gone = kept < n && !a.q ? __ldg(a.draft + (size_t)s * T_ + kept) : -1;
-        const int per = (V + C * VF_THREADS - 1) / (C * VF_THREADS);
-        const int lo = min((rank * VF_THREADS + tid) * per, V), hi = min(lo + per, V);
-        double mine = 0.0;
-        for (int j = lo; j < hi; j++) mine += term(row, j, top, inv);
-        const double slice = block_sum(mine, red);
-        if (tid == 0) part[0] = slice;
-        cluster.sync();
-        double z = 0.0;
-        for (int r = 0; r < C; r++) z += *cluster.map_shared_rank(part, r);
-        const double iz = 1.0 / z;
-        bool whole = false;  // p itself, where the residual is all zero
-        double total, before, own;
-        int top_place;
-        auto weight = [&](int j) {
-            const double p = term(row, j, top, inv) * iz;
-            if (whole) return p;
-            if (q) {
-                const double r = p - (double)__ldg(q + j);
-                return r < 0.0 ? 0.0 : r;
-            }
-            return j == gone ? 0.0 : p;
-        };
-        while (true) {
-            own = 0.0, top_place = -1;
-            for (int j = lo; j < hi; j++) {
-                const double w = weight(j);
-                own += w;
-                if (w > 0.0) top_place = j;
-            }
-            // what lies before this thread's slice, and in all
-            double incl = own;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double up = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += up;
-            }
-            before = __shfl_up_sync(0xffffffffu, incl, 1);
-            if (lane == 0) before = 0.0;
+    for (; kept < n; kept++) {
+        int v = verdict[kept];
+        if (v == 2) {  // the same for every thread: the row's sum in f64
+            RowStats st = rows[kept];
+            double z = 0.0;
+            for (int j = tid; j < V; j += VF_DRAW) z += term(l0 + kept * a.l_row, j, st.top, tp.inv);
+            z = warp_sum(z);
+            if (lane == 0) sums[0][warp] = z;
             __syncthreads();
-            if (lane == 31) red[warp] = incl;
+            st.sum = 0.0;
+            for (int w = 0; w < VF_WARPS; w++) st.sum += sums[0][w];
+            double p;
+            v = judge(kept, st, true, &p);
             __syncthreads();
-            double all = 0.0;
-            for (int w = 0; w < VF_THREADS / 32; w++) {
-                if (w == warp) before += all;
-                all += red[w];
-            }
-            if (tid == 0) part[1] = all;
-            cluster.sync();
-            total = 0.0;
-            for (int r = 0; r < C; r++) {
-                if (r == rank) before += total;
-                total += cluster.map_shared_rank(part, r)[1];
-            }
-            if (total != 0.0 || whole) break;
-            whole = true;
-            cluster.sync();
+            if (tid == 0) probs[kept] = p;
         }
-        if (total > 0.0) {
-            const double target = fmin(fmax((double)__ldg(u + T_), 0.0), 1.0) * total;
-            // the first value at which the running sum passes the target; threads
-            // just behind it look too, in case a slice's sum and the next one's
-            // start differ in the last bit
-            if (top_place >= 0 && before <= target * (1.0 + 1e-9) && before + own > target * (1.0 - 1e-9)) {
-                double cum = before;
-                for (int j = lo; j < hi; j++) {
-                    const double w = weight(j);
-                    cum += w;
-                    if (w > 0.0 && cum > target) {
-                        atomicMin(cluster.map_shared_rank(&found, 0), j);
-                        break;
-                    }
-                }
-            }
-            if (top_place >= 0) atomicMax(&last, top_place);
-            cluster.sync();
-            token = *cluster.map_shared_rank(&found, 0);
-            if (token >= V) {  // u is 1, or the last bits differ at the very end
-                token = -1;
-                for (int r = 0; r < C; r++) token = max(token, *cluster.map_shared_rank(&last, r));
-            }
-            if (token >= 0) prob = (float)(term(row, token, top, inv) * iz);
-        } else {
-            cluster.sync();
-        }
+        if (v == 0) break;
     }
-    if (rank == 0)
-        for (int i = tid; i <= T_; i += VF_THREADS) {
-            const size_t o = (size_t)s * (T_ + 1) + i;
-            a.tokens[o] = i < kept ? __ldg(a.draft + (size_t)s * T_ + i) : i == kept ? token : -1;
-            a.probs[o] = i < kept ? probs[i] : i == kept ? prob : 0.f;
+    __syncthreads();
+
+    const size_t o = (size_t)s * (T_ + 1);
+    auto finish = [&](int token, double p) { a.tokens[o + kept] = token, a.probs[o + kept] = (float)p; };
+    if (rank == 0) {
+        for (int i = tid; i <= T_; i += VF_DRAW) {
+            if (i == kept) continue;
+            a.tokens[o + i] = i < kept ? __ldg(a.draft + (size_t)s * T_ + i) : -1;
+            a.probs[o + i] = i < kept ? (float)probs[i] : 0.f;
         }
-    if (rank == 0 && tid == 0) a.accepted[s] = kept;
-    cluster.sync();  // no CTA leaves while others read its shared memory
+        if (tid == 0) a.accepted[s] = kept;
+    }
+    const RowStats st = rows[kept];
+    if (st.at < 0 || tp.greedy) {
+        // no distribution; or one at st.at, which what q takes from it leaves the only token
+        if (rank == 0 && tid == 0) finish(st.at, st.at < 0 ? 0.0 : 1.0);
+        return;
+    }
+
+    // the drawn row: this warp's run, its terms kept where they fit
+    const T* row = l0 + kept * a.l_row;
+    const float* q = kept < n && a.q ? a.q + s * a.q_seq + kept * a.q_row : nullptr;
+    const int gone = kept < n && !a.q ? __ldg(a.draft + (size_t)s * T_ + kept) : -1;
+    const int runs = C * VF_WARPS, run = rank * VF_WARPS + warp;
+    const int per = ((V + runs - 1) / runs + 31) / 32 * 32, lo = (int)min((long long)run * per, (long long)V), hi = min(lo + per, V);
+    double* cache = cache_all + warp * VF_CACHE;
+    double mine = 0.0;
+#pragma unroll 4
+    for (int j = lo + lane; j < hi; j += 32) {
+        const double e = term(row, j, st.top, tp.inv);
+        if (j - lo < VF_CACHE) cache[j - lo] = e;
+        mine += e;
+    }
+    mine = warp_sum(mine);
+    if (lane == 0) sums[0][warp] = mine;
+    // every run's sum from its CTA: lane l of each warp gets those of runs
+    // 4 l .., what lies before them, and the whole
+    double v[4], ahead;
+    auto gather = [&](int which) {
+        cluster.sync();
+        if (tid < 8 * VF_WARPS) all[tid] = tid < runs ? cluster.map_shared_rank(&sums[which][0], tid / VF_WARPS)[tid % VF_WARPS] : 0.0;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = all[4 * lane + k];
+        const double own = (v[0] + v[1]) + (v[2] + v[3]);
+        double incl = own;
+#pragma unroll
+        for (int k = 1; k < 32; k *= 2) {
+            const double up = __shfl_up_sync(0xffffffffu, incl, k);
+            if (lane >= k) incl += up;
+        }
+        ahead = __shfl_up_sync(0xffffffffu, incl, 1);
+        if (lane == 0) ahead = 0.0;
+        return __shfl_sync(0xffffffffu, incl, 31);
+    };
+    const double iz = 1.0 / gather(0);
+    bool whole = false;  // p itself, where the residual is all zero
+    auto weight = [&](int j) {
+        const double p = (j - lo < VF_CACHE ? cache[j - lo] : term(row, j, st.top, tp.inv)) * iz;
+        if (whole) return p;
+        if (q) {
+            const double r = p - (double)__ldg(q + j);
+            return r < 0.0 ? 0.0 : r;
+        }
+        return j == gone ? 0.0 : p;
+    };
+    double total;
+    while (true) {
+        mine = 0.0;
+#pragma unroll 4
+        for (int j = lo + lane; j < hi; j += 32) mine += weight(j);
+        mine = warp_sum(mine);
+        if (lane == 0) sums[1][warp] = mine;
+        total = gather(1);
+        if (total != 0.0 || whole) break;
+        whole = true;
+        cluster.sync();  // the others have read the sums
+    }
+    if (total > 0.0) {
+        // the first run in which the running sum passes the target, or where
+        // none does (u is 1) the last that has something to draw
+        const double target = fmin(fmax((double)__ldg(u + T_), 0.0), 1.0) * total;
+        double cum = ahead, before = 0.0, last_before = 0.0;
+        int at = -1, last = -1;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (v[k] > 0.0) {
+                last = 4 * lane + k, last_before = cum;
+                if (at < 0 && cum + v[k] > target) at = last, before = cum;
+            }
+            cum += v[k];
+        }
+        const uint32_t hits = __ballot_sync(0xffffffffu, at >= 0), some = __ballot_sync(0xffffffffu, last >= 0);
+        const bool passed = hits != 0;
+        const int from = passed ? __ffs(hits) - 1 : 31 - __clz(some);
+        at = __shfl_sync(0xffffffffu, passed ? at : last, from);
+        before = __shfl_sync(0xffffffffu, passed ? before : last_before, from);
+        if (at == run) {
+            int token = -1;
+            for (int j0 = lo; j0 < hi; j0 += 32) {
+                const double w = j0 + lane < hi ? weight(j0 + lane) : 0.0;
+                double incl = w;
+#pragma unroll
+                for (int k = 1; k < 32; k *= 2) {
+                    const double up = __shfl_up_sync(0xffffffffu, incl, k);
+                    if (lane >= k) incl += up;
+                }
+                const uint32_t some = __ballot_sync(0xffffffffu, w > 0.0);
+                const uint32_t past = __ballot_sync(0xffffffffu, w > 0.0 && before + incl > target);
+                if (some) token = j0 + 31 - __clz(some);  // should the sums' last bits differ: the last one
+                if (passed && past) {
+                    token = j0 + __ffs(past) - 1;
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0) finish(token, term(row, token, st.top, tp.inv) * iz);
+        }
+    } else if (rank == 0 && tid == 0) {
+        finish(-1, 0.0);
+    }
+    cluster.sync();  // no CTA leaves while others read its sums
+}
+
+static int verify_parts(int seqs, int T, int V) {
+    // few rows: enough CTAs for the GPU, a chunk each at least
+    const long long rows = (long long)seqs * (T + 1), chunks = (V + VF_CHUNK - 1) / VF_CHUNK;
+    return (int)std::max(1LL, std::min({chunks, (long long)VF_MAX_PARTS, 592 / rows}));
+}
+
+static unsigned long long verify_ws(int seqs, int T, int V) {
+    return (unsigned long long)seqs * (T + 1) * verify_parts(seqs, T, V) * sizeof(RowStats);
 }
 
 template <typename T>
 static void verify_launch(const VerifyArgs& a, const void* logits, int ctas, cudaStream_t st) {
+    auto check = [](cudaError_t e) {
+        if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_verify: ") + cudaGetErrorString(e));
+    };
+    verify_stats_kernel<T><<<(unsigned)a.seqs * (a.T + 1) * a.parts, VF_STATS, 0, st>>>(a, (const T*)logits);
+    op_launched("nd_op_verify");
+    constexpr int SMEM = VF_WARPS * VF_CACHE * sizeof(double);
+    check(cudaFuncSetAttribute(verify_draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)a.seqs * ctas);
-    cfg.blockDim = dim3(VF_THREADS);
+    cfg.blockDim = dim3(VF_DRAW);
+    cfg.dynamicSmemBytes = SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = ctas, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<T>, VerifyArgs(a), (const T*)logits);
-    if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_verify: ") + cudaGetErrorString(e));
+    cfg.numAttrs = st ? 2 : 1;
+    check(cudaLaunchKernelEx(&cfg, verify_draw_kernel<T>, VerifyArgs(a), (const T*)logits));
     add_launches(1);
 }
 
@@ -333,31 +419,43 @@ static void verify_launch(const VerifyArgs& a, const void* logits, int ctas, cud
 
 using namespace nd;
 
-extern "C" int nd_op_verify(int device, int type, const void* logits, long long l_seq, long long l_row, const int* draft,
-                            const int* counts, const float* u, const float* temperature, const float* q, long long q_seq,
-                            long long q_row, int seqs, int T, int V, int* tokens, int* accepted, float* probs, void* stream) {
+extern "C" {
+
+unsigned long long nd_op_verify_ws(int seqs, int T, int V) {
+    return seqs < 1 || seqs > VF_MAX_SEQS || T < 0 || T > VF_MAX_DRAFT || V < 1 ? 0 : verify_ws(seqs, T, V);
+}
+
+int nd_op_verify(int device, int type, const void* logits, long long l_seq, long long l_row, const int* draft,
+                 const int* counts, const float* u, const float* temperature, const float* q, long long q_seq, long long q_row,
+                 int seqs, int T, int V, int* tokens, int* accepted, float* probs, void* ws, unsigned long long ws_bytes,
+                 void* stream) {
     return op_call([&] {
         const char* what = "nd_op_verify";
         auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
         if (type != ND_F32 && type != ND_F16 && type != ND_BF16) fail("unknown type");
-        if (seqs < 1 || seqs > 1 << 20 || T < 0 || T > VF_MAX_DRAFT || V < 1) fail("needs 1 to 2^20 sequences, 0 to 64 drafted tokens, V >= 1");
+        if (seqs < 1 || seqs > VF_MAX_SEQS || T < 0 || T > VF_MAX_DRAFT || V < 1)
+            fail("needs 1 to 2^20 sequences, 0 to 64 drafted tokens, V >= 1");
         if (!logits || !u || !temperature || !tokens || !accepted || !probs || (T && !draft)) fail("null pointer");
         const int e = type == ND_F32 ? 4 : 2;
         if ((uintptr_t)logits % e || (uintptr_t)q % 4) fail("logits and q must be aligned to their types");
         if (l_seq < 0 || l_row < 0 || q_seq < 0 || q_row < 0) fail("negative strides");
+        if (!ws || (uintptr_t)ws % 16 || ws_bytes < verify_ws(seqs, T, V)) fail("the workspace is too small or not 16-byte aligned");
         VerifyArgs a{};
         a.l_seq = l_seq, a.l_row = l_row, a.q_seq = q_seq, a.q_row = q_row;
         a.draft = draft, a.counts = counts, a.u = u, a.temp = temperature, a.q = T ? q : nullptr;
-        a.seqs = seqs, a.T = T, a.V = V;
+        a.seqs = seqs, a.T = T, a.V = V, a.parts = verify_parts(seqs, T, V);
         a.l_vec = (uintptr_t)logits % 16 == 0 && l_seq * e % 16 == 0 && l_row * e % 16 == 0;
+        a.stats = (RowStats*)ws;
         a.tokens = tokens, a.accepted = accepted, a.probs = probs;
         OnDevice on(device, what);
-        // a CTA a row up to eight; more where there are few sequences, to share the drawn row
+        // CTAs a drawn row: until they fill the GPU or a warp's run is short
         int ctas = 1;
-        while (ctas < 8 && (ctas < T + 1 || seqs * 2 * ctas <= device_sm_count())) ctas *= 2;
+        while (ctas < 8 && seqs * ctas < 2 * device_sm_count() && V > 1024 * ctas) ctas *= 2;
         cudaStream_t st = (cudaStream_t)stream;
         if (type == ND_F32) verify_launch<float>(a, logits, ctas, st);
         else if (type == ND_F16) verify_launch<__half>(a, logits, ctas, st);
         else verify_launch<__nv_bfloat16>(a, logits, ctas, st);
     });
 }
+
+}  // extern "C"

@@ -22,7 +22,8 @@ SIGNATURES = {
     "nd_op_pages_fork": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _U, _P]),
     "nd_op_pages_compact_ws": (_U, [_I]),
     "nd_op_pages_compact": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _U, _P]),
-    "nd_op_verify": (_I, [_I, _I, _P, _L, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _P, _P, _P, _P]),
+    "nd_op_verify_ws": (_U, [_I, _I, _I]),
+    "nd_op_verify": (_I, [_I, _I, _P, _L, _L, _P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _P, _P, _P, _P, _U, _P]),
     "nd_op_kv4_append": (_I, [_P, _I, _P, _L, _L, _P, _L, _L, _P]),
     "nd_op_kv4_read": (_I, [_P, _I, _P, _L, _L, _P, _L, _L, _I, _P]),
     "nd_op_kv4_attend_ws": (_U, [_P, _I, _I, _I]),

@@ -24,7 +24,9 @@ _ZERO_REST = 2
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The address of the device's current stream (without the object that
+    torch.cuda.current_stream makes of it, 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _int32(t, n, device, name):
@@ -244,8 +246,11 @@ def op_verify(logits, draft, u, temperature, q=None, counts=None):
     accepted = torch.empty(s, dtype=torch.int32, device=dev)
     probs = torch.empty((s, t1), dtype=torch.float32, device=dev)
     qa = (None, 0, 0) if q is None or not t else (q.data_ptr(), q.stride(0), q.stride(1))
-    if lib().nd_op_verify(dev.index, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
-                          draft.data_ptr(), c, u.data_ptr(), temperature.data_ptr(), *qa, s, t, v, tokens.data_ptr(),
-                          accepted.data_ptr(), probs.data_ptr(), _stream(dev)) != 0:
+    L = lib()
+    size = L.nd_op_verify_ws(s, t, v)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    if L.nd_op_verify(dev.index, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
+                      draft.data_ptr(), c, u.data_ptr(), temperature.data_ptr(), *qa, s, t, v, tokens.data_ptr(),
+                      accepted.data_ptr(), probs.data_ptr(), ws.data_ptr(), size, _stream(dev)) != 0:
         raise _err()
     return tokens, accepted, probs

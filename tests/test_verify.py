@@ -248,10 +248,11 @@ def test_entry_point_refuses_without_a_gpu():
 
     lib = nb.lib()
 
-    def verify(type=0, logits=4096, row=50, draft=4096, q=None, seqs=1, T=2, V=50, tokens=4096):
-        return lib.nd_op_verify(0, type, logits, 150, row, draft, None, 4096, 4096, q, 100, 50, seqs, T, V, tokens, 4096, 4096, None)
+    def verify(type=0, logits=4096, row=50, draft=4096, q=None, seqs=1, T=2, V=50, tokens=4096, ws=4096, nbytes=1 << 20):
+        return lib.nd_op_verify(0, type, logits, 150, row, draft, None, 4096, 4096, q, 100, 50, seqs, T, V, tokens, 4096, 4096, ws,
+                                nbytes, None)
 
     for bad, message in ((dict(type=3), b"type"), (dict(logits=None), b"null"), (dict(logits=4098), b"aligned"), (dict(q=4097), b"aligned"),
                          (dict(row=-1), b"negative"), (dict(draft=None), b"null"), (dict(seqs=0), b"sequences"),
-                         (dict(T=65), b"64"), (dict(T=-1), b"64"), (dict(V=0), b"V >= 1"), (dict(tokens=None), b"null")):
+                         (dict(T=65), b"64"), (dict(T=-1), b"64"), (dict(V=0), b"V >= 1"), (dict(tokens=None), b"null"), (dict(ws=None), b"workspace"), (dict(nbytes=8), b"workspace")):
         assert verify(**bad) == -1 and message in lib.nd_last_error(), bad
