@@ -56,7 +56,11 @@ constexpr int ATT_KT(int nt) { return nt == 4 ? 1 : 2; }
 constexpr int ATT_STAGES(int nt) { return nt == 4 ? 4 : 3; }
 constexpr int ATT_CTAS(int nt, int dv) { return nt == 4 ? 2 : nt == 2 || dv == 128 ? 3 : 4; }  // an SM
 // Tiles: a shorter run of a cut unit costs more to join than it takes.
-constexpr int ATT_MIN_SHARE = 4;
+constexpr int ATT_MIN_SHARE = 8;
+// What beginning and ending a unit costs a warp, in tiles: without it a warp
+// that meets many short units is the last by far (8 sequences, one of a
+// single position among lengths up to 32768: 70 us instead of UNIT_US).
+constexpr int ATT_UNIT_COST = 4;
 // A call whose units all have at most this many tiles deals whole units out
 // to the warps and needs no second kernel.
 constexpr int ATT_WHOLE_TILES = 16;
@@ -146,12 +150,13 @@ __device__ __forceinline__ Tiles block_tiles(const AttendArgs& a, const SeqRows&
     return tiles_of(a, r.pos0 + a.group(x0), r.pos0 + a.group(x1));
 }
 
-// What a sequence and kv head adds to the list of work: its tiles.
+// What a sequence and kv head adds to the list of work: each unit its cost
+// and then its tiles.
 template <int NT>
 __device__ __forceinline__ long long seq_work(const AttendArgs& a, const SeqRows& r) {
     const int blocks = (r.n * (int)a.group.d + 8 * NT - 1) / (8 * NT);
     long long t = 0;
-    for (int b = 0; b < blocks; b++) t += block_tiles<NT>(a, r, b).n;
+    for (int b = 0; b < blocks; b++) t += block_tiles<NT>(a, r, b).n + ATT_UNIT_COST;
     return t;
 }
 
@@ -836,25 +841,28 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         int h = (int)(rem / per_head), b = 0;
         rem -= h * per_head;
         Tiles tl = block_tiles<NT>(a, rows, b);
-        while (rem >= tl.n) {
-            rem -= tl.n;
+        while (rem >= tl.n + ATT_UNIT_COST) {
+            rem -= tl.n + ATT_UNIT_COST;
             tl = block_tiles<NT>(a, rows, ++b);
         }
-        int off = (int)rem;
+        int at = (int)rem;  // place in the unit: its cost, then its tiles
 
         long long cur = begin;
         while (true) {
-            const int m = (int)min((long long)(tl.n - off), end - cur);
+            const int span = (int)min((long long)(tl.n + ATT_UNIT_COST - at), end - cur);
+            const int off = max(at - ATT_UNIT_COST, 0), m = max(at + span - ATT_UNIT_COST, 0) - off;
             const bool starts = off == 0, ends = off + m == tl.n, done = starts && ends;
-            float* part = MERGE ? (starts ? last_part : first_part) : a.parts + ((size_t)wid * 2 + (starts ? 1 : 0)) * PART;
-            attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, off, m, mine, (uint2*)(mine + Sh::RING), done ? nullptr : part);
-            if (!done && lane == 0) {
+            if (m) {
+                float* part = MERGE ? (starts ? last_part : first_part) : a.parts + ((size_t)wid * 2 + (starts ? 1 : 0)) * PART;
+                attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, off, m, mine, (uint2*)(mine + Sh::RING), done ? nullptr : part);
+            }
+            if (m && !done && lane == 0) {
                 if (MERGE) {
                     if (starts) cut_start[warp] = make_int4(s, h, b, 1);
                     else cut_rest[warp] = ends ? 2 : 1;
                 }
                 if (starts) {
-                    const long long last = (cur + tl.n - 1) / share;  // the warp that ends the unit
+                    const long long last = (cur - at + tl.n + ATT_UNIT_COST - 1) / share;  // the warp that ends the unit
                     const int runner = MERGE ? blockIdx.x : wid, further = (int)((MERGE ? last / ATT_WARPS : last) - runner);
                     if (!MERGE) a.joins[wid] = make_int4(s, h, b, further);
                     else cut_start[warp].w = 1 + further;
@@ -862,9 +870,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             }
 
             // the next unit
-            cur += m;
+            cur += span;
             if (cur >= end) break;
-            off = 0;
+            at = 0;
             if (++b * 8 * NT >= rows.n * (int)a.group.d) {
                 b = 0;
                 if (++h == H) {
@@ -989,7 +997,7 @@ static AttendPlan attend_plan(const nd_kv4* kv, int group, int window, int sink)
     if (window > 0) tiles = std::min(table, ((long long)window + 8 * p.nt + 2 * KV4_TILE) / KV4_TILE + (sink + KV4_TILE - 1LL) / KV4_TILE);
     p.whole = tiles <= ATT_WHOLE_TILES;
     const long long units = kv->heads * ((long long)kv->rows * group / (8 * p.nt) + std::min(kv->seqs, kv->rows));
-    const long long runs = p.whole ? units : (units * tiles + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
+    const long long runs = p.whole ? units : (units * (tiles + ATT_UNIT_COST) + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
     const int full = device_sm_count() * ATT_CTAS(p.nt, kv->dv);
     p.ctas = (int)std::max(1LL, std::min<long long>(full, (runs + ATT_WARPS - 1) / ATT_WARPS));
     const size_t runners = (size_t)p.ctas * (p.nt == 1 ? 1 : ATT_WARPS);
@@ -1009,7 +1017,7 @@ static void attend_launch(const AttendArgs& a0, const AttendPlan& plan, const vo
     auto check = [](cudaError_t e) {
         if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
     };
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (smem > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     kernel<<<plan.ctas, 32 * ATT_WARPS, smem, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
     if (plan.whole) return;

@@ -5,16 +5,25 @@
 //
 // Both are a handful of passes over the tables and one word a page, then the
 // copies. The copies are HBM bound (each page read and written once, 16 bytes
-// a thread); the rest is bound by the launches and the passes' dependent
-// loads, so each pass is one launch, issued early behind the one before.
+// a thread); the rest is bound by the passes' dependent loads and the
+// launches. So one cluster of eight CTAs takes all passes, the hardware's
+// cluster barrier between them, and a second launch, issued early, writes
+// the tables and copies. Past PG_SMALL pages or table entries eight CTAs are
+// too few, and each pass is a launch of its own.
+// Measured (us, GPU alone, then of a Python call): 1024 sequences of 51
+// columns over 14,704 pages FORK_US; as launches of their own 16.5 and 36.
 
-#include <climits>
+#include <cooperative_groups.h>
 
 #include "kv4_host.h"
 
 namespace nd {
 
+namespace cg = cooperative_groups;
+
 constexpr int PG_BLOCK = 1024;  // pages or sequences a block of the prefix sums
+constexpr int PG_CLUSTER = 8;
+constexpr int PG_SMALL = 1 << 17;  // pages, and table entries
 
 __device__ __forceinline__ void after_previous() {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -70,8 +79,8 @@ __device__ __forceinline__ Kept kept_of(const ForkArgs& a, int d) {
 // refers to it, nor if all that do will write on it and d is the first.
 __device__ __forceinline__ bool must_copy(const ForkArgs& a, int d, int p) {
     if (a.pinned && a.pinned[p]) return true;
-    const int refs = a.refs[p];
-    return !(refs == 1 || (refs == a.writers[p] && a.first[p] == a.n - d));
+    const int refs = __ldcg(a.refs + p);
+    return !(refs == 1 || (refs == __ldcg(a.writers + p) && __ldcg(a.first + p) == a.n - d));
 }
 
 __global__ void pages_zero_kernel(int32_t* a, int32_t* b, int n) {
@@ -82,10 +91,7 @@ __global__ void pages_zero_kernel(int32_t* a, int32_t* b, int n) {
     }
 }
 
-__global__ void fork_count_kernel(ForkArgs a) {
-    after_previous();
-    const int d = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
-    if (d >= a.n) return;
+__device__ __forceinline__ void count_kept(const ForkArgs& a, int d, int lane) {  // by a warp
     const Kept k = kept_of(a, d);
     for (int c = lane; c < k.nk; c += 32) {
         const int p = __ldg(k.row + c);
@@ -96,6 +102,23 @@ __global__ void fork_count_kernel(ForkArgs a) {
             atomicMax(a.first + p, a.n - d);
         }
     }
+}
+
+__global__ void fork_count_kernel(ForkArgs a) {
+    after_previous();
+    const int d = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    if (d < a.n) count_kept(a, d, threadIdx.x & 31);
+}
+
+// Fresh pages sequence d wants.
+__device__ __forceinline__ int fresh_wanted(const ForkArgs& a, int d) {
+    const Kept k = kept_of(a, d);
+    int f = k.nn - k.nk;
+    if (k.writes) {
+        const int p = __ldg(k.row + k.nk - 1);
+        f += p >= 0 && p < a.pages && must_copy(a, d, p);
+    }
+    return f;
 }
 
 // Sum of `mine` over a block of PG_BLOCK threads; `before`: of the threads before this one.
@@ -128,7 +151,7 @@ __device__ __forceinline__ int block_total(const int32_t* sums, int n) {
     return block_scan(mine, &before);
 }
 
-__device__ __forceinline__ bool page_free(const ForkArgs& a, int p) { return a.refs[p] == 0 && !(a.pinned && a.pinned[p]); }
+__device__ __forceinline__ bool page_free(const ForkArgs& a, int p) { return __ldcg(a.refs + p) == 0 && !(a.pinned && a.pinned[p]); }
 
 // Blocks of pages count the free ones, blocks of sequences the new pages wanted.
 __global__ void __launch_bounds__(PG_BLOCK) fork_sums_kernel(ForkArgs a, int page_blocks) {
@@ -140,12 +163,7 @@ __global__ void __launch_bounds__(PG_BLOCK) fork_sums_kernel(ForkArgs a, int pag
     } else {
         const int d = (blockIdx.x - page_blocks) * PG_BLOCK + threadIdx.x;
         if (d < a.n) {
-            const Kept k = kept_of(a, d);
-            mine = k.nn - k.nk;
-            if (k.writes) {
-                const int p = __ldg(k.row + k.nk - 1);
-                mine += p >= 0 && p < a.pages && must_copy(a, d, p);
-            }
+            mine = fresh_wanted(a, d);
             a.fresh[d] = mine;
         }
     }
@@ -173,6 +191,44 @@ __global__ void __launch_bounds__(PG_BLOCK) fork_lists_kernel(ForkArgs a, int pa
     }
 }
 
+// All passes of a fork but the last, by one cluster; its CTAs have equal
+// slices of the pages and of the sequences. The totals go to sums[0], sums[1].
+__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_BLOCK) fork_plan_kernel(ForkArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = cluster.block_rank(), tid = threadIdx.x, all = rank * PG_BLOCK + tid;
+    __shared__ int mine[2];
+    for (int i = all; i < a.pages; i += PG_CLUSTER * PG_BLOCK) a.refs[i] = a.writers[i] = a.first[i] = 0;
+    cluster.sync();
+    for (int d = all / 32; d < a.n; d += PG_CLUSTER * PG_BLOCK / 32) count_kept(a, d, tid & 31);
+    cluster.sync();
+    const int pages_each = (a.pages + PG_CLUSTER - 1) / PG_CLUSTER, seqs_each = (a.n + PG_CLUSTER - 1) / PG_CLUSTER;
+    const int p0 = rank * pages_each, p1 = min(p0 + pages_each, a.pages), d0 = rank * seqs_each, d1 = min(d0 + seqs_each, a.n);
+    int frees = 0, wanted = 0, x;
+    for (int p = p0 + tid; p < p1; p += PG_BLOCK) frees += page_free(a, p);
+    for (int d = d0 + tid; d < d1; d += PG_BLOCK) wanted += a.fresh[d] = fresh_wanted(a, d);
+    frees = block_scan(frees, &x);
+    wanted = block_scan(wanted, &x);
+    if (tid == 0) mine[0] = frees, mine[1] = wanted;
+    cluster.sync();
+    int free0 = 0, want0 = 0;
+    for (int r = 0; r < rank; r++) free0 += cluster.map_shared_rank(mine, r)[0], want0 += cluster.map_shared_rank(mine, r)[1];
+    for (int p = p0; p < p1; p += PG_BLOCK) {
+        const bool is = p + tid < p1 && page_free(a, p + tid);
+        const int sum = block_scan(is, &x);
+        if (is) a.free_ids[free0 + x] = p + tid;
+        free0 += sum;
+    }
+    for (int d = d0; d < d1; d += PG_BLOCK) {
+        const int f = d + tid < d1 ? a.fresh[d + tid] : 0;  // this thread's own, from above
+        const int sum = block_scan(f, &x);
+        if (d + tid < d1) a.base[d + tid] = want0 + x;
+        want0 += sum;
+    }
+    if (rank == PG_CLUSTER - 1 && tid == 0) a.sums[0] = free0, a.sums[1] = want0, a.info[2] = 0;
+    cluster.sync();  // no CTA leaves while others read its counts
+}
+
 __device__ __forceinline__ void copy_page(const PoolView& v, int from, int to, int part, int parts) {
     const long long units = v.bytes / 16;
     for (int l = 0; l < v.layers; l++) {
@@ -194,11 +250,11 @@ __device__ __forceinline__ void copy_page(const PoolView& v, int from, int to, i
 // A block a new sequence (and part of its copy): the row of the new table,
 // references, the page it copies. Sources of copies stay referenced, so no
 // copy writes what another reads.
-__global__ void __launch_bounds__(128) fork_assign_kernel(ForkArgs a, int blocks) {
+__global__ void __launch_bounds__(128) fork_assign_kernel(ForkArgs a, int totals) {
     after_previous();
     const int d = blockIdx.x;
     const Kept k = kept_of(a, d);
-    const int base = a.base[d], frees = a.sums[blocks];
+    const int base = a.base[d], frees = a.sums[totals];
     auto id = [&](int rank) { return rank < frees ? a.free_ids[rank] : -1; };
     int last = -1;
     if (k.writes) {
@@ -222,7 +278,7 @@ __global__ void __launch_bounds__(128) fork_assign_kernel(ForkArgs a, int blocks
         a.table_out[(size_t)d * a.cols + c] = p;
     }
     if (threadIdx.x == 0 && d == 0) {
-        const int wanted = a.sums[blocks + 1], given = min(wanted, frees);
+        const int wanted = a.sums[totals + 1], given = min(wanted, frees);
         a.info[0] = a.pages - frees + given;
         a.info[1] = given;
         a.info[3] = wanted - given;
@@ -262,7 +318,7 @@ __global__ void compact_count_kernel(CompactArgs a) {
 // (live, live and movable)
 __device__ __forceinline__ int2 page_state(const CompactArgs& a, int p) {
     if (p >= a.pages) return make_int2(0, 0);
-    const bool used = a.refs[p] != 0, pin = a.pinned && a.pinned[p];
+    const bool used = __ldcg(a.refs + p) != 0, pin = a.pinned && a.pinned[p];
     return make_int2(used || pin, used && !pin);
 }
 
@@ -312,11 +368,69 @@ __global__ void __launch_bounds__(PG_BLOCK) compact_lists_kernel(CompactArgs a) 
     }
 }
 
+// The same in one cluster; n and the moves go to sums[0].
+__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_BLOCK) compact_plan_kernel(CompactArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = cluster.block_rank(), tid = threadIdx.x, all = rank * PG_BLOCK + tid;
+    __shared__ int mine[3];
+    for (int i = all; i < a.pages; i += PG_CLUSTER * PG_BLOCK) a.refs[i] = 0;
+    cluster.sync();
+    for (long long i = all; i < (long long)a.seqs * a.cols; i += PG_CLUSTER * PG_BLOCK) {
+        const int p = __ldg(a.table + (size_t)(i / a.cols) * a.table_stride + i % a.cols);
+        if (p >= 0 && p < a.pages) a.refs[p] = 1;
+    }
+    cluster.sync();
+    const int each = (a.pages + PG_CLUSTER - 1) / PG_CLUSTER, p0 = rank * each, p1 = min(p0 + each, a.pages);
+    int live = 0, move = 0, x;
+    for (int p = p0 + tid; p < p1; p += PG_BLOCK) {
+        const int2 st = page_state(a, p);
+        live += st.x, move += st.y;
+    }
+    live = block_scan(live, &x);
+    move = block_scan(move, &x);
+    if (tid == 0) mine[0] = live, mine[1] = move;
+    cluster.sync();
+    int n = 0, live0 = 0, move0 = 0, moves = 0;
+    for (int r = 0; r < PG_CLUSTER; r++) {
+        const int* m = cluster.map_shared_rank(mine, r);
+        if (r < rank) live0 += m[0], move0 += m[1];
+        n += m[0], moves += m[1];
+    }
+    // movable pages of this slice before n
+    int early = 0;
+    for (int p = p0 + tid; p < min(p1, n); p += PG_BLOCK) early += page_state(a, p).y;
+    early = block_scan(early, &x);
+    if (tid == 0) mine[2] = early;
+    cluster.sync();
+    int before_n = 0;
+    for (int r = 0; r < PG_CLUSTER; r++) before_n += cluster.map_shared_rank(mine, r)[2];
+    for (int b = p0; b < p1; b += PG_BLOCK) {
+        const int p = b + tid;
+        const int2 st = p < p1 ? page_state(a, p) : make_int2(0, 0);
+        int l, m;
+        const int ls = block_scan(st.x, &l), ms = block_scan(st.y, &m);
+        l += live0, m += move0;
+        live0 += ls, move0 += ms;
+        if (p < p1) {
+            a.before[p] = m - before_n;
+            if (p >= n && st.y) a.movers[m - before_n] = p;
+            if (p < n && !st.x) a.holes[p - l] = p;
+        }
+    }
+    if (rank == 0 && tid == 0) {
+        a.sums[0] = make_int2(n, moves - before_n);
+        a.info[0] = n;
+        a.info[1] = moves - before_n;
+    }
+    cluster.sync();  // no CTA leaves while others read its counts
+}
+
 // Blocks of pages write the map, blocks of table entries the new table, the
 // others copy.
-__global__ void __launch_bounds__(128) compact_move_kernel(CompactArgs a, int blocks, int map_blocks, int table_blocks) {
+__global__ void __launch_bounds__(128) compact_move_kernel(CompactArgs a, int totals, int map_blocks, int table_blocks) {
     after_previous();
-    const int2 tot = a.sums[blocks];
+    const int2 tot = a.sums[totals];
     const int n = tot.x;
     auto to = [&](int p) {
         const int2 st = page_state(a, p);
@@ -419,13 +533,19 @@ int nd_op_pages_fork(const nd_pages* pool, const int* table, int table_stride, i
         OnDevice on(pool->device, what);
         cudaStream_t st = (cudaStream_t)stream;
         const int sms = device_sm_count();
-        launch_behind(what, pages_zero_kernel, std::min((N + 255) / 256, 4 * sms), 256, st, true, a.refs, a.writers, N);
-        launch_behind(what, fork_count_kernel, (n + 3) / 4, 128, st, false, a);
-        launch_behind(what, fork_sums_kernel, nb + sb, PG_BLOCK, st, false, a, nb);
-        launch_behind(what, fork_lists_kernel, nb + sb, PG_BLOCK, st, false, a, nb);
+        int totals = 0;  // their place in sums
+        if (N <= PG_SMALL && (long long)n * cols <= PG_SMALL) {
+            launch_behind(what, fork_plan_kernel, PG_CLUSTER, PG_BLOCK, st, true, a);
+        } else {
+            totals = nb + sb;
+            launch_behind(what, pages_zero_kernel, std::min((N + 255) / 256, 4 * sms), 256, st, true, a.refs, a.writers, N);
+            launch_behind(what, fork_count_kernel, (n + 3) / 4, 128, st, false, a);
+            launch_behind(what, fork_sums_kernel, nb + sb, PG_BLOCK, st, false, a, nb);
+            launch_behind(what, fork_lists_kernel, nb + sb, PG_BLOCK, st, false, a, nb);
+        }
         // 8 KB of a layer's page a block at least, 2 CTAs an SM of copies at most
         const long long parts = std::min<long long>((pool->page_bytes + 8191) / 8192, std::max(1, 2 * sms / n));
-        launch_behind(what, fork_assign_kernel, dim3(n, (unsigned)parts), 128, st, false, a, nb + sb);
+        launch_behind(what, fork_assign_kernel, dim3(n, (unsigned)parts), 128, st, false, a, totals);
     });
 }
 
@@ -450,12 +570,18 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
         OnDevice on(pool->device, what);
         cudaStream_t st = (cudaStream_t)stream;
         const int sms = device_sm_count();
-        launch_behind(what, pages_zero_kernel, std::min((N + 255) / 256, 4 * sms), 256, st, true, a.refs, (int32_t*)nullptr, N);
-        launch_behind(what, compact_count_kernel, (seqs + 3) / 4, 128, st, false, a);
-        launch_behind(what, compact_sums_kernel, nb, PG_BLOCK, st, false, a);
-        launch_behind(what, compact_lists_kernel, nb, PG_BLOCK, st, false, a);
+        int totals = 0;  // their place in sums
+        if (N <= PG_SMALL && (long long)seqs * cols <= PG_SMALL) {
+            launch_behind(what, compact_plan_kernel, PG_CLUSTER, PG_BLOCK, st, true, a);
+        } else {
+            totals = nb;
+            launch_behind(what, pages_zero_kernel, std::min((N + 255) / 256, 4 * sms), 256, st, true, a.refs, (int32_t*)nullptr, N);
+            launch_behind(what, compact_count_kernel, (seqs + 3) / 4, 128, st, false, a);
+            launch_behind(what, compact_sums_kernel, nb, PG_BLOCK, st, false, a);
+            launch_behind(what, compact_lists_kernel, nb, PG_BLOCK, st, false, a);
+        }
         const int map_blocks = (N + 127) / 128, table_blocks = (int)(((long long)seqs * cols + 127) / 128);
-        launch_behind(what, compact_move_kernel, map_blocks + table_blocks + std::min(N, 16 * sms), 128, st, false, a, nb, map_blocks, table_blocks);
+        launch_behind(what, compact_move_kernel, map_blocks + table_blocks + std::min(N, 16 * sms), 128, st, false, a, totals, map_blocks, table_blocks);
     });
 }
 

@@ -53,8 +53,8 @@ class KV4Pool:
         self.data, self.dk, self.dv = data, dk, dv
         self.num_pages, self.heads, self.page = n, h, tiles * _TILE
         self.device = data.device
-        self._fixed = (data.device.index, data.data_ptr(), data.stride(0) if n > 1 else h * tiles * tile, n, self.page, h,
-                       dk, dv)
+        self._fixed = bytes(_KV4(data.device.index, data.data_ptr(), data.stride(0) if n > 1 else h * tiles * tile, n,
+                                 self.page, h, dk, dv))
 
     @staticmethod
     def tile_bytes(dk, dv):
@@ -70,9 +70,12 @@ class KV4Pool:
     def _args(self, table, lens, start, rows):
         """The C view of a call; its tensors must outlive the call."""
         dev = self.device
-        s, p, stride = _table(table, dev)
-        return C.byref(_KV4(*self._fixed, table.data_ptr(), stride, p, s, _int32(lens, s, dev, "lens"),
-                            None if start is None else _int32(start, s + 1, dev, "start"), rows))
+        s, a = table.shape[0], _KV4.from_buffer_copy(self._fixed)
+        a.seqs, a.max_pages, a.table_stride = _table(table, dev)
+        a.table, a.lens, a.rows = table.data_ptr(), _int32(lens, s, dev, "lens"), rows
+        if start is not None:
+            a.start = _int32(start, s + 1, dev, "start")
+        return C.byref(a)
 
     def _rows(self, x, heads, d, name):
         if (x.dtype not in _TYPES or x.dim() != 3 or x.device != self.device or x.shape[1] != heads or x.shape[2] != d
@@ -148,9 +151,12 @@ def _pages(pool, axis):
         raise ValueError("pool must be a CUDA tensor [pages, ..], or [layers, pages, ..] with axis=1")
     n, layers = pool.shape[axis], pool.shape[0] if axis else 1
     size = pool.element_size()
-    nbytes = pool.numel() // (n * layers) * size
-    if not pool[0 if axis == 0 else (0, 0)].is_contiguous():
-        raise ValueError("a page must be contiguous")
+    inner = 1
+    for d in range(pool.dim() - 1, axis, -1):
+        if pool.stride(d) != inner and pool.shape[d] != 1:
+            raise ValueError("a page must be contiguous")
+        inner *= pool.shape[d]
+    nbytes = inner * size
     return C.byref(_PAGES(pool.device.index, pool.data_ptr(), pool.stride(axis) * size if n > 1 else nbytes,
                           pool.stride(0) * size if axis and layers > 1 else 0, nbytes, n, layers)), n
 
@@ -189,13 +195,13 @@ def op_pages_fork(pool, table, src, keep, need, page, pinned=None, axis=0):
         raise ValueError("src must name at least one sequence")
     out = torch.empty((n, p), dtype=torch.int32, device=dev)
     refs = torch.empty(n_pages, dtype=torch.int32, device=dev)
-    info = torch.empty(4, dtype=torch.int32, device=dev)
     L = lib()
     size = L.nd_op_pages_fork_ws(n_pages, n)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = torch.empty(4 + (size + 3) // 4, dtype=torch.int32, device=dev)
+    info = ws[:4]
     if L.nd_op_pages_fork(pv, table.data_ptr(), stride, s, p, page, _int32(src, n, dev, "src"), _int32(keep, n, dev, "keep"),
                           _int32(need, n, dev, "need"), n, _pinned(pinned, n_pages, dev), out.data_ptr(), refs.data_ptr(),
-                          info.data_ptr(), ws.data_ptr(), size, _stream(dev)) != 0:
+                          ws.data_ptr(), ws.data_ptr() + 16, size, _stream(dev)) != 0:
         raise _err()
     return out, refs, info
 
@@ -209,12 +215,12 @@ def op_pages_compact(pool, table, pinned=None, axis=0):
     s, p, stride = _table(table, dev)
     out = torch.empty((s, p), dtype=torch.int32, device=dev)
     to = torch.empty(n_pages, dtype=torch.int32, device=dev)
-    info = torch.empty(2, dtype=torch.int32, device=dev)
     L = lib()
     size = L.nd_op_pages_compact_ws(n_pages)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = torch.empty(4 + (size + 3) // 4, dtype=torch.int32, device=dev)
+    info = ws[:2]
     if L.nd_op_pages_compact(pv, table.data_ptr(), stride, s, p, _pinned(pinned, n_pages, dev), out.data_ptr(), to.data_ptr(),
-                             info.data_ptr(), ws.data_ptr(), size, _stream(dev)) != 0:
+                             ws.data_ptr(), ws.data_ptr() + 16, size, _stream(dev)) != 0:
         raise _err()
     return out, to, info
 

@@ -175,6 +175,21 @@ def test_fork_drawn(cuda_device, seed):
     check_fork(table, src, keep, need, page, pages, pinned, layers=1 + seed % 3, elems=8 * int(r.integers(1, 40)), seed=seed)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,cols,n,pages", [(300, 400, 500, 140000), (40, 20, 9000, 2000), (700, 300, 20, 70000)])
+def test_large_sets(cuda_device, seqs, cols, n, pages):
+    """Past what one cluster takes: pages, entries of the new and of the old table."""
+    r = np.random.default_rng(seqs)
+    table = np.full(seqs * cols, -1)
+    some = r.permutation(pages)[: seqs * cols // 3]
+    table[: len(some)] = some
+    table = table.reshape(seqs, cols)
+    src = r.integers(0, seqs // 4 + 1, n)
+    keep = r.integers(0, 16 * cols, n)
+    check_fork(table, src, keep, keep + r.integers(0, 40, n), 16, pages, elems=8)
+    check_compact(table, pages, elems=8)
+
+
 def check_compact(table, pages, pinned=None, layers=1, elems=24, seed=0):
     import needle_b200 as nb
     import torch
