@@ -26,6 +26,7 @@ struct RowSplit {
 };
 
 constexpr int ROW_WARPS = 8;
+constexpr int ROW_AHEAD = 4;  // vectors whose loads a warp has in flight
 
 template <int DK, int DV, typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_append_kernel(Kv4Args a, const T* __restrict__ k, long long k_row, long long k_head,
@@ -39,45 +40,59 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_append_kernel(Kv4Args a, c
     uint8_t* tile0 = kv4_tile_of(a, s, pos, TB);
     if (!tile0) return;
     const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
-    for (int j = blockIdx.y * PER + lane / L; j - lane / L < 2 * a.heads; j += gridDim.y * PER) {
-        const bool val = j >= a.heads;
-        const int h = val ? j - a.heads : j, D = val ? DV : DK;
-        const bool on = j < 2 * a.heads && d0 < D;
-        float x[8];
-        float lo = FLT_MAX, hi = -FLT_MAX;
-        bool bad = false;
-        if (on) {
-            load8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x);
+    const int step = gridDim.y * PER;
+    for (int j0 = blockIdx.y * PER + lane / L; j0 - lane / L < 2 * a.heads; j0 += ROW_AHEAD * step) {
+        float x[ROW_AHEAD][8];
+        bool on[ROW_AHEAD];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                bad |= !(fabsf(x[i]) <= FLT_MAX);
-                lo = fminf(lo, x[i]);
-                hi = fmaxf(hi, x[i]);
+        for (int w = 0; w < ROW_AHEAD; w++) {
+            const int j = j0 + w * step;
+            const bool val = j >= a.heads;
+            const int h = val ? j - a.heads : j;
+            on[w] = j < 2 * a.heads && d0 < (val ? DV : DK);
+            if (on[w]) load8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < ROW_AHEAD; w++) {
+            const int j = j0 + w * step;
+            if (j - lane / L >= 2 * a.heads) break;  // for the whole warp
+            const bool val = j >= a.heads;
+            const int h = val ? j - a.heads : j, D = val ? DV : DK;
+            float lo = FLT_MAX, hi = -FLT_MAX;
+            bool bad = false;
+            if (on[w]) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    bad |= !(fabsf(x[w][i]) <= FLT_MAX);
+                    lo = fminf(lo, x[w][i]);
+                    hi = fmaxf(hi, x[w][i]);
+                }
             }
-        }
 #pragma unroll
-        for (int o = 1; o < L; o *= 2) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
-        }
-        if (!on) continue;
-        __half sh = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), 65504.0f));
-        __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
-        const float sf = __half2float(sh), mf = __half2float(mh);
-        uint32_t w = 0;
-        if (bad) {
-            sh = mh = __ushort_as_half(0x7fff);
-        } else if (sf > 0.f) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), sf)), 0.f), 15.f);
-                w |= (uint32_t)(int)c << (4 * i);
+            for (int o = 1; o < L; o *= 2) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
             }
+            const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+            bad = (bads >> (lane & ~(L - 1)) & ((1ull << L) - 1)) != 0;
+            if (!on[w]) continue;
+            __half sh = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), 65504.0f));
+            __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
+            const float sf = __half2float(sh), mf = __half2float(mh);
+            uint32_t codes = 0;
+            if (bad) {
+                sh = mh = __ushort_as_half(0x7fff);
+            } else if (sf > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[w][i], mf), sf)), 0.f), 15.f);
+                    codes |= (uint32_t)(int)c << (4 * i);
+                }
+            }
+            uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
+            *(uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub) = codes;
+            if (sub == 0) *(__half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot) = __halves2half2(sh, mh);
         }
-        uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
-        *(uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub) = w;
-        if (sub == 0) *(__half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot) = __halves2half2(sh, mh);
     }
 }
 
@@ -97,23 +112,36 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_read_kernel(Kv4Args a, T* 
         return;
     }
     const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
-    for (int j = blockIdx.y * PER + lane / L; j < 2 * a.heads; j += gridDim.y * PER) {
-        const bool val = j >= a.heads;
-        const int h = val ? j - a.heads : j, D = val ? DV : DK;
-        if (d0 >= D) continue;
-        float x[8];
-        if (tile0) {
-            const uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
-            const uint32_t w = *(const uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub);
-            const float2 sm = __half22float2(*(const __half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot));
+    const int step = gridDim.y * PER;
+    for (int j0 = blockIdx.y * PER + lane / L; j0 < 2 * a.heads; j0 += ROW_AHEAD * step) {
+        uint32_t codes[ROW_AHEAD], params[ROW_AHEAD];
+        bool on[ROW_AHEAD];
+#pragma unroll
+        for (int w = 0; w < ROW_AHEAD; w++) {
+            const int j = j0 + w * step;
+            const bool val = j >= a.heads;
+            const int h = val ? j - a.heads : j, D = val ? DV : DK;
+            on[w] = j < 2 * a.heads && d0 < D;
+            codes[w] = params[w] = 0;  // no such position: zeros
+            if (on[w] && tile0) {
+                const uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
+                codes[w] = *(const uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub);
+                params[w] = *(const uint32_t*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot);
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < ROW_AHEAD; w++) {
+            if (!on[w]) continue;
+            const int j = j0 + w * step;
+            const bool val = j >= a.heads;
+            const int h = val ? j - a.heads : j;
+            const float2 sm = __half22float2(*(const __half2*)&params[w]);
+            float x[8];
             // the product of an f16 and a code is exact: one rounding
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = __fmaf_rn(sm.x, (float)((w >> (4 * i)) & 15), sm.y);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.f;
+            for (int i = 0; i < 8; i++) x[i] = __fmaf_rn(sm.x, (float)((codes[w] >> (4 * i)) & 15), sm.y);
+            store8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x);
         }
-        store8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x);
     }
 }
 

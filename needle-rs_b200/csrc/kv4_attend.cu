@@ -52,18 +52,20 @@
 namespace nd {
 
 constexpr int ATT_WARPS = 4;
-constexpr int ATT_KT(int nt) { return nt == 4 ? 1 : 2; }
-constexpr int ATT_STAGES(int nt) { return nt == 4 ? 4 : 3; }
-constexpr int ATT_CTAS(int nt, int dv) { return nt == 4 ? 2 : nt == 2 || dv == 128 ? 3 : 4; }  // an SM
+constexpr int ATT_KT = 2, ATT_STAGES = 3;
+constexpr int ATT_CTAS(int nt, int dv) { return nt == 2 || dv == 128 ? 3 : 4; }  // an SM: what registers and shared memory allow
 // Tiles: a shorter run of a cut unit costs more to join than it takes.
 constexpr int ATT_MIN_SHARE = 8;
 // What beginning and ending a unit costs a warp, in tiles: without it a warp
 // that meets many short units is the last by far (8 sequences, one of a
 // single position among lengths up to 32768: 70 us instead of UNIT_US).
 constexpr int ATT_UNIT_COST = 4;
-// A call whose units all have at most this many tiles deals whole units out
-// to the warps and needs no second kernel.
-constexpr int ATT_WHOLE_TILES = 16;
+// Calls whose units all have at most this many tiles take them whole, a warp
+// or, where units are too few to fill the GPU, a CTA a unit, and need no
+// second kernel. Measured (us, with cut units, a warp, a CTA a unit): 32
+// sequences of up to 256 positions 14.4, 10.1, 6.7; 512 of them -, 15.4, 18.0;
+// 32 of up to 1000 14.9, -, 11.1.
+constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
 
 // n / d for 0 <= n < 2^31 by a multiplication.
 struct FastDiv {
@@ -80,32 +82,37 @@ struct AttendArgs {
     long long q_row, q_head, o_row, o_head;
     FastDiv group;       // query heads a kv head
     FastDiv page_tiles;
-    int window, sink;
+    int window, sink, places;
     float scale_log2e;
     bool q_vec, o_vec, zero_rest;
     float* parts;   // [runners][2][8 NT * (DV + 2)]; a runner is a warp, for NT = 1 a CTA
     int4* joins;    // [runners]: (sequence, kv head, query block, further runners) of the cut unit that starts there, w < 0: none
 };
 
-// Whole units are numbered without sums: sequence s has the places
-// from s + start[s] * group / (8 NT) on, one more than its whole blocks of
-// rows at least, of which it leaves at most one empty.
+// Whole units are numbered without sums. Places 0 .. seqs - 1 are the
+// sequences' first blocks; the further blocks of sequence s are at most the
+// places from further_place(s) to further_place(s + 1): ceil(y - x) - 1 <=
+// floor(y) - floor(x). Places that no block has are left at once.
 template <int NT>
-__device__ __forceinline__ int first_place(const AttendArgs& a, int s) {
-    return s + (int)((long long)kv4_first_row(a.kv, s) * a.group.d / (8 * NT));
+__device__ __forceinline__ int further_place(const AttendArgs& a, int s) {
+    return (int)((long long)kv4_first_row(a.kv, s) * a.group.d / (8 * NT));
 }
 
-// The sequence of place u, by the whole warp 32 at a time.
+// The sequence of place u (by the whole warp, 32 sequences at a time) and its block.
 template <int NT>
-__device__ __forceinline__ int seq_of_place(const AttendArgs& a, int u, int lane) {
-    int lo = 0, size = a.kv.seqs;  // sequences that may begin at or before u
+__device__ __forceinline__ int seq_of_place(const AttendArgs& a, int u, int lane, int* block) {
+    *block = 0;
+    if (u < a.kv.seqs) return u;
+    u -= a.kv.seqs;
+    int lo = 0, size = a.kv.seqs;  // how many begin at or before u
     while (size > 0) {
         const int step = (size + 31) / 32, at = lane * step + step - 1;
-        const bool before = at < size && first_place<NT>(a, lo + at) <= u;
+        const bool before = at < size && further_place<NT>(a, lo + at) <= u;
         const int c = __popc(__ballot_sync(0xffffffffu, before));
         lo += c * step;
         size = min(step - 1, size - c * step);
     }
+    if (lo > 0) *block = 1 + u - further_place<NT>(a, lo - 1);
     return lo - 1;
 }
 
@@ -246,7 +253,7 @@ struct AttendShape {
     static constexpr bool Q_SMEM = QOPS > 16;      // else they stay in registers
     // Tiles a round of the main loop, and rounds in flight: two tiles give a
     // warp two independent chains of products, and share a round's overhead.
-    static constexpr int KT = ATT_KT(NT), STAGES = ATT_STAGES(NT);
+    static constexpr int KT = ATT_KT, STAGES = ATT_STAGES;
     // For one block of eight rows the warps of a CTA join their parts in
     // shared memory first: decoding cuts few units into many parts.
     static constexpr bool MERGE = NT == 1;
@@ -259,7 +266,19 @@ struct AttendShape {
     static constexpr int CTAS = ATT_CTAS(NT, DV);
 };
 
-// acc (8 VW g + .. as the main loop holds it), M, l of a part of 8 rows.
+// Where query row x of a sequence and kv head has its result.
+template <typename T>
+struct OutRows {
+    T* out;
+    const AttendArgs& a;
+    int first, h, nrows;
+    __device__ __forceinline__ T* at(int x) const {
+        const int tok = a.group(x);
+        return out + (long long)(first + tok) * a.o_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.o_head;
+    }
+};
+
+// A part of 8 rows as a warp holds it.
 template <int DV>
 struct PartRegs {
     float v[2][DV / 8], M[2], l[2];  // rows 2 c, 2 c + 1; dimensions (DV / 8) g ..
@@ -271,6 +290,20 @@ struct PartRegs {
             for (int k = 0; k < DV / 32; k++) *(float4*)&v[j][4 * k] = *(const float4*)(p + y * DV + (DV / 8) * g + 4 * k);
             M[j] = p[8 * DV + y];
             l[j] = p[8 * (DV + 1) + y];
+        }
+    }
+    // the quotients, for rows x0 ..
+    template <typename T>
+    __device__ __forceinline__ void write(const OutRows<T>& to, int x0, int g, int c) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int x = x0 + 2 * c + j;
+            const float norm = l[j] == 0.f ? 0.f : 1.f / l[j];
+#pragma unroll
+            for (int k = 0; k < DV / 8; k++) v[j][k] *= norm;
+            if (x < to.nrows)
+#pragma unroll
+                for (int k = 0; k < DV / 64; k++) store8(to.at(x) + (DV / 8) * g + 8 * k, to.a.o_vec, v[j] + 8 * k);
         }
     }
     __device__ __forceinline__ void add(const PartRegs& o) {
@@ -286,17 +319,6 @@ struct PartRegs {
     }
 };
 
-// rows y (of a block) from x0 on of one sequence and kv head
-template <typename T>
-struct OutRows {
-    T* out;
-    const AttendArgs& a;
-    int first, h, nrows;
-    __device__ __forceinline__ T* at(int x) const {
-        const int tok = a.group(x);
-        return out + (long long)(first + tok) * a.o_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.o_head;
-    }
-};
 
 // A warp's part of a unit: tiles off .. off + m - 1 of query block b of
 // sequence s and kv head h. With `part` NULL they are all it has and the
@@ -748,25 +770,46 @@ __device__ __forceinline__ void zero_rest(const AttendArgs& a, T* out, int wid, 
             for (int d = lane; d < DV; d += 32) out[r * a.o_row + hq * a.o_head + d] = (T)0.f;
 }
 
-// Short units, dealt out whole: unit by unit, no sums over the sequences, no joins.
-template <int DK, int DV, int NT, typename T>
+// Short units without sums over the sequences and without joins. SHARED: a
+// CTA a unit, its warps share the tiles and join their parts in shared
+// memory; else a warp a unit. blockIdx.x counts places, blockIdx.y kv heads.
+template <int DK, int DV, int NT, typename T, bool SHARED>
 __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CTAS)
     kv4_attend_whole_kernel(AttendArgs a, const T* __restrict__ q, T* __restrict__ out) {
     using Sh = AttendShape<DK, DV, NT, T>;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int warps = gridDim.x * ATT_WARPS, wid = blockIdx.x * ATT_WARPS + warp;
-    zero_rest<DV>(a, out, wid, warps, lane);
-    uint8_t* ring = smem + warp * (Sh::RING + Sh::QBYTES);
-    const long long units = ((long long)a.kv.seqs + (long long)a.kv.rows * a.group.d / (8 * NT)) * a.kv.heads;
-    for (long long x = wid; x < units; x += warps) {
-        const int u = (int)(x / a.kv.heads), h = (int)(x % a.kv.heads), s = seq_of_place<NT>(a, u, lane);
-        if (s < 0) continue;
-        const int b = u - first_place<NT>(a, s);
-        const SeqRows rows = seq_rows(a, s);
-        if (b * 8 * NT >= rows.n * (int)a.group.d) continue;
-        const Tiles tl = block_tiles<NT>(a, rows, b);
-        attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, 0, tl.n, ring, (uint2*)(ring + Sh::RING), nullptr);
+    if (blockIdx.y == 0) zero_rest<DV>(a, out, blockIdx.x * ATT_WARPS + warp, gridDim.x * ATT_WARPS, lane);
+    uint8_t* mine = smem + warp * (Sh::RING + Sh::QBYTES);
+    uint2* qsm = (uint2*)(mine + Sh::RING);
+    const int u = SHARED ? blockIdx.x : blockIdx.x * ATT_WARPS + warp, h = blockIdx.y;
+    if (u >= a.places) return;
+    int b;
+    const int s = seq_of_place<NT>(a, u, lane, &b);
+    if (s < 0) return;
+    const SeqRows rows = seq_rows(a, s);
+    if ((long long)b * 8 * NT >= (long long)rows.n * a.group.d) return;
+    const Tiles tl = block_tiles<NT>(a, rows, b);
+    if (!SHARED) {
+        attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, 0, tl.n, mine, qsm, nullptr);
+        return;
+    }
+    if constexpr (SHARED) {
+        // as few warps as have a round each
+        const int rounds = (tl.n + Sh::KT - 1) / Sh::KT, each = (rounds + ATT_WARPS - 1) / ATT_WARPS * Sh::KT;
+        const int off = warp * each, m = min(each, tl.n - off), used = (tl.n + each - 1) / each;
+        float* part = (float*)mine;  // over the ring
+        if (m > 0) attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, off, m, mine, qsm, used == 1 ? nullptr : part);
+        if (used == 1) return;
+        __syncthreads();
+        if (warp) return;
+        PartRegs<DV> sum, more;
+        sum.load(part, lane >> 2, lane & 3);
+        for (int w = 1; w < used; w++) {
+            more.load((const float*)(mine + w * (Sh::RING + Sh::QBYTES)), lane >> 2, lane & 3);
+            sum.add(more);
+        }
+        sum.write(OutRows<T>{out, a, rows.first, h, rows.n * (int)a.group.d}, b * 8, lane >> 2, lane & 3);
     }
 }
 
@@ -902,17 +945,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             if (start && ended) {
                 const int4 u = cut_start[warp];
                 const SeqRows rows = seq_rows(a, u.x);
-                const OutRows<T> to{out, a, rows.first, u.y, rows.n * (int)a.group.d};
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int x = u.z * 8 + 2 * c + j;
-                    const float norm = sum.l[j] == 0.f ? 0.f : 1.f / sum.l[j];
-#pragma unroll
-                    for (int k = 0; k < DV / 8; k++) sum.v[j][k] *= norm;
-                    if (x < to.nrows)
-#pragma unroll
-                        for (int k = 0; k < DV / 64; k++) store8(to.at(x) + (DV / 8) * g + 8 * k, a.o_vec, sum.v[j] + 8 * k);
-                }
+                sum.write(OutRows<T>{out, a, rows.first, u.y, rows.n * (int)a.group.d}, u.z * 8, g, c);
                 return false;
             }
             float* part = a.parts + ((size_t)blockIdx.x * 2 + (start ? 1 : 0)) * PART;
@@ -974,16 +1007,23 @@ __global__ void __launch_bounds__(512) kv4_join_kernel(AttendArgs a, T* __restri
     }
 }
 
-// Query rows a block: the fewest blocks of 8, 16 or 32 rows that hold what a
-// sequence brings on average.
+// Blocks of 8 query rows, or of 16 where sequences bring many: the wider
+// block halves the unpacking of codes a product, the narrower one splits over
+// more warps and needs fewer registers. Measured (us, 8 against 16 rows): 5
+// tokens of 6 heads a kv head, 256 sequences 50 and 52; 32 tokens of 4 heads
+// 42 and 51; 512 tokens 393 and 339.
 static int query_tiles(const nd_kv4* kv, int group) {
-    const long long mean = ((long long)kv->rows + kv->seqs - 1) / kv->seqs * group;
-    return mean <= 8 ? 1 : mean <= 16 ? 2 : 4;
+    return ((long long)kv->rows + kv->seqs - 1) / kv->seqs * group <= 256 ? 1 : 2;
 }
 
+// How a call is split:
+// CUT   runs of equal work, units cut where they end, two kernels;
+// WARP  a warp a unit, CTA  four warps a unit: units of few tiles.
+enum AttendMode { CUT, WARP, CTA };
+
 struct AttendPlan {
-    int nt, ctas;
-    bool whole;
+    int nt, ctas, places;
+    AttendMode mode;
     size_t ws;
 };
 
@@ -995,13 +1035,18 @@ static AttendPlan attend_plan(const nd_kv4* kv, int group, int window, int sink)
     const long long table = (long long)kv->max_pages * (kv->page / KV4_TILE);
     long long tiles = table;
     if (window > 0) tiles = std::min(table, ((long long)window + 8 * p.nt + 2 * KV4_TILE) / KV4_TILE + (sink + KV4_TILE - 1LL) / KV4_TILE);
-    p.whole = tiles <= ATT_WHOLE_TILES;
-    const long long units = kv->heads * ((long long)kv->rows * group / (8 * p.nt) + std::min(kv->seqs, kv->rows));
-    const long long runs = p.whole ? units : (units * (tiles + ATT_UNIT_COST) + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
-    const int full = device_sm_count() * ATT_CTAS(p.nt, kv->dv);
+    const long long full = (long long)device_sm_count() * ATT_CTAS(p.nt, kv->dv);
+    const long long further = (long long)kv->rows * group / (8 * p.nt);
+    p.places = (int)(further + kv->seqs);
+    const long long units = kv->heads * std::max<long long>(further, std::min(kv->seqs, kv->rows));  // as many as there are likely to be
+    const long long most = kv->heads * (further + std::min(kv->seqs, kv->rows));
+    p.mode = CUT;
+    if (p.nt == 1 && tiles <= ATT_CTA_TILES && units <= full) p.mode = CTA;
+    else if (tiles <= ATT_WARP_TILES) p.mode = WARP;
+    const long long runs = (most * (tiles + ATT_UNIT_COST) + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
     p.ctas = (int)std::max(1LL, std::min<long long>(full, (runs + ATT_WARPS - 1) / ATT_WARPS));
     const size_t runners = (size_t)p.ctas * (p.nt == 1 ? 1 : ATT_WARPS);
-    p.ws = p.whole ? 0 : runners * (sizeof(int4) + 2 * sizeof(float) * 8 * p.nt * (kv->dv + 2));
+    p.ws = p.mode == CUT ? runners * (sizeof(int4) + 2 * sizeof(float) * 8 * p.nt * (kv->dv + 2)) : 0;
     return p;
 }
 
@@ -1009,18 +1054,28 @@ template <int DK, int DV, int NT, typename T>
 static void attend_launch(const AttendArgs& a0, const AttendPlan& plan, const void* q, void* out, void* ws, cudaStream_t st) {
     using Sh = AttendShape<DK, DV, NT, T>;
     AttendArgs a = a0;
-    const int runners = plan.ctas * (Sh::MERGE ? 1 : ATT_WARPS);
-    a.joins = (int4*)ws;
-    a.parts = (float*)((char*)ws + (size_t)runners * sizeof(int4));
-    auto kernel = plan.whole ? kv4_attend_whole_kernel<DK, DV, NT, T> : kv4_attend_kernel<DK, DV, NT, T>;
-    const int smem = plan.whole ? Sh::WHOLE_SMEM : Sh::SMEM;
+    a.places = plan.places;
     auto check = [](cudaError_t e) {
         if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
     };
-    if (smem > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<plan.ctas, 32 * ATT_WARPS, smem, st>>>(a, (const T*)q, (T*)out);
+    auto prepare = [&](auto kernel, int smem) {
+        if (smem > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        return kernel;
+    };
+    if (plan.mode == WARP) {
+        prepare(kv4_attend_whole_kernel<DK, DV, NT, T, false>, Sh::WHOLE_SMEM)<<<dim3((plan.places + ATT_WARPS - 1) / ATT_WARPS, a.kv.heads), 32 * ATT_WARPS, Sh::WHOLE_SMEM, st>>>(a, (const T*)q, (T*)out);
+        return op_launched("nd_op_kv4_attend");
+    }
+    if constexpr (NT == 1)
+        if (plan.mode == CTA) {
+            prepare(kv4_attend_whole_kernel<DK, DV, NT, T, true>, Sh::WHOLE_SMEM)<<<dim3(plan.places, a.kv.heads), 32 * ATT_WARPS, Sh::WHOLE_SMEM, st>>>(a, (const T*)q, (T*)out);
+            return op_launched("nd_op_kv4_attend");
+        }
+    const int runners = plan.ctas * (Sh::MERGE ? 1 : ATT_WARPS);
+    a.joins = (int4*)ws;
+    a.parts = (float*)((char*)ws + (size_t)runners * sizeof(int4));
+    prepare(kv4_attend_kernel<DK, DV, NT, T>, Sh::SMEM)<<<plan.ctas, 32 * ATT_WARPS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
-    if (plan.whole) return;
     // launched early where the stream allows it; it waits for the first kernel's results
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(runners);
@@ -1038,8 +1093,7 @@ static void attend_launch(const AttendArgs& a0, const AttendPlan& plan, const vo
 template <int DK, int DV, typename T>
 static void attend_nt(const AttendArgs& a, const AttendPlan& p, const void* q, void* out, void* ws, cudaStream_t st) {
     if (p.nt == 1) attend_launch<DK, DV, 1, T>(a, p, q, out, ws, st);
-    else if (p.nt == 2) attend_launch<DK, DV, 2, T>(a, p, q, out, ws, st);
-    else attend_launch<DK, DV, 4, T>(a, p, q, out, ws, st);
+    else attend_launch<DK, DV, 2, T>(a, p, q, out, ws, st);
 }
 
 template <int DK, int DV>

@@ -37,7 +37,7 @@ constexpr int VF_MAX_DRAFT = 64, VF_MAX_SEQS = 1 << 20;
 constexpr int VF_STATS = 256;        // threads of the first kernel
 constexpr int VF_CHUNK = 4096;       // logits a CTA of it takes at a time
 constexpr int VF_MAX_PARTS = 32;
-constexpr int VF_DRAW = 512, VF_WARPS = VF_DRAW / 32;
+constexpr int VF_DRAW = 256, VF_WARPS = VF_DRAW / 32;  // of the second
 constexpr int VF_CACHE = 512;        // f64 terms of its run that a warp keeps
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -95,13 +95,18 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
     float top = -INFINITY, sum = 0.f;
     int at = a.V;
     bool nan = false;
+    uint4 raw[LOADS];  // the next chunk, where 16-byte loads reach all of it
+    auto whole = [&](int ch) { return a.l_vec && ch < hi && (ch + 1) * VF_CHUNK <= a.V; };
+    auto fetch = [&](int ch) {
+        if (whole(ch))
+#pragma unroll
+            for (int k = 0; k < LOADS; k++) raw[k] = __ldg((const uint4*)(row + ch * VF_CHUNK) + k * VF_STATS + tid);
+    };
+    fetch(lo);
     for (int ch = lo; ch < hi; ch++) {
         float x[N];
         const int base = ch * VF_CHUNK;
-        if (a.l_vec && base + VF_CHUNK <= a.V) {
-            uint4 raw[LOADS];
-#pragma unroll
-            for (int k = 0; k < LOADS; k++) raw[k] = __ldg((const uint4*)(row + base) + k * VF_STATS + tid);
+        if (whole(ch)) {
 #pragma unroll
             for (int k = 0; k < LOADS; k++) {
                 const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
@@ -115,6 +120,7 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
                     }
                 }
             }
+            fetch(ch + 1);
         } else {  // the same places one by one
 #pragma unroll
             for (int j = 0; j < N; j++) {
@@ -292,15 +298,16 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
     mine = warp_sum(mine);
     if (lane == 0) sums[0][warp] = mine;
     // every run's sum from its CTA: lane l of each warp gets those of runs
-    // 4 l .., what lies before them, and the whole
-    double v[4], ahead;
+    // EACH l .., what lies before them, and the whole
+    constexpr int EACH = 8 * VF_WARPS / 32;
+    double v[EACH], ahead;
     auto gather = [&](int which) {
         cluster.sync();
         if (tid < 8 * VF_WARPS) all[tid] = tid < runs ? cluster.map_shared_rank(&sums[which][0], tid / VF_WARPS)[tid % VF_WARPS] : 0.0;
         __syncthreads();
+        double own = 0.0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = all[4 * lane + k];
-        const double own = (v[0] + v[1]) + (v[2] + v[3]);
+        for (int k = 0; k < EACH; k++) v[k] = all[EACH * lane + k], own += v[k];
         double incl = own;
 #pragma unroll
         for (int k = 1; k < 32; k *= 2) {
@@ -341,9 +348,9 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
         double cum = ahead, before = 0.0, last_before = 0.0;
         int at = -1, last = -1;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < EACH; k++) {
             if (v[k] > 0.0) {
-                last = 4 * lane + k, last_before = cum;
+                last = EACH * lane + k, last_before = cum;
                 if (at < 0 && cum + v[k] > target) at = last, before = cum;
             }
             cum += v[k];
