@@ -398,8 +398,8 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
  * +infinity at a temperature above 0, or nothing above -infinity accepts
  * nothing and draws -1 with probability 0; so does a residual that holds a
  * NaN. A drafted id outside [0, V) is refused. Sums and comparisons that
- * decide are exact to f64 rounding. At most 2^20 sequences. ws:
- * nd_op_verify_ws(seqs, T, V) bytes, 16-byte aligned. */
+ * decide are exact to f64 rounding. At most 2^20 sequences,
+ * V at most 2^30. ws: nd_op_verify_ws(seqs, T, V) bytes, 16-byte aligned. */
 unsigned long long nd_op_verify_ws(int seqs, int T, int V);
 int nd_op_verify(int device, int type, const void* logits, long long l_seq, long long l_row, const int* draft,
                  const int* counts, const float* u, const float* temperature, const float* q, long long q_seq,

@@ -15,18 +15,54 @@
 namespace nd {
 
 // A warp takes one row of the call: its 2 * heads vectors, L lanes each with
-// eight values a lane (so a lane forms one 32-bit word of codes), 32 / L
-// vectors at a time. HBM bound: each value is read once by 16-byte loads and
-// the codes leave as runs of dk / 2 bytes; the search for the row's sequence
-// costs two or three dependent loads of a warp, not log2(seqs).
+// sixteen values a lane (so a lane forms 64 bits of codes), 32 / L vectors at
+// a time. Bound by instructions, not by HBM: a vector costs about as many for
+// its minimum, its place and its parameters as for its codes, which is why a
+// lane has sixteen values and not the eight of one load (12,000 rows of 8
+// heads of 128 bf16, in and out again: 45 us, with eight 50). The search for
+// the row's sequence costs two or three dependent loads of a warp, not
+// log2(seqs), and the first values are on their way meanwhile.
 template <int DK, int DV>
 struct RowSplit {
-    static constexpr int L = DK > 64 || DV > 64 ? 16 : 8;
+    static constexpr int L = DK > 64 || DV > 64 ? 8 : 4;
     static constexpr int PER = 32 / L;
 };
 
 constexpr int ROW_WARPS = 8;
-constexpr int ROW_AHEAD = 4;  // vectors whose loads a warp has in flight
+
+// Sixteen values to codes, given their row's scale and minimum. A code is the
+// nearest whole number to the f32 quotient of d = x - m by s. By a reciprocal
+// the quotient is off by 2^-21 of it at most: its nearest whole number r is
+// the right one unless d lies near the middle between two, |d - r s| near s /
+// 2 (or r was cut to 0 or 15), and those are divided out. Adding 1.5 * 2^23
+// rounds to a whole number that the low bits hold.
+__device__ __forceinline__ uint2 codes_of(const float* x, float sf, float mf) {
+    if (!(sf > 0.f)) return make_uint2(0, 0);  // all values alike, or no numbers
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
+    const f32x2 m2 = pair(-mf, -mf), inv2 = pair(inv, inv), s2 = pair(-sf, -sf);
+    const f32x2 up = pair(12582912.f, 12582912.f), down = pair(-12582912.f, -12582912.f);
+    float off = 0.f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        const f32x2 d = add2(pair(x[i], x[i + 1]), m2);
+        float2 y = unpair(mul2(d, inv2));
+        y.x = fminf(fmaxf(y.x, 0.f), 15.f), y.y = fminf(fmaxf(y.y, 0.f), 15.f);
+        const f32x2 t = add2(pair(y.x, y.y), up);
+        const float2 e = unpair(fma2(add2(t, down), s2, d)), f = unpair(t);
+        off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
+        w[i / 8] += (__float_as_uint(f.x) << (4 * (i % 8))) + (__float_as_uint(f.y) << (4 * (i % 8) + 4));
+    }
+    w[0] -= 0x4b400000u * 0x11111111u, w[1] -= 0x4b400000u * 0x11111111u;  // the constants
+    if (__builtin_expect(!(off < 0.4999f * sf), 0)) {
+        w[0] = w[1] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            w[i / 8] |= (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], mf), sf)), 0.f), 15.f) << (4 * (i % 8));
+    }
+    return make_uint2(w[0], w[1]);
+}
 
 template <int DK, int DV, typename T>
 __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_append_kernel(Kv4Args a, const T* __restrict__ k, long long k_row, long long k_head,
@@ -34,65 +70,56 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_append_kernel(Kv4Args a, c
     constexpr int TB = kv4_tile_bytes(DK, DV), L = RowSplit<DK, DV>::L, PER = RowSplit<DK, DV>::PER;
     const int lane = threadIdx.x & 31, r = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     if (r >= a.rows) return;
+    const int sub = lane % L, d0 = 16 * sub, step = gridDim.y * PER;
+    int j = blockIdx.y * PER + lane / L;
+    float x[16];
+    auto fetch = [&]() {
+        const bool val = j >= a.heads;
+        if (j >= 2 * a.heads || d0 >= (val ? DV : DK)) return;
+        const T* p = val ? v + r * v_row + (j - a.heads) * v_head + d0 : k + r * k_row + j * k_head + d0;
+        load8(p, vec, x);
+        load8(p + 8, vec, x + 8);
+    };
+    fetch();
     int s, first, n;
     if (!kv4_find_row(a, r, lane, &s, &first, &n)) return;
     const long long pos = (long long)__ldg(a.lens + s) - n + (r - first);
     uint8_t* tile0 = kv4_tile_of(a, s, pos, TB);
     if (!tile0) return;
-    const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
-    const int step = gridDim.y * PER;
-    for (int j0 = blockIdx.y * PER + lane / L; j0 - lane / L < 2 * a.heads; j0 += ROW_AHEAD * step) {
-        float x[ROW_AHEAD][8];
-        bool on[ROW_AHEAD];
+    const int slot = (int)(pos % KV4_TILE);
+    while (true) {
+        const bool val = j >= a.heads;
+        const int h = val ? j - a.heads : j, D = val ? DV : DK;
+        const bool on = j < 2 * a.heads && d0 < D;
+        float lo = FLT_MAX, hi = -FLT_MAX;
+        bool bad = false;
+        if (on) {
+            f32x2 zero = 0;  // NaN where a value is not finite
 #pragma unroll
-        for (int w = 0; w < ROW_AHEAD; w++) {
-            const int j = j0 + w * step;
-            const bool val = j >= a.heads;
-            const int h = val ? j - a.heads : j;
-            on[w] = j < 2 * a.heads && d0 < (val ? DV : DK);
-            if (on[w]) load8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x[w]);
+            for (int i = 0; i < 16; i += 2) zero = fma2(pair(x[i], x[i + 1]), 0, zero);
+#pragma unroll
+            for (int i = 0; i < 16; i++) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
+            const float2 z = unpair(zero);
+            bad = !(z.x == 0.f && z.y == 0.f);
         }
 #pragma unroll
-        for (int w = 0; w < ROW_AHEAD; w++) {
-            const int j = j0 + w * step;
-            if (j - lane / L >= 2 * a.heads) break;  // for the whole warp
-            const bool val = j >= a.heads;
-            const int h = val ? j - a.heads : j, D = val ? DV : DK;
-            float lo = FLT_MAX, hi = -FLT_MAX;
-            bool bad = false;
-            if (on[w]) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    bad |= !(fabsf(x[w][i]) <= FLT_MAX);
-                    lo = fminf(lo, x[w][i]);
-                    hi = fmaxf(hi, x[w][i]);
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < L; o *= 2) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-            bad = (bads >> (lane & ~(L - 1)) & ((1ull << L) - 1)) != 0;
-            if (!on[w]) continue;
+        for (int o = 1; o < L; o *= 2) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        bad = (__ballot_sync(0xffffffffu, bad) >> (lane & ~(L - 1)) & ((1u << L) - 1)) != 0;
+        if (on) {
             __half sh = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), 65504.0f));
             __half mh = __float2half_rn(fminf(fmaxf(lo, -65504.0f), 65504.0f));
-            const float sf = __half2float(sh), mf = __half2float(mh);
-            uint32_t codes = 0;
-            if (bad) {
-                sh = mh = __ushort_as_half(0x7fff);
-            } else if (sf > 0.f) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[w][i], mf), sf)), 0.f), 15.f);
-                    codes |= (uint32_t)(int)c << (4 * i);
-                }
-            }
+            if (bad) sh = mh = __ushort_as_half(0x7fff);
+            const uint2 w = codes_of(x, __half2float(sh), __half2float(mh));
             uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
-            *(uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub) = codes;
+            *(uint2*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 8 * sub) = w;
             if (sub == 0) *(__half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot) = __halves2half2(sh, mh);
         }
+        j += step;
+        if (j - lane / L >= 2 * a.heads) break;
+        fetch();
     }
 }
 
@@ -111,37 +138,33 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) kv4_read_kernel(Kv4Args a, T* 
     } else if (!zero_rest) {
         return;
     }
-    const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 8 * sub;
-    const int step = gridDim.y * PER;
-    for (int j0 = blockIdx.y * PER + lane / L; j0 < 2 * a.heads; j0 += ROW_AHEAD * step) {
-        uint32_t codes[ROW_AHEAD], params[ROW_AHEAD];
-        bool on[ROW_AHEAD];
-#pragma unroll
-        for (int w = 0; w < ROW_AHEAD; w++) {
-            const int j = j0 + w * step;
-            const bool val = j >= a.heads;
-            const int h = val ? j - a.heads : j, D = val ? DV : DK;
-            on[w] = j < 2 * a.heads && d0 < D;
-            codes[w] = params[w] = 0;  // no such position: zeros
-            if (on[w] && tile0) {
-                const uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
-                codes[w] = *(const uint32_t*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 4 * sub);
-                params[w] = *(const uint32_t*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot);
-            }
+    const int slot = (int)(pos % KV4_TILE), sub = lane % L, d0 = 16 * sub;
+#pragma unroll 2
+    for (int j = blockIdx.y * PER + lane / L; j < 2 * a.heads; j += gridDim.y * PER) {
+        const bool val = j >= a.heads;
+        const int h = val ? j - a.heads : j, D = val ? DV : DK;
+        if (d0 >= D) continue;
+        uint2 w = make_uint2(0, 0);  // no such position: zeros
+        float2 sm = make_float2(0.f, 0.f);
+        if (tile0) {
+            const uint8_t* t = tile0 + (size_t)h * a.page_tiles * TB;
+            w = *(const uint2*)(t + (val ? 8 * DK : 0) + slot * (D / 2) + 8 * sub);
+            sm = __half22float2(*(const __half2*)(t + 8 * (DK + DV) + (val ? 64 : 0) + 4 * slot));
         }
+        float x[16];
+        // 2^23 + c has the code in its low bits; the product of an f16 and a
+        // code is exact: one rounding
+        const f32x2 s2 = pair(sm.x, sm.x), m2 = pair(sm.y, sm.y), down = pair(-8388608.f, -8388608.f);
 #pragma unroll
-        for (int w = 0; w < ROW_AHEAD; w++) {
-            if (!on[w]) continue;
-            const int j = j0 + w * step;
-            const bool val = j >= a.heads;
-            const int h = val ? j - a.heads : j;
-            const float2 sm = __half22float2(*(const __half2*)&params[w]);
-            float x[8];
-            // the product of an f16 and a code is exact: one rounding
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = __fmaf_rn(sm.x, (float)((codes[w] >> (4 * i)) & 15), sm.y);
-            store8(val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0, vec, x);
+        for (int i = 0; i < 16; i += 2) {
+            const uint32_t c = (i < 8 ? w.x : w.y) >> (4 * (i % 8));
+            const f32x2 f = add2(pair(__uint_as_float((c & 15) | 0x4b000000u), __uint_as_float((c >> 4 & 15) | 0x4b000000u)), down);
+            const float2 y = unpair(fma2(s2, f, m2));
+            x[i] = y.x, x[i + 1] = y.y;
         }
+        T* p = val ? v + r * v_row + h * v_head + d0 : k + r * k_row + h * k_head + d0;
+        store8(p, vec, x);
+        store8(p + 8, vec, x + 8);
     }
 }
 

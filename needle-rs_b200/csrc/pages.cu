@@ -144,6 +144,30 @@ __device__ __forceinline__ int block_scan(int mine, int* before) {
     return __shfl_sync(0xffffffffu, w, 31);
 }
 
+// The same of two numbers at once.
+__device__ __forceinline__ int2 block_scan2(int2 mine, int2* before) {
+    __shared__ int2 warp_sums[PG_BLOCK / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int2 incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+        if (lane >= o) incl.x += x, incl.y += y;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    int2 w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, w.x, o), y = __shfl_up_sync(0xffffffffu, w.y, o);
+        if (lane >= o) w.x += x, w.y += y;
+    }
+    const int ux = __shfl_sync(0xffffffffu, w.x, max(warp - 1, 0)), uy = __shfl_sync(0xffffffffu, w.y, max(warp - 1, 0));
+    *before = make_int2(incl.x - mine.x + (warp ? ux : 0), incl.y - mine.y + (warp ? uy : 0));
+    return make_int2(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31));
+}
+
 // Sum of sums[0 .. n) by a block.
 __device__ __forceinline__ int block_total(const int32_t* sums, int n) {
     int mine = 0, before;
@@ -191,41 +215,61 @@ __global__ void __launch_bounds__(PG_BLOCK) fork_lists_kernel(ForkArgs a, int pa
     }
 }
 
-// All passes of a fork but the last, by one cluster; its CTAs have equal
-// slices of the pages and of the sequences. The totals go to sums[0], sums[1].
+// All passes of a fork but the last, by one cluster. A thread has a run of
+// pages and one of sequences, so that one prefix sum places both. The totals
+// go to sums[0], sums[1].
 __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_BLOCK) fork_plan_kernel(ForkArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
+    constexpr int ALL = PG_CLUSTER * PG_BLOCK, SEQS = PG_BLOCK;
     const int rank = cluster.block_rank(), tid = threadIdx.x, all = rank * PG_BLOCK + tid;
-    __shared__ int mine[2];
-    for (int i = all; i < a.pages; i += PG_CLUSTER * PG_BLOCK) a.refs[i] = a.writers[i] = a.first[i] = 0;
-    cluster.sync();
-    for (int d = all / 32; d < a.n; d += PG_CLUSTER * PG_BLOCK / 32) count_kept(a, d, tid & 31);
-    cluster.sync();
-    const int pages_each = (a.pages + PG_CLUSTER - 1) / PG_CLUSTER, seqs_each = (a.n + PG_CLUSTER - 1) / PG_CLUSTER;
-    const int p0 = rank * pages_each, p1 = min(p0 + pages_each, a.pages), d0 = rank * seqs_each, d1 = min(d0 + seqs_each, a.n);
-    int frees = 0, wanted = 0, x;
-    for (int p = p0 + tid; p < p1; p += PG_BLOCK) frees += page_free(a, p);
-    for (int d = d0 + tid; d < d1; d += PG_BLOCK) wanted += a.fresh[d] = fresh_wanted(a, d);
-    frees = block_scan(frees, &x);
-    wanted = block_scan(wanted, &x);
-    if (tid == 0) mine[0] = frees, mine[1] = wanted;
-    cluster.sync();
-    int free0 = 0, want0 = 0;
-    for (int r = 0; r < rank; r++) free0 += cluster.map_shared_rank(mine, r)[0], want0 += cluster.map_shared_rank(mine, r)[1];
-    for (int p = p0; p < p1; p += PG_BLOCK) {
-        const bool is = p + tid < p1 && page_free(a, p + tid);
-        const int sum = block_scan(is, &x);
-        if (is) a.free_ids[free0 + x] = p + tid;
-        free0 += sum;
+    __shared__ int2 mine;
+    __shared__ Kept kept[SEQS];
+    for (int i = all; i < a.pages; i += ALL) a.refs[i] = a.writers[i] = a.first[i] = 0;
+    // what this CTA's sequences keep, SEQS at a time; then their table entries
+    const int each = (a.n + PG_CLUSTER - 1) / PG_CLUSTER, d0 = rank * each, d1 = min(d0 + each, a.n);
+    bool zeroed = false;
+    for (int base = d0; base < d1 || !zeroed; base += SEQS) {
+        const int n = max(min(SEQS, d1 - base), 0);
+        __syncthreads();
+        if (tid < n) kept[tid] = kept_of(a, base + tid);
+        if (!zeroed) cluster.sync(), zeroed = true;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid; i < n * a.cols; i += PG_BLOCK) {
+            const int s = i / a.cols, c = i - s * a.cols;
+            const Kept& k = kept[s];
+            if (c >= k.nk) continue;
+            const int p = __ldg(k.row + c);
+            if (p < 0 || p >= a.pages) continue;
+            atomicAdd(a.refs + p, 1);
+            if (k.writes && c == k.nk - 1) {
+                atomicAdd(a.writers + p, 1);
+                atomicMax(a.first + p, a.n - (base + s));
+            }
+        }
     }
-    for (int d = d0; d < d1; d += PG_BLOCK) {
-        const int f = d + tid < d1 ? a.fresh[d + tid] : 0;  // this thread's own, from above
-        const int sum = block_scan(f, &x);
-        if (d + tid < d1) a.base[d + tid] = want0 + x;
-        want0 += sum;
+    cluster.sync();
+    const int pages_each = (a.pages + ALL - 1) / ALL, seqs_each = (a.n + ALL - 1) / ALL;
+    const int p0 = min(all * pages_each, a.pages), p1 = min(p0 + pages_each, a.pages);
+    const int s0 = min(all * seqs_each, a.n), s1 = min(s0 + seqs_each, a.n);
+    int2 own = make_int2(0, 0), before;
+    for (int p = p0; p < p1; p++) own.x += page_free(a, p);
+    for (int d = s0; d < s1; d++) own.y += a.fresh[d] = fresh_wanted(a, d);
+    const int2 sum = block_scan2(own, &before);
+    if (tid == 0) mine = sum;
+    cluster.sync();
+    for (int r = 0; r < rank; r++) {
+        const int2 m = *cluster.map_shared_rank(&mine, r);
+        before.x += m.x, before.y += m.y;
     }
-    if (rank == PG_CLUSTER - 1 && tid == 0) a.sums[0] = free0, a.sums[1] = want0, a.info[2] = 0;
+    for (int p = p0; p < p1; p++)
+        if (page_free(a, p)) a.free_ids[before.x++] = p;
+    for (int d = s0; d < s1; d++) {
+        a.base[d] = before.y;
+        before.y += a.fresh[d];  // this thread's own, from above
+    }
+    if (all == ALL - 1) a.sums[0] = before.x, a.sums[1] = before.y, a.info[2] = 0;
     cluster.sync();  // no CTA leaves while others read its counts
 }
 
@@ -372,53 +416,49 @@ __global__ void __launch_bounds__(PG_BLOCK) compact_lists_kernel(CompactArgs a) 
 __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_BLOCK) compact_plan_kernel(CompactArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
+    constexpr int ALL = PG_CLUSTER * PG_BLOCK;
     const int rank = cluster.block_rank(), tid = threadIdx.x, all = rank * PG_BLOCK + tid;
-    __shared__ int mine[3];
-    for (int i = all; i < a.pages; i += PG_CLUSTER * PG_BLOCK) a.refs[i] = 0;
+    __shared__ int2 mine;
+    __shared__ int early;  // of the first CTA: movable pages before n
+    for (int i = all; i < a.pages; i += ALL) a.refs[i] = 0;
     cluster.sync();
-    for (long long i = all; i < (long long)a.seqs * a.cols; i += PG_CLUSTER * PG_BLOCK) {
-        const int p = __ldg(a.table + (size_t)(i / a.cols) * a.table_stride + i % a.cols);
+    const int entries = a.seqs * a.cols;
+#pragma unroll 4
+    for (int i = all; i < entries; i += ALL) {
+        const int s = i / a.cols, p = __ldg(a.table + (size_t)s * a.table_stride + (i - s * a.cols));
         if (p >= 0 && p < a.pages) a.refs[p] = 1;
     }
     cluster.sync();
-    const int each = (a.pages + PG_CLUSTER - 1) / PG_CLUSTER, p0 = rank * each, p1 = min(p0 + each, a.pages);
-    int live = 0, move = 0, x;
-    for (int p = p0 + tid; p < p1; p += PG_BLOCK) {
+    const int each = (a.pages + ALL - 1) / ALL, p0 = min(all * each, a.pages), p1 = min(p0 + each, a.pages);
+    int2 own = make_int2(0, 0), before;
+    for (int p = p0; p < p1; p++) {
         const int2 st = page_state(a, p);
-        live += st.x, move += st.y;
+        own.x += st.x, own.y += st.y;
     }
-    live = block_scan(live, &x);
-    move = block_scan(move, &x);
-    if (tid == 0) mine[0] = live, mine[1] = move;
+    const int2 sum = block_scan2(own, &before);
+    if (tid == 0) mine = sum;
     cluster.sync();
-    int n = 0, live0 = 0, move0 = 0, moves = 0;
+    int n = 0, moves = 0;
     for (int r = 0; r < PG_CLUSTER; r++) {
-        const int* m = cluster.map_shared_rank(mine, r);
-        if (r < rank) live0 += m[0], move0 += m[1];
-        n += m[0], moves += m[1];
+        const int2 m = *cluster.map_shared_rank(&mine, r);
+        if (r < rank) before.x += m.x, before.y += m.y;
+        n += m.x, moves += m.y;
     }
-    // movable pages of this slice before n
-    int early = 0;
-    for (int p = p0 + tid; p < min(p1, n); p += PG_BLOCK) early += page_state(a, p).y;
-    early = block_scan(early, &x);
-    if (tid == 0) mine[2] = early;
+    if (p0 < n ? n <= p1 : all == 0 && n == 0) {  // the run that n lies in or ends
+        int e = before.y;
+        for (int p = p0; p < n; p++) e += page_state(a, p).y;
+        *cluster.map_shared_rank(&early, 0) = e;
+    }
     cluster.sync();
-    int before_n = 0;
-    for (int r = 0; r < PG_CLUSTER; r++) before_n += cluster.map_shared_rank(mine, r)[2];
-    for (int b = p0; b < p1; b += PG_BLOCK) {
-        const int p = b + tid;
-        const int2 st = p < p1 ? page_state(a, p) : make_int2(0, 0);
-        int l, m;
-        const int ls = block_scan(st.x, &l), ms = block_scan(st.y, &m);
-        l += live0, m += move0;
-        live0 += ls, move0 += ms;
-        if (p < p1) {
-            a.before[p] = m - before_n;
-            if (p >= n && st.y) a.movers[m - before_n] = p;
-            if (p < n && !st.x) a.holes[p - l] = p;
-        }
+    const int before_n = *cluster.map_shared_rank(&early, 0);
+    for (int p = p0; p < p1; p++) {
+        const int2 st = page_state(a, p);
+        a.before[p] = before.y - before_n;
+        if (p >= n && st.y) a.movers[before.y - before_n] = p;
+        if (p < n && !st.x) a.holes[p - before.x] = p;
+        before.x += st.x, before.y += st.y;
     }
-    if (rank == 0 && tid == 0) {
+    if (all == 0) {
         a.sums[0] = make_int2(n, moves - before_n);
         a.info[0] = n;
         a.info[1] = moves - before_n;

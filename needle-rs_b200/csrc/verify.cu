@@ -33,16 +33,17 @@ namespace nd {
 
 namespace cg = cooperative_groups;
 
-constexpr int VF_MAX_DRAFT = 64, VF_MAX_SEQS = 1 << 20;
+constexpr int VF_MAX_DRAFT = 64, VF_MAX_SEQS = 1 << 20, VF_MAX_V = 1 << 30;
 constexpr int VF_STATS = 256;        // threads of the first kernel
 constexpr int VF_CHUNK = 4096;       // logits a CTA of it takes at a time
 constexpr int VF_MAX_PARTS = 32;
 constexpr int VF_DRAW = 256, VF_WARPS = VF_DRAW / 32;  // of the second
-constexpr int VF_CACHE = 512;        // f64 terms of its run that a warp keeps
+constexpr int VF_CACHE = 512, BATCH = 4;  // values of its run that a warp keeps; that a lane takes at a time
 constexpr float LOG2E = 1.4426950408889634f;
 
-// Of a row, or a part of it: the largest logit, its first place (-1: a NaN is
-// there), and sum exp((l - top) / temperature).
+// Of a row, or a part of it: the largest logit; its first place where the
+// draw is greedy, else 0 (-1: no distribution, a NaN is there); sum exp((l -
+// top) / temperature) where it is not greedy.
 struct RowStats {
     float top;
     int at;
@@ -88,7 +89,9 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts, s = r / (a.T + 1), i = r % (a.T + 1), tid = threadIdx.x;
     if (i > drafts_of(a, s)) return;
-    const float scale2 = Temperature(__ldg(a.temp + s)).scale2;
+    const Temperature tp(__ldg(a.temp + s));
+    const float scale2 = tp.scale2;
+    const bool greedy = tp.greedy;
     const T* row = logits + s * a.l_seq + i * a.l_row;
     const int chunks = (a.V + VF_CHUNK - 1) / VF_CHUNK, per = (chunks + a.parts - 1) / a.parts;
     const int lo = min(part * per, chunks), hi = min(lo + per, chunks);
@@ -128,17 +131,27 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
                 x[j] = p < a.V ? (float)row[p] : -INFINITY;
             }
         }
-        float m = top;
+        if (greedy) {  // the place; NaN by itself
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            nan |= x[j] != x[j];
-            if (x[j] > m) m = x[j], at = base + (j / PER * VF_STATS + tid) * PER + j % PER;
+            for (int j = 0; j < N; j++) {
+                nan |= x[j] != x[j];
+                if (x[j] > top) top = x[j], at = base + (j / PER * VF_STATS + tid) * PER + j % PER;
+            }
+        } else {  // the sum, which a NaN spoils, as +infinity does
+            float m = top;
+#pragma unroll
+            for (int j = 0; j < N; j++) m = fmaxf(m, x[j]);
+            if (m == -INFINITY) {
+#pragma unroll
+                for (int j = 0; j < N; j++) nan |= x[j] != x[j];
+                continue;
+            }
+            if (m > top) sum *= vf_ex2((top - m) * scale2), top = m;  // top = -infinity: sum is 0
+#pragma unroll
+            for (int j = 0; j < N; j++) sum += vf_ex2((x[j] - top) * scale2);
         }
-        if (m == -INFINITY) continue;
-        if (m > top) sum *= vf_ex2((top - m) * scale2), top = m;  // top = -infinity: sum is 0
-#pragma unroll
-        for (int j = 0; j < N; j++) sum += vf_ex2((x[j] - top) * scale2);
     }
+    if (!greedy) nan |= sum != sum, at = top > -INFINITY ? 0 : a.V;
     // the block's largest, its first place, the sum against it
     __shared__ float tops[VF_STATS / 32];
     __shared__ int ats[VF_STATS / 32];
@@ -172,9 +185,37 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
     }
 }
 
+// exp(x) for x <= 0 (NaN stays), without branches, so that the terms of a run
+// overlap: x = k ln 2 + r with ln 2 in two parts (Cody and Waite; the first
+// has 40 bits, k times it is exact), Taylor's series to r^13 (|r| <= 0.35:
+// 4e-18 left), times 2^k. Within 2^-52 of itself; below e^-708, 0.
+__device__ __forceinline__ double exp_below(double x) {
+    const bool tiny = x < -708.0;
+    const double y = tiny ? -708.0 : x;
+    const double t = __fma_rn(y, 1.4426950408889634, 6755399441055744.0);  // 1.5 * 2^52: its low bits hold k
+    const double k = t - 6755399441055744.0;
+    const double r = __fma_rn(k, 1.7239444525614835e-13, __fma_rn(k, -0.6931471805601177, y));
+    double p = 1.6059043836821613e-10;
+    p = __fma_rn(p, r, 2.08767569878681e-09);  // 1 / 12!
+    p = __fma_rn(p, r, 2.505210838544172e-08);  // 1 / 11!
+    p = __fma_rn(p, r, 2.755731922398589e-07);  // 1 / 10!
+    p = __fma_rn(p, r, 2.7557319223985893e-06);  // 1 / 9!
+    p = __fma_rn(p, r, 2.48015873015873e-05);  // 1 / 8!
+    p = __fma_rn(p, r, 0.0001984126984126984);  // 1 / 7!
+    p = __fma_rn(p, r, 0.001388888888888889);  // 1 / 6!
+    p = __fma_rn(p, r, 0.008333333333333333);  // 1 / 5!
+    p = __fma_rn(p, r, 0.041666666666666664);  // 1 / 4!
+    p = __fma_rn(p, r, 0.16666666666666666);  // 1 / 3!
+    p = __fma_rn(p, r, 0.5);
+    p = __fma_rn(p, r, 1.0);
+    p = __fma_rn(p, r, 1.0);
+    const double e = p * __hiloint2double((__double2loint(t) + 1023) << 20, 0);
+    return tiny ? 0.0 : e;
+}
+
 template <typename T>
 __device__ __forceinline__ double term(const T* row, int j, float top, double inv) {
-    return exp(((double)(float)row[j] - (double)top) * inv);
+    return exp_below(((double)(float)row[j] - (double)top) * inv);
 }
 
 __device__ __forceinline__ double warp_sum(double x) {
@@ -287,13 +328,27 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
     const int gone = kept < n && !a.q ? __ldg(a.draft + (size_t)s * T_ + kept) : -1;
     const int runs = C * VF_WARPS, run = rank * VF_WARPS + warp;
     const int per = ((V + runs - 1) / runs + 31) / 32 * 32, lo = (int)min((long long)run * per, (long long)V), hi = min(lo + per, V);
-    double* cache = cache_all + warp * VF_CACHE;
+    double* cache = cache_all + warp * VF_CACHE;  // the run's terms, then what can be drawn of it
+    const bool fits = per <= VF_CACHE;
+    // BATCH values at j, j + stride, .. at a time, without branches between
+    // them, so that their loads and their chains of products overlap
+    auto terms = [&](int j, int stride, double* e) {
+        float x[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) x[k] = (float)row[min(j + k * stride, V - 1)];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) e[k] = exp_below(((double)x[k] - (double)st.top) * tp.inv);
+    };
     double mine = 0.0;
-#pragma unroll 4
-    for (int j = lo + lane; j < hi; j += 32) {
-        const double e = term(row, j, st.top, tp.inv);
-        if (j - lo < VF_CACHE) cache[j - lo] = e;
-        mine += e;
+    for (int j = lo + lane; j - lane < hi; j += 32 * BATCH) {
+        double e[BATCH];
+        terms(j, 32, e);
+#pragma unroll
+        for (int k = 0; k < BATCH; k++)
+            if (j + 32 * k < hi) {
+                if (fits) cache[j + 32 * k - lo] = e[k];
+                mine += e[k];
+            }
     }
     mine = warp_sum(mine);
     if (lane == 0) sums[0][warp] = mine;
@@ -320,20 +375,33 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
     };
     const double iz = 1.0 / gather(0);
     bool whole = false;  // p itself, where the residual is all zero
-    auto weight = [&](int j) {
-        const double p = (j - lo < VF_CACHE ? cache[j - lo] : term(row, j, st.top, tp.inv)) * iz;
-        if (whole) return p;
-        if (q) {
-            const double r = p - (double)__ldg(q + j);
-            return r < 0.0 ? 0.0 : r;
+    // what can be drawn of those values (0 from `end` on)
+    auto weights = [&](int j, int stride, int end, double* w) {
+        if (fits) {
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) w[k] = cache[max(min(j + k * stride, hi - 1) - lo, 0)];
+        } else {
+            terms(j, stride, w);
         }
-        return j == gone ? 0.0 : p;
+        float qv[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) qv[k] = q && !whole ? __ldg(q + min(j + k * stride, V - 1)) : 0.f;
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+            double r = w[k] * iz - (double)qv[k];
+            if (r < 0.0 || j + k * stride >= end || (j + k * stride == gone && !whole)) r = 0.0;
+            w[k] = r;
+        }
     };
     double total;
     while (true) {
         mine = 0.0;
-#pragma unroll 4
-        for (int j = lo + lane; j < hi; j += 32) mine += weight(j);
+        for (int j = lo + lane; j - lane < hi; j += 32 * BATCH) {
+            double w[BATCH];
+            weights(j, 32, hi, w);
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) mine += w[k];
+        }
         mine = warp_sum(mine);
         if (lane == 0) sums[1][warp] = mine;
         total = gather(1);
@@ -361,20 +429,41 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
         at = __shfl_sync(0xffffffffu, passed ? at : last, from);
         before = __shfl_sync(0xffffffffu, passed ? before : last_before, from);
         if (at == run) {
-            int token = -1;
-            for (int j0 = lo; j0 < hi; j0 += 32) {
-                const double w = j0 + lane < hi ? weight(j0 + lane) : 0.0;
-                double incl = w;
+            // the lanes share the run, per / 32 values each in order, and all
+            // of them the values of the one that holds the place
+            auto prefix = [&](double w, double* incl) {
+                *incl = w;
 #pragma unroll
                 for (int k = 1; k < 32; k *= 2) {
-                    const double up = __shfl_up_sync(0xffffffffu, incl, k);
-                    if (lane >= k) incl += up;
+                    const double up = __shfl_up_sync(0xffffffffu, *incl, k);
+                    if (lane >= k) *incl += up;
                 }
-                const uint32_t some = __ballot_sync(0xffffffffu, w > 0.0);
-                const uint32_t past = __ballot_sync(0xffffffffu, w > 0.0 && before + incl > target);
-                if (some) token = j0 + 31 - __clz(some);  // should the sums' last bits differ: the last one
-                if (passed && past) {
-                    token = j0 + __ffs(past) - 1;
+            };
+            const int each = per / 32;
+            double own = 0.0, incl;
+            bool some = false;
+            for (int j = lo + lane * each, end = min(j + each, hi); __any_sync(0xffffffffu, j < end); j += BATCH) {
+                double w[BATCH];
+                weights(j, 1, end, w);
+#pragma unroll
+                for (int k = 0; k < BATCH; k++) own += w[k], some |= w[k] > 0.0;
+            }
+            prefix(own, &incl);
+            // should the sums' last bits differ, the last lane that has something
+            const uint32_t past = __ballot_sync(0xffffffffu, some && passed && before + incl > target);
+            const int from = past ? __ffs(past) - 1 : 31 - __clz(__ballot_sync(0xffffffffu, some));
+            before += __shfl_sync(0xffffffffu, incl - own, from);
+            int token = -1;
+            for (int j0 = lo + from * each, end = min(j0 + each, hi); j0 < end; j0 += 32) {
+                double ws[BATCH];
+                weights(j0 + lane, 32, min(end, j0 + 32), ws);  // one each: the others lie past the end
+                const double w = ws[0];
+                prefix(w, &incl);
+                const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0);
+                const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && past && before + incl > target);
+                if (any) token = j0 + 31 - __clz(any);
+                if (hit) {
+                    token = j0 + __ffs(hit) - 1;
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, incl, 31);
@@ -429,7 +518,7 @@ using namespace nd;
 extern "C" {
 
 unsigned long long nd_op_verify_ws(int seqs, int T, int V) {
-    return seqs < 1 || seqs > VF_MAX_SEQS || T < 0 || T > VF_MAX_DRAFT || V < 1 ? 0 : verify_ws(seqs, T, V);
+    return seqs < 1 || seqs > VF_MAX_SEQS || T < 0 || T > VF_MAX_DRAFT || V < 1 || V > VF_MAX_V ? 0 : verify_ws(seqs, T, V);
 }
 
 int nd_op_verify(int device, int type, const void* logits, long long l_seq, long long l_row, const int* draft,
@@ -440,8 +529,8 @@ int nd_op_verify(int device, int type, const void* logits, long long l_seq, long
         const char* what = "nd_op_verify";
         auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
         if (type != ND_F32 && type != ND_F16 && type != ND_BF16) fail("unknown type");
-        if (seqs < 1 || seqs > VF_MAX_SEQS || T < 0 || T > VF_MAX_DRAFT || V < 1)
-            fail("needs 1 to 2^20 sequences, 0 to 64 drafted tokens, V >= 1");
+        if (seqs < 1 || seqs > VF_MAX_SEQS || T < 0 || T > VF_MAX_DRAFT || V < 1 || V > VF_MAX_V)
+            fail("needs 1 to 2^20 sequences, 0 to 64 drafted tokens, 1 <= V <= 2^30");
         if (!logits || !u || !temperature || !tokens || !accepted || !probs || (T && !draft)) fail("null pointer");
         const int e = type == ND_F32 ? 4 : 2;
         if ((uintptr_t)logits % e || (uintptr_t)q % 4) fail("logits and q must be aligned to their types");
@@ -455,9 +544,9 @@ int nd_op_verify(int device, int type, const void* logits, long long l_seq, long
         a.stats = (RowStats*)ws;
         a.tokens = tokens, a.accepted = accepted, a.probs = probs;
         OnDevice on(device, what);
-        // CTAs a drawn row: until they fill the GPU or a warp's run is short
+        // CTAs a drawn row: until a warp's terms fit its cache, or while they do not fill the GPU and runs are not short
         int ctas = 1;
-        while (ctas < 8 && seqs * ctas < 2 * device_sm_count() && V > 1024 * ctas) ctas *= 2;
+        while (ctas < 8 && V > 1024 * ctas && (V > VF_WARPS * VF_CACHE * ctas || seqs * ctas < 2 * device_sm_count())) ctas *= 2;
         cudaStream_t st = (cudaStream_t)stream;
         if (type == ND_F32) verify_launch<float>(a, logits, ctas, st);
         else if (type == ND_F16) verify_launch<__half>(a, logits, ctas, st);

@@ -254,5 +254,5 @@ def test_entry_point_refuses_without_a_gpu():
 
     for bad, message in ((dict(type=3), b"type"), (dict(logits=None), b"null"), (dict(logits=4098), b"aligned"), (dict(q=4097), b"aligned"),
                          (dict(row=-1), b"negative"), (dict(draft=None), b"null"), (dict(seqs=0), b"sequences"),
-                         (dict(T=65), b"64"), (dict(T=-1), b"64"), (dict(V=0), b"V >= 1"), (dict(tokens=None), b"null"), (dict(ws=None), b"workspace"), (dict(nbytes=8), b"workspace")):
+                         (dict(T=65), b"64"), (dict(T=-1), b"64"), (dict(V=0), b"1 <= V"), (dict(tokens=None), b"null"), (dict(ws=None), b"workspace"), (dict(nbytes=8), b"workspace")):
         assert verify(**bad) == -1 and message in lib.nd_last_error(), bad
