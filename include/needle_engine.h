@@ -333,7 +333,7 @@ int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long lo
  * that sees nothing. out must not overlap q. ws:
  * nd_op_kv4_attend_ws(the same arguments) bytes, 16-byte aligned; NULL where
  * that is 0. */
-unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads, int window, int sink);
+unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int type, int q_heads, int window, int sink);
 int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row, long long q_head, int q_heads, float scale,
                      int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
                      int flags, void* stream);

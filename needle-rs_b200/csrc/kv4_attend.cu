@@ -46,7 +46,7 @@
 #include <cstring>
 
 #include "kernels.h"
-#include "kv4.cuh"
+#include "kv4_attend.cuh"
 #include "kv4_host.h"
 
 namespace nd {
@@ -65,29 +65,10 @@ constexpr int ATT_UNIT_COST = 4;
 // second kernel. Measured (us, with cut units, a warp, a CTA a unit): 32
 // sequences of up to 256 positions 14.4, 10.1, 6.7; 512 of them -, 15.4, 18.0;
 // 32 of up to 1000 14.9, -, 11.1.
+// Query rows a sequence brings to a kv head on average from which 16-bit rows
+// go to the tcgen05 kernel.
+constexpr int ATT_TC_ROWS = 192;
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
-
-// n / d for 0 <= n < 2^31 by a multiplication.
-struct FastDiv {
-    uint32_t d, mul, shift;
-    FastDiv(uint32_t x = 1) : d(x), mul(0), shift(0) {
-        while ((1ull << shift) < d) shift++;
-        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
-    }
-    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
-};
-
-struct AttendArgs {
-    Kv4Args kv;
-    long long q_row, q_head, o_row, o_head;
-    FastDiv group;       // query heads a kv head
-    FastDiv page_tiles;
-    int window, sink, places;
-    float scale_log2e;
-    bool q_vec, o_vec, zero_rest;
-    float* parts;   // [runners][2][8 NT * (DV + 2)]; a runner is a warp, for NT = 1 a CTA
-    int4* joins;    // [runners]: (sequence, kv head, query block, further runners) of the cut unit that starts there, w < 0: none
-};
 
 // Whole units are numbered without sums. Places 0 .. seqs - 1 are the
 // sequences' first blocks; the further blocks of sequence s are at most the
@@ -116,47 +97,6 @@ __device__ __forceinline__ int seq_of_place(const AttendArgs& a, int u, int lane
     return lo - 1;
 }
 
-// The key tiles a block of query rows reads: those of the first `sink`
-// positions, then lo .. of the window.
-struct Tiles {
-    int sink, lo, n;  // n >= 1, so that a block that sees nothing is still written
-    __device__ __forceinline__ int at(int i) const { return i < sink ? i : lo + (i - sink); }
-};
-
-__device__ __forceinline__ Tiles tiles_of(const AttendArgs& a, long long first, long long last) {
-    const int cap = a.kv.max_pages * a.kv.page_tiles * KV4_TILE;  // positions of the table: below 2^31
-    const int end = last < 0 ? 0 : (int)min(last, (long long)cap - 1) / KV4_TILE + 1;
-    Tiles t;
-    t.lo = t.sink = 0;
-    if (a.window > 0) {
-        t.lo = (int)(min(max(first - a.window + 1, 0LL), (long long)cap)) / KV4_TILE;
-        if (a.sink > 0) t.sink = min((min(a.sink, cap) - 1) / KV4_TILE + 1, min(t.lo, end));
-    }
-    t.n = max(1, t.sink + max(0, end - t.lo));
-    return t;
-}
-
-struct SeqRows {
-    int first, n;    // rows of the call
-    long long pos0;  // position of the first
-};
-
-__device__ __forceinline__ SeqRows seq_rows(const AttendArgs& a, int s) {
-    SeqRows r;
-    r.first = kv4_first_row(a.kv, s);
-    r.n = max(kv4_first_row(a.kv, s + 1) - r.first, 0);
-    r.pos0 = (long long)__ldg(a.kv.lens + s) - r.n;
-    return r;
-}
-
-// Query rows of a sequence and kv head are numbered token-major: row x is
-// head x % group of token x / group. Block b holds 8 NT of them.
-template <int NT>
-__device__ __forceinline__ Tiles block_tiles(const AttendArgs& a, const SeqRows& r, int b) {
-    const int x0 = b * 8 * NT, x1 = min(x0 + 8 * NT, r.n * (int)a.group.d) - 1;
-    return tiles_of(a, r.pos0 + a.group(x0), r.pos0 + a.group(x1));
-}
-
 // What a sequence and kv head adds to the list of work: each unit its cost
 // and then its tiles.
 template <int NT>
@@ -167,16 +107,6 @@ __device__ __forceinline__ long long seq_work(const AttendArgs& a, const SeqRows
     return t;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -187,32 +117,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *(const uint32_t*)&h;
-}
-__device__ __forceinline__ float2 unpack_half2(uint32_t x) { return __half22float2(*(const __half2*)&x); }
-// Codes (in the low four bits of each half; in the next four) to f16 c - 8:
-// 1024 + c and 1024 + 16 c are the f16 with those bits under 1024's exponent.
-__device__ __forceinline__ uint32_t code_mid(uint32_t x) {
-    x |= 0x64006400u;
-    uint32_t y;
-    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0xe408e408u));  // -1032
-    return y;
-}
-__device__ __forceinline__ uint32_t code16_mid(uint32_t x) {
-    x |= 0x64006400u;
-    uint32_t y;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
-    return y;
-}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {  // 16 of them, or none and zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-
-// Below every score that is not -infinity: the softmax's reference before the
-// first key is seen.
-constexpr float ATT_LOW = -3.0e38f;
 
 template <int DK, int DV, int NT, typename T>
 struct AttendShape {
@@ -236,18 +143,6 @@ struct AttendShape {
     static constexpr int WARP_SMEM = RING + QBYTES + (MERGE ? 4 * PART : 0);
     static constexpr int SMEM = ATT_WARPS * WARP_SMEM, WHOLE_SMEM = ATT_WARPS * (RING + QBYTES);
     static constexpr int CTAS = ATT_CTAS(NT, DV);
-};
-
-// Where query row x of a sequence and kv head has its result.
-template <typename T>
-struct OutRows {
-    T* out;
-    const AttendArgs& a;
-    int first, h, nrows;
-    __device__ __forceinline__ T* at(int x) const {
-        const int tok = a.group(x);
-        return out + (long long)(first + tok) * a.o_row + (long long)(h * (int)a.group.d + x - tok * (int)a.group.d) * a.o_head;
-    }
 };
 
 // A part of 8 rows as a warp holds it.
@@ -733,15 +628,6 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
     }
 }
 
-// Output rows behind the last sequence, where the caller wants them zero.
-template <int DV, typename T>
-__device__ __forceinline__ void zero_rest(const AttendArgs& a, T* out, int wid, int warps, int lane) {
-    if (!a.zero_rest || !a.kv.start) return;
-    for (int r = kv4_first_row(a.kv, a.kv.seqs) + wid; r < a.kv.rows; r += warps)
-        for (int hq = 0; hq < a.kv.heads * (int)a.group.d; hq++)
-            for (int d = lane; d < DV; d += 32) out[r * a.o_row + hq * a.o_head + d] = (T)0.f;
-}
-
 // Short units without sums over the sequences and without joins. SHARED: a
 // CTA a unit, its warps share the tiles and join their parts in shared
 // memory; else a warp a unit. blockIdx.x counts places, blockIdx.y kv heads.
@@ -947,38 +833,6 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
     }
 }
 
-// out = sum_w 2^(M_w - M) acc_w / sum_w 2^(M_w - M) l_w over the runners w
-// that share a unit, in their order. A CTA per runner of the first kernel;
-// those where no cut unit starts return at once.
-template <int DV, int NT, typename T>
-__global__ void __launch_bounds__(512) kv4_join_kernel(AttendArgs a, T* __restrict__ out) {
-    constexpr int PART = 8 * NT * (DV + 2), ROWS = 512 / DV;
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const int4 job = a.joins[blockIdx.x];
-    if (job.w < 0) return;
-    const SeqRows rows = seq_rows(a, job.x);
-    const OutRows<T> to{out, a, rows.first, job.y, rows.n * (int)a.group.d};
-    const float* part = a.parts + (size_t)blockIdx.x * 2 * PART;
-    const int d = threadIdx.x % DV;
-    for (int y = threadIdx.x / DV; y < 8 * NT; y += ROWS) {
-        const int x = job.z * 8 * NT + y;
-        if (x >= to.nrows) return;
-        // the starting runner's second slot, then the first slot of each further one
-        float M = part[PART + 8 * NT * DV + y];
-#pragma unroll 8
-        for (int i = 1; i <= job.w; i++) M = fmaxf(M, part[(size_t)i * 2 * PART + 8 * NT * DV + y]);
-        float l = 0.f, v = 0.f;
-#pragma unroll 8
-        for (int i = 0; i <= job.w; i++) {
-            const float* p = part + (i ? (size_t)i * 2 * PART : PART);
-            const float r = ex2(p[8 * NT * DV + y] - M);
-            l = __fmaf_rn(p[8 * NT * (DV + 1) + y], r, l);
-            v = __fmaf_rn(p[y * DV + d], r, v);
-        }
-        to.at(x)[d] = (T)(l == 0.f ? 0.f : v / l);
-    }
-}
-
 // Blocks of 8 query rows, or of 16 where sequences bring many: the wider
 // block halves the unpacking of codes a product, the narrower one splits over
 // more warps and needs fewer registers. Measured (us, 8 against 16 rows): 5
@@ -991,7 +845,8 @@ static int query_tiles(const nd_kv4* kv, int group) {
 // How a call is split:
 // CUT   runs of equal work, units cut where they end, two kernels;
 // WARP  a warp a unit, CTA  four warps a unit: units of few tiles.
-enum AttendMode { CUT, WARP, CTA };
+// ROWS  blocks of 256 rows on tcgen05 (kv4_prefill.cu).
+enum AttendMode { CUT, WARP, CTA, ROWS };
 
 struct AttendPlan {
     int nt, ctas, places;
@@ -1000,8 +855,13 @@ struct AttendPlan {
 };
 
 // Grid and workspace from what the host knows: the sizes, not the lengths.
-static AttendPlan attend_plan(const nd_kv4* kv, int group, int window, int sink) {
-    AttendPlan p;
+static AttendPlan attend_plan(const nd_kv4* kv, int group, int type, int window, int sink) {
+    AttendPlan p{};
+    if (type != ND_F32 && (long long)kv->rows * group >= (long long)ATT_TC_ROWS * kv->seqs) {
+        p.mode = ROWS;
+        p.ws = prefill_ws_bytes(kv->dv, &p.ctas);
+        return p;
+    }
     p.nt = query_tiles(kv, group);
     // tiles a unit can have: the table's, or those of the window (of 8 nt rows' tokens) and the sinks
     const long long table = (long long)kv->max_pages * (kv->page / KV4_TILE);
@@ -1091,14 +951,15 @@ using namespace nd;
 
 extern "C" {
 
-unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int q_heads, int window, int sink) {
+unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int type, int q_heads, int window, int sink) {
     unsigned long long bytes = 0;
     op_call([&] {
         const char* what = "nd_op_kv4_attend_ws";
         kv4_args(kv, what);
         const int group = attend_group(kv, q_heads, window, sink, what);
+        if (type != ND_F32 && type != ND_F16 && type != ND_BF16) throw std::runtime_error("nd_op_kv4_attend_ws: unknown type");
         OnDevice on(kv->device, what);
-        bytes = attend_plan(kv, group, window, sink).ws;
+        bytes = attend_plan(kv, group, type, window, sink).ws;
     });
     return bytes;
 }
@@ -1125,10 +986,11 @@ int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row,
         a.q_vec = kv4_vec(type, q, q_row, q_head), a.o_vec = kv4_vec(type, out, o_row, o_head);
         a.zero_rest = flags & ND_ZERO_REST;
         OnDevice on(kv->device, what);
-        const AttendPlan plan = attend_plan(kv, group, window, sink);
+        const AttendPlan plan = attend_plan(kv, group, type, window, sink);
         if (plan.ws && (!ws || ws_bytes < plan.ws)) fail("the workspace is too small");
         cudaStream_t st = (cudaStream_t)stream;
-        if (kv->dk == 48) attend_type<48, 64>(type, a, plan, q, out, ws, st);
+        if (plan.mode == ROWS) prefill_launch(a, kv->dk, type, q, out, ws, st);
+        else if (kv->dk == 48) attend_type<48, 64>(type, a, plan, q, out, ws, st);
         else if (kv->dk == 64) attend_type<64, 64>(type, a, plan, q, out, ws, st);
         else attend_type<128, 128>(type, a, plan, q, out, ws, st);
     });

@@ -1,0 +1,579 @@
+// Attention over the paged 4-bit cache for many query rows a sequence
+// (prompts): the same mathematics as kv4_attend.cu (see there) on the
+// fifth-generation tensor cores, for bf16 and f16 rows.
+//
+// A CTA has 256 query rows of one kv head (two blocks of 128, tokens times
+// the heads that share the kv head) and walks the visible keys 64 at a time:
+//  - four warps read codes two stages ahead and write them to shared memory as
+//    the f16 c - 8 (exact), keys as rows of K, values transposed, both in the
+//    128-byte swizzle that the products read; so the unpacking is paid once
+//    for 256 rows, and scales and minima stay in f32 beside them;
+//  - one thread issues tcgen05.mma: S = Q C^T into tensor memory (two buffers
+//    a block), O += P E with P from tensor memory;
+//  - eight warps, a thread a row, turn S into weights: x = sk_j S_ij + r_i mk_j,
+//    p = 2^(f_i x - M_i), w = p sv_j rounded to f16 (in two terms for f16
+//    rows) and written over S; the row's sums of p and p mv stay in registers.
+// M_i is raised only when a new exponent passes it by 4, and then O is
+// rescaled in tensor memory; sv enters by its stage's largest, so that w is
+// at most 16.
+// The work is one list of equal runs as in kv4_attend.cu, cut at stages; cut
+// units are joined by the same second kernel.
+//
+// Every wait is bounded; should one expire, the CTA's remaining rows are NaN.
+
+#include "kernels.h"
+#include "kv4_attend.cuh"
+#include "kv4_host.h"
+#include "tc.cuh"
+
+namespace nd {
+
+constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 32 * 13;
+constexpr int PRE_NT = PRE_ROWS / 8;   // as block_tiles counts rows
+constexpr int PRE_UNIT_COST = 3;       // of beginning and ending a unit, in stages
+
+template <int DK, int DV, typename T>
+struct PreShape {
+    static constexpr int TB = kv4_tile_bytes(DK, DV);
+    static constexpr int WS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2;  // f16 terms of a weight
+    static constexpr int ATOMS = DK > 64 ? 2 : 1;                             // 128-byte columns of a row of Q or K
+    static constexpr int QB = 128 * 128 * ATOMS, KB = PRE_KEYS * 128 * ATOMS, VB = DV * 128;
+    static constexpr int PART = PRE_ROWS * (DV + 2);
+    static constexpr int SMEM = 1024 + 2 * QB + PRE_STAGES * (KB + VB);
+};
+
+// Of a stage's keys: scale, middle (minimum + 8 scales) of key and value;
+// log2 of the largest value scale (by half); which of its four tiles exist.
+struct StageKeys {
+    float ks[PRE_KEYS], km[PRE_KEYS], vs[PRE_KEYS], vm[PRE_KEYS];
+    float lg[2];
+    uint32_t have, unused;
+};
+
+__device__ __forceinline__ int stages_of(const Tiles& t) { return (t.n + 3) / 4; }
+
+__device__ __forceinline__ long long pre_work(const AttendArgs& a, const SeqRows& r) {
+    const int blocks = (r.n * (int)a.group.d + PRE_ROWS - 1) / PRE_ROWS;
+    long long t = 0;
+    for (int b = 0; b < blocks; b++) t += stages_of(block_tiles<PRE_NT>(a, r, b)) + PRE_UNIT_COST;
+    return t;
+}
+
+template <int DK, int DV, typename T>
+__global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs a, const T* __restrict__ q, T* __restrict__ out) {
+    using Sh = PreShape<DK, DV, T>;
+    constexpr int TB = Sh::TB, QB = Sh::QB, KB = Sh::KB, VB = Sh::VB, ST = PRE_STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ long long sums[PRE_THREADS + 1];
+    __shared__ long long warp_sums[PRE_THREADS / 32];
+    __shared__ __align__(16) StageKeys keys[ST];
+    __shared__ __align__(8) uint64_t bars[2 * ST + 4 + 2 + 2 + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    volatile int* abort = &abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int H = a.kv.heads, S = a.kv.seqs, G = (int)a.group.d;
+    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;  // for the swizzle
+    uint8_t* gbase = smem_raw + (base - tc::smem_u32(smem_raw));
+    const uint32_t bar0 = tc::smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+    auto sfull = [&](int b, int buf) { return bar0 + 8u * (2 * ST + 2 * b + buf); };
+    auto pready = [&](int b) { return bar0 + 8u * (2 * ST + 4 + b); };
+    auto odone = [&](int b) { return bar0 + 8u * (2 * ST + 6 + b); };
+    const uint32_t qready = bar0 + 8u * (2 * ST + 8);
+    // a warp's wait: all its lanes go on, or none
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::bar_wait(bar, parity, abort)) != 0; };
+
+    zero_rest<DV>(a, out, blockIdx.x * (PRE_THREADS / 32) + warp, gridDim.x * (PRE_THREADS / 32), lane);
+    if (tid == 0) {
+        for (int s = 0; s < ST; s++) tc::bar_init(full(s), 4), tc::bar_init(empty(s), 1);
+        for (int b = 0; b < 2; b++) {
+            tc::bar_init(sfull(b, 0), 1), tc::bar_init(sfull(b, 1), 1);
+            tc::bar_init(pready(b), 4), tc::bar_init(odone(b), 1);
+        }
+        tc::bar_init(qready, 8);
+        abort_flag = 0;
+        a.joins[blockIdx.x] = make_int4(0, 0, 0, -1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc::smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    // the list's length, and its prefix at every chunk of `per` sequences
+    const int per = (S + PRE_THREADS - 1) / PRE_THREADS;
+    {
+        long long mine = 0;
+        for (int s = tid * per; s < min((tid + 1) * per, S); s++) mine += pre_work(a, seq_rows(a, s)) * H;
+        long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) warp_sums[warp] = incl;
+        tc::fence_before();
+        __syncthreads();
+        tc::fence_after();
+        for (int w = 0; w < warp; w++) incl += warp_sums[w];
+        sums[tid + 1] = incl;
+        if (tid == 0) sums[0] = 0;
+        __syncthreads();
+    }
+    const uint32_t tmem = tmem_slot;
+    const long long total = sums[PRE_THREADS];
+    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)(2 * PRE_UNIT_COST));
+    const long long begin = min(blockIdx.x * share, total), end = min(begin + share, total);
+
+    // Calls f(s, h, b, rows, tiles, first stage, stages, its number in this
+    // CTA, stages before it) for each part of a unit in this CTA's run. All
+    // roles walk the same parts.
+    auto for_parts = [&](auto&& f) {
+        if (begin >= end) return;
+        int s;
+        {
+            int lo = 0, hi = PRE_THREADS;  // sums[lo] <= begin < sums[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (sums[mid] <= begin) lo = mid;
+                else hi = mid;
+            }
+            s = lo;
+        }
+        long long rem = begin - sums[s];
+        s *= per;
+        SeqRows rows = seq_rows(a, s);
+        long long per_head = pre_work(a, rows);
+        while (rem >= per_head * H) {
+            rem -= per_head * H;
+            rows = seq_rows(a, ++s);
+            per_head = pre_work(a, rows);
+        }
+        int h = (int)(rem / per_head), b = 0;
+        rem -= h * per_head;
+        Tiles tl = block_tiles<PRE_NT>(a, rows, 0);
+        while (rem >= stages_of(tl) + PRE_UNIT_COST) {
+            rem -= stages_of(tl) + PRE_UNIT_COST;
+            tl = block_tiles<PRE_NT>(a, rows, ++b);
+        }
+        int at = (int)rem, part = 0, it = 0;
+        for (long long cur = begin;;) {
+            const int ns = stages_of(tl), span = (int)min((long long)(ns + PRE_UNIT_COST - at), end - cur);
+            const int off = max(at - PRE_UNIT_COST, 0), m = max(at + span - PRE_UNIT_COST, 0) - off;
+            if (m) {
+                f(s, h, b, rows, tl, off, m, part, it, cur - at + ns + PRE_UNIT_COST - 1);
+                part++, it += m;
+            }
+            cur += span;
+            if (cur >= end) break;
+            at = 0;
+            if (++b * PRE_ROWS >= rows.n * G) {
+                b = 0;
+                if (++h == H) {
+                    h = 0;
+                    do rows = seq_rows(a, ++s);
+                    while (rows.n == 0);
+                }
+            }
+            tl = block_tiles<PRE_NT>(a, rows, b);
+        }
+    };
+
+    if (warp < 8) {
+        // ---- a thread a query row
+        const int blk = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t scol = tmem + lanes + blk * 256, ocol = scol + 128;
+        uint8_t* qs = gbase + blk * QB;
+        bool ok = true;
+        for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
+            const int nrows = rows.n * G, x0 = b * PRE_ROWS + blk * 128, x = x0 + row;
+            const bool active = x0 < nrows, on = x < nrows;
+            const int tok = a.group(min(x, nrows - 1));
+            // the row's queries as f16 of 2^14 at the largest, in the order in
+            // which codes are unpacked: 0 4 1 5 2 6 3 7 of every eight
+            float f = 0.f, r = 0.f;
+            if (active) {
+                float top = 0.f, sum = 0.f;
+                bool bad = false;
+                const T* p = q + (long long)(rows.first + tok) * a.q_row + (long long)(h * G + x - tok * G) * a.q_head;
+                float v[8];
+#pragma unroll 4
+                for (int c = 0; c < DK / 8; c++) {
+                    if (on) load8(p + 8 * c, a.q_vec, v);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (!on) v[i] = 0.f;
+                        top = fmaxf(top, fabsf(v[i]));
+                        bad |= !(fabsf(v[i]) <= FLT_MAX);
+                        sum += v[i];
+                    }
+                }
+                const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
+                const float sign = a.scale_log2e < 0.f ? -1.f : 1.f;
+                const float up = bad ? 0.f : sign * __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                // exponents are f x: f positive, so that the largest x has the largest
+                f = fmaxf(fabsf(a.scale_log2e) * __uint_as_float((uint32_t)(e - 14 + 127) << 23), 1e-37f);
+                r = sum * up;
+                if (bad) f = r = __uint_as_float(0x7fc00000u);
+#pragma unroll 4
+                for (int c = 0; c < DK / 8; c++) {
+                    if (on) load8(p + 8 * c, a.q_vec, v);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = on && !bad ? v[i] * up : 0.f;
+                    uint4 w = make_uint4(pack_half2(v[0], v[4]), pack_half2(v[1], v[5]), pack_half2(v[2], v[6]), pack_half2(v[3], v[7]));
+                    *(uint4*)(qs + (c / 8) * (128 * 128) + row * 128 + ((c % 8) ^ (row & 7)) * 16) = w;
+                }
+                tc::fence_async_smem();
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(qready);
+
+            const long long qpos = rows.pos0 + tok;
+            const int hi = on ? (int)min(max(qpos, -1LL), 0x7fffffffLL) : -1;
+            const int x_last = min(x0 + 128, nrows) - 1;
+            const long long p_first = rows.pos0 + a.group(min(x0, nrows - 1)), p_last = rows.pos0 + a.group(x_last);
+            const int all_hi = (int)min(max(p_first, -1LL), 0x7fffffffLL) - 15;
+            const int all_lo = a.window > 0 ? (int)min(max(p_last - a.window, -1LL), 0x7fffffffLL) : -1;
+            const f32x2 f2 = pair(f, f), r2 = pair(r, r);
+            float M = ATT_LOW;
+            f32x2 l2 = 0, mn2 = 0;
+
+#pragma unroll 1
+            for (int i = 0; i < m; i++) {
+                const int k = it0 + i, slot = k % ST, buf = k & 1;
+                if (ok) ok = warp_wait(sfull(blk, buf), (k >> 1) & 1) && warp_wait(full(slot), (k / ST) & 1);
+                if (active && ok) {
+                    tc::fence_after();
+                    const StageKeys& sk = keys[slot];
+                    float xs[PRE_KEYS];
+                    tc::ld32(scol + buf * 64, xs);
+                    tc::ld32(scol + buf * 64 + 32, xs + 32);
+                    tc::ld_wait32(xs);
+                    tc::ld_wait32(xs + 32);
+                    bool whole = sk.have == 15;
+                    int k0[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        k0[u] = tl.at(4 * (off + i) + u) * KV4_TILE;
+                        whole &= k0[u] <= all_hi && (k0[u] > all_lo || k0[u] + 15 < a.sink);
+                    }
+#pragma unroll
+                    for (int j = 0; j < PRE_KEYS; j += 4) {
+                        const float4 ks = *(const float4*)&sk.ks[j], km = *(const float4*)&sk.km[j];
+                        const float2 y = unpair(fma2(pair(xs[j], xs[j + 1]), pair(ks.x, ks.y), mul2(r2, pair(km.x, km.y))));
+                        const float2 z = unpair(fma2(pair(xs[j + 2], xs[j + 3]), pair(ks.z, ks.w), mul2(r2, pair(km.z, km.w))));
+                        xs[j] = y.x, xs[j + 1] = y.y, xs[j + 2] = z.x, xs[j + 3] = z.y;
+                    }
+                    if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+                        for (int j = 0; j < PRE_KEYS; j++) {
+                            const int key = k0[j / 16] + j % 16;
+                            if (!((sk.have >> (j / 16) & 1) && key <= hi && (a.window <= 0 || key > hi - a.window || key < a.sink))) xs[j] = -INFINITY;
+                        }
+                    }
+                    float top = xs[0];
+#pragma unroll
+                    for (int j = 1; j < PRE_KEYS; j++) top = fmaxf(top, xs[j]);
+                    const float lg = fmaxf(sk.lg[0], sk.lg[1]), want = __fmaf_rn(top, f, lg);
+                    const bool raise = want > M + 4.f;
+                    if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
+                        const float to = raise ? want : M, scale = ex2(M - to);
+                        M = to;
+                        l2 = mul2(l2, pair(scale, scale)), mn2 = mul2(mn2, pair(scale, scale));
+                        if (i > 0) {
+                            ok = warp_wait(odone(blk), (k - 1) & 1);
+                            tc::fence_after();
+#pragma unroll
+                            for (int c = 0; c < DV; c += 32) {
+                                float o[32];
+                                tc::ld32(ocol + c, o);
+                                tc::ld_wait32(o);
+#pragma unroll
+                                for (int j = 0; j < 32; j++) o[j] *= scale;
+                                tc::st32(ocol + c, (const uint32_t*)o);
+                            }
+                        }
+                    }
+                    const f32x2 nM = pair(-M, -M);
+                    uint32_t hi_w[32], lo_w[Sh::WS == 2 ? 32 : 1];
+                    auto weigh = [&](bool clean) {
+#pragma unroll
+                        for (int j = 0; j < PRE_KEYS; j += 4) {
+                            const float4 vs = *(const float4*)&sk.vs[j], vm = *(const float4*)&sk.vm[j];
+#pragma unroll
+                            for (int half = 0; half < 2; half++) {
+                                const float2 xx = make_float2(xs[j + 2 * half], xs[j + 2 * half + 1]);
+                                const float2 e = unpair(fma2(pair(xx.x, xx.y), f2, nM));
+                                const f32x2 p = pair(ex2(e.x), ex2(e.y));
+                                f32x2 s2 = half ? pair(vs.z, vs.w) : pair(vs.x, vs.y), m2 = half ? pair(vm.z, vm.w) : pair(vm.x, vm.y);
+                                if (clean) {  // a masked place may hold NaN or infinity
+                                    const float2 sf = unpair(s2), mf = unpair(m2);
+                                    s2 = pair(xx.x == -INFINITY ? 0.f : sf.x, xx.y == -INFINITY ? 0.f : sf.y);
+                                    m2 = pair(xx.x == -INFINITY ? 0.f : mf.x, xx.y == -INFINITY ? 0.f : mf.y);
+                                }
+                                l2 = add2(l2, p);
+                                mn2 = fma2(p, m2, mn2);
+                                const float2 w = unpair(mul2(p, s2));
+                                const uint32_t hw = pack_half2(w.x, w.y);
+                                hi_w[j / 2 + half] = hw;
+                                if (Sh::WS == 2) {
+                                    const float2 back = unpack_half2(hw);
+                                    lo_w[Sh::WS == 2 ? j / 2 + half : 0] = pack_half2(w.x - back.x, w.y - back.y);
+                                }
+                            }
+                        }
+                    };
+                    if (__builtin_expect(whole, 1)) weigh(false);
+                    else weigh(true);
+                    tc::st32(scol + buf * 64, hi_w);
+                    if constexpr (Sh::WS == 2) tc::st32(scol + buf * 64 + 32, lo_w);
+                    tc::st_wait();
+                    tc::fence_before();
+                }
+                // the last product's phase is seen before this stage's weights
+                // are announced: a parity tells only neighbouring phases apart,
+                // here of odone and for the issuing thread of pready
+                if (ok && i > 0) ok = warp_wait(odone(blk), (k - 1) & 1);
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(pready(blk));
+            }
+
+            // the last product, and the result or this CTA's part of it
+            if (ok) ok = warp_wait(odone(blk), (it0 + m - 1) & 1);
+            const bool starts = off == 0, ends = off + m == stages_of(tl), done = starts && ends;
+            if (active) {
+                tc::fence_after();
+                const float2 lp = unpair(l2), mp = unpair(mn2);
+                float l = lp.x + lp.y;
+                const float mn = mp.x + mp.y;
+                if (!ok) l = __uint_as_float(0x7fc00000u);
+                const float norm = done ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                const OutRows<T> to{out, a, rows.first, h, nrows};
+                float* part = a.parts + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Sh::PART;
+                const int y = blk * 128 + row;
+                T* o_row = to.at(min(x, nrows - 1));
+#pragma unroll
+                for (int c = 0; c < DV; c += 32) {
+                    float o[32];
+                    tc::ld32(ocol + c, o);
+                    tc::ld_wait32(o);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) o[j] = (o[j] + mn) * norm;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        if (!done) store8(part + (size_t)y * DV + c + j, true, o + j);
+                        else if (on) store8(o_row + c + j, a.o_vec, o + j);
+                    }
+                }
+                if (!done) part[PRE_ROWS * DV + y] = M, part[PRE_ROWS * (DV + 1) + y] = l;
+                tc::fence_before();
+            }
+            if (starts && !ends && tid == 0) a.joins[blockIdx.x] = make_int4(s, h, b, (int)(last / share - blockIdx.x));
+        });
+    } else if (warp < 12) {
+        // ---- codes to operands
+        const int t = tid - 256, half = t >> 6, key = t & 63, w4 = warp - 8;
+        constexpr int KW = DK / 16, VWW = DV / 32;  // words of a half key row; of a quarter value row
+        bool ok = true;
+        for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
+            const int first = 4 * off, n = min(4 * m, tl.n - first);  // tiles of this part
+            const int32_t* trow = a.kv.table + (size_t)s * a.kv.table_stride;
+            const uint8_t* head = a.kv.pool + (size_t)h * a.kv.page_tiles * TB;
+            const long long len = rows.pos0 + rows.n;
+            auto fetch = [&](int i) -> unsigned long long {  // the i-th tile's address, 0: no such page
+                if (i >= n) return 0;
+                const int tile = tl.at(first + i), p = a.page_tiles(tile);
+                const int page = p < a.kv.max_pages ? __ldg(trow + p) : -1;
+                if (page < 0 || page >= a.kv.num_pages) return 0;
+                return (unsigned long long)(head + (size_t)page * a.kv.page_stride + (size_t)(tile - p * a.kv.page_tiles) * TB);
+            };
+            unsigned long long src = fetch(lane), src_next = fetch(32 + lane);
+            uint32_t kw[KW], vw[2][VWW], kp = 0, vp = 0, have = 0;
+            auto load = [&](int i) {  // stage i's words
+                if (i && (i & 7) == 0) src = src_next, src_next = fetch(4 * i + 32 + lane);
+                const unsigned long long ka = __shfl_sync(0xffffffffu, src, (4 * i + (key >> 4)) & 31);
+                const unsigned long long va = __shfl_sync(0xffffffffu, src, (4 * i + (lane >> 3)) & 31);
+                have = __ballot_sync(0xffffffffu, src != 0) >> (4 * i & 31) & 15;
+#pragma unroll
+                for (int w = 0; w < KW; w++) kw[w] = 0x88888888u;  // c - 8 = 0
+#pragma unroll
+                for (int w = 0; w < VWW; w++) vw[0][w] = vw[1][w] = 0x88888888u;
+                kp = vp = 0;
+                if (ka) {
+                    const uint8_t* p = (const uint8_t*)ka + (key & 15) * (DK / 2) + half * (DK / 4);
+                    if constexpr (DK == 48) {
+#pragma unroll
+                        for (int w = 0; w < KW; w++) kw[w] = __ldg((const uint32_t*)p + w);
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < KW; w += 4) {
+                            const uint4 x = __ldg((const uint4*)p + w / 4);
+                            kw[w] = x.x, kw[w + 1] = x.y, kw[w + 2] = x.z, kw[w + 3] = x.w;
+                        }
+                    }
+                    if (half == 0 && tl.at(first + 4 * i + (key >> 4)) * (long long)KV4_TILE + (key & 15) < len) {
+                        const uint8_t* pp = (const uint8_t*)ka + 8 * (DK + DV) + 4 * (key & 15);
+                        kp = __ldg((const uint32_t*)pp), vp = __ldg((const uint32_t*)(pp + 64));
+                    }
+                }
+                if (va) {
+                    const uint8_t* p = (const uint8_t*)va + 8 * DK + (2 * lane & 15) * (DV / 2) + w4 * (DV / 8);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if constexpr (VWW == 4) {
+                            const uint4 x = __ldg((const uint4*)(p + u * (DV / 2)));
+                            vw[u][0] = x.x, vw[u][1] = x.y, vw[u][2] = x.z, vw[u][3] = x.w;
+                        } else {
+                            const uint2 x = __ldg((const uint2*)(p + u * (DV / 2)));
+                            vw[u][0] = x.x, vw[u][1] = x.y;
+                        }
+                    }
+                }
+            };
+            load(0);
+#pragma unroll 1
+            for (int i = 0; i < m; i++) {
+                const int k = it0 + i, slot = k % ST;
+                if (ok && k >= ST) ok = warp_wait(empty(slot), ((k / ST) - 1) & 1);
+                uint8_t* ks = gbase + 2 * QB + slot * (KB + VB);
+                uint8_t* vs = ks + KB;
+#pragma unroll
+                for (int w = 0; w < KW; w++) {  // eight dimensions: 16 bytes of the key's row
+                    const int c = half * KW + w;
+                    const uint32_t x = kw[w], y = x >> 8;
+                    *(uint4*)(ks + (c / 8) * (PRE_KEYS * 128) + key * 128 + ((c % 8) ^ (key & 7)) * 16) =
+                        make_uint4(code_mid(x & 0x000f000fu), code16_mid(x & 0x00f000f0u), code_mid(y & 0x000f000fu), code16_mid(y & 0x00f000f0u));
+                }
+#pragma unroll
+                for (int w = 0; w < VWW; w++)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; q4++) {  // dimensions 2 q4, 2 q4 + 1 of keys 2 lane, 2 lane + 1
+                        const uint32_t x = __byte_perm(vw[0][w], vw[1][w], q4 < 2 ? 0x5410 : 0x7632) >> (q4 & 1 ? 8 : 0);
+                        const int d = w4 * (DV / 4) + 8 * w + 2 * q4;
+                        uint8_t* p = vs + (lane & 3) * 4;
+                        *(uint32_t*)(p + d * 128 + (((lane >> 2) ^ (d & 7)) * 16)) = code_mid(x & 0x000f000fu);
+                        *(uint32_t*)(p + (d + 1) * 128 + (((lane >> 2) ^ ((d + 1) & 7)) * 16)) = code16_mid(x & 0x00f000f0u);
+                    }
+                if (half == 0) {
+                    StageKeys& sk = keys[slot];
+                    const float2 kf = unpack_half2(kp), vf = unpack_half2(vp);
+                    sk.ks[key] = kf.x, sk.km[key] = __fmaf_rn(8.f, kf.x, kf.y);
+                    sk.vs[key] = vf.x, sk.vm[key] = __fmaf_rn(8.f, vf.x, vf.y);
+                    float lg = lg2(fmaxf(vf.x, 5.9604645e-8f));
+#pragma unroll
+                    for (int o = 16; o; o /= 2) lg = fmaxf(lg, __shfl_xor_sync(0xffffffffu, lg, o));
+                    if (lane == 0) sk.lg[w4] = lg;
+                    if (t == 0) sk.have = have;
+                }
+                tc::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(full(slot));
+                if (i + 1 < m) load(i + 1);
+            }
+        });
+    } else {
+        // ---- the products: lane 0 waits and issues
+        bool ok = true;
+        int issued = 0;
+        for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
+            if (lane == 0) {
+                const int blocks = b * PRE_ROWS + 128 < rows.n * G ? 2 : 1;
+                if (ok) ok = tc::bar_wait(qready, part_no & 1, abort);
+                auto scores = [&](int k) {
+                    const int slot = k % ST;
+                    if (ok) ok = tc::bar_wait(full(slot), (k / ST) & 1, abort);
+                    if (!ok) return;
+                    tc::fence_after();
+                    const uint32_t ks = base + 2 * QB + slot * (KB + VB);
+                    for (int blk = 0; blk < 2; blk++) {
+                        if (blk < blocks)
+#pragma unroll
+                            for (int c = 0; c < DK / 16; c++)
+                                tc::mma_ss(tmem + blk * 256 + (k & 1) * 64, tc::sw128_desc(base + blk * QB + c / 4 * (128 * 128) + c % 4 * 32),
+                                           tc::sw128_desc(ks + c / 4 * (PRE_KEYS * 128) + c % 4 * 32), tc::f16_idesc(PRE_KEYS), c > 0);
+                        tc::commit(sfull(blk, k & 1));
+                    }
+                };
+                scores(it0);
+                for (int i = 0; i < m && ok; i++) {
+                    const int k = it0 + i, slot = k % ST;
+                    if (i + 1 < m) scores(k + 1);
+                    const uint32_t vs = base + 2 * QB + slot * (KB + VB) + KB;
+                    for (int blk = 0; blk < 2; blk++) {
+                        if (ok) ok = tc::bar_wait(pready(blk), k & 1, abort);
+                        if (!ok) break;
+                        tc::fence_after();
+                        if (blk < blocks)
+#pragma unroll
+                            for (int term = 0; term < Sh::WS; term++)
+#pragma unroll
+                                for (int c = 0; c < PRE_KEYS / 16; c++)
+                                    tc::mma_ts(tmem + blk * 256 + 128, tmem + blk * 256 + (k & 1) * 64 + term * 32 + c * 8,
+                                               tc::sw128_desc(vs + c * 32), tc::f16_idesc(DV), i > 0 || term > 0 || c > 0);
+                        tc::commit(odone(blk));
+                    }
+                    if (ok) tc::commit(empty(slot)), issued = k + 1;
+                }
+            }
+            __syncwarp();
+        });
+        // every product issued is over before the memory is freed
+        if (lane == 0 && issued > 0) tc::bar_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1, abort);
+        __syncwarp();
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc::fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+size_t prefill_ws_bytes(int dv, int* ctas) {
+    *ctas = device_sm_count();
+    return (size_t)*ctas * (sizeof(int4) + 2 * sizeof(float) * PRE_ROWS * (dv + 2));
+}
+
+template <int DK, int DV, typename T>
+static void launch(const AttendArgs& a0, const void* q, void* out, void* ws, cudaStream_t st) {
+    using Sh = PreShape<DK, DV, T>;
+    AttendArgs a = a0;
+    const int ctas = device_sm_count();
+    a.joins = (int4*)ws;
+    a.parts = (float*)((char*)ws + (size_t)ctas * sizeof(int4));
+    auto check = [](cudaError_t e) {
+        if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
+    };
+    check(cudaFuncSetAttribute(kv4_prefill_kernel<DK, DV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    kv4_prefill_kernel<DK, DV, T><<<ctas, PRE_THREADS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
+    op_launched("nd_op_kv4_attend");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas, 8);
+    cfg.blockDim = dim3(512);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = st ? 1 : 0;
+    check(cudaLaunchKernelEx(&cfg, kv4_join_kernel<DV, PRE_NT, T>, AttendArgs(a), (T*)out));
+    add_launches(1);
+}
+
+template <typename T>
+static void launch_dk(const AttendArgs& a, int dk, const void* q, void* out, void* ws, cudaStream_t st) {
+    if (dk == 48) launch<48, 64, T>(a, q, out, ws, st);
+    else if (dk == 64) launch<64, 64, T>(a, q, out, ws, st);
+    else launch<128, 128, T>(a, q, out, ws, st);
+}
+
+void prefill_launch(const AttendArgs& a, int dk, int type, const void* q, void* out, void* ws, cudaStream_t st) {
+    if (type == ND_F16) launch_dk<__half>(a, dk, q, out, ws, st);
+    else launch_dk<__nv_bfloat16>(a, dk, q, out, ws, st);
+}
+
+}  // namespace nd

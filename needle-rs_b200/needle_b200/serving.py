@@ -136,7 +136,7 @@ def op_kv4_attend(kv, q, table, lens, start=None, scale=None, window=0, sink=0, 
         raise ValueError("out must have q's type and rows")
     oa = kv._rows(out, hq, kv.dv, "out")
     L = lib()
-    n = L.nd_op_kv4_attend_ws(a, hq, window, sink)
+    n = L.nd_op_kv4_attend_ws(a, _TYPES[q.dtype], hq, window, sink)
     ws = torch.empty(n, dtype=torch.uint8, device=kv.device) if n else None
     if L.nd_op_kv4_attend(a, _TYPES[q.dtype], *qa, hq, 1 / math.sqrt(kv.dk) if scale is None else scale, window, sink, *oa,
                           ws.data_ptr() if n else None, n, _ZERO_REST if new else 0, _stream(kv.device)) != 0:

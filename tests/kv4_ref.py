@@ -71,13 +71,16 @@ class Cache:
         b, top = np.zeros((rows, hq, 1)), np.zeros((rows, hq, 1))
         for s in range(len(lens)):
             n = start[s + 1] - start[s]
+            places = [self.place(table, s, j) for j in range(max(int(lens[s]), 0))]
+            exists = np.array([p is not None for p in places], bool)
+            where = np.array([p or (0, 0) for p in places]).reshape(-1, 2)
+            key = np.arange(len(places))
             for i in range(n):
                 pos = int(lens[s]) - n + i
-                seen = [j for j in range(pos + 1) if (window <= 0 or j > pos - window or j < sink)]
-                at = [a for a in (self.place(table, s, j) for j in seen) if a]
-                if not at:
+                seen = exists & (key <= pos) & ((key > pos - window) | (key < sink) | (window <= 0))
+                if not seen.any():
                     continue
-                pg, sl = np.array(at).T
+                pg, sl = where[seen].T
                 r = start[s] + i
                 for g in range(hq):
                     h = g // (hq // H)

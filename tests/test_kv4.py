@@ -238,6 +238,67 @@ def test_attend_ragged_rows(cuda_device, heads, dtype, n, window, sink):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("n,lens", [([200], [200]), ([64, 70, 0], [300, 70, 40]), ([100, 257], [900, 1000])])
+@pytest.mark.parametrize("window,sink", [(0, 0), (90, 20)])
+def test_attend_many_rows(cuda_device, heads, dtype, n, lens, window, sink):
+    """Prompts: several blocks of rows, the last partly filled, keys cut
+    between CTAs, a bad page, rows behind the last sequence."""
+    import needle_b200 as nb
+    import torch
+
+    st = Setup(heads, dtype, lens, n, 32, seed=sum(n), extra_rows=3).append()
+    out = torch.full((st.rows, st.hq, st.dv), 5.0, dtype=st.t, device="cuda")
+    nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start), window=window, sink=sink, out=out)
+    assert (out[-3:] == 5).all()
+    _check(st, dtype, out, window, sink)
+    st.table[0, 3] = -1
+    got = nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start), window=window, sink=sink)
+    assert (got[-3:] == 0).all()
+    _check(st, dtype, got, window, sink)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attend_many_rows_odd_values(cuda_device, dtype):
+    """In the kernel for many rows: values of very small and large scale,
+    constant values, wide scores, NaN rows of keys and queries, scale 0 and
+    below."""
+    import needle_b200 as nb
+    import torch
+
+    for heads, factor in (("wide", 1e-4), ("small", 1e4), ("needle", 0.0)):
+        st = Setup(heads, dtype, [300, 230], [250, 210], 32, seed=7)
+        st.v *= factor
+        if factor == 0.0:
+            st.v += 1.5
+        st.append()
+        _check(st, dtype, nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start)))
+    st = Setup("wide", dtype, [280, 200], [260, 200], 32, seed=8, qscale=30.0).append()
+    args = (st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start))
+    for scale in (None, 0.0, -0.01):
+        _check(st, dtype, nb.op_kv4_attend(*args, scale=scale), scale=scale)
+    st = Setup("small", dtype, [300], [250], 16, seed=9)
+    st.k[100, 1] = float("nan")
+    st.v[200, 2] = float("inf")
+    st.append()
+    st.q[7, 0, 3] = float("nan")
+    st.q[40, 3, 1] = float("inf")
+    got = _np(nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start)))
+    nan = np.zeros((250, 4), bool)
+    pos = np.arange(50, 300)
+    nan[pos >= 100, 1] = True
+    nan[pos >= 200, 2] = True
+    nan[7, 0] = nan[40, 3] = True
+    assert np.array_equal(np.isnan(got).any(-1), nan) and np.array_equal(np.isnan(got).all(-1), nan)
+    got = _np(nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start), window=30))
+    nan[pos >= 130, 1] = False
+    nan[pos >= 230, 2] = False
+    assert np.array_equal(np.isnan(got).any(-1), nan)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("heads", ["needle", "wide"])
 def test_attend_split_over_warps(cuda_device, heads, dtype):
