@@ -28,9 +28,13 @@
 
 namespace nd {
 
-constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 32 * 13;
+constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 512;
 constexpr int PRE_NT = PRE_ROWS / 8;   // as block_tiles counts rows
 constexpr int PRE_UNIT_COST = 3;       // of beginning and ending a unit, in stages
+// Registers of a thread: launched with 128, then shared out by warpgroup (the
+// rows' two, the operands', the issuer's), which sums to what was launched.
+constexpr int PRE_REGS_ROWS = 176, PRE_REGS_CODES = 80, PRE_REGS_ISSUE = 80;
+static_assert(2 * PRE_REGS_ROWS + PRE_REGS_CODES + PRE_REGS_ISSUE <= 4 * 128, "registers of the four warpgroups");
 
 template <int DK, int DV, typename T>
 struct PreShape {
@@ -183,6 +187,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
 
     if (warp < 8) {
         // ---- a thread a query row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ROWS));
         const int blk = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t scol = tmem + lanes + blk * 256, ocol = scol + 128;
@@ -287,7 +292,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                         if (i > 0) {
                             ok = warp_wait(odone(blk), (k - 1) & 1);
                             tc::fence_after();
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < DV; c += 32) {
                                 float o[32];
                                 tc::ld32(ocol + c, o);
@@ -299,17 +304,18 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                         }
                     }
                     const f32x2 nM = pair(-M, -M);
-                    uint32_t hi_w[32], lo_w[Sh::WS == 2 ? 32 : 1];
-                    auto weigh = [&](bool clean) {
+                    // by halves of 32 keys: weights over the half's own scores
+                    auto weigh = [&](float* xh, int half, bool clean) {
+                        uint32_t w[16 * Sh::WS];
 #pragma unroll
-                        for (int j = 0; j < PRE_KEYS; j += 4) {
-                            const float4 vs = *(const float4*)&sk.vs[j], vm = *(const float4*)&sk.vm[j];
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 vs = *(const float4*)&sk.vs[32 * half + j], vm = *(const float4*)&sk.vm[32 * half + j];
 #pragma unroll
-                            for (int half = 0; half < 2; half++) {
-                                const float2 xx = make_float2(xs[j + 2 * half], xs[j + 2 * half + 1]);
+                            for (int t = 0; t < 2; t++) {
+                                const float2 xx = make_float2(xh[j + 2 * t], xh[j + 2 * t + 1]);
                                 const float2 e = unpair(fma2(pair(xx.x, xx.y), f2, nM));
                                 const f32x2 p = pair(ex2(e.x), ex2(e.y));
-                                f32x2 s2 = half ? pair(vs.z, vs.w) : pair(vs.x, vs.y), m2 = half ? pair(vm.z, vm.w) : pair(vm.x, vm.y);
+                                f32x2 s2 = t ? pair(vs.z, vs.w) : pair(vs.x, vs.y), m2 = t ? pair(vm.z, vm.w) : pair(vm.x, vm.y);
                                 if (clean) {  // a masked place may hold NaN or infinity
                                     const float2 sf = unpair(s2), mf = unpair(m2);
                                     s2 = pair(xx.x == -INFINITY ? 0.f : sf.x, xx.y == -INFINITY ? 0.f : sf.y);
@@ -317,20 +323,20 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                                 }
                                 l2 = add2(l2, p);
                                 mn2 = fma2(p, m2, mn2);
-                                const float2 w = unpair(mul2(p, s2));
-                                const uint32_t hw = pack_half2(w.x, w.y);
-                                hi_w[j / 2 + half] = hw;
+                                const float2 v = unpair(mul2(p, s2));
+                                const uint32_t hw = pack_half2(v.x, v.y);
+                                w[j / 2 + t] = hw;
                                 if (Sh::WS == 2) {
                                     const float2 back = unpack_half2(hw);
-                                    lo_w[Sh::WS == 2 ? j / 2 + half : 0] = pack_half2(w.x - back.x, w.y - back.y);
+                                    w[16 * (Sh::WS - 1) + j / 2 + t] = pack_half2(v.x - back.x, v.y - back.y);
                                 }
                             }
                         }
+                        if constexpr (Sh::WS == 2) tc::st32(scol + buf * 64 + 32 * half, w);
+                        else tc::st16(scol + buf * 64 + 32 * half, w);
                     };
-                    if (__builtin_expect(whole, 1)) weigh(false);
-                    else weigh(true);
-                    tc::st32(scol + buf * 64, hi_w);
-                    if constexpr (Sh::WS == 2) tc::st32(scol + buf * 64 + 32, lo_w);
+                    if (__builtin_expect(whole, 1)) weigh(xs, 0, false), weigh(xs + 32, 1, false);
+                    else weigh(xs, 0, true), weigh(xs + 32, 1, true);
                     tc::st_wait();
                     tc::fence_before();
                 }
@@ -356,7 +362,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 float* part = a.parts + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Sh::PART;
                 const int y = blk * 128 + row;
                 T* o_row = to.at(min(x, nrows - 1));
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DV; c += 32) {
                     float o[32];
                     tc::ld32(ocol + c, o);
@@ -376,6 +382,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
         });
     } else if (warp < 12) {
         // ---- codes to operands
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_CODES));
         const int t = tid - 256, half = t >> 6, key = t & 63, w4 = warp - 8;
         constexpr int KW = DK / 16, VWW = DV / 32;  // words of a half key row; of a quarter value row
         bool ok = true;
@@ -476,10 +483,11 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             }
         });
     } else {
-        // ---- the products: lane 0 waits and issues
+        // ---- the products: lane 0 of the first of four warps waits and issues
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ISSUE));
         bool ok = true;
         int issued = 0;
-        for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
+        if (warp == 12) for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
             if (lane == 0) {
                 const int blocks = b * PRE_ROWS + 128 < rows.n * G ? 2 : 1;
                 if (ok) ok = tc::bar_wait(qready, part_no & 1, abort);
@@ -512,7 +520,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                             for (int term = 0; term < Sh::WS; term++)
 #pragma unroll
                                 for (int c = 0; c < PRE_KEYS / 16; c++)
-                                    tc::mma_ts(tmem + blk * 256 + 128, tmem + blk * 256 + (k & 1) * 64 + term * 32 + c * 8,
+                                    tc::mma_ts(tmem + blk * 256 + 128, tmem + blk * 256 + (k & 1) * 64 + c / 2 * 32 + term * 16 + c % 2 * 8,
                                                tc::sw128_desc(vs + c * 32), tc::f16_idesc(DV), i > 0 || term > 0 || c > 0);
                         tc::commit(odone(blk));
                     }
@@ -522,7 +530,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             __syncwarp();
         });
         // every product issued is over before the memory is freed
-        if (lane == 0 && issued > 0) tc::bar_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1, abort);
+        if (warp == 12 && lane == 0 && issued > 0) tc::bar_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1, abort);
         __syncwarp();
     }
     tc::fence_before();
@@ -552,7 +560,7 @@ static void launch(const AttendArgs& a0, const void* q, void* out, void* ws, cud
     kv4_prefill_kernel<DK, DV, T><<<ctas, PRE_THREADS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, 8);
+    cfg.gridDim = dim3(ctas, 32);
     cfg.blockDim = dim3(512);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
