@@ -131,33 +131,39 @@ __device__ __forceinline__ void zero_rest(const AttendArgs& a, T* out, int wid, 
 // those where no cut unit starts return at once.
 template <int DV, int NT, typename T>
 __global__ void __launch_bounds__(512) kv4_join_kernel(AttendArgs a, T* __restrict__ out) {
-    constexpr int PART = 8 * NT * (DV + 2), ROWS = 512 / DV;
+    constexpr int PART = 8 * NT * (DV + 2), LANES = DV / 4, ROWS = 512 / LANES;  // four dimensions a thread
     asm volatile("griddepcontrol.wait;\n" ::: "memory");
     const int4 job = a.joins[blockIdx.x];
     if (job.w < 0) return;
     const SeqRows rows = seq_rows(a, job.x);
     const OutRows<T> to{out, a, rows.first, job.y, rows.n * (int)a.group.d};
     const float* part = a.parts + (size_t)blockIdx.x * 2 * PART;
-    const int d = threadIdx.x % DV;
-    for (int y = blockIdx.y * ROWS + threadIdx.x / DV; y < 8 * NT; y += gridDim.y * ROWS) {
+    const int d = threadIdx.x % LANES * 4;
+    for (int y = blockIdx.y * ROWS + threadIdx.x / LANES; y < 8 * NT; y += gridDim.y * ROWS) {
         const int x = job.z * 8 * NT + y;
         if (x >= to.nrows) return;
         // the starting runner's second slot, then the first slot of each further one
-        float M = part[PART + 8 * NT * DV + y];
-#pragma unroll 8
+        const float* p0 = part + PART;
+        float M = p0[8 * NT * DV + y];
+#pragma unroll 4
         for (int i = 1; i <= job.w; i++) M = fmaxf(M, part[(size_t)i * 2 * PART + 8 * NT * DV + y]);
-        float l = 0.f, v = 0.f;
-#pragma unroll 8
-        for (int i = 0; i <= job.w; i++) {
-            const float* p = part + (i ? (size_t)i * 2 * PART : PART);
+        const float r0 = ex2(p0[8 * NT * DV + y] - M);
+        float l = p0[8 * NT * (DV + 1) + y] * r0;
+        float4 v = *(const float4*)(p0 + y * DV + d);
+        v.x *= r0, v.y *= r0, v.z *= r0, v.w *= r0;
+#pragma unroll 4
+        for (int i = 1; i <= job.w; i++) {
+            const float* p = part + (size_t)i * 2 * PART;
             const float r = ex2(p[8 * NT * DV + y] - M);
+            const float4 u = *(const float4*)(p + y * DV + d);
             l = __fmaf_rn(p[8 * NT * (DV + 1) + y], r, l);
-            v = __fmaf_rn(p[y * DV + d], r, v);
+            v.x = __fmaf_rn(u.x, r, v.x), v.y = __fmaf_rn(u.y, r, v.y), v.z = __fmaf_rn(u.z, r, v.z), v.w = __fmaf_rn(u.w, r, v.w);
         }
-        to.at(x)[d] = (T)(l == 0.f ? 0.f : v / l);
+        const float norm = l == 0.f ? 0.f : 1.f / l;
+        T* o = to.at(x) + d;
+        o[0] = (T)(v.x * norm), o[1] = (T)(v.y * norm), o[2] = (T)(v.z * norm), o[3] = (T)(v.w * norm);
     }
 }
-
 
 // The tcgen05 kernel for long runs of query rows (kv4_prefill.cu): rows a
 // unit, workspace and launch. `dk` chooses the head dimensions; 16-bit types.

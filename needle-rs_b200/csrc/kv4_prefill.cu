@@ -10,12 +10,13 @@
 //    for 256 rows, and scales and minima stay in f32 beside them;
 //  - one thread issues tcgen05.mma: S = Q C^T into tensor memory (two buffers
 //    a block), O += P E with P from tensor memory;
-//  - eight warps, a thread a row, turn S into weights: x = sk_j S_ij + r_i mk_j,
-//    p = 2^(f_i x - M_i), w = p sv_j rounded to f16 (in two terms for f16
-//    rows) and written over S; the row's sums of p and p mv stay in registers.
+//  - sixteen warps, two threads a row with 32 of the 64 keys each, turn S into
+//    weights: x = sk_j S_ij + r_i mk_j, p = 2^(f_i x - M_i), w = p sv_j rounded
+//    to f16 (in two terms for f16 rows) and written over S; the row's sums of
+//    p and p mv stay in registers.
 // M_i is raised only when a new exponent passes it by 4, and then O is
-// rescaled in tensor memory; sv enters by its stage's largest, so that w is
-// at most 16.
+// rescaled in tensor memory; sv enters by its half stage's largest, so that w
+// is at most 16.
 // The work is one list of equal runs as in kv4_attend.cu, cut at stages; cut
 // units are joined by the same second kernel.
 //
@@ -28,13 +29,13 @@
 
 namespace nd {
 
-constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 512;
+constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 768;
 constexpr int PRE_NT = PRE_ROWS / 8;   // as block_tiles counts rows
 constexpr int PRE_UNIT_COST = 3;       // of beginning and ending a unit, in stages
-// Registers of a thread: launched with 128, then shared out by warpgroup (the
-// rows' two, the operands', the issuer's), which sums to what was launched.
-constexpr int PRE_REGS_ROWS = 176, PRE_REGS_CODES = 80, PRE_REGS_ISSUE = 80;
-static_assert(2 * PRE_REGS_ROWS + PRE_REGS_CODES + PRE_REGS_ISSUE <= 4 * 128, "registers of the four warpgroups");
+// Registers of a thread: launched with 80, then shared out by warpgroup (the
+// rows' four, the operands', the issuer's), which sums to what was launched.
+constexpr int PRE_REGS_ROWS = 88, PRE_REGS_CODES = 56, PRE_REGS_ISSUE = 72;
+static_assert(4 * PRE_REGS_ROWS + PRE_REGS_CODES + PRE_REGS_ISSUE <= 6 * 80, "registers of the six warpgroups");
 
 template <int DK, int DV, typename T>
 struct PreShape {
@@ -47,11 +48,13 @@ struct PreShape {
 };
 
 // Of a stage's keys: scale, middle (minimum + 8 scales) of key and value;
-// log2 of the largest value scale (by half); which of its four tiles exist.
+// log2 of the largest value scale of each half; its four tiles' first
+// positions and which of them exist; whether each block's rows all see all.
 struct StageKeys {
     float ks[PRE_KEYS], km[PRE_KEYS], vs[PRE_KEYS], vm[PRE_KEYS];
     float lg[2];
-    uint32_t have, unused;
+    uint32_t have, whole;  // bits: tiles; blocks
+    int k0[4];
 };
 
 __device__ __forceinline__ int stages_of(const Tiles& t) { return (t.n + 3) / 4; }
@@ -74,6 +77,10 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
     __shared__ __align__(8) uint64_t bars[2 * ST + 4 + 2 + 2 + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    // between the two warps of 32 rows: who wants a higher M, by stage parity;
+    // the factors at the start, the sums at the end
+    __shared__ int wish[2][2][8];
+    __shared__ float wants[2][2][PRE_ROWS], half_l[PRE_ROWS], half_mn[PRE_ROWS];
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     volatile int* abort = &abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -95,14 +102,14 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
         for (int s = 0; s < ST; s++) tc::bar_init(full(s), 4), tc::bar_init(empty(s), 1);
         for (int b = 0; b < 2; b++) {
             tc::bar_init(sfull(b, 0), 1), tc::bar_init(sfull(b, 1), 1);
-            tc::bar_init(pready(b), 4), tc::bar_init(odone(b), 1);
+            tc::bar_init(pready(b), 8), tc::bar_init(odone(b), 1);
         }
-        tc::bar_init(qready, 8);
+        tc::bar_init(qready, 16);
         abort_flag = 0;
         a.joins[blockIdx.x] = make_int4(0, 0, 0, -1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc::smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
@@ -185,64 +192,80 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
         }
     };
 
-    if (warp < 8) {
-        // ---- a thread a query row
+    if (warp < 16) {
+        // ---- two threads a query row: block, half of the keys, row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ROWS));
-        const int blk = warp >> 2, row = tid & 127;
+        const int blk = warp >> 3, half = warp >> 2 & 1, row = tid & 127, pair_no = blk * 4 + (warp & 3);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t scol = tmem + lanes + blk * 256, ocol = scol + 128;
+        const uint32_t scol = tmem + lanes + blk * 256 + 32 * half, ocol = tmem + lanes + blk * 256 + 128 + DV / 2 * half;
         uint8_t* qs = gbase + blk * QB;
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;\n" ::"r"(1 + pair_no) : "memory"); };
         bool ok = true;
         for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
             const int nrows = rows.n * G, x0 = b * PRE_ROWS + blk * 128, x = x0 + row;
             const bool active = x0 < nrows, on = x < nrows;
             const int tok = a.group(min(x, nrows - 1));
-            // the row's queries as f16 of 2^14 at the largest, in the order in
-            // which codes are unpacked: 0 4 1 5 2 6 3 7 of every eight
+            // the rows' queries as f16 of 2^14 at the largest, in the order in
+            // which codes are unpacked: 0 4 1 5 2 6 3 7 of every eight. The
+            // warp has sixteen rows, LQ lanes a row, all loads under way at
+            // once; each row's factors go to its threads through shared memory
             float f = 0.f, r = 0.f;
             if (active) {
-                float top = 0.f, sum = 0.f;
-                bool bad = false;
-                const T* p = q + (long long)(rows.first + tok) * a.q_row + (long long)(h * G + x - tok * G) * a.q_head;
-                float v[8];
-#pragma unroll 4
-                for (int c = 0; c < DK / 8; c++) {
-                    if (on) load8(p + 8 * c, a.q_vec, v);
+                constexpr int LQ = DK > 64 ? 16 : 8, PER = 32 / LQ, TURNS = 16 / PER;
+                const int sub = lane % LQ, y0 = 32 * (warp & 3) + 16 * half + lane / LQ;
+                float v[TURNS][8];
+#pragma unroll
+                for (int t = 0; t < TURNS; t++) {
+                    const int xq = x0 + y0 + PER * t, tq = a.group(min(xq, nrows - 1));
+                    const bool have_q = xq < nrows && 8 * sub < DK;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[t][i] = 0.f;
+                    if (have_q)
+                        load8(q + (long long)(rows.first + tq) * a.q_row + (long long)(h * G + xq - tq * G) * a.q_head + 8 * sub, a.q_vec, v[t]);
+                }
+                const float sign = a.scale_log2e < 0.f ? -1.f : 1.f;
+#pragma unroll
+                for (int t = 0; t < TURNS; t++) {
+                    const int y = y0 + PER * t;
+                    float top = 0.f, sum = 0.f;
+                    bool bad = false;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        if (!on) v[i] = 0.f;
-                        top = fmaxf(top, fabsf(v[i]));
-                        bad |= !(fabsf(v[i]) <= FLT_MAX);
-                        sum += v[i];
+                        top = fmaxf(top, fabsf(v[t][i]));
+                        bad |= !(fabsf(v[t][i]) <= FLT_MAX);
+                        sum += v[t][i];
+                    }
+#pragma unroll
+                    for (int o = 1; o < LQ; o *= 2) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
+                    }
+                    const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
+                    const float up = bad ? 0.f : sign * __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                    if (8 * sub < DK) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[t][i] = bad ? 0.f : v[t][i] * up;
+                        *(uint4*)(qs + (sub / 8) * (128 * 128) + y * 128 + ((sub % 8) ^ (y & 7)) * 16) =
+                            make_uint4(pack_half2(v[t][0], v[t][4]), pack_half2(v[t][1], v[t][5]), pack_half2(v[t][2], v[t][6]), pack_half2(v[t][3], v[t][7]));
+                    }
+                    if (sub == 0) {
+                        // exponents are f x: f positive, so that the largest x has the largest
+                        const float nan = __uint_as_float(0x7fc00000u);
+                        half_l[blk * 128 + y] = bad ? nan : fmaxf(fabsf(a.scale_log2e) * __uint_as_float((uint32_t)(e - 14 + 127) << 23), 1e-37f);
+                        half_mn[blk * 128 + y] = bad ? nan : sum * up;
                     }
                 }
-                const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
-                const float sign = a.scale_log2e < 0.f ? -1.f : 1.f;
-                const float up = bad ? 0.f : sign * __uint_as_float((uint32_t)(14 - e + 127) << 23);
-                // exponents are f x: f positive, so that the largest x has the largest
-                f = fmaxf(fabsf(a.scale_log2e) * __uint_as_float((uint32_t)(e - 14 + 127) << 23), 1e-37f);
-                r = sum * up;
-                if (bad) f = r = __uint_as_float(0x7fc00000u);
-#pragma unroll 4
-                for (int c = 0; c < DK / 8; c++) {
-                    if (on) load8(p + 8 * c, a.q_vec, v);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = on && !bad ? v[i] * up : 0.f;
-                    uint4 w = make_uint4(pack_half2(v[0], v[4]), pack_half2(v[1], v[5]), pack_half2(v[2], v[6]), pack_half2(v[3], v[7]));
-                    *(uint4*)(qs + (c / 8) * (128 * 128) + row * 128 + ((c % 8) ^ (row & 7)) * 16) = w;
-                }
                 tc::fence_async_smem();
+                pair_sync();
+                f = half_l[blk * 128 + row], r = half_mn[blk * 128 + row];
+                pair_sync();
             }
             tc::fence_before();
             __syncwarp();
             if (lane == 0) tc::bar_arrive(qready);
 
-            const long long qpos = rows.pos0 + tok;
-            const int hi = on ? (int)min(max(qpos, -1LL), 0x7fffffffLL) : -1;
-            const int x_last = min(x0 + 128, nrows) - 1;
-            const long long p_first = rows.pos0 + a.group(min(x0, nrows - 1)), p_last = rows.pos0 + a.group(x_last);
-            const int all_hi = (int)min(max(p_first, -1LL), 0x7fffffffLL) - 15;
-            const int all_lo = a.window > 0 ? (int)min(max(p_last - a.window, -1LL), 0x7fffffffLL) : -1;
+            const int hi = on ? (int)min(max(rows.pos0 + tok, -1LL), 0x7fffffffLL) : -1;
             const f32x2 f2 = pair(f, f), r2 = pair(r, r);
             float M = ATT_LOW;
             f32x2 l2 = 0, mn2 = 0;
@@ -251,68 +274,73 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             for (int i = 0; i < m; i++) {
                 const int k = it0 + i, slot = k % ST, buf = k & 1;
                 if (ok) ok = warp_wait(sfull(blk, buf), (k >> 1) & 1) && warp_wait(full(slot), (k / ST) & 1);
-                if (active && ok) {
+                if (active) {
+                    // both warps of the rows come here whether or not a wait has failed
                     tc::fence_after();
                     const StageKeys& sk = keys[slot];
-                    float xs[PRE_KEYS];
+                    float xs[32];
                     tc::ld32(scol + buf * 64, xs);
-                    tc::ld32(scol + buf * 64 + 32, xs + 32);
                     tc::ld_wait32(xs);
-                    tc::ld_wait32(xs + 32);
-                    bool whole = sk.have == 15;
-                    int k0[4];
+                    const bool whole = sk.whole >> blk & 1;
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        k0[u] = tl.at(4 * (off + i) + u) * KV4_TILE;
-                        whole &= k0[u] <= all_hi && (k0[u] > all_lo || k0[u] + 15 < a.sink);
-                    }
-#pragma unroll
-                    for (int j = 0; j < PRE_KEYS; j += 4) {
-                        const float4 ks = *(const float4*)&sk.ks[j], km = *(const float4*)&sk.km[j];
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 ks = *(const float4*)&sk.ks[32 * half + j], km = *(const float4*)&sk.km[32 * half + j];
                         const float2 y = unpair(fma2(pair(xs[j], xs[j + 1]), pair(ks.x, ks.y), mul2(r2, pair(km.x, km.y))));
                         const float2 z = unpair(fma2(pair(xs[j + 2], xs[j + 3]), pair(ks.z, ks.w), mul2(r2, pair(km.z, km.w))));
                         xs[j] = y.x, xs[j + 1] = y.y, xs[j + 2] = z.x, xs[j + 3] = z.y;
                     }
                     if (__builtin_expect(!whole, 0)) {
 #pragma unroll
-                        for (int j = 0; j < PRE_KEYS; j++) {
-                            const int key = k0[j / 16] + j % 16;
-                            if (!((sk.have >> (j / 16) & 1) && key <= hi && (a.window <= 0 || key > hi - a.window || key < a.sink))) xs[j] = -INFINITY;
+                        for (int j = 0; j < 32; j++) {
+                            const int tile = 2 * half + j / 16, key = sk.k0[tile] + j % 16;
+                            if (!((sk.have >> tile & 1) && key <= hi && (a.window <= 0 || key > hi - a.window || key < a.sink))) xs[j] = -INFINITY;
                         }
                     }
-                    float top = xs[0];
+                    float t4[4] = {xs[0], xs[1], xs[2], xs[3]};
 #pragma unroll
-                    for (int j = 1; j < PRE_KEYS; j++) top = fmaxf(top, xs[j]);
-                    const float lg = fmaxf(sk.lg[0], sk.lg[1]), want = __fmaf_rn(top, f, lg);
-                    const bool raise = want > M + 4.f;
-                    if (__builtin_expect(__any_sync(0xffffffffu, raise), 0)) {
-                        const float to = raise ? want : M, scale = ex2(M - to);
+                    for (int j = 4; j < 32; j++) t4[j & 3] = fmaxf(t4[j & 3], xs[j]);
+                    const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                    const float want = __fmaf_rn(top, f, sk.lg[half]);
+                    const bool any = __any_sync(0xffffffffu, want > M + 4.f);
+                    if (lane == 0) wish[buf][half][pair_no] = any;
+                    if (any) wants[buf][half][blk * 128 + row] = want;
+                    pair_sync();
+                    const bool other = wish[buf][half ^ 1][pair_no];
+                    if (__builtin_expect(any || other, 0)) {
+                        float to = M;
+                        if (any && want > M + 4.f) to = want;
+                        if (other) {
+                            const float w = wants[buf][half ^ 1][blk * 128 + row];
+                            if (w > M + 4.f) to = fmaxf(to, w);
+                        }
+                        const float scale = ex2(M - to);
                         M = to;
                         l2 = mul2(l2, pair(scale, scale)), mn2 = mul2(mn2, pair(scale, scale));
                         if (i > 0) {
-                            ok = warp_wait(odone(blk), (k - 1) & 1);
+                            if (ok) ok = warp_wait(odone(blk), (k - 1) & 1);
                             tc::fence_after();
+                            if (ok)
 #pragma unroll 1
-                            for (int c = 0; c < DV; c += 32) {
-                                float o[32];
-                                tc::ld32(ocol + c, o);
-                                tc::ld_wait32(o);
+                                for (int c = 0; c < DV / 2; c += 16) {
+                                    float o[16];
+                                    tc::ld16(ocol + c, o);
+                                    tc::ld_wait16(o);
 #pragma unroll
-                                for (int j = 0; j < 32; j++) o[j] *= scale;
-                                tc::st32(ocol + c, (const uint32_t*)o);
-                            }
+                                    for (int j = 0; j < 16; j++) o[j] *= scale;
+                                    tc::st16(ocol + c, (const uint32_t*)o);
+                                }
                         }
                     }
                     const f32x2 nM = pair(-M, -M);
-                    // by halves of 32 keys: weights over the half's own scores
-                    auto weigh = [&](float* xh, int half, bool clean) {
+                    // weights over the half's own scores
+                    auto weigh = [&](bool clean) {
                         uint32_t w[16 * Sh::WS];
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 vs = *(const float4*)&sk.vs[32 * half + j], vm = *(const float4*)&sk.vm[32 * half + j];
 #pragma unroll
                             for (int t = 0; t < 2; t++) {
-                                const float2 xx = make_float2(xh[j + 2 * t], xh[j + 2 * t + 1]);
+                                const float2 xx = make_float2(xs[j + 2 * t], xs[j + 2 * t + 1]);
                                 const float2 e = unpair(fma2(pair(xx.x, xx.y), f2, nM));
                                 const f32x2 p = pair(ex2(e.x), ex2(e.y));
                                 f32x2 s2 = t ? pair(vs.z, vs.w) : pair(vs.x, vs.y), m2 = t ? pair(vm.z, vm.w) : pair(vm.x, vm.y);
@@ -332,11 +360,11 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                                 }
                             }
                         }
-                        if constexpr (Sh::WS == 2) tc::st32(scol + buf * 64 + 32 * half, w);
-                        else tc::st16(scol + buf * 64 + 32 * half, w);
+                        if constexpr (Sh::WS == 2) tc::st32(scol + buf * 64, w);
+                        else tc::st16(scol + buf * 64, w);
                     };
-                    if (__builtin_expect(whole, 1)) weigh(xs, 0, false), weigh(xs + 32, 1, false);
-                    else weigh(xs, 0, true), weigh(xs + 32, 1, true);
+                    if (__builtin_expect(whole, 1)) weigh(false);
+                    else weigh(true);
                     tc::st_wait();
                     tc::fence_before();
                 }
@@ -354,36 +382,45 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             if (active) {
                 tc::fence_after();
                 const float2 lp = unpair(l2), mp = unpair(mn2);
-                float l = lp.x + lp.y;
-                const float mn = mp.x + mp.y;
+                float l = lp.x + lp.y, mn = mp.x + mp.y;
                 if (!ok) l = __uint_as_float(0x7fc00000u);
+                const int y = blk * 128 + row;
+                // the halves' sums, each row's in one order
+                if (half) half_l[y] = l, half_mn[y] = mn;
+                pair_sync();
+                if (!half) {
+                    l += half_l[y], mn += half_mn[y];
+                    half_l[y] = l, half_mn[y] = mn;
+                }
+                pair_sync();
+                l = half_l[y], mn = half_mn[y];
                 const float norm = done ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 const OutRows<T> to{out, a, rows.first, h, nrows};
                 float* part = a.parts + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Sh::PART;
-                const int y = blk * 128 + row;
                 T* o_row = to.at(min(x, nrows - 1));
 #pragma unroll 1
-                for (int c = 0; c < DV; c += 32) {
-                    float o[32];
-                    tc::ld32(ocol + c, o);
-                    tc::ld_wait32(o);
+                for (int c = 0; c < DV / 2; c += 16) {
+                    float o[16];
+                    tc::ld16(ocol + c, o);
+                    tc::ld_wait16(o);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) o[j] = (o[j] + mn) * norm;
+                    for (int j = 0; j < 16; j++) o[j] = (o[j] + mn) * norm;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        if (!done) store8(part + (size_t)y * DV + c + j, true, o + j);
-                        else if (on) store8(o_row + c + j, a.o_vec, o + j);
+                    for (int j = 0; j < 16; j += 8) {
+                        const int d = DV / 2 * half + c + j;
+                        if (!done) store8(part + (size_t)y * DV + d, true, o + j);
+                        else if (on) store8(o_row + d, a.o_vec, o + j);
                     }
                 }
-                if (!done) part[PRE_ROWS * DV + y] = M, part[PRE_ROWS * (DV + 1) + y] = l;
+                if (!done && !half) part[PRE_ROWS * DV + y] = M, part[PRE_ROWS * (DV + 1) + y] = l;
                 tc::fence_before();
             }
             if (starts && !ends && tid == 0) a.joins[blockIdx.x] = make_int4(s, h, b, (int)(last / share - blockIdx.x));
         });
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ---- codes to operands
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_CODES));
-        const int t = tid - 256, half = t >> 6, key = t & 63, w4 = warp - 8;
+        const int t = tid - 512, half = t >> 6, key = t & 63, w4 = warp - 16;
         constexpr int KW = DK / 16, VWW = DV / 32;  // words of a half key row; of a quarter value row
         bool ok = true;
         for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
@@ -391,6 +428,14 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             const int32_t* trow = a.kv.table + (size_t)s * a.kv.table_stride;
             const uint8_t* head = a.kv.pool + (size_t)h * a.kv.page_tiles * TB;
             const long long len = rows.pos0 + rows.n;
+            // tiles wholly inside every row's span of a block need no masks
+            int all_hi[2], all_lo[2];
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++) {
+                const int x0 = min(b * PRE_ROWS + blk * 128, rows.n * G - 1), x1 = min(b * PRE_ROWS + blk * 128 + 128, rows.n * G) - 1;
+                all_hi[blk] = (int)min(max(rows.pos0 + a.group(x0), -1LL), 0x7fffffffLL) - 15;
+                all_lo[blk] = a.window > 0 ? (int)min(max(rows.pos0 + a.group(max(x1, 0)) - a.window, -1LL), 0x7fffffffLL) : -1;
+            }
             auto fetch = [&](int i) -> unsigned long long {  // the i-th tile's address, 0: no such page
                 if (i >= n) return 0;
                 const int tile = tl.at(first + i), p = a.page_tiles(tile);
@@ -474,7 +519,18 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
 #pragma unroll
                     for (int o = 16; o; o /= 2) lg = fmaxf(lg, __shfl_xor_sync(0xffffffffu, lg, o));
                     if (lane == 0) sk.lg[w4] = lg;
-                    if (t == 0) sk.have = have;
+                    if (t == 0) {
+                        uint32_t see = have == 15 ? 3 : 0;
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int k0 = tl.at(first + 4 * i + u) * KV4_TILE;
+                            sk.k0[u] = k0;
+#pragma unroll
+                            for (int blk = 0; blk < 2; blk++)
+                                if (!(k0 <= all_hi[blk] && (k0 > all_lo[blk] || k0 + 15 < a.sink))) see &= ~(1u << blk);
+                        }
+                        sk.have = have, sk.whole = see;
+                    }
                 }
                 tc::fence_async_smem();
                 __syncwarp();
@@ -487,7 +543,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ISSUE));
         bool ok = true;
         int issued = 0;
-        if (warp == 12) for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
+        if (warp == 20) for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
             if (lane == 0) {
                 const int blocks = b * PRE_ROWS + 128 < rows.n * G ? 2 : 1;
                 if (ok) ok = tc::bar_wait(qready, part_no & 1, abort);
@@ -530,12 +586,12 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             __syncwarp();
         });
         // every product issued is over before the memory is freed
-        if (warp == 12 && lane == 0 && issued > 0) tc::bar_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1, abort);
+        if (warp == 20 && lane == 0 && issued > 0) tc::bar_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1, abort);
         __syncwarp();
     }
     tc::fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc::fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -560,7 +616,7 @@ static void launch(const AttendArgs& a0, const void* q, void* out, void* ws, cud
     kv4_prefill_kernel<DK, DV, T><<<ctas, PRE_THREADS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, 32);
+    cfg.gridDim = dim3(ctas, 8);
     cfg.blockDim = dim3(512);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
