@@ -228,19 +228,17 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 for (int t = 0; t < TURNS; t++) {
                     const int y = y0 + PER * t;
                     float top = 0.f, sum = 0.f;
-                    bool bad = false;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         top = fmaxf(top, fabsf(v[t][i]));
-                        bad |= !(fabsf(v[t][i]) <= FLT_MAX);
                         sum += v[t][i];
                     }
 #pragma unroll
                     for (int o = 1; o < LQ; o *= 2) {
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
                     }
+                    const bool bad = !(top <= FLT_MAX && sum == sum);  // an infinity, a NaN
                     const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 127);
                     const float up = bad ? 0.f : sign * __uint_as_float((uint32_t)(14 - e + 127) << 23);
                     if (8 * sub < DK) {
