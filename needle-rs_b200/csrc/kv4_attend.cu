@@ -58,7 +58,7 @@ constexpr int ATT_CTAS(int nt, int dv) { return nt == 2 || dv == 128 ? 3 : 4; } 
 constexpr int ATT_MIN_SHARE = 8;
 // What beginning and ending a unit costs a warp, in tiles: without it a warp
 // that meets many short units is the last by far (8 sequences, one of a
-// single position among lengths up to 32768: 70 us instead of UNIT_US).
+// single position among lengths up to 32768: 70 us instead of 57).
 constexpr int ATT_UNIT_COST = 4;
 // Calls whose units all have at most this many tiles take them whole, a warp
 // or, where units are too few to fill the GPU, a CTA a unit, and need no
@@ -890,24 +890,24 @@ static void attend_launch(const AttendArgs& a0, const AttendPlan& plan, const vo
     auto check = [](cudaError_t e) {
         if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
     };
-    auto prepare = [&](auto kernel, int smem) {
-        if (smem > 48 * 1024) check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        return kernel;
-    };
+    const char* what = "nd_op_kv4_attend";
     if (plan.mode == WARP) {
-        prepare(kv4_attend_whole_kernel<DK, DV, NT, T, false>, Sh::WHOLE_SMEM)<<<dim3((plan.places + ATT_WARPS - 1) / ATT_WARPS, a.kv.heads), 32 * ATT_WARPS, Sh::WHOLE_SMEM, st>>>(a, (const T*)q, (T*)out);
-        return op_launched("nd_op_kv4_attend");
+        allow_smem<kv4_attend_whole_kernel<DK, DV, NT, T, false>>(Sh::WHOLE_SMEM, what);
+        kv4_attend_whole_kernel<DK, DV, NT, T, false><<<dim3((plan.places + ATT_WARPS - 1) / ATT_WARPS, a.kv.heads), 32 * ATT_WARPS, Sh::WHOLE_SMEM, st>>>(a, (const T*)q, (T*)out);
+        return op_launched(what);
     }
     if constexpr (NT == 1)
         if (plan.mode == CTA) {
-            prepare(kv4_attend_whole_kernel<DK, DV, NT, T, true>, Sh::WHOLE_SMEM)<<<dim3(plan.places, a.kv.heads), 32 * ATT_WARPS, Sh::WHOLE_SMEM, st>>>(a, (const T*)q, (T*)out);
-            return op_launched("nd_op_kv4_attend");
+            allow_smem<kv4_attend_whole_kernel<DK, DV, NT, T, true>>(Sh::WHOLE_SMEM, what);
+            kv4_attend_whole_kernel<DK, DV, NT, T, true><<<dim3(plan.places, a.kv.heads), 32 * ATT_WARPS, Sh::WHOLE_SMEM, st>>>(a, (const T*)q, (T*)out);
+            return op_launched(what);
         }
     const int runners = plan.ctas * (Sh::MERGE ? 1 : ATT_WARPS);
     a.joins = (int4*)ws;
     a.parts = (float*)((char*)ws + (size_t)runners * sizeof(int4));
-    prepare(kv4_attend_kernel<DK, DV, NT, T>, Sh::SMEM)<<<plan.ctas, 32 * ATT_WARPS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
-    op_launched("nd_op_kv4_attend");
+    allow_smem<kv4_attend_kernel<DK, DV, NT, T>>(Sh::SMEM, what);
+    kv4_attend_kernel<DK, DV, NT, T><<<plan.ctas, 32 * ATT_WARPS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
+    op_launched(what);
     // launched early where the stream allows it; it waits for the first kernel's results
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(runners);

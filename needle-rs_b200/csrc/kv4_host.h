@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <exception>
 #include <stdexcept>
 #include <string>
@@ -60,6 +61,21 @@ inline void op_launched(const char* what, int kernels = 1) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
     add_launches(kernels);
+}
+
+// Lets a kernel have `bytes` of shared memory, once a device: the call costs
+// a microsecond.
+template <auto Kernel>
+void allow_smem(int bytes, const char* what) {
+    static std::atomic<unsigned long long> done{0};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit);
+    }
+    if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 Kv4Args kv4_args(const nd_kv4* kv, const char* what);

@@ -610,7 +610,7 @@ static void launch(const AttendArgs& a0, const void* q, void* out, void* ws, cud
     auto check = [](cudaError_t e) {
         if (e != cudaSuccess) throw std::runtime_error(std::string("nd_op_kv4_attend: ") + cudaGetErrorString(e));
     };
-    check(cudaFuncSetAttribute(kv4_prefill_kernel<DK, DV, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM));
+    allow_smem<kv4_prefill_kernel<DK, DV, T>>(Sh::SMEM, "nd_op_kv4_attend");
     kv4_prefill_kernel<DK, DV, T><<<ctas, PRE_THREADS, Sh::SMEM, st>>>(a, (const T*)q, (T*)out);
     op_launched("nd_op_kv4_attend");
     cudaLaunchConfig_t cfg{};

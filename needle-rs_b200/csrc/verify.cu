@@ -19,9 +19,12 @@
 // shared memory, each CTA adds them up in order, and the warp whose run holds
 // the place walks it 32 values at a time.
 //
-// Measured (us, GPU alone; 256 sequences of up to 7 drafts, 16384 f32 logits,
-// 98 MB in all): one kernel with a CTA a row and f64 terms taken twice 236; as
-// it is now VERIFY_US.
+// Measured (us, GPU alone; 256 sequences of up to 7 drafts, 16384 f32 logits):
+// one kernel with a CTA a row 236; two kernels 64, the second waiting for
+// its f64 terms one after another; with terms in batches without branches 53.
+// A warp's run of 1024 (two CTAs a row, which fills the GPU) beat runs of 512
+// and 256 on four and eight CTAs, 66 and 67, whose waits for one another are
+// paid more often.
 
 #include <cooperative_groups.h>
 
@@ -494,7 +497,7 @@ static void verify_launch(const VerifyArgs& a, const void* logits, int ctas, cud
     verify_stats_kernel<T><<<(unsigned)a.seqs * (a.T + 1) * a.parts, VF_STATS, 0, st>>>(a, (const T*)logits);
     op_launched("nd_op_verify");
     constexpr int SMEM = VF_WARPS * VF_CACHE * sizeof(double);
-    check(cudaFuncSetAttribute(verify_draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    allow_smem<verify_draw_kernel<T>>(SMEM, "nd_op_verify");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)a.seqs * ctas);
     cfg.blockDim = dim3(VF_DRAW);

@@ -31,7 +31,7 @@ def _stream(device):
 
 def _int32(t, n, device, name):
     """The address of a contiguous int32 vector of n."""
-    if t.dtype is not torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor [{n}] on {device}")
     return t.data_ptr()
 
@@ -78,11 +78,11 @@ class KV4Pool:
         return C.byref(a)
 
     def _rows(self, x, heads, d, name):
-        if (x.dtype not in _TYPES or x.dim() != 3 or x.device != self.device or x.shape[1] != heads or x.shape[2] != d
-                or x.stride(2) != 1):
+        shape, stride = x.shape, x.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != d or stride[2] != 1 or x.dtype not in _TYPES or x.device != self.device:
             raise ValueError(f"{name} must be a float32, float16 or bfloat16 tensor [rows, {heads}, {d}] on {self.device}, "
                              "its last dimension contiguous")
-        return x.data_ptr(), x.stride(0), x.stride(1)
+        return x.data_ptr(), stride[0], stride[1]
 
 
 def op_kv4_append(kv, k, v, table, lens, start=None):
@@ -109,10 +109,11 @@ def op_kv4_read(kv, table, lens, start=None, rows=None, dtype=torch.float32):
         raise ValueError("dtype must be float32, float16 or bfloat16")
     rows = table.shape[0] if rows is None else rows
     a = kv._args(table, lens, start, rows)
-    k = torch.empty((rows, kv.heads, kv.dk), dtype=dtype, device=kv.device)
-    v = torch.empty((rows, kv.heads, kv.dv), dtype=dtype, device=kv.device)
-    if lib().nd_op_kv4_read(a, _TYPES[dtype], *kv._rows(k, kv.heads, kv.dk, "k"), *kv._rows(v, kv.heads, kv.dv, "v"),
-                            _ZERO_REST, _stream(kv.device)) != 0:
+    k = kv.data.new_empty((rows, kv.heads, kv.dk), dtype=dtype)
+    v = kv.data.new_empty((rows, kv.heads, kv.dv), dtype=dtype)
+    hk, hv = kv.heads * kv.dk, kv.heads * kv.dv
+    if lib().nd_op_kv4_read(a, _TYPES[dtype], k.data_ptr(), hk, kv.dk, v.data_ptr(), hv, kv.dv, _ZERO_REST,
+                            _stream(kv.device)) != 0:
         raise _err()
     return k, v
 
@@ -124,20 +125,23 @@ def op_kv4_attend(kv, q, table, lens, start=None, scale=None, window=0, sink=0, 
     ``window`` of them and the first ``sink``. ``scale`` defaults to
     1 / sqrt(dk). Rows behind the last sequence are left as they were in a
     given ``out`` and are zeros in a new one."""
-    if q.dim() != 3 or not q.shape[1] or q.shape[1] % kv.heads:
+    shape = q.shape
+    if len(shape) != 3 or not shape[1] or shape[1] % kv.heads:
         raise ValueError(f"q must be [rows, q_heads, dk] with a multiple of {kv.heads} heads")
-    rows, hq, _ = q.shape
+    rows, hq = shape[0], shape[1]
     qa = kv._rows(q, hq, kv.dk, "q")
     a = kv._args(table, lens, start, rows)
     new = out is None
     if new:
-        out = torch.empty((rows, hq, kv.dv), dtype=q.dtype, device=kv.device)
-    elif out.dtype is not q.dtype or out.shape[:1] != q.shape[:1]:
-        raise ValueError("out must have q's type and rows")
-    oa = kv._rows(out, hq, kv.dv, "out")
+        out = q.new_empty((rows, hq, kv.dv))
+        oa = out.data_ptr(), hq * kv.dv, kv.dv
+    else:
+        if out.dtype is not q.dtype or out.shape[:1] != q.shape[:1]:
+            raise ValueError("out must have q's type and rows")
+        oa = kv._rows(out, hq, kv.dv, "out")
     L = lib()
     n = L.nd_op_kv4_attend_ws(a, _TYPES[q.dtype], hq, window, sink)
-    ws = torch.empty(n, dtype=torch.uint8, device=kv.device) if n else None
+    ws = kv.data.new_empty(n) if n else None
     if L.nd_op_kv4_attend(a, _TYPES[q.dtype], *qa, hq, 1 / math.sqrt(kv.dk) if scale is None else scale, window, sink, *oa,
                           ws.data_ptr() if n else None, n, _ZERO_REST if new else 0, _stream(kv.device)) != 0:
         raise _err()
@@ -193,11 +197,10 @@ def op_pages_fork(pool, table, src, keep, need, page, pinned=None, axis=0):
     n = src.shape[0] if src.dim() else 0
     if not n:
         raise ValueError("src must name at least one sequence")
-    out = torch.empty((n, p), dtype=torch.int32, device=dev)
-    refs = torch.empty(n_pages, dtype=torch.int32, device=dev)
+    out, refs = table.new_empty((n, p)), table.new_empty(n_pages)
     L = lib()
     size = L.nd_op_pages_fork_ws(n_pages, n)
-    ws = torch.empty(4 + (size + 3) // 4, dtype=torch.int32, device=dev)
+    ws = table.new_empty(4 + (size + 3) // 4)
     info = ws[:4]
     if L.nd_op_pages_fork(pv, table.data_ptr(), stride, s, p, page, _int32(src, n, dev, "src"), _int32(keep, n, dev, "keep"),
                           _int32(need, n, dev, "need"), n, _pinned(pinned, n_pages, dev), out.data_ptr(), refs.data_ptr(),
@@ -213,11 +216,10 @@ def op_pages_compact(pool, table, pinned=None, axis=0):
     dev = pool.device
     pv, n_pages = _pages(pool, axis)
     s, p, stride = _table(table, dev)
-    out = torch.empty((s, p), dtype=torch.int32, device=dev)
-    to = torch.empty(n_pages, dtype=torch.int32, device=dev)
+    out, to = table.new_empty((s, p)), table.new_empty(n_pages)
     L = lib()
     size = L.nd_op_pages_compact_ws(n_pages)
-    ws = torch.empty(4 + (size + 3) // 4, dtype=torch.int32, device=dev)
+    ws = table.new_empty(4 + (size + 3) // 4)
     info = ws[:2]
     if L.nd_op_pages_compact(pv, table.data_ptr(), stride, s, p, _pinned(pinned, n_pages, dev), out.data_ptr(), to.data_ptr(),
                              ws.data_ptr(), ws.data_ptr() + 16, size, _stream(dev)) != 0:
@@ -248,13 +250,11 @@ def op_verify(logits, draft, u, temperature, q=None, counts=None):
                           or (t and q.stride(2) != 1 and v > 1)):
         raise ValueError(f"q must be a float32 tensor [{s}, {t}, {v}] on {dev}, rows contiguous")
     c = None if counts is None else _int32(counts, s, dev, "counts")
-    tokens = torch.empty((s, t1), dtype=torch.int32, device=dev)
-    accepted = torch.empty(s, dtype=torch.int32, device=dev)
-    probs = torch.empty((s, t1), dtype=torch.float32, device=dev)
+    tokens, accepted, probs = draft.new_empty((s, t1)), draft.new_empty(s), u.new_empty((s, t1))
     qa = (None, 0, 0) if q is None or not t else (q.data_ptr(), q.stride(0), q.stride(1))
     L = lib()
     size = L.nd_op_verify_ws(s, t, v)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = u.new_empty(size // 4)
     if L.nd_op_verify(dev.index, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
                       draft.data_ptr(), c, u.data_ptr(), temperature.data_ptr(), *qa, s, t, v, tokens.data_ptr(),
                       accepted.data_ptr(), probs.data_ptr(), ws.data_ptr(), size, _stream(dev)) != 0:
