@@ -67,7 +67,7 @@ constexpr int ATT_UNIT_COST = 4;
 // 32 of up to 1000 14.9, -, 11.1.
 // Query rows a sequence brings to a kv head on average from which 16-bit rows
 // go to the tcgen05 kernel.
-constexpr int ATT_TC_ROWS = 192;
+constexpr int ATT_TC_ROWS = 128;
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
 
 // Whole units are numbered without sums. Places 0 .. seqs - 1 are the

@@ -57,6 +57,17 @@ struct StageKeys {
     int k0[4];
 };
 
+// Four values of a row, by one store where `vec` says eight are aligned.
+__device__ __forceinline__ void store4(__half* p, bool vec, float4 v) {
+    if (vec) *(uint2*)p = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+    else p[0] = __float2half_rn(v.x), p[1] = __float2half_rn(v.y), p[2] = __float2half_rn(v.z), p[3] = __float2half_rn(v.w);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, bool vec, float4 v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    if (vec) *(uint2*)p = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+    else p[0] = a.x, p[1] = a.y, p[2] = b.x, p[3] = b.y;
+}
+
 __device__ __forceinline__ int stages_of(const Tiles& t) { return (t.n + 3) / 4; }
 
 __device__ __forceinline__ long long pre_work(const AttendArgs& a, const SeqRows& r) {
@@ -395,23 +406,39 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 const float norm = done ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 const OutRows<T> to{out, a, rows.first, h, nrows};
                 float* part = a.parts + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Sh::PART;
-                T* o_row = to.at(min(x, nrows - 1));
+                // by way of the queries' shared memory, which this block's
+                // products are done with, so that rows leave as whole lines:
+                // a thread a row has 32 of them open at once, which took 8 to
+                // 12 thousand cycles a part
+                constexpr int CR = DK > 64 ? 32 : 16, QUADS = CR / 4;  // dimensions a turn
+                float4* stage = (float4*)(qs + ((warp & 3) * 2 + half) * (32 * CR * 4));
 #pragma unroll 1
-                for (int c = 0; c < DV / 2; c += 16) {
-                    float o[16];
-                    tc::ld16(ocol + c, o);
-                    tc::ld_wait16(o);
+                for (int c = 0; c < DV / 2; c += CR) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) o[j] = (o[j] + mn) * norm;
+                    for (int u = 0; u < CR; u += 16) {
+                        float o[16];
+                        tc::ld16(ocol + c + u, o);
+                        tc::ld_wait16(o);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 8) {
-                        const int d = DV / 2 * half + c + j;
-                        if (!done) store8(part + (size_t)y * DV + d, true, o + j);
-                        else if (on) store8(o_row + d, a.o_vec, o + j);
+                        for (int j = 0; j < 16; j += 4)
+                            stage[lane * QUADS + (((u + j) / 4) ^ (lane & (QUADS - 1)))] =
+                                make_float4((o[j] + mn) * norm, (o[j + 1] + mn) * norm, (o[j + 2] + mn) * norm, (o[j + 3] + mn) * norm);
                     }
+                    __syncwarp();
+#pragma unroll
+                    for (int t = 0; t < QUADS; t++) {
+                        const int yy = t * (32 / QUADS) + lane / QUADS, quad = lane % QUADS;
+                        const float4 v = stage[yy * QUADS + (quad ^ (yy & (QUADS - 1)))];
+                        const int yb = blk * 128 + 32 * (warp & 3) + yy, xr = b * PRE_ROWS + yb, d = DV / 2 * half + c + 4 * quad;
+                        if (!done) *(float4*)(part + (size_t)yb * DV + d) = v;
+                        else if (xr < nrows) store4(to.at(xr) + d, a.o_vec, v);
+                    }
+                    __syncwarp();
                 }
                 if (!done && !half) part[PRE_ROWS * DV + y] = M, part[PRE_ROWS * (DV + 1) + y] = l;
                 tc::fence_before();
+                // the queries' place is written again by any of the block's warps
+                asm volatile("bar.sync %0, 256;\n" ::"r"(9 + blk) : "memory");
             }
             if (starts && !ends && tid == 0) a.joins[blockIdx.x] = make_int4(s, h, b, (int)(last / share - blockIdx.x));
         });
