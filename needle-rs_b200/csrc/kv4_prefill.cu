@@ -564,55 +564,68 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             }
         });
     } else {
-        // ---- the products: lane 0 of the first of four warps waits and issues
+        // ---- the products: an elected lane of the first of four warps issues
+        // them. What a product takes is the same in all lanes and known to be
+        // (shuffled), and differs by constants from step to step: with
+        // addresses formed for each product by one lane on its own, issuing a
+        // stage took 3500 cycles, three times what computing it does.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ISSUE));
         bool ok = true;
         int issued = 0;
-        if (warp == 20) for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m, int part_no, int it0, long long last) {
-            if (lane == 0) {
-                const int blocks = b * PRE_ROWS + 128 < rows.n * G ? 2 : 1;
-                if (ok) ok = tc::bar_wait(qready, part_no & 1, abort);
-                auto scores = [&](int k) {
-                    const int slot = k % ST;
-                    if (ok) ok = tc::bar_wait(full(slot), (k / ST) & 1, abort);
-                    if (!ok) return;
-                    tc::fence_after();
-                    const uint32_t ks = base + 2 * QB + slot * (KB + VB);
-                    for (int blk = 0; blk < 2; blk++) {
-                        if (blk < blocks)
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q_lo = tc::sw128_lo(__shfl_sync(0xffffffffu, base, 0));
+        if (warp == 20) for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m_, int part_no, int it0_, long long last) {
+            const int m = __shfl_sync(0xffffffffu, m_, 0), it0 = __shfl_sync(0xffffffffu, it0_, 0);
+            const bool both = __shfl_sync(0xffffffffu, b * PRE_ROWS + 128 < rows.n * G, 0);
+            if (ok) ok = warp_wait(qready, part_no & 1);
+            auto scores = [&](int k) {
+                const int slot = k % ST;
+                if (ok) ok = warp_wait(full(slot), (k / ST) & 1);
+                if (!ok) return;
+                tc::fence_after();
+                const uint32_t k_lo = q_lo + ((2 * QB + slot * (KB + VB)) >> 4), d = tm + (k & 1) * 64;
+                if (tc::elect()) {
 #pragma unroll
-                            for (int c = 0; c < DK / 16; c++)
-                                tc::mma_ss(tmem + blk * 256 + (k & 1) * 64, tc::sw128_desc(base + blk * QB + c / 4 * (128 * 128) + c % 4 * 32),
-                                           tc::sw128_desc(ks + c / 4 * (PRE_KEYS * 128) + c % 4 * 32), tc::f16_idesc(PRE_KEYS), c > 0);
-                        tc::commit(sfull(blk, k & 1));
-                    }
-                };
-                scores(it0);
-                for (int i = 0; i < m && ok; i++) {
-                    const int k = it0 + i, slot = k % ST;
-                    if (i + 1 < m) scores(k + 1);
-                    const uint32_t vs = base + 2 * QB + slot * (KB + VB) + KB;
-                    for (int blk = 0; blk < 2; blk++) {
-                        if (ok) ok = tc::bar_wait(pready(blk), k & 1, abort);
-                        if (!ok) break;
-                        tc::fence_after();
-                        if (blk < blocks)
+                    for (int c = 0; c < DK / 16; c++)
+                        tc::mma_ss(d, q_lo + c / 4 * (128 * 128 >> 4) + c % 4 * 2, k_lo + c / 4 * (PRE_KEYS * 128 >> 4) + c % 4 * 2, tc::f16_idesc(PRE_KEYS), c > 0);
+                    tc::commit(sfull(0, k & 1));
+                    if (both)
+#pragma unroll
+                        for (int c = 0; c < DK / 16; c++)
+                            tc::mma_ss(d + 256, q_lo + (QB >> 4) + c / 4 * (128 * 128 >> 4) + c % 4 * 2, k_lo + c / 4 * (PRE_KEYS * 128 >> 4) + c % 4 * 2,
+                                       tc::f16_idesc(PRE_KEYS), c > 0);
+                    tc::commit(sfull(1, k & 1));
+                }
+                __syncwarp();
+            };
+            scores(it0);
+#pragma unroll 1
+            for (int i = 0; i < m && ok; i++) {
+                const int k = it0 + i, slot = k % ST;
+                if (i + 1 < m) scores(k + 1);
+                const uint32_t v_lo = q_lo + ((2 * QB + slot * (KB + VB) + KB) >> 4), p = tm + (k & 1) * 64;
+#pragma unroll
+                for (int blk = 0; blk < 2; blk++) {
+                    if (ok) ok = warp_wait(pready(blk), k & 1);
+                    if (!ok) break;
+                    tc::fence_after();
+                    if (tc::elect()) {
+                        if (blk == 0 || both)
 #pragma unroll
                             for (int term = 0; term < Sh::WS; term++)
 #pragma unroll
                                 for (int c = 0; c < PRE_KEYS / 16; c++)
-                                    tc::mma_ts(tmem + blk * 256 + 128, tmem + blk * 256 + (k & 1) * 64 + c / 2 * 32 + term * 16 + c % 2 * 8,
-                                               tc::sw128_desc(vs + c * 32), tc::f16_idesc(DV), i > 0 || term > 0 || c > 0);
+                                    tc::mma_ts(tm + blk * 256 + 128, p + blk * 256 + c / 2 * 32 + term * 16 + c % 2 * 8, v_lo + c * 2, tc::f16_idesc(DV),
+                                               term > 0 || c > 0 ? 1u : (uint32_t)(i > 0));
                         tc::commit(odone(blk));
+                        if (blk == 1) tc::commit(empty(slot));
                     }
-                    if (ok) tc::commit(empty(slot)), issued = k + 1;
+                    __syncwarp();
+                    if (blk == 1) issued = k + 1;
                 }
             }
-            __syncwarp();
         });
         // every product issued is over before the memory is freed
-        if (warp == 20 && lane == 0 && issued > 0) tc::bar_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1, abort);
-        __syncwarp();
+        if (warp == 20 && issued > 0) warp_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1);
     }
     tc::fence_before();
     __syncthreads();

@@ -38,24 +38,34 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 
-// A K-major operand in the 128-byte swizzle: rows of 128 bytes, 8-row atoms
-// 1024 bytes apart, version 1, layout SWIZZLE_128B (2).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
+// Descriptor of a K-major operand in the 128-byte swizzle: rows of 128 bytes,
+// 8-row atoms 1024 bytes apart, version 1, layout SWIZZLE_128B (2). The low
+// word holds the address in 16-byte units and is all that differs between the
+// steps of a product, so that they are one addition apart.
+constexpr uint32_t SW128_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+
+// True in one lane of the warp, the same each time.
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
 }
+
 // kind::f16 with f32 sums, f16 operands, both K-major, M = 128.
 __host__ __device__ constexpr uint32_t f16_idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+                 "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SW128_HI)
                  : "memory");
 }
 // A from tensor memory: a lane a row, two values a column.
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\n.reg .b64 b;\nmov.b64 b, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d),
+                 "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(SW128_HI)
                  : "memory");
 }
 // Arrive on `bar` once every tcgen05 operation this thread issued so far has completed.
