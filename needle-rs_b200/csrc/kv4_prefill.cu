@@ -566,9 +566,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
     } else {
         // ---- the products: an elected lane of the first of four warps issues
         // them. What a product takes is the same in all lanes and known to be
-        // (shuffled), and differs by constants from step to step: with
-        // addresses formed for each product by one lane on its own, issuing a
-        // stage took 3500 cycles, three times what computing it does.
+        // (shuffled), and differs by constants from step to step.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ISSUE));
         bool ok = true;
         int issued = 0;

@@ -489,3 +489,109 @@ def test_entry_points_refuse_without_a_gpu():
     a = KV4(**good)
     assert lib.nd_op_kv4_append(C.byref(a), 0, None, 96, 48, 4096, 128, 64, None) == -1 and b"null" in lib.nd_last_error()
     assert lib.nd_op_kv4_read(C.byref(a), 0, 4096, 96, 0, 4096, 128, 64, 0, None) == -1 and b"overlap" in lib.nd_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [[1, 1, 1], [3, 1, 7], [40, 0, 5]])
+def test_attend_many_heads_on_one(cuda_device, dtype, n):
+    """64 query heads on one kv head, the most there may be."""
+    import needle_b200 as nb
+
+    HEADS["mqa"] = (64, 1, 64, 64)
+    st = Setup("mqa", dtype, [100, 33, 300], n, 16, seed=4).append()
+    got = nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start), window=50, sink=7)
+    _check(st, dtype, got, 50, 7)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_device):
+    """Pages that lie more than 4 GB into a pool, and copies between them."""
+    import needle_b200 as nb
+    import torch
+
+    pages, heads = 34000, 8
+    kv = nb.KV4Pool(torch.empty((pages, heads, 8, nb.KV4Pool.tile_bytes(128, 128)), dtype=torch.uint8, device="cuda"), 128, 128)
+    assert kv.data.numel() > 1.08 * 2 ** 32
+    ids = [pages - 1, 5, pages - 2, 31000, pages - 4]
+    table = torch.tensor([ids[:2], ids[2:4]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([250, 140], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 250, 390], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn((390, heads, 128), device="cuda", generator=g) for _ in range(2))
+    nb.op_kv4_append(kv, k, v, table, lens, start)
+    low = nb.KV4Pool.new(4, heads, 128, 128, page=128)
+    low_table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    nb.op_kv4_append(low, k, v, low_table, lens, start)
+    for q in (torch.randn((2, 32, 128), device="cuda", generator=g), torch.randn((200, 32, 128), device="cuda", generator=g).bfloat16()):
+        n = q.shape[0] // 2
+        first = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+        assert torch.equal(nb.op_kv4_attend(kv, q, table, lens, first), nb.op_kv4_attend(low, q, low_table, lens, first))
+    a, b = nb.op_kv4_read(kv, table, lens, start, rows=390), nb.op_kv4_read(low, low_table, lens, start, rows=390)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    # a copy: the second sequence forked, everything below the high pages taken
+    pinned = torch.ones(pages, dtype=torch.bool, device="cuda")
+    pinned[ids] = False
+    src = torch.tensor([1, 1], dtype=torch.int32, device="cuda")
+    keep = torch.tensor([140, 140], dtype=torch.int32, device="cuda")
+    t2, _, info = nb.op_pages_fork(kv.data, table, src, keep, keep + 1, 128, pinned=pinned)
+    assert info[2] == 1 and t2.tolist() == [[pages - 2, 31000], [pages - 2, 5]]
+    assert torch.equal(kv.data[5], kv.data[31000])
+
+
+@pytest.mark.gpu
+def test_calls_side_by_side(cuda_device):
+    """Attention of three kinds on three streams at once, then replayed from
+    three graphs at once: as one after another."""
+    import needle_b200 as nb
+    import torch
+
+    sets = [Setup("wide", "bf16", [900, 1000], [200, 257], 32, seed=1).append(), Setup("wide", "bf16", [3000, 700], [1, 1], 64, seed=2).append(),
+            Setup("needle", "f32", [60, 200, 31], [1, 1, 1], 16, seed=3).append()]
+    args = [(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start)) for st in sets]
+    want = [nb.op_kv4_attend(*a) for a in args]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, a in zip(streams, args):
+            with torch.cuda.stream(s):
+                got.append(nb.op_kv4_attend(*a))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    graphs, outs = [], []
+    for s, a in zip(streams, args):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(nb.op_kv4_attend(*a))
+        graphs.append(g)
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+@pytest.mark.gpu
+def test_prompts_replayed_with_other_lengths(cuda_device):
+    import needle_b200 as nb
+    import torch
+
+    st = Setup("wide", "bf16", [400, 300], [150, 140], 32, seed=6).append()
+    t, lens, start = st.dev(st.table), st.dev(st.lens), st.dev(st.start)
+    nb.op_kv4_attend(st.kv, st.q, t, lens, start)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = nb.op_kv4_attend(st.kv, st.q, t, lens, start)
+    for new_lens, n in (([400, 300], [150, 140]), ([250, 290], [10, 280]), ([0, 5], [0, 290])):
+        st.lens, st.start = np.array(new_lens, np.int32), np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+        lens.copy_(st.dev(st.lens))
+        start.copy_(st.dev(st.start))
+        g.replay()
+        torch.cuda.synchronize()
+        _check(st, "bf16", out)
