@@ -272,7 +272,7 @@ int nd_op_gather(const nd_model* m, const int* ids, int T, float* out, void* str
  * No counterpart in the reference, whose cache is one session's int8 ring.
  * Device pointers of GPU `device`, whichever device is current; queued on
  * `stream` (of that device; NULL = its legacy default stream) and not waited
- * for; 0 on success, -1 with nd_last_error() and nothing queued. No call
+ * for; 0 on success, -1 with nd_last_error() and nothing that would write a result queued. No call
  * allocates or keeps anything, so all may be captured into a graph; a
  * workspace `ws` is the caller's, holds nothing between calls, and must not
  * be used by two calls that overlap on the GPU. Lengths, tables and ids are
@@ -291,8 +291,8 @@ enum { ND_ZERO_REST = 2 };
  * [16][dk / 2], value codes [16][dv / 2] (two a byte, lower dimension in the
  * low nibble), f16 (scale, minimum) of the 16 keys, of the 16 values; a value
  * is minimum + scale * code. page is a multiple of 16; (dk, dv) is (48, 64),
- * (64, 64) or (128, 128); at most 2^20 sequences. table[seqs][max_pages] (rows table_stride apart)
- * names each sequence's pages in order; positions past its columns, or on a
+ * (64, 64) or (128, 128); at most 2^20 sequences. table[seqs][max_pages]
+ * (rows table_stride apart) names each sequence's pages in order; positions past its columns, or on a
  * page id outside [0, num_pages), do not exist. lens[seqs]: positions each
  * sequence holds, this call's rows included. The call's `rows` rows belong to
  * the sequences in order, start[s] .. start[s + 1] - 1 to sequence s
@@ -316,7 +316,9 @@ typedef struct nd_kv4 {
  * places. Per row and head, in f32: scale = f16(min((max - min) / 15, 65504)),
  * minimum = f16(min, clamped to +-65504), code = rint((x - minimum) / scale)
  * in [0, 15], 0 where scale is 0. A row of values holding a NaN or an infinity
- * is stored as NaN. Rows whose position does not exist are dropped. */
+ * is stored as NaN. Rows whose position does not exist are dropped. Two rows
+ * of one call given the same place (a page that two sequences share: fork it
+ * first) leave a mixture. */
 int nd_op_kv4_append(const nd_kv4* kv, int type, const void* k, long long k_row, long long k_head, const void* v,
                      long long v_row, long long v_head, void* stream);
 

@@ -11,7 +11,7 @@
 // the tables and copies. Past PG_SMALL pages or table entries eight CTAs are
 // too few, and each pass is a launch of its own.
 // Measured (us, GPU alone, then of a Python call): 1024 sequences of 51
-// columns over 14,704 pages 22 and 23; as launches of their own 16.5 and 36.
+// columns over 14,704 pages 22 and 21; as launches of their own 16.5 and 36.
 
 #include <cooperative_groups.h>
 
