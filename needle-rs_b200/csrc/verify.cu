@@ -21,10 +21,10 @@
 //
 // Measured (us, GPU alone; 256 sequences of up to 7 drafts, 16384 f32 logits):
 // one kernel with a CTA a row 236; two kernels 64, the second waiting for
-// its f64 terms one after another; with terms in batches without branches 53.
-// A warp's run of 1024 (two CTAs a row, which fills the GPU) beat runs of 512
-// and 256 on four and eight CTAs, 66 and 67, whose waits for one another are
-// paid more often.
+// its f64 terms one after another; with terms in batches of four without
+// branches 53, batches of eight whose places need no checks 44. Runs of 512 on
+// four CTAs instead of 1024 on two took 4 more. An exponential of fewer f64
+// steps (a table of 2^(j/16)) gained nothing: issue and latency bound it.
 
 #include <cooperative_groups.h>
 
@@ -41,7 +41,13 @@ constexpr int VF_STATS = 256;        // threads of the first kernel
 constexpr int VF_CHUNK = 4096;       // logits a CTA of it takes at a time
 constexpr int VF_MAX_PARTS = 32;
 constexpr int VF_DRAW = 256, VF_WARPS = VF_DRAW / 32;  // of the second
-constexpr int VF_CACHE = 512, BATCH = 4;  // values of its run that a warp keeps; that a lane takes at a time
+// Runs are made this short where eight CTAs can; a warp keeps its run's terms
+// up to this length, two CTAs an SM; and up to this where a CTA has an SM to
+// itself, if the grid is at most two rounds of that. Past it they are computed
+// twice (us, twice and kept: 16 sequences of 130,000 logits 65, 36; 32 of
+// 100,000 66, 44; 32 of 130,000 72, 68; but 128 of 130,000 124, 167).
+constexpr int VF_RUN = 1024, VF_CACHE = 1696, VF_CACHE_ALONE = 3392;
+constexpr int BATCH = 8;  // that a lane takes at a time
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Of a row, or a part of it: the largest logit; its first place where the
@@ -61,7 +67,7 @@ struct VerifyArgs {
     const float* temp;      // [seqs]
     const float* q;         // or NULL
     int seqs, T, V, parts;
-    bool l_vec;
+    bool l_vec, kept;  // a drawn row's terms are
     RowStats* stats;             // [seqs][T + 1][parts]
     int32_t *tokens, *accepted;  // [seqs][T + 1], [seqs]
     float* probs;                // [seqs][T + 1]
@@ -247,6 +253,9 @@ __device__ __forceinline__ RowStats join_stats(const RowStats* parts, int n, flo
     return out;
 }
 
+// Values a warp takes of a row that `runs` warps share.
+__host__ __device__ __forceinline__ int run_of(int V, int runs) { return ((V + runs - 1) / runs + 31) / 32 * 32; }
+
 template <typename T>
 __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, const T* __restrict__ logits) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -330,28 +339,30 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
     const float* q = kept < n && a.q ? a.q + s * a.q_seq + kept * a.q_row : nullptr;
     const int gone = kept < n && !a.q ? __ldg(a.draft + (size_t)s * T_ + kept) : -1;
     const int runs = C * VF_WARPS, run = rank * VF_WARPS + warp;
-    const int per = ((V + runs - 1) / runs + 31) / 32 * 32, lo = (int)min((long long)run * per, (long long)V), hi = min(lo + per, V);
-    double* cache = cache_all + warp * VF_CACHE;  // the run's terms, then what can be drawn of it
-    const bool fits = per <= VF_CACHE;
-    // BATCH values at j, j + stride, .. at a time, without branches between
-    // them, so that their loads and their chains of products overlap
-    auto terms = [&](int j, int stride, double* e) {
-        float x[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; k++) x[k] = (float)row[min(j + k * stride, V - 1)];
-#pragma unroll
-        for (int k = 0; k < BATCH; k++) e[k] = exp_below(((double)x[k] - (double)st.top) * tp.inv);
-    };
+    const int per = run_of(V, runs), lo = (int)min((long long)run * per, (long long)V), hi = min(lo + per, V);
+    double* cache = cache_all + warp * per;  // the run's terms, where they fit
+    const bool fits = a.kept;
+    // BATCH values 32 apart at a time, without branches between them, so that
+    // their loads and their chains of products overlap; what is left one by one
     double mine = 0.0;
-    for (int j = lo + lane; j - lane < hi; j += 32 * BATCH) {
+    int j = lo + lane;
+    for (; j - lane + 32 * BATCH <= hi; j += 32 * BATCH) {
+        const T* x = row + j;
         double e[BATCH];
-        terms(j, 32, e);
 #pragma unroll
-        for (int k = 0; k < BATCH; k++)
-            if (j + 32 * k < hi) {
-                if (fits) cache[j + 32 * k - lo] = e[k];
-                mine += e[k];
-            }
+        for (int k = 0; k < BATCH; k++) e[k] = (double)(float)x[32 * k];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) e[k] = exp_below((e[k] - (double)st.top) * tp.inv);
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+            if (fits) cache[j - lo + 32 * k] = e[k];
+            mine += e[k];
+        }
+    }
+    for (; j < hi; j += 32) {
+        const double e = term(row, j, st.top, tp.inv);
+        if (fits) cache[j - lo] = e;
+        mine += e;
     }
     mine = warp_sum(mine);
     if (lane == 0) sums[0][warp] = mine;
@@ -378,33 +389,29 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
     };
     const double iz = 1.0 / gather(0);
     bool whole = false;  // p itself, where the residual is all zero
-    // what can be drawn of those values (0 from `end` on)
-    auto weights = [&](int j, int stride, int end, double* w) {
-        if (fits) {
-#pragma unroll
-            for (int k = 0; k < BATCH; k++) w[k] = cache[max(min(j + k * stride, hi - 1) - lo, 0)];
-        } else {
-            terms(j, stride, w);
-        }
-        float qv[BATCH];
-#pragma unroll
-        for (int k = 0; k < BATCH; k++) qv[k] = q && !whole ? __ldg(q + min(j + k * stride, V - 1)) : 0.f;
-#pragma unroll
-        for (int k = 0; k < BATCH; k++) {
-            double r = w[k] * iz - (double)qv[k];
-            if (r < 0.0 || j + k * stride >= end || (j + k * stride == gone && !whole)) r = 0.0;
-            w[k] = r;
-        }
+    // what can be drawn of value j, of which the term is e
+    auto rest = [&](int j, double e, float qj) {
+        const double r = e * iz - (double)qj;
+        return r < 0.0 || (j == gone && !whole) ? 0.0 : r;
+    };
+    auto weight = [&](int j) {
+        return rest(j, fits ? cache[j - lo] : term(row, j, st.top, tp.inv), q && !whole ? __ldg(q + j) : 0.f);
     };
     double total;
     while (true) {
         mine = 0.0;
-        for (int j = lo + lane; j - lane < hi; j += 32 * BATCH) {
-            double w[BATCH];
-            weights(j, 32, hi, w);
+        j = lo + lane;
+        for (; j - lane + 32 * BATCH <= hi; j += 32 * BATCH) {
+            double e[BATCH];
+            float qj[BATCH];
 #pragma unroll
-            for (int k = 0; k < BATCH; k++) mine += w[k];
+            for (int k = 0; k < BATCH; k++) qj[k] = q && !whole ? __ldg(q + j + 32 * k) : 0.f;
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) e[k] = fits ? cache[j - lo + 32 * k] : term(row, j + 32 * k, st.top, tp.inv);
+#pragma unroll
+            for (int k = 0; k < BATCH; k++) mine += rest(j + 32 * k, e[k], qj[k]);
         }
+        for (; j < hi; j += 32) mine += weight(j);
         mine = warp_sum(mine);
         if (lane == 0) sums[1][warp] = mine;
         total = gather(1);
@@ -445,11 +452,10 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
             const int each = per / 32;
             double own = 0.0, incl;
             bool some = false;
-            for (int j = lo + lane * each, end = min(j + each, hi); __any_sync(0xffffffffu, j < end); j += BATCH) {
-                double w[BATCH];
-                weights(j, 1, end, w);
-#pragma unroll
-                for (int k = 0; k < BATCH; k++) own += w[k], some |= w[k] > 0.0;
+#pragma unroll 4
+            for (int j = lo + lane * each, end = min(j + each, hi); j < end; j++) {
+                const double w = weight(j);
+                own += w, some |= w > 0.0;
             }
             prefix(own, &incl);
             // should the sums' last bits differ, the last lane that has something
@@ -458,9 +464,7 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
             before += __shfl_sync(0xffffffffu, incl - own, from);
             int token = -1;
             for (int j0 = lo + from * each, end = min(j0 + each, hi); j0 < end; j0 += 32) {
-                double ws[BATCH];
-                weights(j0 + lane, 32, min(end, j0 + 32), ws);  // one each: the others lie past the end
-                const double w = ws[0];
+                const double w = j0 + lane < end ? weight(j0 + lane) : 0.0;
                 prefix(w, &incl);
                 const uint32_t any = __ballot_sync(0xffffffffu, w > 0.0);
                 const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && past && before + incl > target);
@@ -496,12 +500,15 @@ static void verify_launch(const VerifyArgs& a, const void* logits, int ctas, cud
     };
     verify_stats_kernel<T><<<(unsigned)a.seqs * (a.T + 1) * a.parts, VF_STATS, 0, st>>>(a, (const T*)logits);
     op_launched("nd_op_verify");
-    constexpr int SMEM = VF_WARPS * VF_CACHE * sizeof(double);
-    allow_smem<verify_draw_kernel<T>>(SMEM, "nd_op_verify");
+    constexpr int MOST = VF_WARPS * VF_CACHE_ALONE * sizeof(double);
+    allow_smem<verify_draw_kernel<T>>(MOST, "nd_op_verify");
+    const int per = run_of(a.V, ctas * VF_WARPS);
+    VerifyArgs b(a);
+    b.kept = per <= ((long long)a.seqs * ctas <= 2 * device_sm_count() ? VF_CACHE_ALONE : VF_CACHE);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)a.seqs * ctas);
     cfg.blockDim = dim3(VF_DRAW);
-    cfg.dynamicSmemBytes = SMEM;
+    cfg.dynamicSmemBytes = b.kept ? VF_WARPS * per * sizeof(double) : 0;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -510,7 +517,7 @@ static void verify_launch(const VerifyArgs& a, const void* logits, int ctas, cud
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = st ? 2 : 1;
-    check(cudaLaunchKernelEx(&cfg, verify_draw_kernel<T>, VerifyArgs(a), (const T*)logits));
+    check(cudaLaunchKernelEx(&cfg, verify_draw_kernel<T>, b, (const T*)logits));
     add_launches(1);
 }
 
@@ -549,7 +556,7 @@ int nd_op_verify(int device, int type, const void* logits, long long l_seq, long
         OnDevice on(device, what);
         // CTAs a drawn row: until a warp's terms fit its cache, or while they do not fill the GPU and runs are not short
         int ctas = 1;
-        while (ctas < 8 && V > 1024 * ctas && (V > VF_WARPS * VF_CACHE * ctas || seqs * ctas < 2 * device_sm_count())) ctas *= 2;
+        while (ctas < 8 && V > 1024 * ctas && (V > VF_WARPS * VF_RUN * ctas || seqs * ctas < 2 * device_sm_count())) ctas *= 2;
         cudaStream_t st = (cudaStream_t)stream;
         if (type == ND_F32) verify_launch<float>(a, logits, ctas, st);
         else if (type == ND_F16) verify_launch<__half>(a, logits, ctas, st);

@@ -256,3 +256,11 @@ def test_entry_point_refuses_without_a_gpu():
                          (dict(row=-1), b"negative"), (dict(draft=None), b"null"), (dict(seqs=0), b"sequences"),
                          (dict(T=65), b"64"), (dict(T=-1), b"64"), (dict(V=0), b"1 <= V"), (dict(tokens=None), b"null"), (dict(ws=None), b"workspace"), (dict(nbytes=8), b"workspace")):
         assert verify(**bad) == -1 and message in lib.nd_last_error(), bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("S,T,V", [(3, 2, 100003), (2, 1, 130001), (1, 1, 300007), (40, 1, 130001), (300, 0, 8200)])
+def test_long_rows(cuda_device, dtype, S, T, V):
+    """Runs that a warp keeps with two CTAs an SM, alone on one, and not at all."""
+    test_matches_reference(cuda_device, dtype, S, T, V, True)
