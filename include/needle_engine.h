@@ -292,12 +292,13 @@ enum { ND_ZERO_REST = 2 };
  * low nibble), f16 (scale, minimum) of the 16 keys, of the 16 values; a value
  * is minimum + scale * code. page is a multiple of 16; (dk, dv) is (48, 64),
  * (64, 64) or (128, 128); at most 2^20 sequences. table[seqs][max_pages]
- * (rows table_stride apart) names each sequence's pages in order; positions past its columns, or on a
- * page id outside [0, num_pages), do not exist. lens[seqs]: positions each
- * sequence holds, this call's rows included. The call's `rows` rows belong to
- * the sequences in order, start[s] .. start[s + 1] - 1 to sequence s
- * (start[seqs + 1], ascending; NULL: rows / seqs each): row i of the n of
- * sequence s is position lens[s] - n + i. Rows behind start[seqs] are left
+ * (rows table_stride apart) names each sequence's pages in order; positions
+ * past its columns, or on a page id outside [0, num_pages), do not exist.
+ * lens[seqs]: positions each sequence holds, this call's rows included. The
+ * call's `rows` rows belong to the sequences in order, start[s] .. start[s +
+ * 1] - 1 to sequence s (start[seqs + 1], ascending from 0; NULL: rows / seqs
+ * each): row i of the n of sequence s is position lens[s] - n + i. Rows behind
+ * start[seqs] are left
  * alone. */
 typedef struct nd_kv4 {
     int device;

@@ -94,7 +94,7 @@ __device__ __forceinline__ int seq_of_place(const AttendArgs& a, int u, int lane
         size = min(step - 1, size - c * step);
     }
     if (lo > 0) *block = 1 + u - further_place<NT>(a, lo - 1);
-    return lo - 1;
+    return *block > 0 ? lo - 1 : -1;  // no place before its first, should `start` not ascend
 }
 
 // What a sequence and kv head adds to the list of work: each unit its cost

@@ -351,9 +351,10 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                             for (int t = 0; t < 2; t++) {
                                 const float2 xx = make_float2(xs[j + 2 * t], xs[j + 2 * t + 1]);
                                 const float2 e = unpair(fma2(pair(xx.x, xx.y), f2, nM));
-                                const f32x2 p = pair(ex2(e.x), ex2(e.y));
+                                f32x2 p = pair(ex2(e.x), ex2(e.y));
                                 f32x2 s2 = t ? pair(vs.z, vs.w) : pair(vs.x, vs.y), m2 = t ? pair(vm.z, vm.w) : pair(vm.x, vm.y);
-                                if (clean) {  // a masked place may hold NaN or infinity
+                                if (clean) {  // a masked place, or its query, may hold NaN or infinity
+                                    p = pair(xx.x == -INFINITY ? 0.f : ex2(e.x), xx.y == -INFINITY ? 0.f : ex2(e.y));
                                     const float2 sf = unpair(s2), mf = unpair(m2);
                                     s2 = pair(xx.x == -INFINITY ? 0.f : sf.x, xx.y == -INFINITY ? 0.f : sf.y);
                                     m2 = pair(xx.x == -INFINITY ? 0.f : mf.x, xx.y == -INFINITY ? 0.f : mf.y);

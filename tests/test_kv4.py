@@ -595,3 +595,50 @@ def test_prompts_replayed_with_other_lengths(cuda_device):
         g.replay()
         torch.cuda.synchronize()
         _check(st, "bf16", out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_queries_of_nan_that_see_nothing(cuda_device, dtype):
+    """Rows before position 0 are zeros whatever their queries hold."""
+    import needle_b200 as nb
+
+    st = Setup("small", dtype, [60, 60], [60, 60], 16).append()
+    st.n = np.array([200, 200], np.int32)  # rows 0 .. 139 of each lie before position 0
+    st.start = np.array([0, 200, 400], np.int32)
+    st.rows = 400
+    import torch
+
+    st.q = torch.randn((400, st.hq, st.dk), device="cuda").to(st.t)
+    st.q[5, 0, 3] = st.q[150, 1, 0] = float("nan")
+    st.q[250, 2, 7] = float("inf")
+    got = _np(nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start)))
+    assert (got[:140] == 0).all() and (got[200:340] == 0).all()
+    nan = np.zeros((400, st.hq), bool)
+    nan[150, 1] = True
+    assert np.array_equal(np.isnan(got).any(-1), nan)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(60, 1), (60, 40), (4000, 1), (4000, 40)])
+def test_offsets_that_do_not_ascend(cuda_device, dtype, rows, cols):
+    """What such a call writes is not specified; it stays among its rows."""
+    import needle_b200 as nb
+    import torch
+
+    rng = np.random.default_rng(rows)
+    S = 12
+    kv = nb.KV4Pool.new(S * cols, 2, 48, 64, page=16)
+    table = torch.arange(S * cols, dtype=torch.int32, device="cuda").view(S, cols)
+    lens = torch.full((S,), 16 * cols, dtype=torch.int32, device="cuda")
+    room = torch.full((rows + 200, 12, 64), 7.0, device="cuda").to(_torch_type(dtype))
+    k, v = torch.randn((rows, 2, 48), device="cuda"), torch.randn((rows, 2, 64), device="cuda")
+    q = torch.randn((rows, 12, 48), device="cuda").to(room.dtype)
+    for start in ([0, rows] * 6 + [0], rng.integers(-5, rows + 9, S + 1), rng.integers(-2 ** 31, 2 ** 31, S + 1), [rows] * (S + 1)):
+        start = torch.tensor(np.asarray(start), dtype=torch.int32, device="cuda")
+        nb.op_kv4_append(kv, k, v, table, lens, start)
+        nb.op_kv4_attend(kv, q, table, lens, start, out=room[100:-100])
+        nb.op_kv4_read(kv, table, lens, start, rows=rows)
+    torch.cuda.synchronize()
+    assert (room[:100] == 7).all() and (room[-100:] == 7).all()
