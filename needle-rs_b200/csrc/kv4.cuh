@@ -73,6 +73,16 @@ __device__ __forceinline__ uint8_t* kv4_tile_of(const Kv4Args& a, int s, long lo
     return a.pool + (size_t)page * a.page_stride + (size_t)(tile % a.page_tiles) * tile_bytes;
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv(uint32_t x = 1) : d(x), mul(0), shift(0) {
+        while ((1ull << shift) < d) shift++;
+        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+    }
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+
 // Two f32 operations in one instruction.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b) {

@@ -9,16 +9,6 @@
 
 namespace nd {
 
-// n / d for 0 <= n < 2^31 by a multiplication.
-struct FastDiv {
-    uint32_t d, mul, shift;
-    FastDiv(uint32_t x = 1) : d(x), mul(0), shift(0) {
-        while ((1ull << shift) < d) shift++;
-        mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
-    }
-    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
-};
-
 struct AttendArgs {
     Kv4Args kv;
     long long q_row, q_head, o_row, o_head;

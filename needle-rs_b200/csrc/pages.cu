@@ -6,12 +6,14 @@
 // Both are a handful of passes over the tables and one word a page, then the
 // copies. The copies are HBM bound (each page read and written once, 16 bytes
 // a thread); the rest is bound by the passes' dependent loads and the
-// launches. So one cluster of eight CTAs takes all passes, the hardware's
-// cluster barrier between them, and a second launch, issued early, writes
-// the tables and copies. Past PG_SMALL pages or table entries eight CTAs are
-// too few, and each pass is a launch of its own.
+// launches. So a fork's passes are one cluster of eight CTAs, the hardware's
+// cluster barrier between them, and a second launch, issued early, writes the
+// tables and copies. A compaction needs a bit a page, not a count, and its
+// plan is CTAs that each have all bits and wait for nobody. Past PG_SMALL
+// pages or table entries that is too few CTAs, and each pass is a launch.
 // Measured (us, GPU alone, then of a Python call): 1024 sequences of 51
-// columns over 14,704 pages 22 and 21; as launches of their own 16.5 and 36.
+// columns over 14,704 pages forked 22 and 21, as launches of their own 16.5 and
+// 36; 24,576 pages compacted, half live, 26, planned by a cluster 29.
 
 #include <cooperative_groups.h>
 
@@ -23,6 +25,7 @@ namespace cg = cooperative_groups;
 
 constexpr int PG_BLOCK = 1024;  // pages or sequences a block of the prefix sums
 constexpr int PG_CLUSTER = 8;
+constexpr int PG_PLAN = 32;  // CTAs that each plan a compaction
 constexpr int PG_SMALL = 1 << 17;  // pages, and table entries
 
 __device__ __forceinline__ void after_previous() {
@@ -40,6 +43,7 @@ struct ForkArgs {
     PoolView pool;
     const int32_t* table;
     int table_stride, seqs, cols, pages, page;
+    FastDiv by_cols;
     const int32_t *src, *keep, *need;
     int n;  // new sequences
     const uint8_t* pinned;
@@ -237,7 +241,7 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_BLOCK) f
         __syncthreads();
 #pragma unroll 4
         for (int i = tid; i < n * a.cols; i += PG_BLOCK) {
-            const int s = i / a.cols, c = i - s * a.cols;
+            const int s = a.by_cols(i), c = i - s * a.cols;
             const Kept& k = kept[s];
             if (c >= k.nk) continue;
             const int p = __ldg(k.row + c);
@@ -340,6 +344,7 @@ struct CompactArgs {
     PoolView pool;
     const int32_t* table;
     int table_stride, seqs, cols, pages;
+    FastDiv by_cols;
     const uint8_t* pinned;
     int32_t *table_out, *map, *info;
     // workspace
@@ -412,62 +417,84 @@ __global__ void __launch_bounds__(PG_BLOCK) compact_lists_kernel(CompactArgs a) 
     }
 }
 
-// The same in one cluster; n and the moves go to sums[0].
-__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_BLOCK) compact_plan_kernel(CompactArgs a) {
+// The same where all pages' bits fit a CTA's shared memory: each of a few CTAs
+// reads the whole table and counts for itself, so that none waits for
+// another, and writes its share of the map. Thread t has words 4 t .. 4 t + 3.
+constexpr int PG_WORDS = PG_SMALL / 32;
+static_assert(PG_WORDS == 4 * PG_BLOCK, "four words a thread");
+
+__global__ void __launch_bounds__(PG_BLOCK) compact_plan_kernel(CompactArgs a) {
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    cg::cluster_group cluster = cg::this_cluster();
-    constexpr int ALL = PG_CLUSTER * PG_BLOCK;
-    const int rank = cluster.block_rank(), tid = threadIdx.x, all = rank * PG_BLOCK + tid;
-    __shared__ int2 mine;
-    __shared__ int early;  // of the first CTA: movable pages before n
-    for (int i = all; i < a.pages; i += ALL) a.refs[i] = 0;
-    cluster.sync();
+    __shared__ uint32_t live[PG_WORDS], move[PG_WORDS];  // referred to or pinned; only referred to
+    __shared__ int2 count[PG_BLOCK];                     // of those, before the thread's words
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) live[tid + i * PG_BLOCK] = 0;
+    __syncthreads();
     const int entries = a.seqs * a.cols;
-#pragma unroll 4
-    for (int i = all; i < entries; i += ALL) {
-        const int s = i / a.cols, p = __ldg(a.table + (size_t)s * a.table_stride + (i - s * a.cols));
-        if (p >= 0 && p < a.pages) a.refs[p] = 1;
+#pragma unroll 8
+    for (int i = tid; i < entries; i += PG_BLOCK) {
+        const int s = a.by_cols(i), p = __ldg(a.table + (size_t)s * a.table_stride + (i - s * a.cols));
+        if (p >= 0 && p < a.pages) atomicOr(&live[p >> 5], 1u << (p & 31));
     }
-    cluster.sync();
-    const int each = (a.pages + ALL - 1) / ALL, p0 = min(all * each, a.pages), p1 = min(p0 + each, a.pages);
+    __syncthreads();
+    if (a.pinned) {
+        for (int p = tid; p < (a.pages + 31) / 32 * 32; p += PG_BLOCK) {
+            const uint32_t pin = __ballot_sync(0xffffffffu, p < a.pages && a.pinned[p]);
+            if ((tid & 31) == 0) move[p >> 5] = live[p >> 5] & ~pin, live[p >> 5] |= pin;
+        }
+        __syncthreads();
+    }
+    const uint32_t* mv = a.pinned ? move : live;
+    const int W = (a.pages + 31) / 32;
     int2 own = make_int2(0, 0), before;
-    for (int p = p0; p < p1; p++) {
-        const int2 st = page_state(a, p);
-        own.x += st.x, own.y += st.y;
+#pragma unroll
+    for (int i = 4 * tid; i < 4 * tid + 4; i++)
+        if (i < W) own.x += __popc(live[i]), own.y += __popc(mv[i]);
+    const int2 all = block_scan2(own, &before);
+    count[tid] = before;
+    __syncthreads();
+    // movable pages before p
+    auto rank = [&](int p) {
+        const int w = p >> 5;
+        int r = count[w >> 2].y + __popc(mv[w] & ((1u << (p & 31)) - 1));
+        for (int i = w & ~3; i < w; i++) r += __popc(mv[i]);
+        return r;
+    };
+    // the r-th page that is not live, r below their number
+    auto hole = [&](int r) {
+        int lo = 0, hi = PG_BLOCK;  // 128 lo - count[lo].x <= r, not so at hi
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (128 * mid - count[mid].x <= r) lo = mid;
+            else hi = mid;
+        }
+        r -= 128 * lo - count[lo].x;
+        int w = 4 * lo;
+        while (w < 4 * lo + 3 && r >= 32 - __popc(live[w])) r -= 32 - __popc(live[w]), w++;
+        uint32_t free = ~live[w];
+        for (; r > 0; r--) free &= free - 1;
+        return 32 * w + __ffs(free) - 1;
+    };
+    const int n = all.x, before_n = n < a.pages ? rank(n) : all.y;
+    for (int p = blockIdx.x * PG_BLOCK + tid; p < a.pages; p += gridDim.x * PG_BLOCK) {
+        int to = live[p >> 5] >> (p & 31) & 1 ? p : -1;
+        if (p >= n && (mv[p >> 5] >> (p & 31) & 1)) {
+            const int r = rank(p) - before_n;
+            to = hole(r);
+            a.movers[r] = p, a.holes[r] = to;
+        }
+        a.map[p] = to;
     }
-    const int2 sum = block_scan2(own, &before);
-    if (tid == 0) mine = sum;
-    cluster.sync();
-    int n = 0, moves = 0;
-    for (int r = 0; r < PG_CLUSTER; r++) {
-        const int2 m = *cluster.map_shared_rank(&mine, r);
-        if (r < rank) before.x += m.x, before.y += m.y;
-        n += m.x, moves += m.y;
-    }
-    if (p0 < n ? n <= p1 : all == 0 && n == 0) {  // the run that n lies in or ends
-        int e = before.y;
-        for (int p = p0; p < n; p++) e += page_state(a, p).y;
-        *cluster.map_shared_rank(&early, 0) = e;
-    }
-    cluster.sync();
-    const int before_n = *cluster.map_shared_rank(&early, 0);
-    for (int p = p0; p < p1; p++) {
-        const int2 st = page_state(a, p);
-        a.before[p] = before.y - before_n;
-        if (p >= n && st.y) a.movers[before.y - before_n] = p;
-        if (p < n && !st.x) a.holes[p - before.x] = p;
-        before.x += st.x, before.y += st.y;
-    }
-    if (all == 0) {
-        a.sums[0] = make_int2(n, moves - before_n);
+    if (blockIdx.x == 0 && tid == 0) {
+        a.sums[0] = make_int2(n, all.y - before_n);
         a.info[0] = n;
-        a.info[1] = moves - before_n;
+        a.info[1] = all.y - before_n;
     }
-    cluster.sync();  // no CTA leaves while others read its counts
 }
 
-// Blocks of pages write the map, blocks of table entries the new table, the
-// others copy.
+// Blocks of pages write the map (where the plan has not: no such blocks),
+// blocks of table entries the new table, the others copy.
 __global__ void __launch_bounds__(128) compact_move_kernel(CompactArgs a, int totals, int map_blocks, int table_blocks) {
     after_previous();
     const int2 tot = a.sums[totals];
@@ -486,8 +513,8 @@ __global__ void __launch_bounds__(128) compact_move_kernel(CompactArgs a, int to
     if (b < table_blocks) {
         const long long i = b * 128LL + threadIdx.x;
         if (i < (long long)a.seqs * a.cols) {
-            const int p = __ldg(a.table + (size_t)(i / a.cols) * a.table_stride + i % a.cols);
-            a.table_out[i] = p >= 0 && p < a.pages ? to(p) : -1;
+            const int s = a.by_cols((int)i), p = __ldg(a.table + (size_t)s * a.table_stride + (i - (long long)s * a.cols));
+            a.table_out[i] = p < 0 || p >= a.pages ? -1 : map_blocks ? to(p) : __ldcg(a.map + p);
         }
         return;
     }
@@ -565,7 +592,7 @@ int nd_op_pages_fork(const nd_pages* pool, const int* table, int table_stride, i
         if (table_out == table) fail("the new table must not be the old one");
         if (!ws || (uintptr_t)ws % 16 || ws_bytes < fork_ws(pool->num_pages, n)) fail("the workspace is too small or not 16-byte aligned");
         const int N = pool->num_pages, nb = blocks_of(N), sb = blocks_of(n);
-        a.table = table, a.table_stride = table_stride, a.seqs = seqs, a.cols = cols, a.pages = N, a.page = page;
+        a.table = table, a.table_stride = table_stride, a.seqs = seqs, a.cols = cols, a.pages = N, a.page = page, a.by_cols = FastDiv(cols);
         a.src = src, a.keep = keep, a.need = need, a.n = n, a.pinned = pinned;
         a.table_out = table_out, a.refs = refs, a.info = info;
         a.writers = (int32_t*)ws, a.first = a.writers + N, a.free_ids = a.first + N, a.fresh = a.free_ids + N;
@@ -603,7 +630,7 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
         if (table_out == table) fail("the new table must not be the old one");
         if (!ws || (uintptr_t)ws % 16 || ws_bytes < compact_ws(pool->num_pages)) fail("the workspace is too small or not 16-byte aligned");
         const int N = pool->num_pages, nb = blocks_of(N);
-        a.table = table, a.table_stride = table_stride, a.seqs = seqs, a.cols = cols, a.pages = N, a.pinned = pinned;
+        a.table = table, a.table_stride = table_stride, a.seqs = seqs, a.cols = cols, a.pages = N, a.by_cols = FastDiv(cols), a.pinned = pinned;
         a.table_out = table_out, a.map = map, a.info = info;
         a.sums = (int2*)ws;
         a.refs = (int32_t*)(a.sums + nb + 1), a.before = a.refs + N, a.movers = a.before + N, a.holes = a.movers + N;
@@ -612,7 +639,7 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
         const int sms = device_sm_count();
         int totals = 0;  // their place in sums
         if (N <= PG_SMALL && (long long)seqs * cols <= PG_SMALL) {
-            launch_behind(what, compact_plan_kernel, PG_CLUSTER, PG_BLOCK, st, true, a);
+            launch_behind(what, compact_plan_kernel, std::min(nb, PG_PLAN), PG_BLOCK, st, true, a);
         } else {
             totals = nb;
             launch_behind(what, pages_zero_kernel, std::min((N + 255) / 256, 4 * sms), 256, st, true, a.refs, (int32_t*)nullptr, N);
@@ -620,8 +647,8 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
             launch_behind(what, compact_sums_kernel, nb, PG_BLOCK, st, false, a);
             launch_behind(what, compact_lists_kernel, nb, PG_BLOCK, st, false, a);
         }
-        const int map_blocks = (N + 127) / 128, table_blocks = (int)(((long long)seqs * cols + 127) / 128);
-        launch_behind(what, compact_move_kernel, map_blocks + table_blocks + std::min(N, 16 * sms), 128, st, false, a, totals, map_blocks, table_blocks);
+        const int map_blocks = totals ? (N + 127) / 128 : 0, table_blocks = (int)(((long long)seqs * cols + 127) / 128);
+        launch_behind(what, compact_move_kernel, map_blocks + table_blocks + std::min(N, 32 * sms), 128, st, false, a, totals, map_blocks, table_blocks);
     });
 }
 

@@ -316,3 +316,16 @@ def test_entry_points_refuse_without_a_gpu():
         assert fork(**bad) == -1 and message in lib.nd_last_error(), (bad, lib.nd_last_error())
     assert lib.nd_op_pages_compact(None, 4096, 2, 1, 2, None, 8192, 4096, 4096, 4096, 1 << 20, None) == -1
     assert lib.nd_op_pages_fork_ws(0, 1) == 0 and lib.nd_op_pages_compact_ws(-1) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [131072, 131071, 131073, 32, 33, 128, 129])
+@pytest.mark.parametrize("dense,pins", [(0.02, False), (0.98, True), (0.5, True)])
+def test_compact_whole_words_and_all_a_plan_takes(cuda_device, pages, dense, pins):
+    r = np.random.default_rng(pages)
+    some = r.permutation(pages)[: max(1, int(dense * pages))]
+    cols = 7
+    table = np.full(-(-len(some) // cols) * cols, -1)
+    table[: len(some)] = some
+    pinned = r.random(pages) < 0.01 if pins else None
+    check_compact(table.reshape(-1, cols), pages, pinned, elems=8)
