@@ -60,15 +60,23 @@ constexpr int ATT_MIN_SHARE = 8;
 // that meets many short units is the last by far (8 sequences, one of a
 // single position among lengths up to 32768: 70 us instead of 57).
 constexpr int ATT_UNIT_COST = 4;
-// Calls whose units all have at most this many tiles take them whole, a warp
-// or, where units are too few to fill the GPU, a CTA a unit, and need no
-// second kernel. Measured (us, with cut units, a warp, a CTA a unit): 32
-// sequences of up to 256 positions 14.4, 10.1, 6.7; 512 of them -, 15.4, 18.0;
-// 32 of up to 1000 14.9, -, 11.1.
 // Query rows a sequence brings to a kv head on average from which 16-bit rows
 // go to the tcgen05 kernel.
 constexpr int ATT_TC_ROWS = 128;
+// Calls whose units all have few tiles take them whole, a warp or, where units
+// are too few to fill the GPU twice, a CTA a unit, and need no second kernel
+// and no place in a list, 8 us of the cut units' time. A warp a unit: up to
+// ATT_WARP_TILES, and where there are more units than CTAs at once to
+// ATT_WARP_MOST (a warp's own time shows with more).
+// A CTA: up to ATT_CTA_TILES, half for two rounds. Measured (us; one token of 6
+// heads a kv head, f32; cut units, a warp, a CTA a unit): 32 sequences of up to
+// 256 positions 14.4, 10.1, 6.7; 512 of them 21.9, 14.7, 16.1; 32 of up to 1000
+// 14.9, -, 11.1; 512 of up to 640 29.0, 27.8, 23.4; 1024 of up to 400 35.5,
+// 25.9, 34.4; of up to 740 49.6, 43.4, -; of up to 1000 59.0, 56.0, 57.5, and
+// in a window of 74 tiles, five tokens, 256 sequences 51.5, 54.1. Heads of 128
+// bf16, 256 of up to 400 39.0, 34.8, 47.2; 128 of up to 740 34.0, 37.5, -.
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
+constexpr int ATT_WARP_MOST(int dv) { return dv == 128 ? 32 : 48; }
 
 // Whole units are numbered without sums. Places 0 .. seqs - 1 are the
 // sequences' first blocks; the further blocks of sequence s are at most the
@@ -873,8 +881,9 @@ static AttendPlan attend_plan(const nd_kv4* kv, int group, int type, int window,
     const long long units = kv->heads * std::max<long long>(further, std::min(kv->seqs, kv->rows));  // as many as there are likely to be
     const long long most = kv->heads * (further + std::min(kv->seqs, kv->rows));
     p.mode = CUT;
-    if (p.nt == 1 && tiles <= ATT_CTA_TILES && units <= full) p.mode = CTA;
-    else if (tiles <= ATT_WARP_TILES) p.mode = WARP;
+    const long long rounds = (units + full - 1) / full;  // of a GPU full of CTAs
+    if (p.nt == 1 && rounds <= 2 && rounds * tiles <= ATT_CTA_TILES && (rounds == 1 || tiles > ATT_WARP_TILES)) p.mode = CTA;
+    else if (tiles <= ATT_WARP_TILES || (rounds > 1 && tiles <= ATT_WARP_MOST(kv->dv))) p.mode = WARP;
     const long long runs = (most * (tiles + ATT_UNIT_COST) + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
     p.ctas = (int)std::max(1LL, std::min<long long>(full, (runs + ATT_WARPS - 1) / ATT_WARPS));
     const size_t runners = (size_t)p.ctas * (p.nt == 1 ? 1 : ATT_WARPS);

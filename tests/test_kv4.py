@@ -642,3 +642,18 @@ def test_offsets_that_do_not_ascend(cuda_device, dtype, rows, cols):
         nb.op_kv4_read(kv, table, lens, start, rows=rows)
     torch.cuda.synchronize()
     assert (room[:100] == 7).all() and (room[-100:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,dtype,seqs,most", [("needle", "f32", 700, 600), ("needle", "bf16", 400, 900), ("wide", "f16", 750, 500),
+                                                   ("small", "f32", 450, 760)])
+def test_attend_many_short_sequences(cuda_device, heads, dtype, seqs, most):
+    """Units taken whole, a warp or four each, over more tiles than one round of the GPU."""
+    import needle_b200 as nb
+
+    lens = np.random.default_rng(seqs).integers(1, most + 1, seqs)
+    lens[:2] = 1, most
+    st = Setup(heads, dtype, lens, [1] * seqs, 16).append()
+    for window, sink in ((0, 0), (300, 20)):
+        got = nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), window=window, sink=sink)
+        _check(st, dtype, got, window=window, sink=sink)
