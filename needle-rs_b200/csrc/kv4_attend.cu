@@ -60,9 +60,15 @@ constexpr int ATT_MIN_SHARE = 8;
 // that meets many short units is the last by far (8 sequences, one of a
 // single position among lengths up to 32768: 70 us instead of 57).
 constexpr int ATT_UNIT_COST = 4;
-// Query rows a sequence brings to a kv head on average from which 16-bit rows
-// go to the tcgen05 kernel.
+// 16-bit rows that would be cut go to the tcgen05 kernel from this many query
+// rows a sequence and kv head on average, and this many tiles by blocks of
+// eight rows: it takes 30 us (heads of 128: 40) at the least. Measured (us,
+// this kernel, that one; bf16): 4 heads of 128 a kv head, 4 sequences of 64 rows
+// over 740 positions 24, 40; 8 of them 40, 43; 16 of them 61, 56; one of 128
+// over 2000 45, 42, over 4000 65, 50; 6 heads of 64, one of 512 over 740 47, 34,
+// of 128 over 4096 33, 34, over 20000 66, 54.
 constexpr int ATT_TC_ROWS = 128;
+constexpr long long ATT_TC_WORK(int dv) { return dv == 128 ? 1 << 16 : 1 << 15; }
 // Calls whose units all have few tiles take them whole, a warp or, where units
 // are too few to fill the GPU twice, a CTA a unit, and need no second kernel
 // and no place in a list, 8 us of the cut units' time. A warp a unit: up to
@@ -74,7 +80,8 @@ constexpr int ATT_TC_ROWS = 128;
 // 14.9, -, 11.1; 512 of up to 640 29.0, 27.8, 23.4; 1024 of up to 400 35.5,
 // 25.9, 34.4; of up to 740 49.6, 43.4, -; of up to 1000 59.0, 56.0, 57.5, and
 // in a window of 74 tiles, five tokens, 256 sequences 51.5, 54.1. Heads of 128
-// bf16, 256 of up to 400 39.0, 34.8, 47.2; 128 of up to 740 34.0, 37.5, -.
+// bf16, 256 of up to 400 39.0, 34.8, 47.2; 128 of up to 740 34.0, 37.5, -. Whole
+// prompts of 118 rows, 6 heads, bf16, 256 of them: a warp a unit 79, on tcgen05 134.
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
 constexpr int ATT_WARP_MOST(int dv) { return dv == 128 ? 32 : 48; }
 
@@ -865,11 +872,6 @@ struct AttendPlan {
 // Grid and workspace from what the host knows: the sizes, not the lengths.
 static AttendPlan attend_plan(const nd_kv4* kv, int group, int type, int window, int sink) {
     AttendPlan p{};
-    if (type != ND_F32 && (long long)kv->rows * group >= (long long)ATT_TC_ROWS * kv->seqs) {
-        p.mode = ROWS;
-        p.ws = prefill_ws_bytes(kv->dv, &p.ctas);
-        return p;
-    }
     p.nt = query_tiles(kv, group);
     // tiles a unit can have: the table's, or those of the window (of 8 nt rows' tokens) and the sinks
     const long long table = (long long)kv->max_pages * (kv->page / KV4_TILE);
@@ -884,6 +886,12 @@ static AttendPlan attend_plan(const nd_kv4* kv, int group, int type, int window,
     const long long rounds = (units + full - 1) / full;  // of a GPU full of CTAs
     if (p.nt == 1 && rounds <= 2 && rounds * tiles <= ATT_CTA_TILES && (rounds == 1 || tiles > ATT_WARP_TILES)) p.mode = CTA;
     else if (tiles <= ATT_WARP_TILES || (rounds > 1 && tiles <= ATT_WARP_MOST(kv->dv))) p.mode = WARP;
+    if (p.mode == CUT && type != ND_F32 && (long long)kv->rows * group >= (long long)ATT_TC_ROWS * kv->seqs &&
+        (long long)kv->heads * kv->rows * group / 8 * tiles >= ATT_TC_WORK(kv->dv)) {
+        p.mode = ROWS;
+        p.ws = prefill_ws_bytes(kv->dv, &p.ctas);
+        return p;
+    }
     const long long runs = (most * (tiles + ATT_UNIT_COST) + ATT_MIN_SHARE - 1) / ATT_MIN_SHARE;
     p.ctas = (int)std::max(1LL, std::min<long long>(full, (runs + ATT_WARPS - 1) / ATT_WARPS));
     const size_t runners = (size_t)p.ctas * (p.nt == 1 ? 1 : ATT_WARPS);

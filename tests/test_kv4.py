@@ -657,3 +657,61 @@ def test_attend_many_short_sequences(cuda_device, heads, dtype, seqs, most):
     for window, sink in ((0, 0), (300, 20)):
         got = nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), window=window, sink=sink)
         _check(st, dtype, got, window=window, sink=sink)
+
+
+# The many-row kernel is chosen by what the table could hold, so the tests
+# above reach it with tables that have columns to spare.
+@pytest.fixture
+def wide_tables(monkeypatch):
+    init = Setup.__init__
+
+    def wide(self, *a, **k):
+        init(self, *a, **k)
+        self.table = np.pad(self.table, ((0, 0), (0, 40000)), constant_values=-1)
+
+    monkeypatch.setattr(Setup, "__init__", wide)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("n,lens", [([200], [200]), ([64, 70, 0], [300, 70, 40]), ([100, 257], [900, 1000])])
+@pytest.mark.parametrize("window,sink", [(0, 0), (200000, 0), (90, 20)])
+def test_many_rows_wide_table(cuda_device, wide_tables, heads, dtype, n, lens, window, sink):
+    test_attend_many_rows(cuda_device, heads, dtype, n, lens, window, sink)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_odd_values_wide_table(cuda_device, wide_tables, dtype):
+    test_attend_many_rows_odd_values(cuda_device, dtype)
+    test_queries_of_nan_that_see_nothing(cuda_device, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [[40, 0, 5], [3, 90, 7]])
+def test_many_heads_wide_table(cuda_device, wide_tables, dtype, n):
+    test_attend_many_heads_on_one(cuda_device, dtype, n)
+
+
+@pytest.mark.gpu
+def test_prompts_replayed_wide_table(cuda_device, wide_tables):
+    test_prompts_replayed_with_other_lengths(cuda_device)
+
+
+@pytest.mark.gpu
+def test_calls_side_by_side_wide_table(cuda_device, wide_tables):
+    test_calls_side_by_side(cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("window,sink", [(0, 0), (900, 40)])
+def test_attend_long_prompts(cuda_device, heads, dtype, window, sink):
+    import needle_b200 as nb
+
+    st = Setup(heads, dtype, [1500, 900, 3, 700], [700, 500, 0, 150], 64).append()
+    got = nb.op_kv4_attend(st.kv, st.q, st.dev(st.table), st.dev(st.lens), st.dev(st.start), window=window, sink=sink)
+    _check(st, dtype, got, window=window, sink=sink)
