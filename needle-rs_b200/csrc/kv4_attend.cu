@@ -15,8 +15,9 @@
 // bits make 16 c * 2^-24, whose 16 is taken out of the matching query value
 // beforehand (q is scaled per row by a power of two so that its f16 keeps it)
 // or out of the accumulator row afterwards. 2^24 is put back in f32.
-// Weights p sv are split into two f16 terms (22 bits) for f32 and f16 rows;
-// bf16 rows take one: its 2^-12 is far below the output's own 2^-9.
+// Weights p sv are split into two f16 terms (22 bits, down to 2^-36 of the
+// row's largest weight, see ATT_TOP) for f32 and f16 rows; bf16 rows take
+// one: its 2^-12 is far below the output's own 2^-9.
 //
 // f32 rows. The tensor cores truncate their sums near the 24th bit, and codes
 // counted from the minimum add up to much more than the result, so what is
@@ -27,13 +28,15 @@
 //   2^24 units: it is exact, whatever the order.
 // - value codes are made the f16 e - 8 (one more instruction a pair), each
 //   tile's sum starts at zero and is added to the accumulator rounded.
-// Measured: 5e-7 of the result against 64 bits where the plain way had 4e-5
-// (keys and values with outlying channels).
+// - sums of 32 rounds are carried in f64 (ATT_ROUNDS).
+// Measured: 6e-7 of the result against 64 bits where the plain way had 4e-5
+// (keys and values with outlying channels); below 3e-6 over a run of 32,768
+// equal keys behind one that is 10 to 18 nats ahead.
 //
 // A warp keeps the softmax's running reference M per query row (a power-of-
 // two argument: scores carry log2 e) and rescales only when a new exponent
 // passes it by more than 4, since only the quotient counts. The reference is
-// taken over score + log2 sv, so that the f16 weight p sv is at most 16
+// taken over score + log2 sv, so that the f16 weight p sv is at most 2^15
 // whatever the values' scale.
 //
 // Work split: the tiles of all (sequence, kv head, query block) units are one
@@ -53,6 +56,15 @@ namespace nd {
 
 constexpr int ATT_WARPS = 4;
 constexpr int ATT_KT = 2, ATT_STAGES = 3;
+// A row's reference puts its largest weight so far between 2^ATT_TOP and
+// 2^(ATT_TOP + 4), just below f16's end: what f16's last step, 2^-24, takes
+// from a weight is then 2^-36 of the largest. At 1 instead of 2^11 a key 18
+// nats ahead of 32,768 others cost f32 rows 5e-4 of their result.
+constexpr float ATT_TOP = 11.f;
+// Rounds after which a run's sums go to memory (f64 for f32 rows) and begin
+// anew: in f32 small terms beside a large sum lose up to 2^-25 of it each,
+// which thousands of equal ones add up. Few runs are that long.
+constexpr int ATT_ROUNDS = 32;
 constexpr int ATT_CTAS(int nt, int dv) { return nt == 2 || dv == 128 ? 3 : 4; }  // an SM: what registers and shared memory allow
 // Tiles: a shorter run of a cut unit costs more to join than it takes.
 constexpr int ATT_MIN_SHARE = 8;
@@ -84,6 +96,7 @@ constexpr long long ATT_TC_WORK(int dv) { return dv == 128 ? 1 << 16 : 1 << 15; 
 // prompts of 118 rows, 6 heads, bf16, 256 of them: a warp a unit 79, on tcgen05 134.
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
 constexpr int ATT_WARP_MOST(int dv) { return dv == 128 ? 32 : 48; }
+static_assert(ATT_WARP_MOST(64) <= ATT_ROUNDS * ATT_KT && ATT_CTA_TILES / ATT_WARPS + ATT_KT <= ATT_ROUNDS * ATT_KT, "whole units are not LONG");
 
 // Whole units are numbered without sums. Places 0 .. seqs - 1 are the
 // sequences' first blocks; the further blocks of sequence s are at most the
@@ -204,8 +217,9 @@ struct PartRegs {
 
 // A warp's part of a unit: tiles off .. off + m - 1 of query block b of
 // sequence s and kv head h. With `part` NULL they are all it has and the
-// result goes to its place; else the sums go to `part`, unnormalised.
-template <int DK, int DV, int NT, typename T>
+// result goes to its place; else the sums go to `part`, unnormalised. LONG:
+// it may have more than ATT_ROUNDS rounds.
+template <int DK, int DV, int NT, typename T, bool LONG>
 __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __restrict__ q, T* __restrict__ out, int s, int h, int b,
                                             const SeqRows& rows, const Tiles& tl, int off, int m, uint8_t* ring, uint2* qsm0,
                                             float* part) {
@@ -357,6 +371,25 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
 
     float acc[NT][MT][4];
     f32x2 nM[NT], l[NT], mn[NT];  // -M, sum p, sum p mv for columns 2 c, 2 c + 1 (the sums over this lane's keys)
+    // the sums of earlier rounds; through a pointer the compiler cannot see
+    // through, so that they stay out of the registers
+    typedef typename std::conditional<F32, double, float>::type Sum;
+    Sum earlier[NT * (4 * MT + 4)];
+    Sum* past = earlier;
+    asm volatile("" : "+l"(past) : : "memory");
+    auto sums = [&](auto&& f) {  // f(i, value) of every sum; replaces it
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int k = 0; k < MT; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[t][k][j] = f(t * (4 * MT + 4) + 4 * k + j, acc[t][k][j]);
+            float2 x = unpair(l[t]), y = unpair(mn[t]);
+            x.x = f(t * (4 * MT + 4) + 4 * MT, x.x), x.y = f(t * (4 * MT + 4) + 4 * MT + 1, x.y);
+            y.x = f(t * (4 * MT + 4) + 4 * MT + 2, y.x), y.y = f(t * (4 * MT + 4) + 4 * MT + 3, y.y);
+            l[t] = pair(x.x, x.y), mn[t] = pair(y.x, y.y);
+        }
+    };
 #pragma unroll
     for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -371,6 +404,13 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
     uint32_t get_at = 0;
 #pragma unroll 1
     for (int i = 0; i < m; i += KT) {
+        if (LONG && __builtin_expect(i > 0 && i % (ATT_ROUNDS * KT) == 0, 0)) {
+            const bool first = i == ATT_ROUNDS * KT;
+            sums([&](int k, float x) {
+                past[k] = first ? (Sum)x : past[k] + (Sum)x;
+                return 0.f;
+            });
+        }
         asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
         __syncwarp();
         const uint32_t here = have >> ((STAGES - 2) * KT);  // bit KT - 1 - u: tile u of this round
@@ -464,7 +504,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
                 kpa[u].y = __fmaf_rn(8.f, kpa[u].x, kpa[u].y), kpb[u].y = __fmaf_rn(8.f, kpb[u].x, kpb[u].y);
                 vpa[u].y = __fmaf_rn(8.f, vpa[u].x, vpa[u].y), vpb[u].y = __fmaf_rn(8.f, vpb[u].x, vpb[u].y);
             }
-            ta[u] = 4.f - lg2(fmaxf(vpa[u].x, 5.9604645e-8f)), tb[u] = 4.f - lg2(fmaxf(vpb[u].x, 5.9604645e-8f));
+            ta[u] = ATT_TOP + 4.f - lg2(fmaxf(vpa[u].x, 5.9604645e-8f)), tb[u] = ATT_TOP + 4.f - lg2(fmaxf(vpb[u].x, 5.9604645e-8f));
             const f32x2 ksa = pair(kpa[u].x, kpa[u].x), ksb = pair(kpb[u].x, kpb[u].x);
             const f32x2 kma = pair(kpa[u].y, kpa[u].y), kmb = pair(kpb[u].y, kpb[u].y);
 #pragma unroll
@@ -528,19 +568,26 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
                 mn[t] = mul2(mn[t], r);
 #pragma unroll
                 for (int k = 0; k < MT; k++) acc[t][k][0] *= r0, acc[t][k][1] *= r1, acc[t][k][2] *= r0, acc[t][k][3] *= r1;
+                if (LONG && i >= ATT_ROUNDS * KT)
+#pragma unroll 1
+                    for (int k = 0; k < 4 * MT + 4; k += 2) {
+                        Sum* o = past + t * (4 * MT + 4) + k;
+                        o[0] *= r0, o[1] *= r1;
+                    }
 #pragma unroll
                 for (int u = 0; u < KT; u++) xa[u][t] = unpair(add2(sa[u][t], nM[t])), xb[u][t] = unpair(add2(sb[u][t], nM[t]));
             }
         }
         // weights, and their operands: rows of the transpose are query rows
         uint32_t wop[KT][NT][2][WS];
+        f32x2 l1[NT], mn1[NT];  // this round's
 #pragma unroll
         for (int u = 0; u < KT; u++) {
             const f32x2 vsa = pair(vpa[u].x, vpa[u].x), vsb = pair(vpb[u].x, vpb[u].x), vma = pair(vpa[u].y, vpa[u].y), vmb = pair(vpb[u].y, vpb[u].y);
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const f32x2 pa = pair(ex2(xa[u][t].x), ex2(xa[u][t].y)), pb = pair(ex2(xb[u][t].x), ex2(xb[u][t].y));
-                l[t] = add2(l[t], add2(pa, pb));
+                l1[t] = u ? add2(l1[t], add2(pa, pb)) : add2(pa, pb);
                 f32x2 wa2 = mul2(pa, vsa), wb2 = mul2(pb, vsb), ma = mul2(pa, vma), mb = mul2(pb, vmb);
                 if (__builtin_expect(!whole, 0)) {  // a masked place may hold NaN or infinity
                     auto clean = [](f32x2 x, float2 e) {
@@ -549,7 +596,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
                     };
                     wa2 = clean(wa2, xa[u][t]), wb2 = clean(wb2, xb[u][t]), ma = clean(ma, xa[u][t]), mb = clean(mb, xb[u][t]);
                 }
-                mn[t] = add2(mn[t], add2(ma, mb));
+                mn1[t] = u ? add2(mn1[t], add2(ma, mb)) : add2(ma, mb);
                 const float2 fa = unpair(wa2), fb = unpair(wb2);
                 const uint32_t ha = pack_half2(fa.x, fa.y), hb = pack_half2(fb.x, fb.y);
                 wop[u][t][0][0] = transpose8(ha), wop[u][t][1][0] = transpose8(hb);
@@ -560,6 +607,8 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
                 }
             }
         }
+#pragma unroll
+        for (int t = 0; t < NT; t++) l[t] = add2(l[t], l1[t]), mn[t] = add2(mn[t], mn1[t]);
         // values: lane (g, c) holds dimensions 8 (VW g + w) .. + 7 of keys 2c, 2c+1, 2c+8, 2c+9
         uint32_t vw[KT][4][VW];
 #pragma unroll
@@ -606,6 +655,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncwarp();
+    if (LONG && m > ATT_ROUNDS * KT) sums([&](int k, float x) { return (float)(past[k] + (Sum)x); });
 
     // this run's part of the unit: sums over the keys' lanes, 2^24 back
     const bool done = !part;
@@ -664,7 +714,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
     if ((long long)b * 8 * NT >= (long long)rows.n * a.group.d) return;
     const Tiles tl = block_tiles<NT>(a, rows, b);
     if (!SHARED) {
-        attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, 0, tl.n, mine, qsm, nullptr);
+        attend_part<DK, DV, NT, T, false>(a, q, out, s, h, b, rows, tl, 0, tl.n, mine, qsm, nullptr);
         return;
     }
     if constexpr (SHARED) {
@@ -672,7 +722,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
         const int rounds = (tl.n + Sh::KT - 1) / Sh::KT, each = (rounds + ATT_WARPS - 1) / ATT_WARPS * Sh::KT;
         const int off = warp * each, m = min(each, tl.n - off), used = (tl.n + each - 1) / each;
         float* part = (float*)mine;  // over the ring
-        if (m > 0) attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, off, m, mine, qsm, used == 1 ? nullptr : part);
+        if (m > 0) attend_part<DK, DV, NT, T, false>(a, q, out, s, h, b, rows, tl, off, m, mine, qsm, used == 1 ? nullptr : part);
         if (used == 1) return;
         __syncthreads();
         if (warp) return;
@@ -770,7 +820,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, AttendShape<DK, DV, NT, T>::CT
             const bool starts = off == 0, ends = off + m == tl.n, done = starts && ends;
             if (m) {
                 float* part = MERGE ? (starts ? last_part : first_part) : a.parts + ((size_t)wid * 2 + (starts ? 1 : 0)) * PART;
-                attend_part<DK, DV, NT, T>(a, q, out, s, h, b, rows, tl, off, m, mine, (uint2*)(mine + Sh::RING), done ? nullptr : part);
+                attend_part<DK, DV, NT, T, true>(a, q, out, s, h, b, rows, tl, off, m, mine, (uint2*)(mine + Sh::RING), done ? nullptr : part);
             }
             if (m && !done && lane == 0) {
                 if (MERGE) {
