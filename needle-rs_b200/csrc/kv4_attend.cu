@@ -56,11 +56,6 @@ namespace nd {
 
 constexpr int ATT_WARPS = 4;
 constexpr int ATT_KT = 2, ATT_STAGES = 3;
-// A row's reference puts its largest weight so far between 2^ATT_TOP and
-// 2^(ATT_TOP + 4), just below f16's end: what f16's last step, 2^-24, takes
-// from a weight is then 2^-36 of the largest. At 1 instead of 2^11 a key 18
-// nats ahead of 32,768 others cost f32 rows 5e-4 of their result.
-constexpr float ATT_TOP = 11.f;
 // Rounds after which a run's sums go to memory (f64 for f32 rows) and begin
 // anew: in f32 small terms beside a large sum lose up to 2^-25 of it each,
 // which thousands of equal ones add up. Few runs are that long.

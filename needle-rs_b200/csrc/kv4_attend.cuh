@@ -94,6 +94,11 @@ __device__ __forceinline__ uint32_t code16_mid(uint32_t x) {
 // Below every score that is not -infinity: the softmax's reference before the
 // first key is seen.
 constexpr float ATT_LOW = -3.0e38f;
+// A row's reference puts its largest weight so far between 2^ATT_TOP and
+// 2^(ATT_TOP + 4), just below f16's end: what f16's last step, 2^-24, takes
+// from a weight is then 2^-36 of the largest. At 1 instead of 2^11 a key 18
+// nats ahead of 32,768 others cost f32 rows 5e-4 of their result.
+constexpr float ATT_TOP = 11.f;
 
 // Where query row x of a sequence and kv head has its result.
 template <typename T>

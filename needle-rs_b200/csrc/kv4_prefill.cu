@@ -14,9 +14,10 @@
 //    weights: x = sk_j S_ij + r_i mk_j, p = 2^(f_i x - M_i), w = p sv_j rounded
 //    to f16 (in two terms for f16 rows) and written over S; the row's sums of
 //    p and p mv stay in registers.
+// Every PRE_SUMS stages O and the sums leave for the CTA's part in the workspace.
 // M_i is raised only when a new exponent passes it by 4, and then O is
 // rescaled in tensor memory; sv enters by its half stage's largest, so that w
-// is at most 16.
+// is at most 2^15 (ATT_TOP).
 // The work is one list of equal runs as in kv4_attend.cu, cut at stages; cut
 // units are joined by the same second kernel.
 //
@@ -32,6 +33,10 @@ namespace nd {
 constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 768;
 constexpr int PRE_NT = PRE_ROWS / 8;   // as block_tiles counts rows
 constexpr int PRE_UNIT_COST = 3;       // of beginning and ending a unit, in stages
+// Stages after which a unit's sums leave tensor memory and registers and
+// begin anew. The tensor cores truncate a running f32 sum at each product of 16
+// keys: over 262,144 keys that cost f16 rows 3e-3 of the values.
+constexpr int PRE_SUMS = 64;
 // Registers of a thread: launched with 80, then shared out by warpgroup (the
 // rows' four, the operands', the issuer's), which sums to what was launched.
 constexpr int PRE_REGS_ROWS = 88, PRE_REGS_CODES = 56, PRE_REGS_ISSUE = 72;
@@ -48,7 +53,7 @@ struct PreShape {
 };
 
 // Of a stage's keys: scale, middle (minimum + 8 scales) of key and value;
-// log2 of the largest value scale of each half; its four tiles' first
+// log2 of the largest value scale of each half, less ATT_TOP; its four tiles' first
 // positions and which of them exist; whether each block's rows all see all.
 struct StageKeys {
     float ks[PRE_KEYS], km[PRE_KEYS], vs[PRE_KEYS], vm[PRE_KEYS];
@@ -92,6 +97,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
     // the factors at the start, the sums at the end
     __shared__ int wish[2][2][8];
     __shared__ float wants[2][2][PRE_ROWS], half_l[PRE_ROWS], half_mn[PRE_ROWS];
+    __shared__ float4 earlier[2][PRE_ROWS];  // a thread's M, sum p, sum p mv when its sums last left; they lie in its part's place
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     volatile int* abort = &abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -278,6 +284,10 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             const f32x2 f2 = pair(f, f), r2 = pair(r, r);
             float M = ATT_LOW;
             f32x2 l2 = 0, mn2 = 0;
+            const bool starts = off == 0, ends = off + m == stages_of(tl), done = starts && ends;
+            float* part = a.parts + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Sh::PART;
+            // a thread's own dimensions of its row there
+            float* own = part + (size_t)(blk * 128 + row) * DV + DV / 2 * half;
 
 #pragma unroll 1
             for (int i = 0; i < m; i++) {
@@ -344,6 +354,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                     // weights over the half's own scores
                     auto weigh = [&](bool clean) {
                         uint32_t w[16 * Sh::WS];
+                        f32x2 l1 = 0, mn1 = 0;  // this stage's: small terms meet before a large sum
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 vs = *(const float4*)&sk.vs[32 * half + j], vm = *(const float4*)&sk.vm[32 * half + j];
@@ -359,8 +370,8 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                                     s2 = pair(xx.x == -INFINITY ? 0.f : sf.x, xx.y == -INFINITY ? 0.f : sf.y);
                                     m2 = pair(xx.x == -INFINITY ? 0.f : mf.x, xx.y == -INFINITY ? 0.f : mf.y);
                                 }
-                                l2 = add2(l2, p);
-                                mn2 = fma2(p, m2, mn2);
+                                l1 = add2(l1, p);
+                                mn1 = fma2(p, m2, mn1);
                                 const float2 v = unpair(mul2(p, s2));
                                 const uint32_t hw = pack_half2(v.x, v.y);
                                 w[j / 2 + t] = hw;
@@ -370,6 +381,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                                 }
                             }
                         }
+                        l2 = add2(l2, l1), mn2 = add2(mn2, mn1);
                         if constexpr (Sh::WS == 2) tc::st32(scol + buf * 64, w);
                         else tc::st16(scol + buf * 64, w);
                     };
@@ -382,17 +394,52 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 // are announced: a parity tells only neighbouring phases apart,
                 // here of odone and for the issuing thread of pready
                 if (ok && i > 0) ok = warp_wait(odone(blk), (k - 1) & 1);
+                if (__builtin_expect(i > 0 && i % PRE_SUMS == 0, 0) && active && ok) {
+                    // the product of this stage starts from zero
+                    tc::fence_after();
+                    const bool first = i == PRE_SUMS;
+                    float4 e = first ? make_float4(M, 0.f, 0.f, 0.f) : earlier[half][blk * 128 + row];
+                    const float scale = ex2(e.x - M);
+#pragma unroll 1
+                    for (int c = 0; c < DV / 2; c += 16) {
+                        float o[16];
+                        tc::ld16(ocol + c, o);
+                        tc::ld_wait16(o);
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4) {
+                            float4 v = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                            if (!first) {
+                                const float4 w = *(const float4*)(own + c + j);
+                                v.x = __fmaf_rn(w.x, scale, v.x), v.y = __fmaf_rn(w.y, scale, v.y);
+                                v.z = __fmaf_rn(w.z, scale, v.z), v.w = __fmaf_rn(w.w, scale, v.w);
+                            }
+                            *(float4*)(own + c + j) = v;
+                        }
+                    }
+                    // of this stage too, which O has not
+                    const float2 lp = unpair(l2), mp = unpair(mn2);
+                    e.y = __fmaf_rn(e.y, scale, lp.x + lp.y), e.z = __fmaf_rn(e.z, scale, mp.x + mp.y);
+                    l2 = mn2 = 0;
+                    e.x = M;
+                    earlier[half][blk * 128 + row] = e;
+                    tc::fence_before();
+                }
                 __syncwarp();
                 if (lane == 0) tc::bar_arrive(pready(blk));
             }
 
             // the last product, and the result or this CTA's part of it
             if (ok) ok = warp_wait(odone(blk), (it0 + m - 1) & 1);
-            const bool starts = off == 0, ends = off + m == stages_of(tl), done = starts && ends;
             if (active) {
                 tc::fence_after();
                 const float2 lp = unpair(l2), mp = unpair(mn2);
-                float l = lp.x + lp.y, mn = mp.x + mp.y;
+                float l = lp.x + lp.y, mn = mp.x + mp.y, scale = 0.f;
+                const bool more = m > PRE_SUMS && ok;
+                if (more) {
+                    const float4 e = earlier[half][blk * 128 + row];
+                    scale = ex2(e.x - M);
+                    l = __fmaf_rn(e.y, scale, l), mn = __fmaf_rn(e.z, scale, mn);
+                }
                 if (!ok) l = __uint_as_float(0x7fc00000u);
                 const int y = blk * 128 + row;
                 // the halves' sums, each row's in one order
@@ -406,7 +453,6 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 l = half_l[y], mn = half_mn[y];
                 const float norm = done ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 const OutRows<T> to{out, a, rows.first, h, nrows};
-                float* part = a.parts + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Sh::PART;
                 // by way of the queries' shared memory, which this block's
                 // products are done with, so that rows leave as whole lines:
                 // a thread a row has 32 of them open at once, which took 8 to
@@ -420,6 +466,13 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                         float o[16];
                         tc::ld16(ocol + c + u, o);
                         tc::ld_wait16(o);
+                        if (more)
+#pragma unroll
+                            for (int j = 0; j < 16; j += 4) {
+                                const float4 w = *(const float4*)(own + c + u + j);
+                                o[j] = __fmaf_rn(w.x, scale, o[j]), o[j + 1] = __fmaf_rn(w.y, scale, o[j + 1]);
+                                o[j + 2] = __fmaf_rn(w.z, scale, o[j + 2]), o[j + 3] = __fmaf_rn(w.w, scale, o[j + 3]);
+                            }
 #pragma unroll
                         for (int j = 0; j < 16; j += 4)
                             stage[lane * QUADS + (((u + j) / 4) ^ (lane & (QUADS - 1)))] =
@@ -541,7 +594,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                     const float2 kf = unpack_half2(kp), vf = unpack_half2(vp);
                     sk.ks[key] = kf.x, sk.km[key] = __fmaf_rn(8.f, kf.x, kf.y);
                     sk.vs[key] = vf.x, sk.vm[key] = __fmaf_rn(8.f, vf.x, vf.y);
-                    float lg = lg2(fmaxf(vf.x, 5.9604645e-8f));
+                    float lg = lg2(fmaxf(vf.x, 5.9604645e-8f)) - ATT_TOP;
 #pragma unroll
                     for (int o = 16; o; o /= 2) lg = fmaxf(lg, __shfl_xor_sync(0xffffffffu, lg, o));
                     if (lane == 0) sk.lg[w4] = lg;
@@ -614,7 +667,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
 #pragma unroll
                                 for (int c = 0; c < PRE_KEYS / 16; c++)
                                     tc::mma_ts(tm + blk * 256 + 128, p + blk * 256 + c / 2 * 32 + term * 16 + c % 2 * 8, v_lo + c * 2, tc::f16_idesc(DV),
-                                               term > 0 || c > 0 ? 1u : (uint32_t)(i > 0));
+                                               term > 0 || c > 0 ? 1u : (uint32_t)(i % PRE_SUMS != 0));
                         tc::commit(odone(blk));
                         if (blk == 1) tc::commit(empty(slot));
                     }

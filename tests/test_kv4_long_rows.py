@@ -9,7 +9,8 @@ and the background's values repeat a page. So with n background keys
     out = (e^gap v_0 + sum_{1 .. n} v_j) / (e^gap + n)
 
 in 64 bits, from the values as the format holds them. Every sequence reads the
-same two pages, and there are as many sequences as warps, so that each takes a whole row in one run.
+same two pages, and there are as many sequences as warps (or CTAs of the
+many-row kernel), so that each takes a whole row in one run.
 
 Tolerance, relative to the largest value that a row sees (top):
  - half a step of the output type;
@@ -24,7 +25,8 @@ Tolerance, relative to the largest value that a row sees (top):
  - sums: f32 rows add 32 rounds in f32 (2^-25 each) to sums in f64, with the
    codes' part and the middles' part of at most 2 top each; 16-bit rows add
    64 products a term that are truncated at 2^-23 each, and such sums, of
-   1024 keys, in f32.
+   1024 keys, in f32; the many-row kernel has 256 products a term, and sums of 4096
+   keys (64 additions) in f32.
 """
 
 import numpy as np
@@ -32,16 +34,19 @@ import pytest
 
 import kv4_ref
 from test_kv4 import _np, _torch_type
+from test_kv4_many_rows import uses_many_row_kernel
 
 HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
 PAGE = 128
 
 
-def tolerance(dtype, n, gap, share, top, want):
+def tolerance(dtype, n, gap, share, top, want, many_rows):
     d = (gap + 1) * 2.0 ** -22
     weights = (2.0 ** -12 if dtype == "bf16" else 2.0 ** -22) + n * 2.0 ** -36 * 8 / 7
     terms = 1 if dtype == "bf16" else 2
-    if dtype == "f32":
+    if many_rows:
+        sums = 2 * (256 * 2.0 ** -23 * terms + (n / 4096 + 64) * 2.0 ** -24)
+    elif dtype == "f32":
         sums = 2 * 32 * 2.0 ** -25 + 2.0 ** -21
     else:
         sums = 2 * (64 * 2.0 ** -23 * terms + (n / 1024 + 32) * 2.0 ** -24)
@@ -49,7 +54,7 @@ def tolerance(dtype, n, gap, share, top, want):
     return HALF[dtype] * np.abs(want) * (1 + 2.0 ** -7) + floor + (2 * share * (1 - share) * d + weights + sums) * top
 
 
-def run(dtype, dk, dv, keys, rows, seqs, gap, flat, factor=1.0):
+def run(dtype, dk, dv, keys, rows, seqs, gap, flat, many_rows=False, factor=1.0):
     import needle_b200 as nb
     import torch
 
@@ -73,6 +78,8 @@ def run(dtype, dk, dv, keys, rows, seqs, gap, flat, factor=1.0):
     lens = torch.full((seqs,), keys, dtype=torch.int32, device="cuda")
     q = torch.full((seqs * rows, 1, dk), gap / dk, device="cuda", dtype=t)
     assert float(q[0, 0, 0]) * dk == gap
+    if many_rows:
+        assert uses_many_row_kernel(kv, q, table, lens)
     got = _np(nb.op_kv4_attend(kv, q, table, lens, scale=1.0).view(seqs, rows, dv))
     c, s, m = kv4_ref.quantize(_np(v))
     val = (m.astype(np.float64)[..., None] + s.astype(np.float64)[..., None] * c)[:, 0]
@@ -85,7 +92,7 @@ def run(dtype, dk, dv, keys, rows, seqs, gap, flat, factor=1.0):
     share = (pos / (e + pos))[:, None]
     top = np.abs(val).max()
     err = np.abs(got - want)
-    tol = tolerance(dtype, keys, gap, share, top, want)
+    tol = tolerance(dtype, keys, gap, share, top, want, many_rows)
     assert (err <= tol).all(), f"{err.max() / top:.3g} of the values, {(err / tol).max():.3g} of the tolerance"
 
 
@@ -116,6 +123,14 @@ def test_one_key_ahead_of_a_million(cuda_device, dtype, gap):
 def test_blocks_of_sixteen_rows(cuda_device, dtype, dk, dv, gap):
     """f32 prompts: sixteen rows a unit, a warp's run a whole unit."""
     run(dtype, dk, dv, 16384, 272, _sms() * 12 // 17, gap, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128)])
+@pytest.mark.parametrize("gap,keys", [(10, 4096), (14, 16384), (18, 16384), (17.5, 1 << 18)])
+def test_prompts(cuda_device, dtype, dk, dv, gap, keys):
+    run(dtype, dk, dv, keys, 256, _sms(), gap, True, many_rows=True)
 
 
 @pytest.mark.gpu
