@@ -16,8 +16,8 @@
 //    p and p mv stay in registers.
 // Every PRE_SUMS stages O and the sums leave for the CTA's part in the workspace.
 // M_i is raised only when a new exponent passes it by 4, and then O is
-// rescaled in tensor memory; sv enters by its half stage's largest, so that w
-// is at most 2^15 (ATT_TOP).
+// rescaled in tensor memory; sv enters by its half stage's largest where that
+// is near the others (PRE_SPREAD), so that w is at most 2^15 (ATT_TOP).
 // The work is one list of equal runs as in kv4_attend.cu, cut at stages; cut
 // units are joined by the same second kernel.
 //
@@ -32,6 +32,11 @@ namespace nd {
 
 constexpr int PRE_KEYS = 64, PRE_STAGES = 3, PRE_THREADS = 768;
 constexpr int PRE_NT = PRE_ROWS / 8;   // as block_tiles counts rows
+// A half stage whose value scales lie within 2^PRE_SPREAD of one another takes
+// the largest for all in its reference: weights lose that many bits of
+// their range, not of their precision. Others are taken key by key, so that a
+// large value that a row cannot see, or hardly weighs, costs it nothing.
+constexpr float PRE_SPREAD = 4.f;
 constexpr int PRE_UNIT_COST = 3;       // of beginning and ending a unit, in stages
 // Stages after which a unit's sums leave tensor memory and registers and
 // begin anew. The tensor cores truncate a running f32 sum at each product of 16
@@ -53,11 +58,12 @@ struct PreShape {
 };
 
 // Of a stage's keys: scale, middle (minimum + 8 scales) of key and value;
-// log2 of the largest value scale of each half, less ATT_TOP; its four tiles' first
+// log2 of the value scale, less ATT_TOP; of each half the largest of these and
+// how far above the smallest it lies; its four tiles' first
 // positions and which of them exist; whether each block's rows all see all.
-struct StageKeys {
+struct __align__(16) StageKeys {  // read by float4
     float ks[PRE_KEYS], km[PRE_KEYS], vs[PRE_KEYS], vm[PRE_KEYS];
-    float lg[2];
+    float lgs[PRE_KEYS], lg[2], spread[2];
     uint32_t have, whole;  // bits: tiles; blocks
     int k0[4];
 };
@@ -319,7 +325,16 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
 #pragma unroll
                     for (int j = 4; j < 32; j++) t4[j & 3] = fmaxf(t4[j & 3], xs[j]);
                     const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                    const float want = __fmaf_rn(top, f, sk.lg[half]);
+                    float want = __fmaf_rn(top, f, sk.lg[half]);
+                    if (__builtin_expect(sk.spread[half] > PRE_SPREAD, 0)) {
+                        want = -INFINITY;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 lg = *(const float4*)&sk.lgs[32 * half + j];
+                            want = fmaxf(fmaxf(want, fmaxf(__fmaf_rn(xs[j], f, lg.x), __fmaf_rn(xs[j + 1], f, lg.y))),
+                                         fmaxf(__fmaf_rn(xs[j + 2], f, lg.z), __fmaf_rn(xs[j + 3], f, lg.w)));
+                        }
+                    }
                     const bool any = __any_sync(0xffffffffu, want > M + 4.f);
                     if (lane == 0) wish[buf][half][pair_no] = any;
                     if (any) wants[buf][half][blk * 128 + row] = want;
@@ -524,6 +539,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             };
             unsigned long long src = fetch(lane), src_next = fetch(32 + lane);
             uint32_t kw[KW], vw[2][VWW], kp = 0, vp = 0, have = 0;
+            bool held = false;  // this thread's key exists
             auto load = [&](int i) {  // stage i's words
                 if (i && (i & 7) == 0) src = src_next, src_next = fetch(4 * i + 32 + lane);
                 const unsigned long long ka = __shfl_sync(0xffffffffu, src, (4 * i + (key >> 4)) & 31);
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 for (int w = 0; w < KW; w++) kw[w] = 0x88888888u;  // c - 8 = 0
 #pragma unroll
                 for (int w = 0; w < VWW; w++) vw[0][w] = vw[1][w] = 0x88888888u;
-                kp = vp = 0;
+                kp = vp = 0, held = false;
                 if (ka) {
                     const uint8_t* p = (const uint8_t*)ka + (key & 15) * (DK / 2) + half * (DK / 4);
                     if constexpr (DK == 48) {
@@ -548,7 +564,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                     }
                     if (half == 0 && tl.at(first + 4 * i + (key >> 4)) * (long long)KV4_TILE + (key & 15) < len) {
                         const uint8_t* pp = (const uint8_t*)ka + 8 * (DK + DV) + 4 * (key & 15);
-                        kp = __ldg((const uint32_t*)pp), vp = __ldg((const uint32_t*)(pp + 64));
+                        kp = __ldg((const uint32_t*)pp), vp = __ldg((const uint32_t*)(pp + 64)), held = true;
                     }
                 }
                 if (va) {
@@ -594,10 +610,16 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                     const float2 kf = unpack_half2(kp), vf = unpack_half2(vp);
                     sk.ks[key] = kf.x, sk.km[key] = __fmaf_rn(8.f, kf.x, kf.y);
                     sk.vs[key] = vf.x, sk.vm[key] = __fmaf_rn(8.f, vf.x, vf.y);
-                    float lg = lg2(fmaxf(vf.x, 5.9604645e-8f)) - ATT_TOP;
+                    const float lg = lg2(fmaxf(vf.x, 5.9604645e-8f)) - ATT_TOP;
+                    sk.lgs[key] = lg;
+                    // positions that do not exist (their scales are zeros) leave the spread alone
+                    float most = held ? lg : -INFINITY, least = held ? lg : INFINITY;
 #pragma unroll
-                    for (int o = 16; o; o /= 2) lg = fmaxf(lg, __shfl_xor_sync(0xffffffffu, lg, o));
-                    if (lane == 0) sk.lg[w4] = lg;
+                    for (int o = 16; o; o /= 2) {
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+                    }
+                    if (lane == 0) sk.lg[w4] = most, sk.spread[w4] = most - least;
                     if (t == 0) {
                         uint32_t see = have == 15 ? 3 : 0;
 #pragma unroll

@@ -1,6 +1,7 @@
-"""The many-row attention kernel (prompts of 16-bit rows): 64 query heads on
-one kv head, windows that hide keys with NaN among them. Each test asserts that
-its call goes to that kernel, by the size of the workspace it asks for.
+"""The many-row attention kernel (prompts of 16-bit rows): values whose scales
+lie far apart, 64 query heads on one kv head, windows that hide keys with NaN
+among them. Each test asserts that its call goes to that kernel, by the size of
+the workspace it asks for.
 """
 
 import numpy as np
@@ -27,6 +28,63 @@ def attend(st, window=0, sink=0, scale=None):
     t, lens, start = st.dev(st.table), st.dev(st.lens), st.dev(st.start)
     assert uses_many_row_kernel(st.kv, st.q, t, lens, start, window, sink)
     return nb.op_kv4_attend(st.kv, st.q, t, lens, start, window=window, sink=sink, scale=scale)
+
+
+def widen(st):
+    """Columns to spare: the call's plan follows what a table could hold."""
+    st.table = np.pad(st.table, ((0, 0), (0, 40000)), constant_values=-1)
+    return st
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("at", [100, 288, 319, 330])
+def test_a_large_value_that_rows_cannot_see(cuda_device, heads, dtype, at):
+    """One position's values 2^20 times the others': rows before it answer
+    as if it were not there, with the tolerance of what they see."""
+    st = Setup(heads, dtype, [400, 60], [380, 40], 32, seed=at)
+    st.v *= 2.0 ** -8
+    st.v[at] *= 2.0 ** 20
+    widen(st.append())
+    _check(st, dtype, attend(st))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", list(HEADS))
+def test_a_large_value_of_small_weight(cuda_device, heads, dtype):
+    """The same where every later row sees it, with a score some 40 nats
+    below the others. Tolerance: errors follow the weighted magnitude
+    sum p_j max |v_j| of what is seen, not the largest value: (2 d + w) of it
+    with test_kv4's d and w, f16's last step for each key (2^-25 against 2^11
+    and codes to 8), and the truncated sums, keys / 16 of 2^-22."""
+    st = Setup(heads, dtype, [400], [380], 32, seed=5)
+    st.q = (st.q * 0.25 + 1).to(st.t)
+    st.v *= 2.0 ** -8
+    st.v[50] *= 2.0 ** 20
+    st.k *= 0.5
+    st.k[50] = -320.0 / st.dk
+    widen(st.append())
+    scale = 0.125
+    got = _np(attend(st, scale=scale))
+    pages = st.table[0, np.arange(400) // 32]
+    kk, vv = st.ref.k[pages, :, np.arange(400) % 32], st.ref.v[pages, :, np.arange(400) % 32]  # [keys, heads, d]
+    group = st.hq // st.h
+    half = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
+    for g in range(st.hq):
+        x = _np(st.q)[:, g].astype(np.float64) @ kk[:, g // group].T * scale
+        x[np.arange(400)[None] > np.arange(20, 400)[:, None]] = -np.inf
+        p = np.exp(x - x.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        want = p @ vv[:, g // group]
+        mag = (p @ np.abs(vv[:, g // group]).max(1))[:, None]
+        assert (p[31:, 50] < 1e-13).all()
+        b = scale * np.abs(_np(st.q)[:, g]).sum(1, keepdims=True) * 2 * np.abs(kk).max()
+        tol = half * np.abs(want) * (1 + 2.0 ** -7) + 2.0 ** -25 + mag * (
+            2 * (2.0 ** -17 * b + 2.0 ** -20) + (2.0 ** -11 if dtype == "bf16" else 2.0 ** -21) + 400 * 2.0 ** -33 + 400 / 16 * 2.0 ** -22)
+        err = np.abs(got[:, g] - want)
+        assert (err <= tol).all(), f"head {g}: {np.nanmax(err / tol):.3g} of the tolerance"
 
 
 @pytest.mark.gpu
