@@ -28,9 +28,9 @@
 //   2^24 units: it is exact, whatever the order.
 // - value codes are made the f16 e - 8 (one more instruction a pair), each
 //   tile's sum starts at zero and is added to the accumulator rounded.
-// - sums of 32 rounds are carried in f64 (ATT_ROUNDS).
+// - sums of 16 rounds are carried in f64 (ATT_ROUNDS).
 // Measured: 6e-7 of the result against 64 bits where the plain way had 4e-5
-// (keys and values with outlying channels); below 3e-6 over a run of 32,768
+// (keys and values with outlying channels); below 2e-6 over a run of 32,768
 // equal keys behind one that is 10 to 18 nats ahead.
 //
 // A warp keeps the softmax's running reference M per query row (a power-of-
@@ -57,9 +57,9 @@ namespace nd {
 constexpr int ATT_WARPS = 4;
 constexpr int ATT_KT = 2, ATT_STAGES = 3;
 // Rounds after which a run's sums go to memory (f64 for f32 rows) and begin
-// anew: in f32 small terms beside a large sum lose up to 2^-25 of it each,
+// anew: in f32 small terms beside a large sum lose up to 2^-24 of it each,
 // which thousands of equal ones add up. Few runs are that long.
-constexpr int ATT_ROUNDS = 32;
+__host__ __device__ constexpr int ATT_ROUNDS(bool f32) { return f32 ? 16 : 32; }
 constexpr int ATT_CTAS(int nt, int dv) { return nt == 2 || dv == 128 ? 3 : 4; }  // an SM: what registers and shared memory allow
 // Tiles: a shorter run of a cut unit costs more to join than it takes.
 constexpr int ATT_MIN_SHARE = 8;
@@ -91,7 +91,7 @@ constexpr long long ATT_TC_WORK(int dv) { return dv == 128 ? 1 << 16 : 1 << 15; 
 // prompts of 118 rows, 6 heads, bf16, 256 of them: a warp a unit 79, on tcgen05 134.
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
 constexpr int ATT_WARP_MOST(int dv) { return dv == 128 ? 32 : 48; }
-static_assert(ATT_WARP_MOST(64) <= ATT_ROUNDS * ATT_KT && ATT_CTA_TILES / ATT_WARPS + ATT_KT <= ATT_ROUNDS * ATT_KT, "whole units are not LONG");
+static_assert(ATT_WARP_MOST(64) <= ATT_ROUNDS(false) * ATT_KT && ATT_CTA_TILES / ATT_WARPS + ATT_KT <= ATT_ROUNDS(false) * ATT_KT, "whole units are not LONG");
 
 // Whole units are numbered without sums. Places 0 .. seqs - 1 are the
 // sequences' first blocks; the further blocks of sequence s are at most the
@@ -213,7 +213,7 @@ struct PartRegs {
 // A warp's part of a unit: tiles off .. off + m - 1 of query block b of
 // sequence s and kv head h. With `part` NULL they are all it has and the
 // result goes to its place; else the sums go to `part`, unnormalised. LONG:
-// it may have more than ATT_ROUNDS rounds.
+// it may have more rounds than sums in f32 should (ATT_ROUNDS).
 template <int DK, int DV, int NT, typename T, bool LONG>
 __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __restrict__ q, T* __restrict__ out, int s, int h, int b,
                                             const SeqRows& rows, const Tiles& tl, int off, int m, uint8_t* ring, uint2* qsm0,
@@ -221,6 +221,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
     using Sh = AttendShape<DK, DV, NT, T>;
     constexpr int TB = Sh::TB, QS = Sh::QS, WS = Sh::WS, KS = Sh::KSTEPS, MT = DV / 16, VW = DV / 64, KT = Sh::KT, STAGES = Sh::STAGES;
     constexpr bool F32 = Sh::F32;
+    constexpr int ROUNDS = ATT_ROUNDS(F32);
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int nrows = rows.n * (int)a.group.d;
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
@@ -399,8 +400,8 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
     uint32_t get_at = 0;
 #pragma unroll 1
     for (int i = 0; i < m; i += KT) {
-        if (LONG && __builtin_expect(i > 0 && i % (ATT_ROUNDS * KT) == 0, 0)) {
-            const bool first = i == ATT_ROUNDS * KT;
+        if (LONG && __builtin_expect(i > 0 && i % (ROUNDS * KT) == 0, 0)) {
+            const bool first = i == ROUNDS * KT;
             sums([&](int k, float x) {
                 past[k] = first ? (Sum)x : past[k] + (Sum)x;
                 return 0.f;
@@ -563,7 +564,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
                 mn[t] = mul2(mn[t], r);
 #pragma unroll
                 for (int k = 0; k < MT; k++) acc[t][k][0] *= r0, acc[t][k][1] *= r1, acc[t][k][2] *= r0, acc[t][k][3] *= r1;
-                if (LONG && i >= ATT_ROUNDS * KT)
+                if (LONG && i >= ROUNDS * KT)
 #pragma unroll 1
                     for (int k = 0; k < 4 * MT + 4; k += 2) {
                         Sum* o = past + t * (4 * MT + 4) + k;
@@ -650,7 +651,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
     }
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncwarp();
-    if (LONG && m > ATT_ROUNDS * KT) sums([&](int k, float x) { return (float)(past[k] + (Sum)x); });
+    if (LONG && m > ROUNDS * KT) sums([&](int k, float x) { return (float)(past[k] + (Sum)x); });
 
     // this run's part of the unit: sums over the keys' lanes, 2^24 back
     const bool done = !part;

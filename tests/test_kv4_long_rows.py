@@ -22,7 +22,7 @@ Tolerance, relative to the largest value that a row sees (top):
    never more than top in all; and half of f16's last step, 2^-25, for each key
    where the largest weight is 2^11 or more: codes to 8, top at least 7 of
    the value's steps: n 2^-25 2^-11 8 / 7;
- - sums: f32 rows add 32 rounds in f32 (2^-25 each) to sums in f64, with the
+ - sums: f32 rows add 16 rounds in f32 (2^-24 each) to sums in f64, with the
    codes' part and the middles' part of at most 2 top each; 16-bit rows add
    64 products a term that are truncated at 2^-23 each, and such sums, of
    1024 keys, in f32; the many-row kernel has 256 products a term, and sums of 4096
@@ -47,7 +47,7 @@ def tolerance(dtype, n, gap, share, top, want, many_rows):
     if many_rows:
         sums = 2 * (256 * 2.0 ** -23 * terms + (n / 4096 + 64) * 2.0 ** -24)
     elif dtype == "f32":
-        sums = 2 * 32 * 2.0 ** -25 + 2.0 ** -21
+        sums = 2 * 16 * 2.0 ** -24 + 2.0 ** -21
     else:
         sums = 2 * (64 * 2.0 ** -23 * terms + (n / 1024 + 32) * 2.0 ** -24)
     floor = 2.0 ** -25 if dtype == "f16" else 0.0
