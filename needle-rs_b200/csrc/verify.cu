@@ -6,11 +6,14 @@
 // token is drawn from p. What matters here is that a draw is an index that a
 // rounding near a border would change: sums, exponentials and comparisons
 // that decide are in f64. Nearly all of the work is not: a row's maximum is
-// exact in any order, its sum of exponentials is taken in f32 first (off by at
-// most 5e-6: 2^-22 of each ex2, 2^-23 |x| 2^-x of its argument, one rounding a
-// term), and a comparison closer than 1e-4 to its border is decided again
-// with the sum in f64. Only the one row a sequence draws from is summed in
-// f64 throughout.
+// exact in any order, its sum of exponentials is taken from f32 terms first,
+// and a comparison closer than 1e-4 to its border is decided again with the
+// sum in f64. That first sum is off by less than 1e-5 whatever V: 2^-22 of each
+// ex2 and 2^-22 |x| of its argument, where |x| 2^x is below 0.6 or x up to
+// VF_SLACK; five roundings of 2^-24 where a thread adds 16 terms, f64 from
+// there; as much as a term again where parts meet, and at each rescaling, of
+// which at most 11 leave a part that counts. Only the one row a sequence draws
+// from is summed in f64 throughout.
 //
 // Two kernels: one takes every row's statistics (one read of the logits, which
 // bounds the large calls: a CTA a row, or several where rows are few), the
@@ -40,6 +43,7 @@ constexpr int VF_MAX_DRAFT = 64, VF_MAX_SEQS = 1 << 20, VF_MAX_V = 1 << 30;
 constexpr int VF_STATS = 256;        // threads of the first kernel
 constexpr int VF_CHUNK = 4096;       // logits a CTA of it takes at a time
 constexpr int VF_MAX_PARTS = 32;
+constexpr float VF_SLACK = 2.f;      // of an exponent of two
 constexpr int VF_DRAW = 256, VF_WARPS = VF_DRAW / 32;  // of the second
 // Runs are made this short where eight CTAs can; a warp keeps its run's terms
 // up to this length, two CTAs an SM; and up to this where a CTA has an SM to
@@ -104,7 +108,12 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
     const T* row = logits + s * a.l_seq + i * a.l_row;
     const int chunks = (a.V + VF_CHUNK - 1) / VF_CHUNK, per = (chunks + a.parts - 1) / a.parts;
     const int lo = min(part * per, chunks), hi = min(lo + per, chunks);
-    float top = -INFINITY, sum = 0.f;
+    // The sum is against `ref`, which follows the largest logit only when that
+    // is 2^VF_SLACK ahead: each time the sum loses 2^-22 of what is left of it,
+    // which is little. A chunk's terms meet in f32, chunks in f64, so that the
+    // error does not grow with V.
+    float top = -INFINITY, ref = -INFINITY;
+    double sum = 0.0;
     int at = a.V;
     bool nan = false;
     uint4 raw[LOADS];  // the next chunk, where 16-byte loads reach all of it
@@ -155,9 +164,15 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
                 for (int j = 0; j < N; j++) nan |= x[j] != x[j];
                 continue;
             }
-            if (m > top) sum *= vf_ex2((top - m) * scale2), top = m;  // top = -infinity: sum is 0
+            top = m;
+            if ((m - ref) * scale2 > VF_SLACK) sum *= (double)vf_ex2((ref - m) * scale2), ref = m;  // ref = -infinity: sum is 0
+            float part[4];
 #pragma unroll
-            for (int j = 0; j < N; j++) sum += vf_ex2((x[j] - top) * scale2);
+            for (int j = 0; j < N; j++) {
+                const float e = vf_ex2((x[j] - ref) * scale2);
+                part[j & 3] = j < 4 ? e : part[j & 3] + e;
+            }
+            sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
         }
     }
     if (!greedy) nan |= sum != sum, at = top > -INFINITY ? 0 : a.V;
@@ -182,7 +197,7 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
         nan |= ats[w] < 0;
         if (tops[w] > m || (tops[w] == m && ats[w] < at)) m = tops[w], at = ats[w];
     }
-    double z = top == -INFINITY ? 0.0 : (double)sum * (double)vf_ex2((top - m) * scale2);
+    double z = top == -INFINITY ? 0.0 : sum * (double)vf_ex2((ref - m) * scale2);
 #pragma unroll
     for (int o = 16; o; o /= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
     if (lane == 0) sums[warp] = z;

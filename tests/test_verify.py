@@ -264,3 +264,37 @@ def test_entry_point_refuses_without_a_gpu():
 def test_long_rows(cuda_device, dtype, S, T, V):
     """Runs that a warp keeps with two CTAs an SM, alone on one, and not at all."""
     test_matches_reference(cuda_device, dtype, S, T, V, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("below,off", [(0.4875, 4e-4), (0.6125, -5e-4)])
+def test_sums_of_very_long_flat_rows(cuda_device, below, off):
+    """16.8 million logits, all alike but for the first 4096, and drafts whose u
+    lies 4e-4 or 5e-4 of p from their border. Equal terms round the same way, so a
+    running f32 sum of 65,536 of them is off by twice that (these two by -8e-4
+    and +1e-3); the header promises f64's decisions. Probabilities within 5e-6,
+    the bound that the kernel states for its first sum."""
+    import needle_b200 as nb
+    import torch
+
+    S, V = 160, 1 << 24  # 320 rows: a CTA takes a whole one
+    row = torch.full((V,), -below, device="cuda")
+    row[:4096] = 0.0
+    l = row.double().cpu().numpy()
+    e = np.exp(l)
+    p = e / e.sum()
+    draft = np.full((S, 1), 77, np.int32)
+    u = np.random.default_rng(3).random((S, 2)).astype(np.float32)
+    u[:, 0] = p[77] * (1 + off)
+    tokens, accepted, probs = nb.op_verify(row.expand(S, 2, V), _dev(draft), _dev(u), torch.ones(S, device="cuda"))
+    stands = int(off < 0)
+    assert (accepted.cpu().numpy() == stands).all()
+    if not stands:
+        e[77] = 0.0
+    cum = np.cumsum(e)
+    drawn = np.searchsorted(cum, u[:, 1].astype(np.float64) * cum[-1], side="right")
+    tokens, probs = tokens.cpu().numpy(), probs.cpu().numpy()
+    assert np.array_equal(tokens[:, stands], drawn) and (tokens[:, 1 - stands] == (77 if stands else -1)).all()
+    assert (np.abs(probs[:, stands] - p[drawn]) <= 2.0 ** -23 * p[drawn]).all()
+    if stands:
+        assert (np.abs(probs[:, 0] - p[77]) <= 5e-6 * p[77]).all()
