@@ -340,6 +340,11 @@ unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int type, int q_heads, 
 int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row, long long q_head, int q_heads, float scale,
                      int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
                      int flags, void* stream);
+/* The waits inside the kernel for prompts of 16-bit rows are bounded. Should
+ * one run out, which takes a fault elsewhere, what is left of its block's rows
+ * is NaN and the call still returns 0. This sets the bound, in rounds, for the
+ * calls of this process from here on and returns what it was: for tests. */
+unsigned nd_op_kv4_attend_wait_rounds(unsigned rounds);
 
 /* A pool as bytes: page p of layer l lies at pool + p * page_stride + l *
  * layer_stride, page_bytes long (all multiples of 16; pool 16-byte aligned;

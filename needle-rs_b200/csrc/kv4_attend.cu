@@ -51,6 +51,7 @@
 #include "kernels.h"
 #include "kv4_attend.cuh"
 #include "kv4_host.h"
+#include "tc.cuh"
 
 namespace nd {
 
@@ -998,6 +999,8 @@ static void attend_type(int type, const AttendArgs& a, const AttendPlan& p, cons
     else attend_nt<DK, DV, __nv_bfloat16>(a, p, q, out, ws, st);
 }
 
+static std::atomic<uint32_t> wait_rounds{tc::SPIN};
+
 static int attend_group(const nd_kv4* kv, int q_heads, int window, int sink, const char* what) {
     auto fail = [&](const std::string& m) { throw std::runtime_error(std::string(what) + ": " + m); };
     if (q_heads < 1 || q_heads % kv->heads) fail("q_heads must be a multiple of heads");
@@ -1027,6 +1030,8 @@ unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int type, int q_heads, 
     return bytes;
 }
 
+unsigned nd_op_kv4_attend_wait_rounds(unsigned rounds) { return wait_rounds.exchange(rounds); }
+
 int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row, long long q_head, int q_heads, float scale,
                      int window, int sink, void* out, long long o_row, long long o_head, void* ws, unsigned long long ws_bytes,
                      int flags, void* stream) {
@@ -1048,6 +1053,7 @@ int nd_op_kv4_attend(const nd_kv4* kv, int type, const void* q, long long q_row,
         a.scale_log2e = (float)((double)scale * 1.4426950408889634);
         a.q_vec = kv4_vec(type, q, q_row, q_head), a.o_vec = kv4_vec(type, out, o_row, o_head);
         a.zero_rest = flags & ND_ZERO_REST;
+        a.wait_rounds = wait_rounds.load(std::memory_order_relaxed);
         OnDevice on(kv->device, what);
         const AttendPlan plan = attend_plan(kv, group, type, window, sink);
         if (plan.ws && (!ws || ws_bytes < plan.ws)) fail("the workspace is too small");

@@ -15,6 +15,7 @@ struct AttendArgs {
     FastDiv group;       // query heads a kv head
     FastDiv page_tiles;
     int window, sink, places;
+    uint32_t wait_rounds;  // of a wait inside the many-row kernel
     float scale_log2e;
     bool q_vec, o_vec, zero_rest;
     float* parts;   // [runners][2][8 NT * (DV + 2)]; a runner is a warp, for NT = 1 a CTA

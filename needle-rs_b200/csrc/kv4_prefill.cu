@@ -21,7 +21,8 @@
 // The work is one list of equal runs as in kv4_attend.cu, cut at stages; cut
 // units are joined by the same second kernel.
 //
-// Every wait is bounded; should one expire, the CTA's remaining rows are NaN.
+// Every wait is bounded; should one expire, the CTA's remaining rows are NaN, no
+// further product is issued, and those under way are waited for.
 
 #include "kernels.h"
 #include "kv4_attend.cuh"
@@ -96,9 +97,9 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
     __shared__ long long sums[PRE_THREADS + 1];
     __shared__ long long warp_sums[PRE_THREADS / 32];
     __shared__ __align__(16) StageKeys keys[ST];
-    __shared__ __align__(8) uint64_t bars[2 * ST + 4 + 2 + 2 + 1];
+    __shared__ __align__(8) uint64_t bars[2 * ST + 4 + 2 + 2 + 2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag;
+    __shared__ int abort_flag, late;
     // between the two warps of 32 rows: who wants a higher M, by stage parity;
     // the factors at the start, the sums at the end
     __shared__ int wish[2][2][8];
@@ -116,9 +117,9 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
     auto sfull = [&](int b, int buf) { return bar0 + 8u * (2 * ST + 2 * b + buf); };
     auto pready = [&](int b) { return bar0 + 8u * (2 * ST + 4 + b); };
     auto odone = [&](int b) { return bar0 + 8u * (2 * ST + 6 + b); };
-    const uint32_t qready = bar0 + 8u * (2 * ST + 8);
+    const uint32_t qready = bar0 + 8u * (2 * ST + 8), drained = bar0 + 8u * (2 * ST + 9);
     // a warp's wait: all its lanes go on, or none
-    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::bar_wait(bar, parity, abort)) != 0; };
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, tc::bar_wait(bar, parity, abort, a.wait_rounds)) != 0; };
 
     zero_rest<DV>(a, out, blockIdx.x * (PRE_THREADS / 32) + warp, gridDim.x * (PRE_THREADS / 32), lane);
     if (tid == 0) {
@@ -128,7 +129,8 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
             tc::bar_init(pready(b), 8), tc::bar_init(odone(b), 1);
         }
         tc::bar_init(qready, 16);
-        abort_flag = 0;
+        tc::bar_init(drained, 1);
+        abort_flag = late = 0;
         a.joins[blockIdx.x] = make_int4(0, 0, 0, -1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -445,6 +447,9 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
 
             // the last product, and the result or this CTA's part of it
             if (ok) ok = warp_wait(odone(blk), (it0 + m - 1) & 1);
+            // what another role did after giving up may have reached this part
+            __threadfence_block();
+            if (__any_sync(0xffffffffu, *abort)) ok = false;
             if (active) {
                 tc::fence_after();
                 const float2 lp = unpair(l2), mp = unpair(mn2);
@@ -645,7 +650,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
         // (shuffled), and differs by constants from step to step.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(PRE_REGS_ISSUE));
         bool ok = true;
-        int issued = 0;
+        bool issued = false;
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), q_lo = tc::sw128_lo(__shfl_sync(0xffffffffu, base, 0));
         if (warp == 20) for_parts([&](int s, int h, int b, const SeqRows& rows, const Tiles& tl, int off, int m_, int part_no, int it0_, long long last) {
             const int m = __shfl_sync(0xffffffffu, m_, 0), it0 = __shfl_sync(0xffffffffu, it0_, 0);
@@ -657,6 +662,7 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                 if (!ok) return;
                 tc::fence_after();
                 const uint32_t k_lo = q_lo + ((2 * QB + slot * (KB + VB)) >> 4), d = tm + (k & 1) * 64;
+                issued = true;
                 if (tc::elect()) {
 #pragma unroll
                     for (int c = 0; c < DK / 16; c++)
@@ -694,12 +700,16 @@ __global__ void __launch_bounds__(PRE_THREADS, 1) kv4_prefill_kernel(AttendArgs 
                         if (blk == 1) tc::commit(empty(slot));
                     }
                     __syncwarp();
-                    if (blk == 1) issued = k + 1;
                 }
             }
         });
-        // every product issued is over before the memory is freed
-        if (warp == 20 && issued > 0) warp_wait(empty((issued - 1) % ST), ((issued - 1) / ST) & 1);
+        // Every product issued, by the same lane each time, is over before its
+        // memory is freed, also where a wait has expired: this one has its own bound.
+        if (warp == 20 && issued) {
+            if (tc::elect()) tc::commit(drained);
+            __syncwarp();
+            tc::bar_wait(drained, 0, &late);
+        }
     }
     tc::fence_before();
     __syncthreads();

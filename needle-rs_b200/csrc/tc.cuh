@@ -8,7 +8,7 @@
 namespace nd {
 namespace tc {
 
-constexpr uint32_t SPIN = 1u << 18;  // try_wait rounds before a wait counts as failed
+constexpr uint32_t SPIN = 1u << 18;  // try_wait rounds before a wait counts as failed, if the caller has no other number
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -18,10 +18,10 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
-// Wait for phase `parity`, giving up after SPIN rounds or once another role
-// has (*abort set): false then.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-    for (uint32_t it = 0; it < SPIN; it++) {
+// Wait for phase `parity`, giving up after `rounds` or once another role has
+// (*abort set): false then.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t rounds = SPIN) {
+    for (uint32_t it = 0; it < rounds; it++) {
         uint32_t ok;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
                      : "=r"(ok)
@@ -31,6 +31,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         if ((it & 255) == 255 && *abort) return false;
     }
     *abort = 1;
+    __threadfence_block();  // seen by whoever sees what this thread does next
     return false;
 }
 

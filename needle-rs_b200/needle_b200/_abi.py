@@ -27,5 +27,6 @@ SIGNATURES = {
     "nd_op_kv4_append": (_I, [_P, _I, _P, _L, _L, _P, _L, _L, _P]),
     "nd_op_kv4_read": (_I, [_P, _I, _P, _L, _L, _P, _L, _L, _I, _P]),
     "nd_op_kv4_attend_ws": (_U, [_P, _I, _I, _I, _I]),
+    "nd_op_kv4_attend_wait_rounds": (C.c_uint, [C.c_uint]),
     "nd_op_kv4_attend": (_I, [_P, _I, _P, _L, _L, _I, C.c_float, _I, _I, _P, _L, _L, _P, _U, _I, _P]),
 }

@@ -129,3 +129,29 @@ def test_nan_behind_a_window(cuda_device, dtype):
             nan[:, 0] = True
         nan[7, 3] = True
         assert np.array_equal(np.isnan(got).any(-1), nan) and np.array_equal(np.isnan(got).all(-1), nan)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", list(HEADS))
+def test_waits_that_run_out(cuda_device, heads, dtype):
+    """With hardly a round for its waits the kernel gives rows up: what it
+    returns is NaN or right, it ends, and the next call is right. (Nothing that
+    follows a wait takes an address from what was waited for, the barriers among
+    warps are passed either way, and products under way are drained.)"""
+    import needle_b200 as nb
+    import torch
+
+    st = widen(Setup(heads, dtype, [900, 600, 300], [250, 200, 300], 32, seed=2, extra_rows=2).append())
+    want = attend(st)
+    for rounds in (0, 1, 2, 4):
+        was = nb.lib().nd_op_kv4_attend_wait_rounds(rounds)
+        try:
+            got = attend(st)
+            torch.cuda.synchronize()
+        finally:
+            assert nb.lib().nd_op_kv4_attend_wait_rounds(was) == rounds
+        gone = torch.isnan(got)
+        assert (gone | (got == want)).all() and (got[-2:] == 0).all()
+        assert rounds or gone[:-2].all()
+    assert torch.equal(attend(st), want)
