@@ -6,6 +6,7 @@ square root; host code with -ffp-contract=off for the same reason.
 """
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -37,6 +38,20 @@ def _stale(target, sources):
     return any(os.path.getmtime(s) > t for s in sources)
 
 
+def check_registers(source: str, log: str) -> None:
+    """The prompt kernel shares its registers out anew among its warpgroups; a
+    share beyond what the block was launched with would wait for ever. So the
+    build ends here should the compiler (its -v log) give a thread fewer than
+    the PRE_REGS_LAUNCH that the source counts on (registers come in eights)."""
+    need = int(re.search(r"PRE_REGS_LAUNCH = (\d+)", source).group(1))
+    got = [int(n) for name, n in re.findall(r"Compiling entry function '(\S+)'.*?Used (\d+) registers", log, re.S)
+           if "kv4_prefill_kernel" in name]
+    if not got:
+        raise RuntimeError("no register counts of kv4_prefill_kernel in the compiler's log")
+    if any((n + 7) // 8 * 8 < need for n in got):
+        raise RuntimeError(f"kv4_prefill_kernel has {min(got)} registers a thread; its warpgroups share out {need}")
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [
         os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)
@@ -60,13 +75,21 @@ def build(force: bool = False, verbose: bool = False) -> str:
         o = os.path.join(BUILD, f + ".o")
         cmd = [nvcc, *ARCH, *common, "-lineinfo", "-fmad=false", "-prec-div=true", "-prec-sqrt=true",
                "-Xcompiler", "-fPIC,-ffp-contract=off", "-c", os.path.join(CSRC, f), "-o", o]
+        shares = f == "kv4_prefill.cu"
+        if shares:
+            cmd += ["-Xptxas", "-v"]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
-        procs.append((cmd, subprocess.Popen(cmd)))
+        procs.append((cmd, shares, subprocess.Popen(cmd, stderr=subprocess.PIPE if shares else None, text=True)))
         objs.append(o)
-    for cmd, proc in procs:
-        if proc.wait():
+    for cmd, shares, proc in procs:
+        _, log = proc.communicate()
+        if proc.returncode:
+            print(log or "", file=sys.stderr)
             raise subprocess.CalledProcessError(proc.returncode, cmd)
+        if shares:
+            with open(os.path.join(CSRC, "kv4_prefill.cu")) as src:
+                check_registers(src.read(), log)
     tmp = LIB + ".tmp"
     cmd = [nvcc, *ARCH, "-shared", "-o", tmp, *objs, "-lpthread"]
     if verbose:

@@ -43,10 +43,12 @@ constexpr int PRE_UNIT_COST = 3;       // of beginning and ending a unit, in sta
 // begin anew. The tensor cores truncate a running f32 sum at each product of 16
 // keys: over 262,144 keys that cost f16 rows 3e-3 of the values.
 constexpr int PRE_SUMS = 64;
-// Registers of a thread: launched with 80, then shared out by warpgroup (the
-// rows' four, the operands', the issuer's), which sums to what was launched.
+// Registers of a thread: launched with 80 (the build checks that the compiler
+// gave as many), then shared out by warpgroup (the rows' four, the operands',
+// the issuer's), which sums to what was launched.
+constexpr int PRE_REGS_LAUNCH = 80;
 constexpr int PRE_REGS_ROWS = 88, PRE_REGS_CODES = 56, PRE_REGS_ISSUE = 72;
-static_assert(4 * PRE_REGS_ROWS + PRE_REGS_CODES + PRE_REGS_ISSUE <= 6 * 80, "registers of the six warpgroups");
+static_assert(4 * PRE_REGS_ROWS + PRE_REGS_CODES + PRE_REGS_ISSUE <= 6 * PRE_REGS_LAUNCH, "registers of the six warpgroups");
 
 template <int DK, int DV, typename T>
 struct PreShape {
