@@ -29,6 +29,13 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _int(x, name):
+    """x, where a C int holds it: ctypes drops the bits above without a word."""
+    if not -2147483648 <= x <= 2147483647:
+        raise ValueError(f"{name} is beyond 32 bits: {x}")
+    return x
+
+
 def _int32(t, n, device, name):
     """The address of a contiguous int32 vector of n."""
     if t.dtype is not torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
@@ -50,6 +57,7 @@ class KV4Pool:
             raise ValueError(f"a tile of ({dk}, {dv}) holds {self.tile_bytes(dk, dv)} bytes, got {list(data.shape)}")
         if data.stride(3) != 1 or (tiles > 1 and data.stride(2) != tile) or (h > 1 and data.stride(1) != tiles * tile):
             raise ValueError("a page's heads and tiles must be contiguous")
+        _int(max(n, h, tiles * _TILE), "a size of the pool")
         self.data, self.dk, self.dv = data, dk, dv
         self.num_pages, self.heads, self.page = n, h, tiles * _TILE
         self.device = data.device
@@ -72,7 +80,7 @@ class KV4Pool:
         dev = self.device
         s, a = table.shape[0], _KV4.from_buffer_copy(self._fixed)
         a.seqs, a.max_pages, a.table_stride = _table(table, dev)
-        a.table, a.lens, a.rows = table.data_ptr(), _int32(lens, s, dev, "lens"), rows
+        a.table, a.lens, a.rows = table.data_ptr(), _int32(lens, s, dev, "lens"), _int(rows, "rows")
         if start is not None:
             a.start = _int32(start, s + 1, dev, "start")
         return C.byref(a)
@@ -140,6 +148,7 @@ def op_kv4_attend(kv, q, table, lens, start=None, scale=None, window=0, sink=0, 
             raise ValueError("out must have q's type and rows")
         oa = kv._rows(out, hq, kv.dv, "out")
     L = lib()
+    _int(hq, "q_heads"), _int(window, "window"), _int(sink, "sink")
     n = L.nd_op_kv4_attend_ws(a, _TYPES[q.dtype], hq, window, sink)
     ws = kv.data.new_empty(n) if n else None
     if L.nd_op_kv4_attend(a, _TYPES[q.dtype], *qa, hq, 1 / math.sqrt(kv.dk) if scale is None else scale, window, sink, *oa,
@@ -153,7 +162,7 @@ def _pages(pool, axis):
     [layers, pages, ..])."""
     if not pool.is_cuda or axis not in (0, 1) or pool.dim() <= axis or not pool.numel():
         raise ValueError("pool must be a CUDA tensor [pages, ..], or [layers, pages, ..] with axis=1")
-    n, layers = pool.shape[axis], pool.shape[0] if axis else 1
+    n, layers = _int(pool.shape[axis], "pages"), _int(pool.shape[0], "layers") if axis else 1
     size = pool.element_size()
     inner = 1
     for d in range(pool.dim() - 1, axis, -1):
@@ -171,6 +180,7 @@ def _table(table, device):
     (s, p), (stride, inner) = table.shape, table.stride()
     if not s or not p or (inner != 1 and p > 1):
         raise ValueError("table must have sequences and columns, each row contiguous")
+    _int(max(s, p, stride), "a size of the table")
     return s, p, stride if s > 1 else p
 
 
@@ -194,10 +204,11 @@ def op_pages_fork(pool, table, src, keep, need, page, pinned=None, axis=0):
     dev = pool.device
     pv, n_pages = _pages(pool, axis)
     s, p, stride = _table(table, dev)
-    n = src.shape[0] if src.dim() else 0
+    n = _int(src.shape[0], "src's length") if src.dim() else 0
     if not n:
         raise ValueError("src must name at least one sequence")
     out, refs = table.new_empty((n, p)), table.new_empty(n_pages)
+    _int(page, "page")
     L = lib()
     size = L.nd_op_pages_fork_ws(n_pages, n)
     ws = table.new_empty(4 + (size + 3) // 4)
@@ -239,6 +250,7 @@ def op_verify(logits, draft, u, temperature, q=None, counts=None):
     if logits.dtype not in _TYPES or logits.dim() != 3 or not logits.is_cuda or logits.stride(2) != 1 or not logits.numel():
         raise ValueError("logits must be a float32, float16 or bfloat16 CUDA tensor [seqs, T + 1, V], rows contiguous")
     s, t1, v = logits.shape
+    _int(max(s, t1, v), "a size of logits")
     t = t1 - 1
     if draft.dtype is not torch.int32 or draft.shape != (s, t) or draft.device != dev or not draft.is_contiguous():
         raise ValueError(f"draft must be a contiguous int32 tensor [{s}, {t}] on {dev}")
