@@ -43,6 +43,31 @@ def _int32(t, n, device, name):
     return t.data_ptr()
 
 
+def _overlap(a, b):
+    """Whether a value of a and one of b [rows, heads, d] (one type, d
+    contiguous, strides not negative) share memory."""
+    if not a.numel() or not b.numel():
+        return False
+    size, (n, h, da), db = a.element_size(), a.shape, b.shape[2]
+    off = b.data_ptr() - a.data_ptr()
+    if off % size:  # values that lie across one another: by bytes
+        (ra, ha), (rb, hb), da, db = [s * size for s in a.stride()[:2]], [s * size for s in b.stride()[:2]], da * size, db * size
+    else:
+        (ra, ha), (rb, hb), off = a.stride()[:2], b.stride()[:2], off // size
+    heads = b.shape[1]
+    if off >= (n - 1) * ra + (h - 1) * ha + da or -off >= (b.shape[0] - 1) * rb + (heads - 1) * hb + db:
+        return False
+    # parts of one buffer that repeats by heads, or by rows
+    if ha == hb > 0 and ra % ha == 0 and rb % ha == 0 and off % ha >= da and off % ha + db <= ha:
+        return False
+    if ra == rb > 0 and off % ra >= (h - 1) * ha + da and off % ra + (heads - 1) * hb + db <= ra:
+        return False
+    runs = lambda n, r, h, s: (torch.arange(n, device="cpu")[:, None] * r + torch.arange(h, device="cpu") * s).flatten()
+    first, other = runs(n, ra, h, ha).sort().values, runs(b.shape[0], rb, heads, hb) + off
+    at = torch.searchsorted(first, other + db) - 1  # the last run of a that begins before the one of b ends
+    return bool(((at >= 0) & (first[at.clamp(min=0)] + da > other)).any())
+
+
 class KV4Pool:
     """A pool of pages of 4-bit keys and values. ``data`` is a uint8 CUDA
     tensor [pages, heads, page / 16, tile] as the header lays it out (a page's
@@ -132,7 +157,7 @@ def op_kv4_attend(kv, q, table, lens, start=None, scale=None, window=0, sink=0, 
     type. A row sees the positions up to its own, with ``window`` the last
     ``window`` of them and the first ``sink``. ``scale`` defaults to
     1 / sqrt(dk). Rows behind the last sequence are left as they were in a
-    given ``out`` and are zeros in a new one."""
+    given ``out``, which must not overlap ``q``, and are zeros in a new one."""
     shape = q.shape
     if len(shape) != 3 or not shape[1] or shape[1] % kv.heads:
         raise ValueError(f"q must be [rows, q_heads, dk] with a multiple of {kv.heads} heads")
@@ -147,6 +172,8 @@ def op_kv4_attend(kv, q, table, lens, start=None, scale=None, window=0, sink=0, 
         if out.dtype is not q.dtype or out.shape[:1] != q.shape[:1]:
             raise ValueError("out must have q's type and rows")
         oa = kv._rows(out, hq, kv.dv, "out")
+        if _overlap(q, out):
+            raise ValueError("out must not overlap q")
     L = lib()
     _int(hq, "q_heads"), _int(window, "window"), _int(sink, "sink")
     n = L.nd_op_kv4_attend_ws(a, _TYPES[q.dtype], hq, window, sink)
