@@ -333,7 +333,8 @@ int nd_op_kv4_read(const nd_kv4* kv, int type, void* k, long long k_row, long lo
  * head g reads kv head g / (q_heads / heads), q_heads / heads <= 64. A row at
  * position p sees the positions j <= p that exist, with window > 0 only those
  * with j > p - window or j < sink. out = softmax(scale q.k) v; zeros for a row
- * that sees nothing. out must not overlap q. ws:
+ * that sees nothing. Scores are held in f32: queries beyond 2^100 may give NaN.
+ * out must not overlap q. ws:
  * nd_op_kv4_attend_ws(the same arguments) bytes, 16-byte aligned; NULL where
  * that is 0. */
 unsigned long long nd_op_kv4_attend_ws(const nd_kv4* kv, int type, int q_heads, int window, int sink);
@@ -402,7 +403,8 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
  * is all zero) at the first i refused, from p after the last: the first j
  * whose running sum over 0 .. j exceeds u[T] times the whole. accepted[seqs];
  * tokens[seqs][T + 1]: the accepted drafts, the drawn token, then -1;
- * probs[seqs][T + 1]: p of each of them, then 0. A row that holds a NaN, a
+ * probs[seqs][T + 1]: p of each of them (the drawn one's rounded once, an
+ * accepted draft's within 1e-5 of itself), then 0. A row that holds a NaN, a
  * +infinity at a temperature above 0, or nothing above -infinity accepts
  * nothing and draws -1 with probability 0; so does a residual that holds a
  * NaN. A drafted id outside [0, V) is refused. Sums and comparisons that

@@ -66,7 +66,8 @@ constexpr int ATT_CTAS(int nt, int dv) { return nt == 2 || dv == 128 ? 3 : 4; } 
 constexpr int ATT_MIN_SHARE = 8;
 // What beginning and ending a unit costs a warp, in tiles: without it a warp
 // that meets many short units is the last by far (8 sequences, one of a
-// single position among lengths up to 32768: 70 us instead of 57).
+// single position among lengths up to 32768: 70 us instead of 57, before sums
+// were carried on).
 constexpr int ATT_UNIT_COST = 4;
 // 16-bit rows that would be cut go to the tcgen05 kernel from this many query
 // rows a sequence and kv head on average, and this many tiles by blocks of
@@ -90,6 +91,10 @@ constexpr long long ATT_TC_WORK(int dv) { return dv == 128 ? 1 << 16 : 1 << 15; 
 // in a window of 74 tiles, five tokens, 256 sequences 51.5, 54.1. Heads of 128
 // bf16, 256 of up to 400 39.0, 34.8, 47.2; 128 of up to 740 34.0, 37.5, -. Whole
 // prompts of 118 rows, 6 heads, bf16, 256 of them: a warp a unit 79, on tcgen05 134.
+// Tiles here are what the table's columns or the window could hold, as the
+// host knows no lengths: with columns for 4096 positions the same calls are cut
+// or go to tcgen05 (one session 4.8, 10.3; 1024 sequences of up to 256 19.1, 31.2;
+// 32 of them 6.2, 15.4; 16 prompts of 118 rows 10.5, 32.3).
 constexpr int ATT_WARP_TILES = 16, ATT_CTA_TILES = 128;
 constexpr int ATT_WARP_MOST(int dv) { return dv == 128 ? 32 : 48; }
 static_assert(ATT_WARP_MOST(64) <= ATT_ROUNDS(false) * ATT_KT && ATT_CTA_TILES / ATT_WARPS + ATT_KT <= ATT_ROUNDS(false) * ATT_KT, "whole units are not LONG");

@@ -25,7 +25,7 @@
 // Measured (us, GPU alone; 256 sequences of up to 7 drafts, 16384 f32 logits):
 // one kernel with a CTA a row 236; two kernels 64, the second waiting for
 // its f64 terms one after another; with terms in batches of four without
-// branches 53, batches of eight whose places need no checks 44. Runs of 512 on
+// branches 53, batches of eight whose places need no checks 45. Runs of 512 on
 // four CTAs instead of 1024 on two took 4 more. An exponential of fewer f64
 // steps (a table of 2^(j/16)) gained nothing: issue and latency bound it.
 
@@ -43,6 +43,9 @@ constexpr int VF_MAX_DRAFT = 64, VF_MAX_SEQS = 1 << 20, VF_MAX_V = 1 << 30;
 constexpr int VF_STATS = 256;        // threads of the first kernel
 constexpr int VF_CHUNK = 4096;       // logits a CTA of it takes at a time
 constexpr int VF_MAX_PARTS = 32;
+// CTAs that rows are cut for: four an SM. A constant, so that a workspace's
+// size does not depend on which device is current when it is asked for.
+constexpr int VF_FILL = 4 * 148;
 constexpr float VF_SLACK = 2.f;      // of an exponent of two
 constexpr int VF_DRAW = 256, VF_WARPS = VF_DRAW / 32;  // of the second
 // Runs are made this short where eight CTAs can; a warp keeps its run's terms
@@ -501,7 +504,7 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
 static int verify_parts(int seqs, int T, int V) {
     // few rows: enough CTAs for the GPU, a chunk each at least
     const long long rows = (long long)seqs * (T + 1), chunks = (V + VF_CHUNK - 1) / VF_CHUNK;
-    return (int)std::max(1LL, std::min({chunks, (long long)VF_MAX_PARTS, 592 / rows}));
+    return (int)std::max(1LL, std::min({chunks, (long long)VF_MAX_PARTS, VF_FILL / rows}));
 }
 
 static unsigned long long verify_ws(int seqs, int T, int V) {

@@ -6,7 +6,8 @@ drafted tokens.
 Tensors are CUDA tensors of one device; work is queued on that device's
 current torch stream. Tables, lengths and offsets are int32 and read on the
 device, so calls can be captured into a CUDA graph and replayed as they
-change. Bad arguments raise ValueError before anything is queued.
+change. Bad arguments raise ValueError, or RuntimeError where the C entry
+refuses them, before anything is queued.
 """
 
 import ctypes as C
