@@ -91,12 +91,15 @@ __device__ __forceinline__ int drafts_of(const VerifyArgs& a, int s) { return a.
 struct Temperature {
     bool greedy;
     double inv;
-    float scale2;  // of an exponent of two
+    float pre, scale2;  // of an exponent of two: pre is 1, or 2^64 where LOG2E / t is no f32
     __device__ explicit Temperature(float t) {
-        greedy = !(t > 0.f && LOG2E / t <= FLT_MAX);
+        greedy = !(t > 0.f);
         inv = greedy ? 1.0 : 1.0 / (double)t;
-        scale2 = greedy ? LOG2E : LOG2E / t;
+        pre = !greedy && t < 1e-37f ? 18446744073709551616.f : 1.f;
+        scale2 = greedy ? LOG2E : LOG2E / (t * pre);
     }
+    // d / t as an exponent of two
+    __device__ __forceinline__ float two(float d) const { return d * pre * scale2; }
 };
 
 template <typename T>
@@ -106,7 +109,6 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
     const int r = blockIdx.x / a.parts, part = blockIdx.x % a.parts, s = r / (a.T + 1), i = r % (a.T + 1), tid = threadIdx.x;
     if (i > drafts_of(a, s)) return;
     const Temperature tp(__ldg(a.temp + s));
-    const float scale2 = tp.scale2;
     const bool greedy = tp.greedy;
     const T* row = logits + s * a.l_seq + i * a.l_row;
     const int chunks = (a.V + VF_CHUNK - 1) / VF_CHUNK, per = (chunks + a.parts - 1) / a.parts;
@@ -168,11 +170,11 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
                 continue;
             }
             top = m;
-            if ((m - ref) * scale2 > VF_SLACK) sum *= (double)vf_ex2((ref - m) * scale2), ref = m;  // ref = -infinity: sum is 0
+            if (tp.two(m - ref) > VF_SLACK) sum *= (double)vf_ex2(tp.two(ref - m)), ref = m;  // ref = -infinity: sum is 0
             float part[4];
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                const float e = vf_ex2((x[j] - ref) * scale2);
+                const float e = vf_ex2(tp.two(x[j] - ref));
                 part[j & 3] = j < 4 ? e : part[j & 3] + e;
             }
             sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(VF_STATS) verify_stats_kernel(VerifyArgs a, co
         nan |= ats[w] < 0;
         if (tops[w] > m || (tops[w] == m && ats[w] < at)) m = tops[w], at = ats[w];
     }
-    double z = top == -INFINITY ? 0.0 : sum * (double)vf_ex2((ref - m) * scale2);
+    double z = top == -INFINITY ? 0.0 : sum * (double)vf_ex2(tp.two(ref - m));
 #pragma unroll
     for (int o = 16; o; o /= 2) z += __shfl_xor_sync(0xffffffffu, z, o);
     if (lane == 0) sums[warp] = z;
@@ -253,7 +255,7 @@ __device__ __forceinline__ double warp_sum(double x) {
 
 // A row's statistics from its parts, in their order; at < 0 where it is no
 // distribution. For a whole warp.
-__device__ __forceinline__ RowStats join_stats(const RowStats* parts, int n, float scale2, int lane) {
+__device__ __forceinline__ RowStats join_stats(const RowStats* parts, int n, const Temperature& tp, int lane) {
     RowStats r{-INFINITY, 0x7fffffff, 0.0};
     if (lane < n) r = parts[lane];
     float m = r.top;
@@ -267,7 +269,7 @@ __device__ __forceinline__ RowStats join_stats(const RowStats* parts, int n, flo
         nan |= __shfl_xor_sync(0xffffffffu, (int)nan, o) != 0;
     }
     RowStats out{m, nan || m == -INFINITY ? -1 : at, 0.0};
-    out.sum = warp_sum(r.top == -INFINITY ? 0.0 : r.sum * (double)vf_ex2((r.top - m) * scale2));
+    out.sum = warp_sum(r.top == -INFINITY ? 0.0 : r.sum * (double)vf_ex2(tp.two(r.top - m)));
     return out;
 }
 
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(VF_DRAW) verify_draw_kernel(VerifyArgs a, cons
         return uq < *p;
     };
     for (int i = warp; i <= n; i += VF_WARPS) {
-        const RowStats st = join_stats(a.stats + ((size_t)s * (T_ + 1) + i) * a.parts, a.parts, tp.scale2, lane);
+        const RowStats st = join_stats(a.stats + ((size_t)s * (T_ + 1) + i) * a.parts, a.parts, tp, lane);
         if (lane == 0) {
             rows[i] = st;
             if (i < n) verdict[i] = judge(i, st, false, &probs[i]);

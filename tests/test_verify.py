@@ -298,3 +298,22 @@ def test_sums_of_very_long_flat_rows(cuda_device, below, off):
     assert (np.abs(probs[:, stands] - p[drawn]) <= 2.0 ** -23 * p[drawn]).all()
     if stands:
         assert (np.abs(probs[:, 0] - p[77]) <= 5e-6 * p[77]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,V", [(3, 50), (2, 20011)])
+def test_temperatures_below_the_normal_numbers(cuda_device, T, V):
+    """Above 0 is above 0: of tied logits each is drawn, also where 1 /
+    temperature is no f32, and differences as small as the temperature count."""
+    r = np.random.default_rng(V)
+    temp = np.array([1e-39, 1.4e-45, 3e-40, 4.2e-39, 1.2e-38, 1e-41, 0.0])
+    S = len(temp)
+    logits = r.integers(0, 3, (S, T + 1, V)).astype(np.float64)
+    logits[5] = r.integers(0, 2000, (T + 1, V)) * 1e-44
+    draft = logits[:, :T].argmax(-1)
+    q = np.full((S, T, V), 1 / V)
+    u = r.random((S, T + 1))
+    w = run(logits, draft, u, temp, q)
+    assert len({int(t) for t in w[0][np.arange(S), w[1]]}) > 3
+    run(logits, draft, u, temp)
+    run(np.maximum(logits, 1.0), draft, u, temp, dtype="bfloat16")
