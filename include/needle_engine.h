@@ -396,7 +396,7 @@ int nd_op_pages_compact(const nd_pages* pool, const int* table, int table_stride
  * the token after the last one. counts[seqs] (NULL: T each; cut to [0, T])
  * says how many of draft[seqs][T] there are; T <= 64. p_i = softmax(logits_i /
  * temperature[s]), or one at the first largest logit where the temperature
- * is not above 0. q[seqs][T][V] f32 (strides q_seq, q_row; NULL: the draft
+ * is not above 0 (+infinity: all logits above -infinity alike). q[seqs][T][V] f32 (strides q_seq, q_row; NULL: the draft
  * was certain of its tokens): the draft's probabilities. u[seqs][T + 1] in
  * [0, 1). Draft i is accepted, while all before it are, if u[i] q_i(draft_i)
  * < p_i(draft_i). The next token is drawn from max(p_i - q_i, 0) (p_i if that

@@ -94,6 +94,7 @@ struct Temperature {
     float pre, scale2;  // of an exponent of two: pre is 1, or 2^64 where LOG2E / t is no f32
     __device__ explicit Temperature(float t) {
         greedy = !(t > 0.f);
+        t = fminf(t, FLT_MAX);  // an infinite one: the limit, where -infinity still has no part
         inv = greedy ? 1.0 : 1.0 / (double)t;
         pre = !greedy && t < 1e-37f ? 18446744073709551616.f : 1.f;
         scale2 = greedy ? LOG2E : LOG2E / (t * pre);

@@ -317,3 +317,22 @@ def test_temperatures_below_the_normal_numbers(cuda_device, T, V):
     assert len({int(t) for t in w[0][np.arange(S), w[1]]}) > 3
     run(logits, draft, u, temp)
     run(np.maximum(logits, 1.0), draft, u, temp, dtype="bfloat16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("S,T,V", [(2, 2, 9), (5, 3, 20011), (1, 1, 130001)])
+def test_infinite_temperatures(cuda_device, dtype, S, T, V):
+    """The limit of ever larger ones: all tokens alike, but those at -infinity."""
+    logits, draft, u, temp, q = case(S, T, V, 17)
+    w = run(logits, draft, u, np.full(S, np.inf), q, dtype=dtype)
+    assert (w[0][np.arange(S), w[1]] >= 0).all()
+    run(logits, draft, u, np.full(S, 3e38), dtype=dtype)
+    logits[:, :, 1::2] = -np.inf
+    import needle_b200 as nb
+    import torch
+
+    lt = _dev(logits.astype(np.float32)).to(getattr(torch, dtype))
+    got = nb.op_verify(lt, _dev(draft.astype(np.int32)), _dev(u.astype(np.float32)), _dev(np.full(S, np.inf, np.float32)))
+    want = ref_verify(lt.float().cpu().numpy(), draft, u.astype(np.float32), np.full(S, 3e38, np.float32), None, np.full(S, T))
+    assert np.array_equal(got[0].cpu().numpy(), want[0]) and np.array_equal(got[1].cpu().numpy(), want[1])
