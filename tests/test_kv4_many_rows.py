@@ -1,7 +1,8 @@
 """The many-row attention kernel (prompts of 16-bit rows): values whose scales
 lie far apart, 64 query heads on one kv head, windows that hide keys with NaN
 among them. Each test asserts that its call goes to that kernel, by the size of
-the workspace it asks for.
+the workspace it asks for. (test_kv4's tests on wide tables reach it where no
+window, or one of more than 48 tiles, is given: smaller ones make units short.)
 """
 
 import numpy as np
