@@ -582,7 +582,7 @@ __device__ __forceinline__ void attend_part(const AttendArgs& a, const T* __rest
         }
         // weights, and their operands: rows of the transpose are query rows
         uint32_t wop[KT][NT][2][WS];
-        f32x2 l1[NT], mn1[NT];  // this round's
+        f32x2 l1[NT], mn1[NT];  // of these tiles
 #pragma unroll
         for (int u = 0; u < KT; u++) {
             const f32x2 vsa = pair(vpa[u].x, vpa[u].x), vsb = pair(vpb[u].x, vpb[u].x), vma = pair(vpa[u].y, vpa[u].y), vmb = pair(vpb[u].y, vpb[u].y);
